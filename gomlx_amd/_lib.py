@@ -56,6 +56,11 @@ SIGNATURES = [
     ("gq_qdense_norm_bf16_batch", _int, [_int, _vp, _vp, _vp]),
     ("gq_qdense_gated_bf16", _int, [_int, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _int, _vp, _vp]),
     ("gq_embedding_lookup", _int, [_int, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    ("gq_qk_norm_rope", _int, [_int, _vp, _int, _vp, _int, _int, _i64, _vp, _vp, _vp, _i64, _int, _int, _vp, _vp, _int, _vp, _vp, _vp]),
+    ("gq_kv_append", _int, [_vp, _int, _vp, _vp, _vp, _vp]),
+    ("gq_kv_read", _int, [_vp, _vp, _vp, _vp]),
+    ("gq_kv_attention", _int, [_vp, _int, _vp, _int, ctypes.c_float, _i64, _vp, _vp, _vp]),
+    ("gq_kv_evict", _int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp]),
     ("gq_graph_begin", _int, [_vp]),
     ("gq_graph_end", _int, [_vp, ctypes.POINTER(_vp)]),
     ("gq_graph_launch", _int, [_vp, _vp]),
@@ -76,6 +81,17 @@ class DenseDesc(ctypes.Structure):
 class RmsNormDesc(ctypes.Structure):
     """gq_rmsnorm of include/gomlx_hipq.h."""
     _fields_ = [("dGain", _vp), ("eps", ctypes.c_float), ("gain_offset", ctypes.c_float)]
+
+
+class KvCacheDesc(ctypes.Structure):
+    """gq_kv_cache of include/gomlx_hipq.h."""
+    _fields_ = [("dCache", _vp), ("pages", _i64), ("kv_heads", _int), ("head_dim", _int), ("page_tokens", _int), ("max_pages", _int),
+                ("dPageTable", _vp), ("table_stride", _i64), ("dLengths", _vp), ("dStarts", _vp), ("seqs", _i64), ("rows", _i64), ("max_new", _i64)]
+
+
+class HeadRowsDesc(ctypes.Structure):
+    """gq_head_rows of include/gomlx_hipq.h."""
+    _fields_ = [("dX", _vp), ("row_stride", _i64), ("head_stride", _i64)]
 
 
 class HipqError(RuntimeError):

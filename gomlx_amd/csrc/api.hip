@@ -1220,6 +1220,139 @@ int gq_embedding_lookup(int type, const void *dTable, int64_t vocab, int64_t K, 
                                    (hipStream_t)stream);
 }
 
+namespace {
+constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+
+int check_head_rows(const char *fn, const char *what, const gq_head_rows *r, int dtype, int64_t rows, int heads) {
+    if (!r || (!r->dX && rows > 0 && heads > 0)) return fail(GQ_ERR_INVALID, "%s: null %s", fn, what);
+    if (!aligned_to(r->dX, dtype == GQ_BF16 ? 2 : 4)) return fail(GQ_ERR_INVALID, "%s: %s is not aligned to its elements", fn, what);
+    if (r->row_stride < 0 || r->head_stride < 0) return fail(GQ_ERR_INVALID, "%s: negative stride of %s", fn, what);
+    return GQ_OK;
+}
+int check_head_dim(const char *fn, int head_dim) {
+    if (head_dim == 64 || head_dim == 128 || head_dim == 256) return GQ_OK;
+    return fail(GQ_ERR_NOT_IMPLEMENTED, "%s: head_dim %d is not implemented (64, 128, 256)", fn, head_dim);
+}
+int check_float_type(const char *fn, int dtype) {
+    return dtype == GQ_F32 || dtype == GQ_BF16 ? GQ_OK : fail(GQ_ERR_NOT_IMPLEMENTED, "%s: element type %d is not implemented", fn, dtype);
+}
+
+// What the cache's entry points check of its description; *call is it for the kernels.  by_rows: the call has rows of its own.
+int check_kv(const char *fn, const gq_kv_cache *kv, bool by_rows, KvCall *call) {
+    if (!kv) return fail(GQ_ERR_INVALID, "%s: null cache", fn);
+    if (int rc = check_head_dim(fn, kv->head_dim)) return rc;
+    if (kv->pages < 0 || kv->seqs < 0 || kv->max_pages < 0 || kv->kv_heads <= 0 || kv->page_tokens <= 0)
+        return fail(GQ_ERR_INVALID, "%s: sizes of the cache must not be negative, its heads and page tokens positive", fn);
+    if (kv->page_tokens % 32) return fail(GQ_ERR_INVALID, "%s: page_tokens=%d is not a multiple of 32", fn, kv->page_tokens);
+    if (kv->pages > INT32_MAX || (int64_t)kv->max_pages * kv->page_tokens > INT32_MAX - 64)
+        return fail(GQ_ERR_INVALID, "%s: %lld pages, %d pages of %d tokens a sequence: too many", fn, (long long)kv->pages, kv->max_pages, kv->page_tokens);
+    if (kv->seqs > 65535 || kv->kv_heads > 65535)
+        return fail(GQ_ERR_INVALID, "%s: more than 65535 sequences or key heads (%lld, %d)", fn, (long long)kv->seqs, kv->kv_heads);
+    const int64_t rows = by_rows ? kv->rows : kv->seqs, max_new = by_rows ? kv->max_new : 1;
+    if (rows < 0 || max_new < 0 || rows > INT32_MAX || max_new > INT32_MAX - 64) return fail(GQ_ERR_INVALID, "%s: rows=%lld, max_new=%lld", fn, (long long)rows, (long long)max_new);
+    if (by_rows && !kv->dStarts && (rows != kv->seqs || max_new < 1))
+        return fail(GQ_ERR_INVALID, "%s: without dStarts every sequence has one row (%lld rows, %lld sequences, max_new %lld)", fn, (long long)rows, (long long)kv->seqs, (long long)max_new);
+    if (kv->seqs > 0) {
+        if (!kv->dLengths || (kv->max_pages > 0 && !kv->dPageTable) || (kv->pages > 0 && !kv->dCache)) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
+        if (!aligned_to(kv->dLengths, 4) || !aligned_to(kv->dPageTable, 4) || !aligned_to(kv->dStarts, 4)) return fail(GQ_ERR_INVALID, "%s: lengths, starts and page table must be 4-byte aligned", fn);
+        if (!aligned_to(kv->dCache, 16)) return fail(GQ_ERR_INVALID, "%s: the cache must be 16-byte aligned", fn);
+        if (kv->table_stride < (kv->seqs > 1 ? kv->max_pages : 0)) return fail(GQ_ERR_INVALID, "%s: rows of the page table overlap (stride %lld, %d columns)", fn, (long long)kv->table_stride, kv->max_pages);
+    }
+    const bool starts = by_rows && kv->dStarts;
+    *call = KvCall{static_cast<uint8_t *>(kv->dCache), (int)kv->pages, kv->kv_heads, kv->head_dim, kv->page_tokens, kv->dPageTable, kv->table_stride, kv->max_pages,
+                   kv->dLengths, starts ? kv->dStarts : nullptr, (int)kv->seqs, (int)rows, (int)(starts ? std::min(max_new, rows) : 1)};
+    return GQ_OK;
+}
+}  // namespace
+
+int gq_qk_norm_rope(int dtype, const gq_head_rows *q, int q_heads, const gq_head_rows *k, int k_heads, int head_dim, int64_t rows,
+                    const int32_t *dPositions, const float *dCos, const float *dSin, int64_t table_rows, int rot, int interleaved,
+                    const gq_rmsnorm *q_norm, const gq_rmsnorm *k_norm, int out_dtype, void *dQOut, void *dKOut, void *stream) {
+    const char *fn = "gq_qk_norm_rope";
+    if (int rc = check_float_type(fn, dtype)) return rc;
+    if (int rc = check_float_type(fn, out_dtype)) return rc;
+    if (int rc = check_head_dim(fn, head_dim)) return rc;
+    if (rows < 0 || q_heads < 0 || k_heads < 0 || table_rows < 0) return fail(GQ_ERR_INVALID, "%s: negative size", fn);
+    if (rot < 0 || rot > head_dim || rot % 8) return fail(GQ_ERR_INVALID, "%s: rot=%d is not a multiple of 8 of at most %d", fn, rot, head_dim);
+    if (int rc = check_head_rows(fn, "q", q, dtype, rows, q_heads)) return rc;
+    if (int rc = check_head_rows(fn, "k", k, dtype, rows, k_heads)) return rc;
+    const int64_t heads = (int64_t)q_heads + k_heads;
+    if (rows == 0 || heads == 0) return GQ_OK;
+    if (heads > INT32_MAX || rows > kMaxGrid / heads) return fail(GQ_ERR_INVALID, "%s: %lld rows of %lld heads: too many", fn, (long long)rows, (long long)heads);
+    if (!dPositions || (rot > 0 && table_rows > 0 && (!dCos || !dSin)) || (q_heads && !dQOut) || (k_heads && !dKOut)) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
+    if (!aligned_to(dPositions, 4) || !aligned_to(dCos, 16) || !aligned_to(dSin, 16) || !aligned_to(dQOut, 16) || !aligned_to(dKOut, 16))
+        return fail(GQ_ERR_INVALID, "%s: table and outputs must be 16-byte aligned, positions 4-byte", fn);
+    for (const gq_rmsnorm *n : {q_norm, k_norm})
+        if (n && !aligned_to(n->dGain, 4)) return fail(GQ_ERR_INVALID, "%s: gain must be 4-byte aligned", fn);
+    if (int rc = use_device()) return rc;
+    const bool bf16 = dtype == GQ_BF16;
+    const HeadRows hq{q->dX, q->row_stride, q->head_stride, bf16}, hk{k->dX, k->row_stride, k->head_stride, bf16};
+    const RmsNorm nq = q_norm ? RmsNorm{q_norm->dGain, q_norm->eps, q_norm->gain_offset} : RmsNorm{}, nk = k_norm ? RmsNorm{k_norm->dGain, k_norm->eps, k_norm->gain_offset} : RmsNorm{};
+    return launch_qk_norm_rope(hq, q_heads, hk, k_heads, head_dim, rows, dPositions, dCos, dSin, table_rows, rot, interleaved != 0, q_norm ? &nq : nullptr,
+                               k_norm ? &nk : nullptr, out_dtype == GQ_BF16, dQOut, dKOut, (hipStream_t)stream);
+}
+
+int gq_kv_append(const gq_kv_cache *kv, int dtype, const gq_head_rows *k, const gq_head_rows *v, float *dAccounts, void *stream) {
+    const char *fn = "gq_kv_append";
+    KvCall call;
+    if (int rc = check_kv(fn, kv, true, &call)) return rc;
+    if (int rc = check_float_type(fn, dtype)) return rc;
+    if (int rc = check_head_rows(fn, "k", k, dtype, call.rows, call.kv_heads)) return rc;
+    if (int rc = check_head_rows(fn, "v", v, dtype, call.rows, call.kv_heads)) return rc;
+    if (!aligned_to(dAccounts, 4)) return fail(GQ_ERR_INVALID, "%s: accounts must be 4-byte aligned", fn);
+    if (call.seqs == 0 || call.rows == 0 || call.max_new == 0 || call.max_pages == 0 || call.pages == 0) return GQ_OK;
+    if ((int64_t)call.seqs * call.kv_heads > kMaxGrid / ((call.max_new + 14) / 8)) return fail(GQ_ERR_INVALID, "%s: too many sequences, heads and new tokens", fn);
+    if (int rc = use_device()) return rc;
+    const bool bf16 = dtype == GQ_BF16;
+    return launch_kv_append(call, HeadRows{k->dX, k->row_stride, k->head_stride, bf16}, HeadRows{v->dX, v->row_stride, v->head_stride, bf16}, dAccounts, (hipStream_t)stream);
+}
+
+int gq_kv_read(const gq_kv_cache *kv, uint16_t *dK, uint16_t *dV, void *stream) {
+    const char *fn = "gq_kv_read";
+    KvCall call;
+    if (int rc = check_kv(fn, kv, true, &call)) return rc;
+    if (call.seqs == 0 || call.rows == 0 || call.max_new == 0) return GQ_OK;
+    if (!dK || !dV) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
+    if (!aligned_to(dK, 16) || !aligned_to(dV, 16)) return fail(GQ_ERR_INVALID, "%s: outputs must be 16-byte aligned", fn);
+    if ((int64_t)call.seqs * call.kv_heads > kMaxGrid / ((call.max_new + 14) / 8)) return fail(GQ_ERR_INVALID, "%s: too many sequences, heads and new tokens", fn);
+    if (int rc = use_device()) return rc;
+    return launch_kv_read(call, dK, dV, (hipStream_t)stream);
+}
+
+int gq_kv_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int heads, float scale, int64_t window, float *dAccounts, void *dOut,
+                    void *stream) {
+    const char *fn = "gq_kv_attention";
+    KvCall call;
+    if (int rc = check_kv(fn, kv, true, &call)) return rc;
+    if (int rc = check_float_type(fn, dtype)) return rc;
+    if (heads <= 0 || heads % call.kv_heads) return fail(GQ_ERR_INVALID, "%s: %d query heads are not a multiple of %d key heads", fn, heads, call.kv_heads);
+    if (window < 0) return fail(GQ_ERR_INVALID, "%s: negative window", fn);
+    if (int rc = check_head_rows(fn, "q", q, dtype, call.rows, heads)) return rc;
+    if (call.seqs == 0 || call.rows == 0 || call.max_new == 0) return GQ_OK;
+    if (!dOut) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
+    if (!aligned_to(dOut, 16) || !aligned_to(dAccounts, 4)) return fail(GQ_ERR_INVALID, "%s: the output must be 16-byte aligned, accounts 4-byte", fn);
+    // (grids are counted in 32 bits, threads included)
+    if (call.rows > (INT32_MAX >> 7) / heads || call.max_new > INT32_MAX / 2 / heads) return fail(GQ_ERR_INVALID, "%s: %d rows of %d heads: too many", fn, call.rows, heads);
+    if (int rc = use_device()) return rc;
+    CallScope scope;
+    const int room = call.max_pages * call.page_tokens;
+    return launch_kv_attention(call, HeadRows{q->dX, q->row_stride, q->head_stride, dtype == GQ_BF16}, heads, scale, window >= room ? 0 : (int)window, dAccounts, dOut,
+                               (hipStream_t)stream);
+}
+
+int gq_kv_evict(const gq_kv_cache *kv, float *dAccounts, int64_t keep, int64_t recent, int32_t *dKept, int32_t *dNewLengths, void *stream) {
+    const char *fn = "gq_kv_evict";
+    KvCall call;
+    if (int rc = check_kv(fn, kv, false, &call)) return rc;
+    if (keep < 1 || keep > INT32_MAX - 1024) return fail(GQ_ERR_INVALID, "%s: keep=%lld", fn, (long long)keep);
+    if (recent < 0 || recent > keep) return fail(GQ_ERR_INVALID, "%s: recent=%lld is not between 0 and keep=%lld", fn, (long long)recent, (long long)keep);
+    if (call.seqs == 0) return GQ_OK;
+    if (!dAccounts || !dKept || !dNewLengths) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
+    if (!aligned_to(dAccounts, 4) || !aligned_to(dKept, 4) || !aligned_to(dNewLengths, 4)) return fail(GQ_ERR_INVALID, "%s: arrays must be 4-byte aligned", fn);
+    if (int rc = use_device()) return rc;
+    return launch_kv_evict(call, dAccounts, (int)keep, (int)recent, dKept, dNewLengths, (hipStream_t)stream);
+}
+
 int gq_graph_begin(void *stream) {
     if (!stream) return fail(GQ_ERR_INVALID, "gq_graph_begin: recording needs an explicit stream");
     if (profile_state().active) return fail(GQ_ERR_INVALID, "gq_graph_begin: kernel timing is active on this thread");

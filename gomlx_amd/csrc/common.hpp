@@ -146,6 +146,26 @@ int launch_gemm_two_pass_set(int type, const float *x, int64_t M, int64_t K, con
 bool gemm_wreg_supported(int type, int64_t M, int64_t K, int64_t cols);
 int launch_gemm_wreg(int type, bool bf16, const uint16_t *x16, int64_t M, int64_t K, int count, const MmqSetItem *items, const uint8_t *W2,
                      const float *bias2, int act, const float *residual, const float *rowscale, float *partial, int tm, int slices, hipStream_t s);
+// Attention over a 4-bit cache (kv.hpp): what a call says about the cache and its sequences, checked by the entry points.
+struct KvCall {
+    uint8_t *cache;
+    int pages, kv_heads, head_dim, page_tokens;
+    const int32_t *table;
+    int64_t table_stride;
+    int max_pages;
+    const int32_t *lengths, *starts;  // starts null: row b is sequence b's one new token
+    int seqs, rows, max_new;
+};
+// rows of head vectors, strides in elements, the values of a vector side by side
+struct HeadRows { const void *p; int64_t row, head; bool bf16; };
+int launch_qk_norm_rope(const HeadRows &q, int q_heads, const HeadRows &k, int k_heads, int head_dim, int64_t rows, const int32_t *positions, const float *cos,
+                        const float *sin, int64_t table_rows, int rot, bool interleaved, const RmsNorm *q_norm, const RmsNorm *k_norm, bool out_bf16, void *q_out,
+                        void *k_out, hipStream_t s);
+int launch_kv_append(const KvCall &kv, const HeadRows &k, const HeadRows &v, float *accounts, hipStream_t s);
+int launch_kv_read(const KvCall &kv, uint16_t *k, uint16_t *v, hipStream_t s);
+int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float scale, int window, float *accounts, void *out, hipStream_t s);
+int launch_kv_evict(const KvCall &kv, float *accounts, int keep, int recent, int32_t *kept, int32_t *new_lengths, hipStream_t s);
+
 int launch_gemm(int type, bool x_is_bf16, const void *x, int64_t M, int64_t K, const uint8_t *W, int64_t N,
                 const float *bias, int act, float *y, hipStream_t s);
 

@@ -1,0 +1,75 @@
+// The 4-bit key / value cache: its layout in memory, what a call says about it, and how kernels walk it.
+//
+// A group is 32 neighbouring values of a head vector: a scale d and 32 codes c of 4 bits stand for d (c - 8).  d is an fp16
+// number of at most 8 significant bits and |d| <= 8160, c - 8 has at most 3: every value that the cache can hold is an fp16
+// number, normal or not, so that keys and values are exact operands of the fp16 matrix instructions.
+//
+// A tile is 32 tokens of one key head, 36 D bytes in one piece, in the order in which a wavefront wants it as operands of
+// v_mfma_f32_16x16x32_f16 (lane (r = lane % 16, j = lane / 16) holds 8 values of the contraction of operand row r):
+//     key codes    dwords [w / 4][lane][w % 4], w = u G + g (G = D / 32 groups): token 8 (r / 4) + 4 u + r % 4, values 32 g + 8 j + e
+//     value codes  dwords [w / 4][lane][w % 4]: value 16 w + r, tokens 8 j + e
+//     key scales   [token][g], value scales [g][token]
+// Element e = 0 .. 7 of a dword lies in nibble e / 2 + 4 (e % 2): masking the dword (shifted by 0, 4, 8, 12) leaves the pairs
+// (0, 1), (2, 3), ... in its two halves.  With these token orders the scores that a lane gets out of the two key operands
+// (u = 0, 1) of a tile are those of the tokens 8 j .. 8 j + 7 for query r: its share of the second product's operand, in place.
+#pragma once
+
+#include "common.hpp"
+
+namespace gq {
+
+namespace {
+
+constexpr int kTileTokens = 32;
+
+// Byte offsets in a tile of head vectors of D values.
+template <int D> struct KvTile {
+    static constexpr int G = D / 32;
+    static constexpr int kKeys = 0, kValues = 16 * D, kKeyScales = 32 * D, kValueScales = 34 * D, kBytes = 36 * D;
+    // dword w of a lane, of key or value codes
+    __host__ __device__ static constexpr int code(int w, int lane) { return ((w >> 2) * 64 + lane) * 16 + (w & 3) * 4; }
+};
+
+// row of the key operand that token t of a tile is: lane r of operand u
+__device__ __forceinline__ int key_row(int t) { return (t >> 3) * 4 + (t & 3); }
+__device__ __forceinline__ int key_half(int t) { return (t >> 2) & 1; }
+
+// What sequence b of a call has: `length` tokens, the last `news` of them new, their rows from `row0` on.
+struct KvSeq { int length, news, row0; };
+
+// Lengths beyond the page table and rows beyond the call's are cut off, so that no device value leads a kernel out of its buffers.
+__device__ __forceinline__ KvSeq kv_seq(const KvCall &kv, int b) {
+    KvSeq s;
+    const int64_t room = (int64_t)kv.max_pages * kv.page_tokens;
+    int length = kv.lengths[b];
+    length = length < 0 ? 0 : length;
+    s.length = length > room ? (int)room : length;
+    int from = b, to = b + 1;
+    if (kv.starts) { from = kv.starts[b]; to = kv.starts[b + 1]; }
+    from = from < 0 ? 0 : from > kv.rows ? kv.rows : from;
+    to = to < from ? from : to > kv.rows ? kv.rows : to;
+    s.row0 = from;
+    s.news = to - from > kv.max_new ? kv.max_new : to - from;
+    return s;
+}
+
+// Tile `tile` of sequence b and key head h; null where the page table names no page of the cache.
+__device__ __forceinline__ uint8_t *kv_tile(const KvCall &kv, int b, int h, int tile, int tile_bytes) {
+    const int per_page = kv.page_tokens >> 5;
+    const int slot = tile / per_page;
+    const int page = kv.table[b * kv.table_stride + slot];
+    if ((uint32_t)page >= (uint32_t)kv.pages) return nullptr;
+    return kv.cache + (((int64_t)page * kv.kv_heads + h) * per_page + (tile - slot * per_page)) * tile_bytes;
+}
+
+// The account of token p of sequence b and key head h; null as above.
+__device__ __forceinline__ float *kv_account(const KvCall &kv, float *accounts, int b, int h, int p) {
+    const int slot = p / kv.page_tokens;
+    const int page = kv.table[b * kv.table_stride + slot];
+    if ((uint32_t)page >= (uint32_t)kv.pages) return nullptr;
+    return accounts + ((int64_t)page * kv.kv_heads + h) * kv.page_tokens + (p - slot * kv.page_tokens);
+}
+
+}  // namespace
+
+}  // namespace gq

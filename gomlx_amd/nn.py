@@ -327,3 +327,216 @@ def quantized_dense_batch(problems, norm: RMSNorm | None = None) -> list:
             fn = L.gq_qdense_norm_bf16_batch if problems[0][0].dtype == torch.bfloat16 else L.gq_qdense_norm_f32_batch
             _lib.check(fn(len(problems), descs, ctypes.byref(d), _stream_ptr(problems[0][0])))
     return outs
+
+
+# ---- between the q / k / v projections and the output projection of a decoder layer: norms and rotation of queries and keys,
+# ---- a key / value cache held in 4 bits, attention over it, eviction from it (ml/layers/attention, attention/kvcache, attention/pos)
+
+_HEAD_DIMS = (64, 128, 256)
+
+
+def _float_type(name: str, t: torch.Tensor) -> int:
+    if t.dtype == torch.float32:
+        return _lib.F32
+    if t.dtype == torch.bfloat16:
+        return _lib.BF16
+    raise _lib.NotImplementedByBackend(_lib.ERR_NOT_IMPLEMENTED, f"{name}: dtype {t.dtype} is not implemented")
+
+
+def _head_rows(name: str, t: torch.Tensor, heads: int | None = None, dim: int | None = None):
+    """[rows, heads, dim] with the values of a head side by side; rows and heads may be strided (views of a wider projection)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor: this backend has no CPU path")
+    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
+        raise ValueError(f"{name} must be [rows, {'heads' if heads is None else heads}, {'head_dim' if dim is None else dim}], got {tuple(t.shape)}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: the values of a head must lie side by side")
+    return _lib.HeadRowsDesc(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _int32(name: str, t: torch.Tensor, shape: tuple) -> None:
+    _require_cuda(name, t)
+    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be an int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _kv_desc(cache, page_table, lengths, starts=None, max_new=1, rows=None, accounts=None):
+    """gq_kv_cache and the checks that need no look at the device."""
+    _require_cuda("cache", cache)
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[3] not in tuple(36 * d for d in _HEAD_DIMS):
+        raise ValueError("cache must be a Uint8 [pages, kv_heads, page_tokens / 32, 36 * head_dim] tensor (nn.kv_cache)")
+    pages, kv_heads, tiles, tile_bytes = cache.shape
+    if kv_heads < 1 or tiles < 1:
+        raise ValueError(f"cache of shape {tuple(cache.shape)} has no heads or no tokens")
+    if lengths.dim() != 1:
+        raise ValueError("lengths must be an int32 [sequences] tensor")
+    seqs = lengths.shape[0]
+    _int32("lengths", lengths, (seqs,))
+    if not page_table.is_cuda or page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != seqs or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"page_table must be an int32 [{seqs}, pages of a sequence] GPU tensor with neighbouring columns side by side")
+    if starts is None:
+        if rows is not None and rows != seqs:
+            raise ValueError(f"without starts every sequence has one row: got {rows} rows for {seqs} sequences")
+        if max_new != 1:
+            raise ValueError("max_new goes with starts")
+        rows = seqs
+    else:
+        _int32("starts", starts, (seqs + 1,))
+        if rows is None:
+            raise ValueError("rows must be given with starts")
+    if max_new < 1:
+        raise ValueError(f"max_new must be at least 1, got {max_new}")
+    if accounts is not None:
+        _require_cuda("weights", accounts)
+        if accounts.dtype != torch.float32 or tuple(accounts.shape) != (pages, kv_heads, 32 * tiles):
+            raise ValueError(f"weights must be a float32 [{pages}, {kv_heads}, {32 * tiles}] tensor, got {accounts.dtype} {tuple(accounts.shape)}")
+    for name, t in (("page_table", page_table), ("lengths", lengths), ("starts", starts), ("weights", accounts)):
+        if t is not None and t.device != cache.device:
+            raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+    return _lib.KvCacheDesc(cache.data_ptr(), pages, kv_heads, tile_bytes // 36, 32 * tiles, page_table.shape[1], page_table.data_ptr(),
+                            max(page_table.stride(0), page_table.shape[1]) if seqs < 2 else page_table.stride(0), lengths.data_ptr(),
+                            None if starts is None else starts.data_ptr(), seqs, rows, max_new)
+
+
+def rotary_table(positions: int, dim: int, base: float = 10000.0, device="cuda") -> tuple:
+    """(cos, sin) float32 [positions, dim / 2] for ``qk_norm_rope``: angles position * base^(-2 i / dim), formed in 64 bits.  A model
+    with other rates (scaled for long contexts, say) makes its own pair."""
+    if dim < 2 or dim % 2:
+        raise ValueError(f"dim must be a positive even number, got {dim}")
+    rates = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    angles = torch.arange(positions, dtype=torch.float64)[:, None] * rates
+    return angles.cos().float().to(device), angles.sin().float().to(device)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_norm: RMSNorm | None = None,
+                 k_norm: RMSNorm | None = None, interleaved: bool = False, dtype: torch.dtype | None = None) -> tuple:
+    """Norms of queries and keys for each head with the rotation by position in the same pass.
+
+    q: [rows, heads, head_dim], k: [rows, key heads, head_dim], float32 or bfloat16, both of one type; rows and heads may be strided.
+    positions: int32 [rows]; cos, sin: float32 [table rows, rot / 2] (``rotary_table``).  Values i and i + rot / 2 of a head form a
+    pair (``interleaved``: 2 i and 2 i + 1); those from rot on are not rotated.  ``q_norm`` / ``k_norm`` normalise every head over its
+    head_dim values first (gain [head_dim]).  Returns (q, k), contiguous, of ``dtype`` (default: the inputs').  A position outside the
+    table makes its row NaN."""
+    import ctypes
+    xd = _float_type("qk_norm_rope", q)
+    if k.dtype != q.dtype:
+        raise ValueError(f"q and k differ in type: {q.dtype} vs {k.dtype}")
+    dq = _head_rows("q", q)
+    rows, heads, dim = q.shape
+    dk = _head_rows("k", k, dim=dim)
+    if k.shape[0] != rows:
+        raise ValueError(f"q and k differ in rows: {rows} vs {k.shape[0]}")
+    if dim not in _HEAD_DIMS:
+        raise _lib.NotImplementedByBackend(_lib.ERR_NOT_IMPLEMENTED, f"qk_norm_rope: head_dim {dim} is not implemented (64, 128, 256)")
+    _int32("positions", positions, (rows,))
+    for name, t in (("cos", cos), ("sin", sin)):
+        _require_cuda(name, t)
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape:
+            raise ValueError(f"{name} must be a float32 [table rows, rot / 2] tensor, cos and sin of one shape")
+    for name, t in (("k", k), ("positions", positions), ("cos", cos), ("sin", sin)):
+        if t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+    dtype = q.dtype if dtype is None else dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise _lib.NotImplementedByBackend(_lib.ERR_NOT_IMPLEMENTED, f"qk_norm_rope: output dtype {dtype} is not implemented")
+    norms = [None if n is None else n._desc(dim) for n in (q_norm, k_norm)]
+    _init(q.device.index or 0)
+    q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=dtype, device=q.device)
+    _lib.check(_lib.lib().gq_qk_norm_rope(xd, ctypes.byref(dq), heads, ctypes.byref(dk), k.shape[1], dim, rows, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                                          cos.shape[0], 2 * cos.shape[1], int(interleaved), *(None if n is None else ctypes.byref(n) for n in norms),
+                                          _lib.F32 if dtype == torch.float32 else _lib.BF16, q_out.data_ptr(), k_out.data_ptr(), _stream_ptr(q)))
+    return q_out, k_out
+
+
+def kv_cache(pages: int, kv_heads: int, head_dim: int, page_tokens: int = 64, device="cuda") -> torch.Tensor:
+    """An empty key / value cache: uint8 [pages, kv_heads, page_tokens / 32, 36 * head_dim], 4.5 bits a value.
+
+    Groups of 32 neighbouring values of a head share a scale d and stand for d (c - 8) with 4-bit codes c; every value it can hold is
+    a float16 number.  A page holds ``page_tokens`` tokens (a multiple of 32) of every key head; which pages a sequence has, and in which
+    order, is the caller's table: int32 [sequences, pages of a sequence], where the entries of pages that a sequence does not have (yet)
+    may hold anything.  The calls below take it with ``lengths``, int32 [sequences], the tokens of each sequence with the call's new ones.
+    A call's rows are one new token per sequence, or, with ``starts`` (int32 [sequences + 1]), rows ``starts[b]`` to ``starts[b + 1]`` the
+    new tokens of sequence b, at most ``max_new``: in either case the last tokens of the sequence.  Table, lengths and starts are read
+    on the device.  A table may be a slice of the first columns of a wider one: its width bounds the work that is laid out."""
+    if head_dim not in _HEAD_DIMS:
+        raise _lib.NotImplementedByBackend(_lib.ERR_NOT_IMPLEMENTED, f"kv_cache: head_dim {head_dim} is not implemented (64, 128, 256)")
+    if pages < 0 or kv_heads < 1 or page_tokens < 1 or page_tokens % 32:
+        raise ValueError(f"kv_cache: {pages} pages, {kv_heads} heads, {page_tokens} tokens a page (a multiple of 32)")
+    return torch.zeros((pages, kv_heads, page_tokens // 32, 36 * head_dim), dtype=torch.uint8, device=device)
+
+
+def kv_cache_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                    starts: torch.Tensor | None = None, max_new: int = 1, weights: torch.Tensor | None = None) -> None:
+    """Writes keys and values [rows, kv_heads, head_dim] (float32 or bfloat16, strided rows and heads allowed) of the new tokens into the cache.
+
+    The scale of a group is minus an eighth of its value of largest magnitude, rounded to 8 significant bits; codes are rounded to
+    nearest.  A token with a NaN, an infinity or a magnitude of 65408 or more in a head makes rows that attend to it NaN there.
+    ``weights``: the accounts of ``cached_attention``, set to zero for the new tokens."""
+    import ctypes
+    xd = _float_type("kv_cache_append", k)
+    if v.dtype != k.dtype or v.shape != k.shape:
+        raise ValueError(f"k and v differ: {k.dtype} {tuple(k.shape)} vs {v.dtype} {tuple(v.shape)}")
+    d = _kv_desc(cache, page_table, lengths, starts, max_new, k.shape[0] if k.dim() else None, weights)
+    dk, dv = (_head_rows(name, t, d.kv_heads, d.head_dim) for name, t in (("k", k), ("v", v)))
+    if k.device != cache.device or v.device != cache.device:
+        raise ValueError("k, v and the cache must be on one device")
+    _init(cache.device.index or 0)
+    _lib.check(_lib.lib().gq_kv_append(ctypes.byref(d), xd, ctypes.byref(dk), ctypes.byref(dv), None if weights is None else weights.data_ptr(), _stream_ptr(cache)))
+
+
+def kv_cache_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, max_new: int = 1,
+                  rows: int | None = None) -> tuple:
+    """(keys, values) float16 [rows, kv_heads, head_dim] that the cache stands for at the last tokens of every sequence, exact.  Rows in
+    front of a sequence's first token are zero."""
+    import ctypes
+    d = _kv_desc(cache, page_table, lengths, starts, max_new, rows)
+    _init(cache.device.index or 0)
+    k, v = (torch.empty((d.rows, d.kv_heads, d.head_dim), dtype=torch.float16, device=cache.device) for _ in range(2))
+    _lib.check(_lib.lib().gq_kv_read(ctypes.byref(d), k.data_ptr(), v.data_ptr(), _stream_ptr(cache)))
+    return k, v
+
+
+def cached_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None,
+                     max_new: int = 1, scale: float | None = None, window: int = 0, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(scale q . k) v of the new tokens over a 4-bit cache (which already holds them).
+
+    q: [rows, heads, head_dim] float32 or bfloat16, strided rows and heads allowed; ``heads`` is a multiple of the cache's key heads and
+    neighbouring query heads share one.  ``scale`` defaults to head_dim^-1/2.  A token sees itself and the tokens in front of it in its
+    sequence, with a ``window`` the last that many; one that sees nothing gets zeros.  ``weights``: float32 [pages, kv_heads, page_tokens],
+    to which the softmax weights that every cached token receives are added (summed over rows and the query heads of a key head): what
+    ``kv_cache_evict`` goes by.  Every row of q belongs to a sequence.  Returns [rows, heads, head_dim] of q's type, contiguous."""
+    import ctypes
+    xd = _float_type("cached_attention", q)
+    d = _kv_desc(cache, page_table, lengths, starts, max_new, q.shape[0] if q.dim() else None, weights)
+    dq = _head_rows("q", q, dim=d.head_dim)
+    heads = q.shape[1]
+    if heads < 1 or heads % d.kv_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {d.kv_heads} key heads")
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    if q.device != cache.device:
+        raise ValueError("q and the cache must be on one device")
+    _init(cache.device.index or 0)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _lib.check(_lib.lib().gq_kv_attention(ctypes.byref(d), xd, ctypes.byref(dq), heads, d.head_dim ** -0.5 if scale is None else scale, window,
+                                          None if weights is None else weights.data_ptr(), out.data_ptr(), _stream_ptr(cache)))
+    return out
+
+
+def kv_cache_evict(cache: torch.Tensor, weights: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, keep: int, recent: int = 0) -> tuple:
+    """Shrinks every sequence of more than ``keep`` tokens to ``keep``: for each key head the last ``recent`` tokens and the keep - recent
+    others of largest accumulated weight stay (ties: the earlier token), moved to the front of the sequence's pages in their order,
+    with their weights.  Returns (kept, lengths): int32 [sequences, kv_heads, keep] former places of the kept tokens (-1 behind the last), and
+    the new lengths, min(length, keep); ``lengths`` itself is left as it is."""
+    import ctypes
+    d = _kv_desc(cache, page_table, lengths, accounts=weights)
+    if weights is None:
+        raise ValueError("weights must not be None")
+    if keep < 1 or not 0 <= recent <= keep:
+        raise ValueError(f"keep must be positive and recent between 0 and keep: got {keep}, {recent}")
+    _init(cache.device.index or 0)
+    kept = torch.empty((d.seqs, d.kv_heads, keep), dtype=torch.int32, device=cache.device)
+    new_lengths = torch.empty_like(lengths)
+    _lib.check(_lib.lib().gq_kv_evict(ctypes.byref(d), weights.data_ptr(), keep, recent, kept.data_ptr(), new_lengths.data_ptr(), _stream_ptr(cache)))
+    return kept, new_lengths

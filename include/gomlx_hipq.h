@@ -231,6 +231,63 @@ int gq_embedding_lookup(int type, const void *dTable, int64_t vocab, int64_t K,
                         const int32_t *dIndices, int64_t count, float *dOut,
                         int32_t *dErrFlag, void *stream);
 
+/* ---- Attention over a cache held in 4 bits, and what stands around it between a decoder layer's q / k / v projections and
+ * its output projection (the reference's attention and kvcache layers, ml/layers/attention; it has no 4-bit cache).
+ *
+ * A cache is dCache[pages, kv_heads, page_tokens / 32, 36 * head_dim] bytes, zero when it is new, 16-byte aligned; head_dim is
+ * 64, 128 or 256, page_tokens a multiple of 32.  32 neighbouring values of a head vector share a scale d (fp16, 8 significant
+ * bits) and stand for d (c - 8) with 4-bit codes c: 4.5 bits a value, every value an fp16 number.  Token p of sequence b lies
+ * in page dPageTable[b * table_stride + p / page_tokens] (entries of tokens that a sequence does not have are not read).
+ * dLengths[b] counts the tokens of sequence b with its new ones.  The rows dStarts[b] to dStarts[b + 1] of a call's row
+ * arguments are its new tokens, the last ones of it (at most max_new); dStarts == NULL: row b is the one new token of sequence b.
+ * These arrays lie on the device, so that a recorded graph replays over growing sequences.  Device values that lead out of the
+ * buffers are not followed: lengths are cut at the page table's end, rows at `rows`, and a token whose page is none of the
+ * cache's is taken as absent. ---- */
+typedef struct {
+    void *dCache;
+    int64_t pages;
+    int kv_heads, head_dim, page_tokens;
+    int max_pages;               /* columns of the page table: bounds the length of every sequence */
+    const int32_t *dPageTable;   /* [seqs, max_pages], rows table_stride apart */
+    int64_t table_stride;
+    const int32_t *dLengths;     /* [seqs] */
+    const int32_t *dStarts;      /* [seqs + 1] or NULL */
+    int64_t seqs, rows, max_new;
+} gq_kv_cache;
+/* Rows of head vectors: element (row, head, i) lies at dX[row * row_stride + head * head_stride + i]. */
+typedef struct {
+    const void *dX;              /* GQ_F32 or GQ_BF16 elements */
+    int64_t row_stride, head_stride;
+} gq_head_rows;
+
+/* RMSNorm over every query and key head (each norm may be NULL) and the rotation by position behind it:
+ * pairs (a, b) = (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved, become (a cos - b sin, a sin + b cos); values from rot
+ * on stay.  dCos / dSin: [table_rows, rot / 2], 16-byte aligned, rot a multiple of 8, at most head_dim (64, 128 or 256).  Outputs
+ * [rows, heads, head_dim] of type out_dtype, 16-byte aligned.  A position outside the table makes its rows NaN.  Either number of heads may be 0. */
+int gq_qk_norm_rope(int dtype, const gq_head_rows *q, int q_heads, const gq_head_rows *k, int k_heads, int head_dim, int64_t rows,
+                    const int32_t *dPositions, const float *dCos, const float *dSin, int64_t table_rows, int rot, int interleaved,
+                    const gq_rmsnorm *q_norm, const gq_rmsnorm *k_norm, int out_dtype, void *dQOut, void *dKOut, void *stream);
+/* Keys and values of the new tokens into the cache.  A group's scale is fp16(bf16(-m / 8)) of its value m of largest magnitude
+ * (the first of those), a code min(max(floor(x / d + 8.5), 0), 15).  A token with a value not below 65408 in magnitude in a
+ * head's key or value, a NaN among them, is kept as one that makes every row that attends to it NaN (its key reads as NaN, its
+ * value as 0).  dAccounts (may be NULL): [pages, kv_heads, page_tokens], set to 0 for the new tokens. */
+int gq_kv_append(const gq_kv_cache *kv, int dtype, const gq_head_rows *k, const gq_head_rows *v, float *dAccounts, void *stream);
+/* What the cache stands for at the new (last) tokens: fp16 [rows, kv_heads, head_dim], exact; zeros in front of a sequence's first token. */
+int gq_kv_read(const gq_kv_cache *kv, uint16_t *dK, uint16_t *dV, void *stream);
+/* Attention of the new tokens over their sequences, o = softmax(scale q . k) v: a token sees itself and the tokens in front of
+ * it, with window > 0 the last `window` of them.  heads is a multiple of kv_heads; neighbouring query heads share a key head.
+ * q and the output [rows, heads, head_dim] (16-byte aligned) are of one type, GQ_F32 (products in 22 bits and more) or GQ_BF16
+ * (weights rounded to 11 bits); all sums in fp32.  A row that sees nothing gets zeros.  dAccounts (may be NULL): every token's
+ * account grows by the weights that the call's rows gave it, summed over the query heads of a key head.  May use a per-stream
+ * workspace, as the dense entry points: make one call outside a recording first. */
+int gq_kv_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int heads, float scale, int64_t window, float *dAccounts, void *dOut,
+                    void *stream);
+/* Eviction by account: of every sequence longer than `keep` and every key head stay the last `recent` tokens and the
+ * keep - recent others of largest account (ties: the lower token; NaN counts as the largest), moved to the front of its pages
+ * in their order, with their accounts.  dKept[seqs, kv_heads, keep]: their former places, -1 behind the last one;
+ * dNewLengths[seqs] (may be dLengths itself): min(length, keep).  dStarts, rows and max_new are not used.  Sequences must not share pages. */
+int gq_kv_evict(const gq_kv_cache *kv, float *dAccounts, int64_t keep, int64_t recent, int32_t *dKept, int32_t *dNewLengths, void *stream);
+
 /* ---- Executable.Execute of a compiled graph (core/graph/graph.go:669): a sequence of
  * launches recorded once and replayed with one submission (HIP graph).  Between begin
  * and end, entry points called with this stream are recorded, not run.  A graph replays on

@@ -1,0 +1,613 @@
+"""The operators between a layer's q / k / v projections and its output projection on the GPU, against their definition in 64 bits
+(oracle/kv_oracle.py).  Tolerances are bounds that follow from the formats: see attention_bound() and rope_bound()."""
+import numpy as np
+import pytest
+
+from oracle import kv_oracle as ref
+
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24  # half a unit of float32
+
+
+class Case:
+    """Sequences over a cache with scattered pages, filled by kv_cache_append in pieces."""
+
+    def __init__(self, torch, lengths, kv_heads=2, dim=128, page=64, seed=0, wide_table=0, scale=1.0):
+        from gomlx_amd import nn
+        self.torch, self.nn, self.lengths, self.page, self.kv_heads, self.dim = torch, nn, lengths, page, kv_heads, dim
+        self.rng = np.random.default_rng(seed)
+        counts = [-(-n // page) for n in lengths]
+        self.pages = sum(counts) + 2
+        order = list(self.rng.permutation(self.pages))
+        self.table = np.full((len(lengths), max(counts + [1]) + wide_table), -1, np.int32)
+        for b, n in enumerate(counts):
+            self.table[b, :n] = [order.pop() for _ in range(n)]
+        self.cache = nn.kv_cache(self.pages, kv_heads, dim, page)
+        self.d_table = torch.from_numpy(self.table).cuda()
+        self.k = [(scale * self.rng.standard_normal((n, kv_heads, dim))).astype(np.float32) for n in lengths]
+        self.v = [self.rng.standard_normal((n, kv_heads, dim)).astype(np.float32) for n in lengths]
+
+    def ints(self, v):
+        return self.torch.tensor(v, dtype=self.torch.int32, device="cuda")
+
+    def fill(self, accounts=None):
+        """Everything in one ragged call."""
+        starts = np.concatenate([[0], np.cumsum(self.lengths)])
+        if starts[-1]:
+            k, v = (self.torch.from_numpy(np.concatenate(x)).cuda() for x in (self.k, self.v))
+            self.nn.kv_cache_append(self.cache, k, v, self.d_table, self.ints(self.lengths), starts=self.ints(starts), max_new=max(self.lengths), weights=accounts)
+        return self
+
+    def host(self):
+        return self.cache.cpu().numpy()
+
+    def attend(self, news, heads, dtype="f32", window=0, accounts=None, q=None, scale=None, table=None):
+        """(q rows float64, output) of a call with `news` new tokens of each sequence."""
+        torch = self.torch
+        rows = sum(news)
+        if q is None:
+            q = torch.from_numpy(self.rng.standard_normal((rows, heads, self.dim)).astype(np.float32)).cuda()
+        q = q.to({"f32": torch.float32, "bf16": torch.bfloat16}[dtype])
+        single = all(n == 1 for n in news)
+        starts = None if single else self.ints(np.concatenate([[0], np.cumsum(news)]))
+        out = self.nn.cached_attention(q, self.cache, self.d_table if table is None else table, self.ints(self.lengths), starts=starts,
+                                       max_new=1 if single else max(news), window=window, weights=accounts, scale=scale)
+        assert out.dtype == q.dtype and out.shape == q.shape and out.is_contiguous()
+        return q.double().cpu().numpy(), out.double().cpu().numpy()
+
+    def check(self, news, heads, dtype="f32", window=0, with_accounts=False, q=None, scale=None):
+        torch, group = self.torch, heads // self.kv_heads
+        accounts = before = None
+        if with_accounts:
+            before = self.rng.random((self.pages, self.kv_heads, self.page)).astype(np.float32)
+            accounts = torch.from_numpy(before.copy()).cuda()
+        q, out = self.attend(news, heads, dtype, window, accounts, q, scale)
+        host, at = self.host(), 0
+        scale = self.dim ** -0.5 if scale is None else scale
+        expect = None if before is None else before.astype(np.float64)
+        slack = None if before is None else np.abs(expect) * 2 * EPS
+        for b, n in enumerate(news):
+            for h in range(self.kv_heads):
+                keys, values = ref.decode(host, self.table[b], self.lengths[b], h)
+                qb = q[at:at + n, h * group:(h + 1) * group]
+                want, p, s, seen = ref.attention(qb, keys, values, scale, window)
+                got = out[at:at + n, h * group:(h + 1) * group]
+                if n and not seen.any(-1).all():
+                    assert np.all(got[~seen.any(-1)] == 0)
+                bound, eps_p = attention_bound(qb, keys, values, scale, p, s, seen, dtype)
+                bad = np.isnan(want).any(-1)
+                assert np.isnan(got[bad]).all()
+                assert np.all(np.abs(got - want)[~bad] <= (bound + np.abs(want) * (2.0 ** -8 if dtype == "bf16" else 2 * EPS))[~bad]), \
+                    f"sequence {b}, head {h}: {np.max((np.abs(got - want) - bound)[~bad])}"
+                if expect is not None:
+                    for t in range(self.lengths[b]):
+                        add = p[:, :, t][np.broadcast_to(seen[:, None, t], p.shape[:2])]
+                        w = (self.table[b, t // self.page], h, t % self.page)
+                        expect[w] += add.sum()
+                        slack[w] += (np.abs(add) * (np.broadcast_to(eps_p, p.shape[:2])[np.broadcast_to(seen[:, None, t], p.shape[:2])] + (add.size + 4) * EPS)).sum() + expect[w] * EPS
+            at += n
+        if expect is not None:
+            got = accounts.cpu().numpy().astype(np.float64)
+            assert np.all(np.isnan(got) == np.isnan(expect))
+            fine = ~np.isnan(expect)
+            assert np.all(np.abs(got - expect)[fine] <= slack[fine]), np.max((np.abs(got - expect) - slack)[fine])
+        return out
+
+
+def attention_bound(q, keys, values, scale, p, s, seen, dtype):
+    """Largest error of a row's results before the rounding of the output, and relative error of its weights.
+
+    q is used to 2^-22 of its row's largest value (float32; bfloat16 exactly), products are exact, a score is a sum of D of them in
+    float32 and scaled: |ds| <= scale (2^-22 + D 2^-24) max_j sum_d max|q| |k_jd| + 2^-22 max|s|.  exp2 adds 2^-22.  A softmax weight is
+    then off by a factor of at most 1 + 2 (|ds| + 2^-22) (the sum's error included), plus n 2^-24 of the sum's additions.  As operands weights are rounded to 2^-22 (float32) or 2^-12
+    (bfloat16) of themselves or, where tiny, 2^-30 of the largest.  n additions in float32 in the second product."""
+    n = keys.shape[0]
+    if n == 0 or q.size == 0:
+        return np.zeros(q.shape), np.zeros(q.shape[:2])
+    with np.errstate(all="ignore"):
+        k = np.nan_to_num(np.abs(keys))
+        qk = np.abs(q).max(-1) * max(k.sum(-1).max(), 0)
+        top = np.max(np.where(np.isfinite(s), np.abs(s), 0), -1)
+        ds = scale * (2.0 ** -22 + q.shape[-1] * EPS) * qk + 2.0 ** -22 * top
+        eps_p = 2 * (ds + 2.0 ** -22) + n * EPS
+        operand = 2.0 ** -12 if dtype == "bf16" else 2.0 ** -22
+        size = np.einsum("ngt,td->ngd", np.nan_to_num(p), np.abs(values))
+        bound = (eps_p + operand + (n + 8) * EPS)[..., None] * size + n * 2.0 ** -30 * np.abs(values).max(initial=0)
+    return bound, eps_p
+
+
+# ---- the cache --------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim", (64, 128, 256))
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+def test_append_holds_what_the_definition_says(gpu, dim, dtype):
+    """Bit for bit, in one ragged call, token by token, and from strided rows that no vector load fits."""
+    torch = gpu
+    lengths = [1, 7, 33, 100, 65]
+    c = Case(torch, lengths, kv_heads=3, dim=dim, page=32)
+    c.k[3][5, 1] = 0.0                                        # a head of zeros
+    c.k[3][6, 0, :32] = 1e-7                                  # a scale below fp16's smallest
+    c.v[3][7, 2, 3], c.v[3][7, 2, 9] = 4.0, -4.0              # a tie: the first one's sign
+    c.k[4][0] = 60000.0 * np.sign(c.k[4][0])                  # near the largest scale
+    if dtype == "bf16":
+        c.k, c.v = ([torch.from_numpy(x).bfloat16().float().numpy() for x in y] for y in (c.k, c.v))
+    c.fill()
+    want = [ref.quantise(k, v) for k, v in zip(c.k, c.v)]
+    starts = np.concatenate([[0], np.cumsum(lengths)])
+
+    def same(cache):
+        k, v = c.nn.kv_cache_read(cache, c.d_table, c.ints(lengths), starts=c.ints(starts), max_new=100, rows=int(starts[-1]))
+        for got, which in ((k, 0), (v, 1)):
+            got = got.double().cpu().numpy()
+            for b in range(len(lengths)):
+                assert np.array_equal(got[starts[b]:starts[b + 1]], want[b][which])
+
+    same(c.cache)
+    host = c.host()
+    for b, n in enumerate(lengths):  # the bytes themselves
+        for h in range(3):
+            k, v = ref.decode(host, c.table[b], n, h)
+            assert np.array_equal(k, want[b][0][:, h]) and np.array_equal(v, want[b][1][:, h])
+    kind = {"f32": torch.float32, "bf16": torch.bfloat16}[dtype]
+    # token by token: sequences that still grow get one row each
+    again = c.nn.kv_cache(c.pages, 3, dim, 32)
+    wide = torch.zeros(len(lengths), 3 * (2 * dim + 3) + 1, dtype=kind, device="cuda")[:, 1:]  # rows and heads off every vector
+    k, v = (wide.as_strided((len(lengths), 3, dim), (wide.stride(0), 2 * dim + 3, 1), wide.storage_offset() + o) for o in (0, dim + 1))
+    for step in range(max(lengths)):
+        now = [min(step + 1, n) for n in lengths]
+        for b, n in enumerate(now):
+            k[b], v[b] = torch.from_numpy(c.k[b][n - 1]).cuda().to(kind), torch.from_numpy(c.v[b][n - 1]).cuda().to(kind)
+        c.nn.kv_cache_append(again, k, v, c.d_table, c.ints(now))
+    same(again)
+
+
+def test_append_in_pieces_keeps_the_neighbours(gpu):
+    """Pieces that begin and end inside a block of eight tokens, a tile and a page leave every other token as it was, and stay inside
+    the pages of their sequence."""
+    c = Case(gpu, [200, 90], kv_heads=2, dim=64, page=64, seed=3)
+    c.cache.random_(0, 256)
+    before = c.host().copy()
+    done = [0, 0]
+    for pieces in ([5, 3], [1, 1], [60, 29], [64, 0], [70, 57]):
+        done = [a + n for a, n in zip(done, pieces)]
+        starts = np.concatenate([[0], np.cumsum(pieces)])
+        k, v = (gpu.from_numpy(np.concatenate([x[b][done[b] - n:done[b]] for b, n in enumerate(pieces)])).cuda() for x in (c.k, c.v))
+        c.nn.kv_cache_append(c.cache, k, v, c.d_table, c.ints(done), starts=c.ints(starts), max_new=max(pieces))
+    host = c.host()
+    for b, n in enumerate(c.lengths):
+        want = ref.quantise(c.k[b], c.v[b])
+        for h in range(2):
+            k, v = ref.decode(host, c.table[b], n, h)
+            assert np.array_equal(k, want[0][:, h]) and np.array_equal(v, want[1][:, h])
+            # behind the last token: as before
+            whole = -(-n // 64) * 64
+            old, new = (ref.decode(x, c.table[b], whole, h) for x in (before, host))
+            for i in (0, 1):
+                assert np.array_equal(old[i][n:], new[i][n:], equal_nan=True)
+    free = sorted(set(range(c.pages)) - set(c.table[c.table >= 0].tolist()))
+    assert free and np.array_equal(before[free], host[free])
+
+
+def test_append_bad_tokens_and_accounts(gpu):
+    c = Case(gpu, [40], kv_heads=2, dim=128, page=64)
+    c.k[0][3, 0, 5] = np.nan
+    c.v[0][9, 1, 127] = np.inf
+    c.k[0][11, 1, 64] = 65408.0
+    c.v[0][12, 0, 0] = -65407.0
+    accounts = gpu.ones(c.pages, 2, 64, device="cuda")
+    c.fill(accounts)
+    host = c.host()
+    want = ref.quantise(c.k[0], c.v[0])
+    for h in range(2):
+        k, v = ref.decode(host, c.table[0], 40, h)
+        assert np.array_equal(k, want[0][:, h], equal_nan=True) and np.array_equal(v, want[1][:, h])
+    assert np.isnan(want[0]).all(-1).sum() == 3
+    got = accounts.cpu().numpy()
+    assert np.all(got[c.table[0, 0], :, :40] == 0) and got.sum() == got.size - 80
+
+
+def test_read_in_front_of_the_first_token_and_absent_pages(gpu):
+    c = Case(gpu, [5, 70], kv_heads=1, dim=64, page=32).fill()
+    c.d_table[1, 1] = c.pages  # tokens 32 to 63 of the second sequence have no page
+    k, v = c.nn.kv_cache_read(c.cache, c.d_table, c.ints([5, 70]), starts=c.ints([0, 12, 90]), max_new=78, rows=90)
+    k, v = k.double().cpu().numpy(), v.double().cpu().numpy()
+    w0, w1 = ref.quantise(c.k[0], c.v[0]), ref.quantise(c.k[1], c.v[1])
+    for got, i in ((k, 0), (v, 1)):
+        assert np.all(got[:7] == 0) and np.array_equal(got[7:12], w0[i])
+        assert np.all(got[12:20] == 0) and np.array_equal(got[20:52], w1[i][:32]) and np.all(got[52:84] == 0) and np.array_equal(got[84:], w1[i][64:])
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("dim,kv_heads,heads,page", ((64, 3, 3, 32), (128, 2, 8, 64), (128, 1, 7, 96), (256, 2, 4, 32), (64, 1, 40, 64)))
+def test_single_tokens(gpu, dtype, dim, kv_heads, heads, page):
+    """Lengths around tiles and pages, from nothing to several workgroups' worth."""
+    c = Case(gpu, [1, 0, 31, 32, 33, 64, 65, 500, 1285], kv_heads, dim, page, seed=dim + heads).fill()
+    c.check([1] * 9, heads, dtype, with_accounts=True)
+    c.check([1] * 9, heads, dtype, window=40, with_accounts=True)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("dim,kv_heads,heads,window", ((128, 2, 8, 0), (64, 2, 2, 0), (256, 1, 3, 0), (128, 1, 4, 33), (64, 1, 5, 1), (256, 2, 4, 100)))
+def test_several_tokens(gpu, dtype, dim, kv_heads, heads, window):
+    """Ragged prompts on top of caches, sequences without a new token, prompts that are the whole cache."""
+    c = Case(gpu, [300, 70, 129, 1, 64], kv_heads, dim, 64, seed=window + heads).fill()
+    c.check([3, 70, 0, 1, 40], heads, dtype, window, with_accounts=True)
+    c.check([131, 17, 129, 1, 5], heads, dtype, window, with_accounts=True)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+def test_prompt_of_a_thousand_tokens(gpu, dtype):
+    c = Case(gpu, [1217], 1, 128, 128, seed=9).fill()
+    c.check([1001], 4, dtype, with_accounts=True)
+    c.check([1001], 4, dtype, window=300)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("news", (1, 40))
+def test_large_and_small_scores(gpu, dtype, news):
+    """Softmax from nearly one token to nearly flat, large queries and tiny ones, and a scale of the caller's."""
+    c = Case(gpu, [400], 2, 128, 64, seed=4, scale=3.0).fill()
+    q = gpu.randn(news, 4, 128, device="cuda", generator=gpu.Generator("cuda").manual_seed(1))
+    for factor in (1e-30, 1e-4, 1.0, 30.0):
+        c.check([news], 4, dtype, q=q * factor)
+    c.check([news], 4, dtype, q=q, scale=0.7)
+    c.check([news], 4, dtype, q=q * 1e30, scale=1e-31)
+    c.check([news], 4, dtype, q=q, scale=0.0, with_accounts=True)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+def test_tiny_keys_and_values_are_exact_operands(gpu, dtype):
+    """Values whose scales are fp16 denormals: the matrix instructions must not flush them."""
+    c = Case(gpu, [100], 1, 64, 32, seed=5)
+    c.k = [x * np.float32(2e-6) for x in c.k]
+    c.v = [x * np.float32(2e-6) for x in c.v]
+    c.fill()
+    q = 1e6 * gpu.randn(1, 2, 64, device="cuda")
+    out = c.check([1], 2, dtype, q=q)
+    assert np.abs(out).max() > 1e-8
+    c.check([64], 2, dtype, q=1e6 * gpu.randn(64, 2, 64, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("news", (1, 64, 90))
+def test_bad_tokens_reach_only_rows_that_see_them(gpu, dtype, news):
+    """A NaN in a key or value makes the rows that attend to it NaN, and no other: not those in front of it, not those whose window has
+    left it, not other heads; what lies behind a sequence in its pages reaches nobody."""
+    c = Case(gpu, [150, 150], 2, 128, 64, seed=6)
+    c.k[0][100, 0, 3] = np.nan
+    c.v[0][120, 1, 3] = np.inf
+    c.cache.random_(0, 256)  # (scales of every kind in the places that no token has)
+    c.cache[:, :, :, 34 * 128:] = 0
+    c.fill()
+    for window in (0, 20):
+        out = c.check([news, news], 4, dtype, window, with_accounts=True)
+        assert np.isnan(out).any() == (news > 1 or window == 0) and not np.isnan(out).all()
+    q = gpu.randn(2 * news, 4, 128, device="cuda")
+    q[0, 1, 5] = float("nan")
+    c.check([news, news], 4, dtype, q=q)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+def test_rows_of_strange_layout(gpu, dtype):
+    """Queries as a view of a wider projection, and at an offset and strides that no vector load fits: the same results."""
+    torch = gpu
+    c = Case(torch, [77, 200], 2, 64, 32, seed=7).fill()
+    kind = {"f32": torch.float32, "bf16": torch.bfloat16}[dtype]
+    starts = c.ints([0, 40, 43])
+    q = torch.randn(43, 6, 64, device="cuda").to(kind)
+    args = (c.cache, c.d_table, c.ints(c.lengths))
+    want = c.nn.cached_attention(q, *args, starts=starts, max_new=40)
+    wide = torch.zeros(43, 10, 64, device="cuda", dtype=kind)
+    wide[:, 2:8] = q
+    assert torch.equal(c.nn.cached_attention(wide[:, 2:8], *args, starts=starts, max_new=40), want)
+    odd = torch.zeros(43 * 6 * 67 + 1, device="cuda", dtype=kind)[1:].as_strided((43, 6, 64), (6 * 67, 67, 1), 1)
+    odd.copy_(q)
+    assert torch.equal(c.nn.cached_attention(odd, *args, starts=starts, max_new=40), want)
+    # a wider table, and a slice of one
+    wider = torch.full((2, 50), 7, dtype=torch.int32, device="cuda")
+    wider[:, :c.table.shape[1]] = c.d_table
+    got = c.nn.cached_attention(q, c.cache, wider[:, :c.table.shape[1]], c.ints(c.lengths), starts=starts, max_new=40)
+    assert torch.equal(got, want)
+    got = c.nn.cached_attention(q, c.cache, wider, c.ints(c.lengths), starts=starts, max_new=43).double()
+    assert (got - want.double()).abs().max() <= (2.0 ** -8 if dtype == "bf16" else 2.0 ** -18) * want.double().abs().max()
+
+
+def test_device_values_that_lead_nowhere(gpu):
+    """Lengths past the table, starts past the rows, pages that are none of the cache's: cut off or absent, never followed."""
+    torch = gpu
+    c = Case(torch, [100, 90], 2, 64, 32, seed=8, wide_table=1).fill()
+    q = torch.randn(2, 4, 64, device="cuda")
+    table = c.d_table.clone()
+    table[0, 1], table[1, 0] = -5, 10 ** 9
+    out = c.nn.cached_attention(q, c.cache, table, c.ints([100, 90]))
+    host = c.host()
+    for b, gone in ((0, range(32, 64)), (1, range(0, 32))):
+        for h in range(2):
+            keys, values = ref.decode(host, c.table[b], c.lengths[b], h)
+            left = [t for t in range(c.lengths[b]) if t not in gone]
+            want, p, s, seen = ref.attention(q[b:b + 1, 2 * h:2 * h + 2].double().cpu().numpy(), keys[left], values[left], 0.125, 0)
+            bound, _ = attention_bound(q[b:b + 1, 2 * h:2 * h + 2].double().cpu().numpy(), keys[left], values[left], 0.125, p, s, seen, "f32")
+            assert np.all(np.abs(out[b, 2 * h:2 * h + 2].double().cpu().numpy() - want[0]) <= bound[0] + np.abs(want[0]) * 2 * EPS)
+    weights = torch.zeros(c.pages, 2, 32, device="cuda")
+    for lengths, starts in (([10 ** 9, -7], [0, 1, 2]), ([100, 90], [-3, 10 ** 6, 2]), ([100, 90], [2, 1, 0])):
+        c.nn.cached_attention(q, c.cache, c.d_table, c.ints(lengths), starts=c.ints(starts), max_new=2, weights=weights)
+        c.nn.kv_cache_append(c.cache, q[:, :2], q[:, 2:], c.d_table, c.ints(lengths), starts=c.ints(starts), max_new=2, weights=weights)
+        c.nn.kv_cache_read(c.cache, c.d_table, c.ints(lengths), starts=c.ints(starts), max_new=2, rows=2)
+        c.nn.kv_cache_evict(c.cache, weights, c.d_table, c.ints(lengths), 50, 10)
+    torch.cuda.synchronize()
+
+
+def test_cache_past_four_gigabytes(gpu):
+    """Pages whose bytes lie beyond 2^32."""
+    torch = gpu
+    from gomlx_amd import nn
+    pages = (9 << 29) // (8 * 8 * 36 * 256)  # 4.8 GB
+    cache = nn.kv_cache(pages, 8, 256, 256)
+    assert cache.numel() > 1 << 32
+    table = torch.tensor([[pages - 1, 3]], dtype=torch.int32, device="cuda")
+    small, t2 = nn.kv_cache(2, 8, 256, 256), torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    k, v, q = (torch.randn(300, 8, 256, device="cuda") for _ in range(3))
+    n = torch.tensor([300], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    outs = []
+    for c, t in ((cache, table), (small, t2)):
+        w = torch.zeros(c.shape[0], 8, 256, device="cuda")
+        nn.kv_cache_append(c, k, v, t, n, starts=starts, max_new=300)
+        a = nn.cached_attention(q, c, t, n, starts=starts, max_new=300, weights=w)
+        b = nn.cached_attention(q[:1], c, t, n)
+        kept, left = nn.kv_cache_evict(c, w, t, n, 200, 20)
+        outs.append((a, b, kept, *nn.kv_cache_read(c, t, left, starts=torch.tensor([0, 200], dtype=torch.int32, device="cuda"), max_new=200, rows=200)))
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+
+
+# ---- eviction ---------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim,page", ((64, 32), (128, 64), (256, 96)))
+@pytest.mark.parametrize("keep,recent", ((1, 0), (1, 1), (32, 7), (45, 45), (150, 0), (333, 40), (2000, 5)))
+def test_evict(gpu, dim, page, keep, recent):
+    """Places, order, codes, scales and accounts of what stays; sequences within the budget are left alone."""
+    torch = gpu
+    lengths = [0, 1, 32, 45, 150, 700, 1500]
+    c = Case(torch, lengths, 2, dim, page, seed=keep).fill()
+    accounts = np.round(c.rng.standard_normal((c.pages, 2, page)).astype(np.float32) ** 2, 1)  # many exactly equal
+    accounts[c.rng.random(accounts.shape) < 0.3] = 0
+    accounts[c.rng.random(accounts.shape) < 0.01] = np.nan
+    accounts[c.rng.random(accounts.shape) < 0.01] = np.inf
+    accounts[c.rng.random(accounts.shape) < 0.05] *= -1
+    d = torch.from_numpy(accounts).cuda()
+    before = c.host().copy()
+    kept, left = c.nn.kv_cache_evict(c.cache, d, c.d_table, c.ints(lengths), keep, recent)
+    kept, after, d = kept.cpu().numpy(), c.host(), d.cpu().numpy()
+    assert left.tolist() == [min(n, keep) for n in lengths]
+    for b, n in enumerate(lengths):
+        where = [(c.table[b, t // page], t % page) for t in range(n)]
+        for h in range(2):
+            want = ref.evict(np.array([accounts[p, h, s] for p, s in where], np.float32), keep, recent)
+            assert kept[b, h].tolist() == want.tolist() + [-1] * (keep - len(want))
+            old, new = ref.decode(before, c.table[b], n, h), ref.decode(after, c.table[b], n, h)
+            for i in (0, 1):
+                assert np.array_equal(new[i][:len(want)], old[i][want])
+                assert np.array_equal(new[i][len(want):], old[i][len(want):])  # what lies behind is left as it was
+            got = np.array([d[p, h, s] for p, s in where], np.float32)
+            assert np.array_equal(got[:len(want)], np.array([accounts[where[t][0], h, where[t][1]] for t in want], np.float32), equal_nan=True)
+
+
+def test_evict_writes_lengths_in_place_and_goes_on(gpu):
+    """Serving: append, attend with accounts, evict into the same lengths, go on with the shorter sequences."""
+    torch = gpu
+    from gomlx_amd import _lib
+    import ctypes
+    c = Case(torch, [130, 60], 1, 64, 32, seed=2, wide_table=1).fill()
+    weights = torch.zeros(c.pages, 1, 32, device="cuda")
+    q = torch.randn(2, 4, 64, device="cuda")
+    lengths = c.ints([130, 60])
+    c.nn.cached_attention(q, c.cache, c.d_table, lengths, weights=weights)
+    kept = torch.empty(2, 1, 64, dtype=torch.int32, device="cuda")
+    d = c.nn._kv_desc(c.cache, c.d_table, lengths, accounts=weights)
+    _lib.check(_lib.lib().gq_kv_evict(ctypes.byref(d), weights.data_ptr(), 64, 16, kept.data_ptr(), lengths.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    assert lengths.tolist() == [64, 60]
+    k, v = (torch.randn(2, 1, 64, device="cuda") for _ in range(2))
+    c.nn.kv_cache_append(c.cache, k, v, c.d_table, lengths + 1, weights=weights)
+    c.lengths = [65, 61]
+    c.check([1, 1], 4)
+
+
+# ---- norms and rotation ---------------------------------------------------------------------------------------------------
+
+
+def rope_bound(size, want, dtype):
+    """The sum of squares is a sum of D positive terms in float32 (relative error up to D 2^-24 halved by the root), then a root, a
+    division, two products and a sum: under (D / 2 + 8) 2^-24 of the two terms' magnitudes; bfloat16 results are rounded to 2^-8."""
+    return size * (size.shape[-1] / 2 + 8) * EPS + (np.abs(want) * 2.0 ** -8 if dtype == "bf16" else 0)
+
+
+@pytest.mark.parametrize("dim,rot", ((64, 64), (128, 128), (128, 64), (256, 256), (256, 8), (64, 24), (128, 0)))
+@pytest.mark.parametrize("interleaved", (False, True))
+@pytest.mark.parametrize("kind,out", (("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("bf16", "f32")))
+def test_qk_norm_rope(gpu, dim, rot, interleaved, kind, out):
+    torch = gpu
+    from gomlx_amd import nn
+    rng = np.random.default_rng(dim + rot)
+    types = {"f32": torch.float32, "bf16": torch.bfloat16}
+    cos, sin = nn.rotary_table(5000, rot, 10000.0) if rot else (torch.zeros(5000, 0, device="cuda"),) * 2
+    for rows, heads, kv, norm in ((1, 4, 1, True), (37, 6, 2, True), (5, 3, 3, False), (3, 0, 2, True), (0, 4, 2, True)):
+        wide = torch.from_numpy(rng.standard_normal((rows, (heads + 2 * kv) * dim)).astype(np.float32)).cuda().to(types[kind])
+        q, k = wide[:, :heads * dim].view(rows, heads, dim), wide[:, heads * dim:(heads + kv) * dim].view(rows, kv, dim)
+        pos = rng.integers(0, 5000, rows).astype(np.int32)
+        if rows > 4:
+            pos[1], pos[3] = -1, 5000  # outside the table
+        gains = [torch.from_numpy(rng.standard_normal(dim).astype(np.float32)).cuda(), None]
+        norms = [nn.RMSNorm(gain=gains[0], epsilon=1e-5, scale_offset=1.0), nn.RMSNorm(epsilon=1e-6)] if norm else [None, None]
+        got = nn.qk_norm_rope(q, k, torch.from_numpy(pos).cuda(), cos, sin, *norms, interleaved=interleaved, dtype=types[out])
+        for x, y, g, n in zip((q, k), got, gains, norms):
+            assert y.shape == x.shape and y.dtype == types[out] and y.is_contiguous()
+            want, size = ref.norm_rope(x.double().cpu().numpy(), pos, cos.cpu().numpy(), sin.cpu().numpy(), None if g is None else g.cpu().numpy(),
+                                       n.epsilon if n else 0.0, n.scale_offset if n else 0.0, norm, interleaved)
+            y = y.double().cpu().numpy()
+            assert np.array_equal(np.isnan(y), np.isnan(want))
+            fine = ~np.isnan(want)
+            assert np.all(np.abs(y - want)[fine] <= rope_bound(size, want, out)[fine])
+
+
+def test_qk_norm_rope_rows_off_every_vector(gpu):
+    torch = gpu
+    from gomlx_amd import nn
+    cos, sin = nn.rotary_table(64, 128)
+    pos = torch.arange(9, dtype=torch.int32, device="cuda")
+    for kind in (torch.float32, torch.bfloat16):
+        q, k = (torch.randn(9, 2, 128, device="cuda").to(kind) for _ in range(2))
+        odd = [torch.zeros(9 * 2 * 131 + 1, dtype=kind, device="cuda")[1:].as_strided((9, 2, 128), (2 * 131, 131, 1), 1) for _ in range(2)]
+        for o, x in zip(odd, (q, k)):
+            o.copy_(x)
+        for a, b in zip(nn.qk_norm_rope(q, k, pos, cos, sin), nn.qk_norm_rope(*odd, pos, cos, sin)):
+            assert torch.equal(a, b)
+    zero = torch.zeros(9, 2, 128, device="cuda")
+    a, _ = nn.qk_norm_rope(zero, zero, pos, cos, sin, q_norm=nn.RMSNorm())  # eps keeps a head of zeros at zero
+    assert torch.equal(a, zero)
+
+
+# ---- together -----------------------------------------------------------------------------------------------------------
+
+
+def test_recorded_graph_replays_over_growing_sequences(gpu):
+    """rotate, append, attend with accounts as one HIP graph, replayed while lengths and inputs change, with eager work between."""
+    torch = gpu
+    from gomlx_amd import nn
+    dim, kv, heads, page, seqs = 64, 2, 4, 32, 3
+    table = torch.arange(seqs * 6, dtype=torch.int32, device="cuda").view(seqs, 6)
+    cos, sin = nn.rotary_table(256, dim)
+
+    def state():
+        return dict(cache=nn.kv_cache(seqs * 6, kv, dim, page), weights=torch.zeros(seqs * 6, kv, page, device="cuda"),
+                    lengths=torch.tensor([90, 31, 1], dtype=torch.int32, device="cuda"), x=torch.zeros(seqs, heads + 2 * kv, dim, device="cuda"))
+
+    def step(s):
+        q, k = nn.qk_norm_rope(s["x"][:, :heads], s["x"][:, heads:heads + kv], s["lengths"], cos, sin, q_norm=nn.RMSNorm(), k_norm=nn.RMSNorm())
+        nn.kv_cache_append(s["cache"], k, s["x"][:, heads + kv:], table, s["lengths"], weights=s["weights"])
+        return nn.cached_attention(q, s["cache"], table, s["lengths"], weights=s["weights"])
+
+    a, b = state(), state()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(b)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(b)
+    for s in (a, b):
+        s["cache"].zero_()
+        s["weights"].zero_()
+    for i in range(5):
+        x = torch.randn(seqs, heads + 2 * kv, dim, device="cuda")
+        for s in (a, b):
+            s["x"].copy_(x)
+            s["lengths"] += 1
+        want = step(a)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(a["cache"], b["cache"]) and torch.equal(a["weights"], b["weights"])
+
+
+def test_two_streams(gpu):
+    """Calls on two streams have workspaces of their own."""
+    torch = gpu
+    c = Case(torch, [3000], 2, 128, 64, seed=11).fill()
+    qs = [torch.randn(1, 8, 128, device="cuda") for _ in range(2)]
+    n = c.ints([3000])
+    want = [c.nn.cached_attention(q, c.cache, c.d_table, n) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for _ in range(20):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(c.nn.cached_attention(qs[i], c.cache, c.d_table, n))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+def test_same_call_same_bits(gpu):
+    torch = gpu
+    c = Case(torch, [700, 650], 2, 128, 64, seed=12).fill()
+    q = torch.randn(100, 8, 128, device="cuda")
+    starts = c.ints([0, 60, 100])
+    runs = []
+    for _ in range(3):
+        w = torch.zeros(c.pages, 2, 64, device="cuda")
+        runs.append((c.nn.cached_attention(q, c.cache, c.d_table, c.ints(c.lengths), starts=starts, max_new=60, weights=w), w))
+    for o, w in runs[1:]:
+        assert torch.equal(o, runs[0][0]) and torch.equal(w, runs[0][1])
+
+
+def test_refusals(gpu):
+    torch = gpu
+    from gomlx_amd import _lib, nn
+    c = Case(torch, [40, 10], 2, 64, 32).fill()
+    n = c.ints([40, 10])
+    q = torch.zeros(2, 4, 64, device="cuda")
+    k = torch.zeros(2, 2, 64, device="cuda")
+    w = torch.zeros(c.pages, 2, 32, device="cuda")
+    good = dict(q=q, cache=c.cache, page_table=c.d_table, lengths=n)
+    for change, error in ((dict(q=q.half()), _lib.NotImplementedByBackend), (dict(q=q[:, :3]), ValueError), (dict(q=q[:1]), ValueError), (dict(q=q[..., ::2]), ValueError),
+                          (dict(q=q.cpu()), ValueError), (dict(q=q.view(2, 256)), ValueError), (dict(cache=c.cache[..., :-36]), ValueError),
+                          (dict(cache=c.cache.view(torch.int8)), ValueError), (dict(lengths=n.long()), ValueError), (dict(page_table=c.d_table[:1]), ValueError),
+                          (dict(page_table=c.d_table.long()), ValueError), (dict(window=-1), ValueError), (dict(starts=c.ints([0, 2])), ValueError),
+                          (dict(max_new=2), ValueError), (dict(starts=c.ints([0, 1, 2]), max_new=0), ValueError), (dict(weights=w[:, :1]), ValueError),
+                          (dict(weights=w.double()), ValueError)):
+        with pytest.raises(error):
+            nn.cached_attention(**{**good, **change})
+    with pytest.raises(ValueError):
+        nn.kv_cache_append(c.cache, k, k.bfloat16(), c.d_table, n)
+    with pytest.raises(ValueError):
+        nn.kv_cache_append(c.cache, k[:, :1], k[:, :1], c.d_table, n)
+    with pytest.raises(_lib.NotImplementedByBackend):
+        nn.kv_cache_append(c.cache, k.half(), k.half(), c.d_table, n)
+    with pytest.raises(ValueError):
+        nn.kv_cache_read(c.cache, c.d_table, n, starts=c.ints([0, 1, 2]), max_new=1)
+    for keep, recent in ((0, 0), (5, 6), (5, -1)):
+        with pytest.raises(ValueError):
+            nn.kv_cache_evict(c.cache, w, c.d_table, n, keep, recent)
+    with pytest.raises(ValueError):
+        nn.kv_cache_evict(c.cache, None, c.d_table, n, 5, 1)
+    cos, sin = nn.rotary_table(10, 64)
+    pos = c.ints([0, 1])
+    good = dict(q=q, k=k, positions=pos, cos=cos, sin=sin)
+    for change, error in ((dict(q=q.half(), k=k.half()), _lib.NotImplementedByBackend), (dict(k=k.bfloat16()), ValueError), (dict(k=k[:1]), ValueError),
+                          (dict(q=q[..., :32].contiguous(), k=k[..., :32].contiguous()), _lib.NotImplementedByBackend), (dict(positions=pos.long()), ValueError),
+                          (dict(sin=sin[:5]), ValueError), (dict(cos=cos[:, :30].contiguous(), sin=sin[:, :30].contiguous()), _lib.HipqError),
+                          (dict(cos=cos.double(), sin=sin.double()), ValueError), (dict(dtype=torch.float16), _lib.NotImplementedByBackend),
+                          (dict(q_norm=nn.RMSNorm(gain=torch.ones(32, device="cuda"))), ValueError)):
+        with pytest.raises(error):
+            nn.qk_norm_rope(**{**good, **change})
+    for bad in (dict(head_dim=80), dict(page_tokens=33), dict(kv_heads=0)):
+        with pytest.raises((ValueError, _lib.NotImplementedByBackend)):
+            nn.kv_cache(**{**dict(pages=1, kv_heads=1, head_dim=64, page_tokens=32), **bad})
+
+
+def test_empty_calls(gpu):
+    torch = gpu
+    from gomlx_amd import nn
+    cache = nn.kv_cache(0, 2, 64, 32)
+    table, n = torch.zeros(0, 3, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    q = torch.zeros(0, 4, 64, device="cuda")
+    assert nn.cached_attention(q, cache, table, n).shape == (0, 4, 64)
+    nn.kv_cache_append(cache, q[:, :2], q[:, :2], table, n)
+    assert nn.kv_cache_read(cache, table, n)[0].shape == (0, 2, 64)
+    kept, left = nn.kv_cache_evict(cache, torch.zeros(0, 2, 32, device="cuda"), table, n, 4)
+    assert kept.shape == (0, 2, 4) and left.shape == (0,)
+    # one sequence without a page: nothing to see
+    cache, q = nn.kv_cache(1, 2, 64, 32), torch.randn(1, 4, 64, device="cuda")
+    table, n = torch.zeros(1, 0, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert torch.equal(nn.cached_attention(q, cache, table, n, weights=torch.zeros(1, 2, 32, device="cuda")), torch.zeros_like(q))
+    nn.kv_cache_append(cache, q[:, :2], q[:, 2:], table, n + 1)
+    assert not cache.any()
