@@ -115,7 +115,7 @@ _fast_tried = False
 # Entry points the native host path calls, in the order in which csrc/binding.cpp takes them.
 _BOUND = ("gq_qdense_check", "gq_qdense_f32", "gq_qdense_bf16", "gq_qdense_block_f32", "gq_qdense_block_bf16", "gq_qdense_gated_f32",
           "gq_qdense_gated_bf16", "gq_qdense_f32_batch", "gq_qdense_norm_f32_batch", "gq_qdense_norm_bf16_batch", "gq_dequantize",
-          "gq_embedding_lookup", "gq_bytes_per_block", "gq_values_per_block")
+          "gq_embedding_lookup", "gq_bytes_per_block", "gq_values_per_block", "gq_qk_norm_rope", "gq_kv_append", "gq_kv_read", "gq_kv_attention", "gq_kv_evict")
 
 
 def lib() -> ctypes.CDLL:

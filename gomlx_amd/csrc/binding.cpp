@@ -10,9 +10,12 @@
 
 #include <ATen/ATen.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <climits>
+#include <cmath>
 #include <initializer_list>
 
 #include "../../include/gomlx_hipq.h"
@@ -34,8 +37,13 @@ struct Entry {
     decltype(&gq_embedding_lookup) lookup;
     decltype(&gq_bytes_per_block) bytes_per_block;
     decltype(&gq_values_per_block) values_per_block;
+    decltype(&gq_qk_norm_rope) rope;
+    decltype(&gq_kv_append) kv_append;
+    decltype(&gq_kv_read) kv_read;
+    decltype(&gq_kv_attention) kv_attention;
+    decltype(&gq_kv_evict) kv_evict;
 } g;
-constexpr int kEntries = 14;
+constexpr int kEntries = 19;
 bool g_bound = false;
 PyTypeObject *g_activation = nullptr;  // nn.Activation
 PyObject *s_scheme, *s_ggml_type, *s_gain, *s_epsilon, *s_scale_offset;
@@ -304,6 +312,182 @@ PyObject *gather(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
+// ---- rotation, the 4-bit cache and attention over it --------------------------------------------------------------------
+
+bool to_i64(PyObject *o, int64_t &v) {
+    if (!PyLong_Check(o)) return false;
+    v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+int element_type(at::ScalarType t) { return t == at::kFloat ? GQ_F32 : t == at::kBFloat16 ? GQ_BF16 : -1; }
+bool head_dim_served(int64_t d) { return d == 64 || d == 128 || d == 256; }
+
+// [rows, heads, values], the values side by side
+struct HeadRows {
+    const at::Tensor *t = nullptr;
+    gq_head_rows d;
+    bool read(PyObject *o) {
+        if (!THPVariable_CheckExact(o)) return false;
+        t = &THPVariable_Unpack(o);
+        if (!t->is_cuda() || t->dim() != 3 || t->layout() != at::kStrided || element_type(t->scalar_type()) < 0 || t->stride(2) != 1) return false;
+        d = gq_head_rows{t->const_data_ptr(), t->stride(0), t->stride(1)};
+        return true;
+    }
+};
+
+const int32_t *int32_vector(PyObject *o, int64_t n, c10::DeviceIndex device) {
+    const at::Tensor *t = gpu_tensor(o);
+    return t && t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == n && t->get_device() == device ? t->const_data_ptr<int32_t>() : nullptr;
+}
+
+// What nn._kv_desc checks; empty calls are left to it.
+struct Cache {
+    gq_kv_cache d;
+    const at::Tensor *t = nullptr;
+    float *accounts = nullptr;
+    bool read(PyObject *cache, PyObject *table, PyObject *lengths, PyObject *starts, PyObject *max_new, int64_t rows, PyObject *weights) {
+        t = gpu_tensor(cache);
+        if (!t || t->scalar_type() != at::kByte || t->dim() != 4 || t->size(3) % 36 || !head_dim_served(t->size(3) / 36) || t->numel() == 0) return false;
+        if (!THPVariable_CheckExact(table) || !THPVariable_CheckExact(lengths)) return false;
+        const at::Tensor &pt = THPVariable_Unpack(table), &ln = THPVariable_Unpack(lengths);
+        const c10::DeviceIndex device = t->get_device();
+        if (ln.dim() != 1 || ln.size(0) < 1 || !pt.is_cuda() || pt.get_device() != device || pt.scalar_type() != at::kInt || pt.dim() != 2 || pt.size(0) != ln.size(0) ||
+            pt.size(1) < 1 || pt.size(1) > INT_MAX || (pt.size(1) > 1 && pt.stride(1) != 1))
+            return false;
+        d = gq_kv_cache{t->mutable_data_ptr(), t->size(0), (int)t->size(1), (int)(t->size(3) / 36), (int)(32 * t->size(2)), (int)pt.size(1), pt.const_data_ptr<int32_t>(),
+                        ln.size(0) < 2 ? std::max(pt.stride(0), pt.size(1)) : pt.stride(0), int32_vector(lengths, ln.size(0), device), nullptr, ln.size(0), rows, 1};
+        if (!d.dLengths || rows < 1 || !to_i64(max_new, d.max_new) || d.max_new < 1) return false;
+        if (starts != Py_None) {
+            if (!(d.dStarts = int32_vector(starts, d.seqs + 1, device))) return false;
+        } else if (d.max_new != 1 || rows != d.seqs) {
+            return false;
+        }
+        if (weights != Py_None) {
+            const at::Tensor *w = gpu_tensor(weights);
+            if (!w || w->get_device() != device || w->scalar_type() != at::kFloat || w->dim() != 3 || w->size(0) != d.pages || w->size(1) != d.kv_heads || w->size(2) != d.page_tokens)
+                return false;
+            accounts = static_cast<float *>(w->mutable_data_ptr());
+        }
+        return true;
+    }
+};
+
+at::Tensor fresh(const at::Tensor &like, at::IntArrayRef shape, at::ScalarType type) { return at::empty(shape, like.options().dtype(type).requires_grad(false)); }
+
+PyObject *pair(at::Tensor &&a, at::Tensor &&b) {
+    PyObject *out = PyTuple_New(2);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(a)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(b)));
+    return out;
+}
+
+// qk_norm_rope(q, k, positions, cos, sin, q_norm, k_norm, interleaved, dtype)
+PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        HeadRows q, k;
+        Norm qn, kn;
+        if (n != 9 || !q.read(a[0]) || !k.read(a[1]) || !PyBool_Check(a[7])) return none();
+        const int64_t rows = q.t->size(0), dim = q.t->size(2);
+        const c10::DeviceIndex device = q.t->get_device();
+        const at::Tensor *cos = gpu_tensor(a[3]), *sin = gpu_tensor(a[4]);
+        if (!head_dim_served(dim) || k.t->scalar_type() != q.t->scalar_type() || k.t->size(0) != rows || k.t->size(2) != dim || k.t->get_device() != device || !cos || !sin ||
+            cos->scalar_type() != at::kFloat || sin->scalar_type() != at::kFloat || cos->dim() != 2 || cos->sizes() != sin->sizes() || cos->get_device() != device ||
+            sin->get_device() != device || q.t->size(1) > INT_MAX || k.t->size(1) > INT_MAX || cos->size(1) > dim)
+            return none();
+        at::ScalarType type = q.t->scalar_type();
+        if (a[8] != Py_None) {
+            if (!THPDtype_Check(a[8])) return none();
+            type = reinterpret_cast<THPDtype *>(a[8])->scalar_type;
+        }
+        const int32_t *pos = int32_vector(a[2], rows, device);
+        if (element_type(type) < 0 || !pos || !qn.read(a[5], dim) || !kn.read(a[6], dim)) return none();
+        at::Tensor qo = fresh(*q.t, q.t->sizes(), type), ko = fresh(*q.t, k.t->sizes(), type);
+        const float *cp = cos->const_data_ptr<float>(), *sp = sin->const_data_ptr<float>();
+        void *qp = qo.mutable_data_ptr(), *kp = ko.mutable_data_ptr(), *s = stream_of(*q.t);
+        const int rc = without_gil([&] {
+            return g.rope(element_type(q.t->scalar_type()), &q.d, (int)q.t->size(1), &k.d, (int)k.t->size(1), (int)dim, rows, pos, cp, sp, cos->size(0), (int)(2 * cos->size(1)),
+                          a[7] == Py_True, qn.ptr(), kn.ptr(), element_type(type), qp, kp, s);
+        });
+        return rc == GQ_OK ? pair(std::move(qo), std::move(ko)) : none();
+    });
+}
+
+// kv_append(cache, k, v, page_table, lengths, starts, max_new, weights): True where it is done
+PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        HeadRows k, v;
+        Cache c;
+        if (n != 8 || !k.read(a[1]) || !v.read(a[2]) || !c.read(a[0], a[3], a[4], a[5], a[6], k.t->size(0), a[7])) return none();
+        if (k.t->sizes() != v.t->sizes() || k.t->scalar_type() != v.t->scalar_type() || k.t->size(1) != c.d.kv_heads || k.t->size(2) != c.d.head_dim ||
+            k.t->get_device() != c.t->get_device() || v.t->get_device() != c.t->get_device())
+            return none();
+        void *s = stream_of(*c.t);
+        const int rc = without_gil([&] { return g.kv_append(&c.d, element_type(k.t->scalar_type()), &k.d, &v.d, c.accounts, s); });
+        if (rc != GQ_OK) return none();
+        Py_RETURN_TRUE;
+    });
+}
+
+// kv_read(cache, page_table, lengths, starts, max_new, rows)
+PyObject *kv_read(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Cache c;
+        int64_t rows;
+        if (n != 6) return none();
+        if (a[5] == Py_None) {
+            if (a[3] != Py_None || !THPVariable_CheckExact(a[2]) || THPVariable_Unpack(a[2]).dim() != 1) return none();
+            rows = THPVariable_Unpack(a[2]).size(0);
+        } else if (!to_i64(a[5], rows)) {
+            return none();
+        }
+        if (!c.read(a[0], a[1], a[2], a[3], a[4], rows, Py_None)) return none();
+        at::Tensor k = fresh(*c.t, {rows, c.d.kv_heads, c.d.head_dim}, at::kHalf), v = fresh(*c.t, {rows, c.d.kv_heads, c.d.head_dim}, at::kHalf);
+        uint16_t *kp = static_cast<uint16_t *>(k.mutable_data_ptr()), *vp = static_cast<uint16_t *>(v.mutable_data_ptr());
+        void *s = stream_of(*c.t);
+        const int rc = without_gil([&] { return g.kv_read(&c.d, kp, vp, s); });
+        return rc == GQ_OK ? pair(std::move(k), std::move(v)) : none();
+    });
+}
+
+// cached_attention(q, cache, page_table, lengths, starts, max_new, scale | None, window, weights)
+PyObject *cached_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        HeadRows q;
+        Cache c;
+        int64_t window;
+        if (n != 9 || !q.read(a[0]) || !c.read(a[1], a[2], a[3], a[4], a[5], q.t->size(0), a[8]) || !to_i64(a[7], window)) return none();
+        if (q.t->size(2) != c.d.head_dim || q.t->size(1) < 1 || q.t->size(1) % c.d.kv_heads || q.t->size(1) > INT_MAX || q.t->get_device() != c.t->get_device()) return none();
+        double scale;
+        if (a[6] == Py_None) scale = 1.0 / std::sqrt((double)c.d.head_dim);
+        else if (PyFloat_Check(a[6])) scale = PyFloat_AS_DOUBLE(a[6]);
+        else return none();
+        at::Tensor out = fresh(*q.t, q.t->sizes(), q.t->scalar_type());
+        void *op = out.mutable_data_ptr(), *s = stream_of(*c.t);
+        const int rc = without_gil([&] { return g.kv_attention(&c.d, element_type(q.t->scalar_type()), &q.d, (int)q.t->size(1), (float)scale, window, c.accounts, op, s); });
+        return rc == GQ_OK ? THPVariable_Wrap(std::move(out)) : none();
+    });
+}
+
+// kv_evict(cache, weights, page_table, lengths, keep, recent)
+PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Cache c;
+        int64_t keep, recent;
+        if (n != 6 || a[1] == Py_None || !THPVariable_CheckExact(a[3]) || THPVariable_Unpack(a[3]).dim() != 1 || !to_i64(a[4], keep) || !to_i64(a[5], recent)) return none();
+        PyObject *one = PyLong_FromLong(1);  // (a small number: shared)
+        const bool ok = c.read(a[0], a[2], a[3], Py_None, one, THPVariable_Unpack(a[3]).size(0), a[1]);
+        Py_DECREF(one);
+        if (!ok || keep < 1 || recent < 0 || recent > keep) return none();
+        at::Tensor kept = fresh(*c.t, {c.d.seqs, c.d.kv_heads, keep}, at::kInt), left = fresh(*c.t, {c.d.seqs}, at::kInt);
+        int32_t *kp = kept.mutable_data_ptr<int32_t>(), *lp = left.mutable_data_ptr<int32_t>();
+        void *s = stream_of(*c.t);
+        const int rc = without_gil([&] { return g.kv_evict(&c.d, c.accounts, keep, recent, kp, lp, s); });
+        return rc == GQ_OK ? pair(std::move(kept), std::move(left)) : none();
+    });
+}
+
 // bind(Activation, address, ...): the enumeration of nn.py, the entry points in the order of Entry
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != kEntries + 1 || !PyType_Check(a[0])) { PyErr_Format(PyExc_TypeError, "bind takes a type and %d addresses", kEntries); return nullptr; }
@@ -331,6 +515,11 @@ PyMethodDef methods[] = {
     {"batch", (PyCFunction)(void (*)(void))batch, METH_FASTCALL, nullptr},
     {"dequantize", (PyCFunction)(void (*)(void))dequantize, METH_FASTCALL, nullptr},
     {"gather", (PyCFunction)(void (*)(void))gather, METH_FASTCALL, nullptr},
+    {"qk_norm_rope", (PyCFunction)(void (*)(void))qk_norm_rope, METH_FASTCALL, nullptr},
+    {"kv_append", (PyCFunction)(void (*)(void))kv_append, METH_FASTCALL, nullptr},
+    {"kv_read", (PyCFunction)(void (*)(void))kv_read, METH_FASTCALL, nullptr},
+    {"cached_attention", (PyCFunction)(void (*)(void))cached_attention, METH_FASTCALL, nullptr},
+    {"kv_evict", (PyCFunction)(void (*)(void))kv_evict, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -417,6 +417,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos:
     pair (``interleaved``: 2 i and 2 i + 1); those from rot on are not rotated.  ``q_norm`` / ``k_norm`` normalise every head over its
     head_dim values first (gain [head_dim]).  Returns (q, k), contiguous, of ``dtype`` (default: the inputs').  A position outside the
     table makes its row NaN."""
+    if _lib.fast is not None and (out := _lib.fast.qk_norm_rope(q, k, positions, cos, sin, q_norm, k_norm, interleaved, dtype)) is not None:
+        return out
     import ctypes
     xd = _float_type("qk_norm_rope", q)
     if k.dtype != q.dtype:
@@ -473,6 +475,8 @@ def kv_cache_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_
     The scale of a group is minus an eighth of its value of largest magnitude, rounded to 8 significant bits; codes are rounded to
     nearest.  A token with a NaN, an infinity or a magnitude of 65408 or more in a head makes rows that attend to it NaN there.
     ``weights``: the accounts of ``cached_attention``, set to zero for the new tokens."""
+    if _lib.fast is not None and _lib.fast.kv_append(cache, k, v, page_table, lengths, starts, max_new, weights):
+        return
     import ctypes
     xd = _float_type("kv_cache_append", k)
     if v.dtype != k.dtype or v.shape != k.shape:
@@ -489,6 +493,8 @@ def kv_cache_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.
                   rows: int | None = None) -> tuple:
     """(keys, values) float16 [rows, kv_heads, head_dim] that the cache stands for at the last tokens of every sequence, exact.  Rows in
     front of a sequence's first token are zero."""
+    if _lib.fast is not None and (out := _lib.fast.kv_read(cache, page_table, lengths, starts, max_new, rows)) is not None:
+        return out
     import ctypes
     d = _kv_desc(cache, page_table, lengths, starts, max_new, rows)
     _init(cache.device.index or 0)
@@ -506,6 +512,8 @@ def cached_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
     sequence, with a ``window`` the last that many; one that sees nothing gets zeros.  ``weights``: float32 [pages, kv_heads, page_tokens],
     to which the softmax weights that every cached token receives are added (summed over rows and the query heads of a key head): what
     ``kv_cache_evict`` goes by.  Every row of q belongs to a sequence.  Returns [rows, heads, head_dim] of q's type, contiguous."""
+    if _lib.fast is not None and (out := _lib.fast.cached_attention(q, cache, page_table, lengths, starts, max_new, scale, window, weights)) is not None:
+        return out
     import ctypes
     xd = _float_type("cached_attention", q)
     d = _kv_desc(cache, page_table, lengths, starts, max_new, q.shape[0] if q.dim() else None, weights)
@@ -529,6 +537,8 @@ def kv_cache_evict(cache: torch.Tensor, weights: torch.Tensor, page_table: torch
     others of largest accumulated weight stay (ties: the earlier token), moved to the front of the sequence's pages in their order,
     with their weights.  Returns (kept, lengths): int32 [sequences, kv_heads, keep] former places of the kept tokens (-1 behind the last), and
     the new lengths, min(length, keep); ``lengths`` itself is left as it is."""
+    if _lib.fast is not None and (out := _lib.fast.kv_evict(cache, weights, page_table, lengths, keep, recent)) is not None:
+        return out
     import ctypes
     d = _kv_desc(cache, page_table, lengths, accounts=weights)
     if weights is None:
