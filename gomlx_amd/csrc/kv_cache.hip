@@ -22,66 +22,59 @@ __device__ __forceinline__ float round_to_bf16(float v) {  // of finite v, to ne
 // where element e of a dword lies
 __device__ __forceinline__ int nibble_shift(int e) { return ((e >> 1) + 4 * (e & 1)) * 4; }
 
-template <int NE, bool BF16> __device__ __forceinline__ void load_values(float (&v)[NE], const void *p, int64_t at, int wide) {
+// Eight neighbouring values.
+template <bool BF16> __device__ __forceinline__ void load8(float (&v)[8], const void *p, int64_t at, int wide) {
     if constexpr (BF16) {
         const uint16_t *x = static_cast<const uint16_t *>(p) + at;
-        uint32_t u[NE];
-        if (NE == 2 && wide) {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(x);
-            u[0] = w & 0xFFFFu;
-            u[NE - 1] = w >> 16;
-        } else if (NE == 4 && wide) {
-            const u2 w = *reinterpret_cast<const u2 *>(x);
-            u[0] = w.x & 0xFFFFu;
-            u[1 % NE] = w.x >> 16;
-            u[2 % NE] = w.y & 0xFFFFu;
-            u[NE - 1] = w.y >> 16;
-        } else {
+        u4 w;
+        if (wide) w = *reinterpret_cast<const u4 *>(x);
+        else w = u4{x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16};
 #pragma unroll
-            for (int i = 0; i < NE; i++) u[i] = x[i];
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
         }
-#pragma unroll
-        for (int i = 0; i < NE; i++) v[i] = __uint_as_float(u[i] << 16);
     } else {
         const float *x = static_cast<const float *>(p) + at;
-        if (NE == 2 && wide) {
-            const float2 w = *reinterpret_cast<const float2 *>(x);
-            v[0] = w.x;
-            v[NE - 1] = w.y;
-        } else if (NE == 4 && wide) {
-            const float4 w = *reinterpret_cast<const float4 *>(x);
-            v[0] = w.x;
-            v[1 % NE] = w.y;
-            v[2 % NE] = w.z;
-            v[NE - 1] = w.w;
+        if (wide) {
+            const float4 lo = *reinterpret_cast<const float4 *>(x), hi = *reinterpret_cast<const float4 *>(x + 4);
+            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < NE; i++) v[i] = x[i];
+            for (int i = 0; i < 8; i++) v[i] = x[i];
         }
     }
 }
 
-// A group's scale, from the NE values of each of its 32 / NE lanes: minus an eighth of the value of largest magnitude (the
+// A group's scale, from the eight values of each of its four lanes: minus an eighth of the value of largest magnitude (the
 // first of those), rounded to 8 significant bits.  The value itself then has code 0 and none is more than 8 steps away.
-template <int NE> __device__ __forceinline__ float group_scale(const float (&v)[NE]) {
+__device__ __forceinline__ float group_scale(const float (&v)[8]) {
     float m = v[0];
 #pragma unroll
-    for (int i = 1; i < NE; i++) m = fabsf(v[i]) > fabsf(m) ? v[i] : m;
+    for (int i = 1; i < 8; i++) m = fabsf(v[i]) > fabsf(m) ? v[i] : m;
 #pragma unroll
-    for (int s = 1; s < 32 / NE; s <<= 1) {
+    for (int s = 1; s < 4; s <<= 1) {
         const float o = __shfl_xor(m, s);
         const bool take = fabsf(o) > fabsf(m) || (fabsf(o) == fabsf(m) && ((int)threadIdx.x & s));
         m = take ? o : m;
     }
     return half_value(half_bits(round_to_bf16(m * -0.125f)));
 }
-__device__ __forceinline__ uint32_t code_of(float v, float d) {
-    return d == 0.0f ? 8u : (uint32_t)fminf(fmaxf(floorf(v / d + 8.5f), 0.0f), 15.0f);
+// floor(v / d + 8.5) within 0 .. 15, the quotient rounded once: inv is 1 / d rounded to nearest, and a product with it, corrected by its
+// exact remainder, is then the rounded quotient (quotients so small that the remainder leaves fp32's range give 8 either way).
+__device__ __forceinline__ uint32_t code_of(float v, float d, float inv) {
+    const float q = v * inv, quotient = fmaf(fmaf(-q, d, v), inv, q);
+    return (uint32_t)fminf(fmaxf(floorf(quotient + 8.5f), 0.0f), 15.0f);
 }
 
-// Eight tokens of one block (a lane's share of a value operand: their codes share dwords) per wavefront, key head and sequence;
-// a lane holds D / 64 values of every token.  A dword of value codes belongs to one lane of one wavefront of the launch, so
-// that tokens that share bytes need no atomics.
+// Eight tokens of one block (a lane's share of a value operand: their codes share dwords) per wavefront, key head and sequence.
+// A lane takes eight values of a token, D / 8 lanes a token, and D / 64 rounds the block: a lane's key codes are one dword.  Its
+// value codes are eight dwords that other lanes hold other tokens of; the lanes of equal values exchange halves until each has
+// D / 64 whole ones.  A dword belongs to one lane of one wavefront of the launch, so that tokens that share bytes need no atomics.
+//
+// A few new tokens: the chain length -> page -> bytes of a partly filled dword bounds it (4 us for 32 sequences of 8 heads); many:
+// the inputs' bytes.
 struct AppendArgs {
     KvCall kv;
     HeadRows k, v;
@@ -92,7 +85,7 @@ struct AppendArgs {
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
     typedef KvTile<D> T;
-    constexpr int NE = D / 64, G = T::G;
+    constexpr int G = T::G, L = D / 8, ROUNDS = D / 64, PER = 8 / ROUNDS;  // lanes of a token, rounds, tokens of a round
     const KvCall &kv = a.kv;
     const int64_t unit = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
     const int per = kv.kv_heads * a.blocks;
@@ -105,58 +98,79 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
     if (p0 >= s.length || s.news == 0) return;
     uint8_t *tile = kv_tile(kv, b, h, p0 >> 5, T::kBytes);
     if (!tile) return;
-    const int lane = (int)threadIdx.x & 63, x = lane * NE;  // first value of the lane
+    const int lane = (int)threadIdx.x & 63, l = lane % L, x = l * 8, mine = lane / L;  // the lane's values; its token of a round
     const int j = (p0 >> 3) & 3, g = x >> 5;
+    const bool account = a.accounts && l == 0;
+    const int live_from = from > p0 ? from - p0 : 0, live_to = s.length - p0 < 8 ? s.length - p0 : 8;  // new tokens of the block
 
-    float k[8][NE], v[8][NE];
+    float k[ROUNDS][8], v[ROUNDS][8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const int p = p0 + e;
-        const bool live = p >= from && p < s.length;
-        const int64_t row = live ? s.row0 + (p - first) : s.row0;
-        load_values<NE, BF16>(k[e], a.k.p, row * a.k.row + h * a.k.head + x, a.wide);
-        load_values<NE, BF16>(v[e], a.v.p, row * a.v.row + h * a.v.head + x, a.wide);
+    for (int n = 0; n < ROUNDS; n++) {
+        const int e = n * PER + mine;
+        if (e >= live_from && e < live_to) {
+            const int64_t row = s.row0 + (p0 + e - first);
+            load8<BF16>(k[n], a.k.p, row * a.k.row + h * a.k.head + x, a.wide);
+            load8<BF16>(v[n], a.v.p, row * a.v.row + h * a.v.head + x, a.wide);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) k[n][i] = v[n][i] = 0.0f;
+        }
     }
-    uint32_t bits[NE] = {}, live_mask = 0;
+    uint32_t bits[8] = {};
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const int p = p0 + e;
-        if (p < from || p >= s.length) continue;
+    for (int n = 0; n < ROUNDS; n++) {
+        const int e = n * PER + mine, p = p0 + e;
+        const bool live = e >= live_from && e < live_to;
         bool good = true;
 #pragma unroll
-        for (int i = 0; i < NE; i++) good = good && fabsf(k[e][i]) < kLargest && fabsf(v[e][i]) < kLargest;
-        good = __all(good);
+        for (int i = 0; i < 8; i++) good = good && fabsf(k[n][i]) < kLargest && fabsf(v[n][i]) < kLargest;
+        const uint64_t token = (L == 64 ? ~0ull : ((1ull << (L & 63)) - 1)) << (mine * L);
+        good = (__ballot(good) & token) == token;
         if (!good) {
 #pragma unroll
-            for (int i = 0; i < NE; i++) k[e][i] = v[e][i] = 0.0f;
+            for (int i = 0; i < 8; i++) k[n][i] = v[n][i] = 0.0f;
         }
-        const float dk = group_scale<NE>(k[e]), dv = group_scale<NE>(v[e]);
+        const float dk = group_scale(k[n]), dv = group_scale(v[n]);
+        const float ik = dk == 0.0f ? 0.0f : 1.0f / dk, iv = dv == 0.0f ? 0.0f : 1.0f / dv;  // (no scale: every code is 8)
         uint32_t word = 0;
+        const int at = nibble_shift(e);
 #pragma unroll
-        for (int i = 0; i < NE; i++) {
-            word |= code_of(k[e][i], dk) << nibble_shift((x + i) & 7);
-            bits[i] |= code_of(v[e][i], dv) << nibble_shift(e);
+        for (int i = 0; i < 8; i++) {
+            word |= code_of(k[n][i], dk, ik) << nibble_shift(i);
+            bits[i] |= (live ? code_of(v[n][i], dv, iv) : 0u) << at;
         }
-        live_mask |= 0xFu << nibble_shift(e);
-#pragma unroll
-        for (int m = 1; m < 8 / NE; m <<= 1) word |= (uint32_t)__shfl_xor((int)word, m);
-        const int t = p & 31;
-        if ((x & 7) == 0) {
-            const int w = key_half(t) * G + g, l = key_row(t) + 16 * ((x >> 3) & 3);
-            *reinterpret_cast<uint32_t *>(tile + T::kKeys + T::code(w, l)) = word;
-        }
-        if ((x & 31) == 0) {
-            reinterpret_cast<uint16_t *>(tile + T::kKeyScales)[t * G + g] = (uint16_t)(good ? half_bits(dk) : kNanHalf);
-            reinterpret_cast<uint16_t *>(tile + T::kValueScales)[g * 32 + t] = (uint16_t)half_bits(dv);
-        }
-        if (a.accounts && lane == 0) {
-            float *at = kv_account(kv, a.accounts, b, h, p);
-            if (at) *at = 0.0f;
+        if (live) {
+            const int t = p & 31;
+            *reinterpret_cast<uint32_t *>(tile + T::kKeys + T::code(key_half(t) * G + g, key_row(t) + 16 * (l & 3))) = word;
+            if ((l & 3) == 0) {
+                reinterpret_cast<uint16_t *>(tile + T::kKeyScales)[t * G + g] = (uint16_t)(good ? half_bits(dk) : kNanHalf);
+                reinterpret_cast<uint16_t *>(tile + T::kValueScales)[g * 32 + t] = (uint16_t)half_bits(dv);
+            }
+            if (account) {
+                float *q = kv_account(kv, a.accounts, b, h, p);
+                if (q) *q = 0.0f;
+            }
         }
     }
+    // lanes of equal values, L, 2 L, ... apart, pass each other the dwords that the other one finishes
+    int count = 8, base = 0;
 #pragma unroll
-    for (int i = 0; i < NE; i++) {
-        const int c = x + i;
+    for (int m = 32; m >= L; m >>= 1) {
+        count >>= 1;
+        const bool upper = lane & m;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i >= count) break;
+            const uint32_t give = upper ? bits[i] : bits[i + count], keep = upper ? bits[i + count] : bits[i];
+            bits[i] = keep | (uint32_t)__shfl_xor((int)give, m);
+        }
+        base += upper ? count : 0;
+    }
+    uint32_t live_mask = 0;
+    for (int e = live_from; e < live_to; e++) live_mask |= 0xFu << nibble_shift(e);
+#pragma unroll
+    for (int i = 0; i < ROUNDS; i++) {
+        const int c = x + base + i;
         uint32_t *at = reinterpret_cast<uint32_t *>(tile + T::kValues + T::code(c >> 4, (c & 15) + 16 * j));
         *at = live_mask == 0xFFFFFFFFu ? bits[i] : (*at & ~live_mask) | bits[i];
     }
@@ -224,7 +238,8 @@ __device__ __forceinline__ uint32_t account_key(float f) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+constexpr int kBins = 2048;
 
 // The sum of v over the threads in front, and over all.
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *waves, uint32_t &total) {
@@ -240,7 +255,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *waves, uint
     __syncthreads();
     uint32_t before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kSelectThreads / 64; i++) {
+    for (int i = 0; i < kSelectWaves; i++) {
         const uint32_t n = waves[i];
         before += i < w ? n : 0;
         all += n;
@@ -249,9 +264,15 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *waves, uint
     return before + inc - v;
 }
 
-__global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall kv, float *__restrict__ accounts, int keep, int recent, int32_t *__restrict__ kept) {
-    __shared__ uint32_t hist[256], waves[kSelectThreads / 64], found[2];
-    const int h = (int)blockIdx.x, b = (int)blockIdx.y, tid = (int)threadIdx.x;
+// One workgroup per sequence and key head.  A wavefront owns a run of neighbouring tokens, 64 at a time, and holds their keys in
+// registers where IT rounds of them suffice (IT = 0: reads them again for every pass).  The smallest kept key is found digit by
+// digit, eleven bits at a time of its distance from the smallest key there is, so that keys of similar size spread over the
+// histogram (those that equal the smallest, zeros mostly, are left out of it); a wavefront then counts what it keeps, and
+// writes its tokens behind those of the wavefronts in front.
+template <int IT>
+__global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall kv, const float *__restrict__ accounts, int keep, int recent, int32_t *__restrict__ kept) {
+    __shared__ uint32_t hist[kBins], waves[kSelectWaves], found[2], ends[2][kSelectWaves];
+    const int h = (int)blockIdx.x, b = (int)blockIdx.y, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const KvSeq s = kv_seq(kv, b);
     int32_t *out = kept + ((int64_t)b * kv.kv_heads + h) * keep;
     if (s.length <= keep) {
@@ -260,50 +281,122 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall 
     }
     const int n = s.length - recent;
     uint32_t want = (uint32_t)(keep - recent);  // of the first n tokens (n > want)
+    for (int i = tid; i < recent; i += kSelectThreads) out[want + i] = n + i;
+    if (want == 0) return;
+    const int rounds = IT ? IT : (n + kSelectThreads - 1) / kSelectThreads;
+    const int t0 = wave * rounds * 64 + lane;
     // (an account without a page counts as the smallest)
     const auto key_at = [&](int t) {
-        const float *p = kv_account(kv, accounts, b, h, t);
+        const float *p = kv_account(kv, const_cast<float *>(accounts), b, h, t);
         return p ? account_key(*p) : 0u;
     };
-    // the want-th largest key, eight bits at a time; `want` counts down to how many of the tokens that equal it are kept
-    uint32_t key = 0;
-    for (int shift = 24; shift >= 0 && want; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
-        __syncthreads();
-        for (int t = tid; t < n; t += kSelectThreads) {
-            const uint32_t u = key_at(t);
-            if (shift == 24 || (u >> (shift + 8)) == (key >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255u], 1u);
+    uint32_t keys[IT ? IT : 1];
+    if constexpr (IT > 0) {
+#pragma unroll
+        for (int i = 0; i < IT; i++) keys[i] = t0 + 64 * i < n ? key_at(t0 + 64 * i) : 0u;
+    }
+    const auto each = [&](auto f) {  // f(token, key) for the thread's tokens
+        if constexpr (IT > 0) {
+#pragma unroll
+            for (int i = 0; i < IT; i++)
+                if (t0 + 64 * i < n) f(t0 + 64 * i, keys[i]);
+        } else {
+            for (int i = 0; i < rounds; i++)
+                if (t0 + 64 * i < n) f(t0 + 64 * i, key_at(t0 + 64 * i));
         }
+    };
+    uint32_t low = 0xFFFFFFFFu, high = 0;
+    each([&](int, uint32_t u) {
+        low = min(low, u);
+        high = max(high, u);
+    });
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        low = min(low, (uint32_t)__shfl_xor((int)low, m));
+        high = max(high, (uint32_t)__shfl_xor((int)high, m));
+    }
+    if (lane == 0) { ends[0][wave] = low; ends[1][wave] = high; }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSelectWaves; i++) {
+        low = min(low, ends[0][i]);
+        high = max(high, ends[1][i]);
+    }
+    __syncthreads();
+    // digits of u - low; `want` counts down to how many of the tokens that equal the key are kept
+    int width = 32 - __clz(high - low);  // bits that are open (0: every key is the same)
+    uint32_t key = low;                  // the smallest key that the open bits allow
+    while (width > 0) {
+        const int shift = width > 11 ? width - 11 : 0;
+        const uint32_t top = width < 32 ? 1u << width : 0u;  // keys from key to key + top - 1 are looked at (0: all)
+        for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
         __syncthreads();
-        const uint32_t mine = tid < 256 ? hist[255 - tid] : 0;  // the largest digits first
+        each([&](int, uint32_t u) {
+            const uint32_t at = u - key;
+            if (u > low && u >= key && (top == 0 || at < top)) atomicAdd(&hist[at >> shift], 1u);
+        });
+        __syncthreads();
+        const int bin = kBins - 1 - 2 * tid;  // the largest digits first, two a thread
+        const uint32_t first = hist[bin], second = hist[bin - 1];
         uint32_t total;
-        const uint32_t before = block_scan(mine, waves, total);
-        if (tid < 256 && before < want && want <= before + mine) { found[0] = 255u - tid; found[1] = want - before; }
+        const uint32_t before = block_scan(first + second, waves, total);
+        if (before < want && want <= before + first) { found[0] = (uint32_t)bin; found[1] = want - before; }
+        else if (before + first < want && want <= before + first + second) { found[0] = (uint32_t)bin - 1; found[1] = want - before - first; }
+        if (tid == 0 && want > total) { found[0] = 0xFFFFFFFFu; found[1] = want - total; }  // down to those that equal the smallest
         __syncthreads();
-        key |= found[0] << shift;
+        const uint32_t digit = found[0];
         want = found[1];
         __syncthreads();
+        if (digit == 0xFFFFFFFFu) {
+            key = low;
+            break;
+        }
+        key += digit << shift;
+        width = shift;
     }
-    const bool some = keep > recent;
-    uint32_t at = 0, equal = 0;  // kept so far; tokens equal to the key so far
-    for (int t0 = 0; t0 < s.length; t0 += kSelectThreads) {
-        const int t = t0 + tid;
-        const uint32_t u = t < n && some ? key_at(t) : 0;
-        const bool same = t < n && some && u == key;
-        uint32_t sames, all;
-        const uint32_t rank = equal + block_scan(same ? 1u : 0u, waves, sames);
-        const bool keeps = t < n ? some && (u > key || (same && rank < want)) : t < s.length;
-        const uint32_t place = at + block_scan(keeps ? 1u : 0u, waves, all);
-        if (keeps) out[place] = t;
-        equal += sames;
-        at += all;
+    // u > key stay, and the first `want` that equal it
+    uint32_t more = 0, same = 0;
+    each([&](int, uint32_t u) {
+        more += u > key;
+        same += u == key;
+    });
+    uint32_t mores = more, sames = same;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        mores += (uint32_t)__shfl_xor((int)mores, m);
+        sames += (uint32_t)__shfl_xor((int)sames, m);
+    }
+    if (lane == 0) { ends[0][wave] = mores; ends[1][wave] = sames; }
+    __syncthreads();
+    uint32_t at = 0, equal = 0;  // kept, and equal to the key, in front
+    for (int i = 0; i < wave; i++) {
+        const uint32_t e = ends[1][i];
+        at += ends[0][i] + (equal < want ? min(e, want - equal) : 0);
+        equal += e;
+    }
+    const auto place = [&](int t, uint32_t u) {  // the whole wavefront, tokens in order of lanes
+        const uint64_t below = (1ull << lane) - 1;
+        const bool here = t < n, is = here && u == key;
+        const uint64_t equals = __ballot(is);
+        const bool stays = here && (u > key || (is && equal + (uint32_t)__popcll(equals & below) < want));
+        const uint64_t stay = __ballot(stays);
+        if (stays) out[at + (uint32_t)__popcll(stay & below)] = t;
+        at += (uint32_t)__popcll(stay);
+        equal += (uint32_t)__popcll(equals);
+    };
+    if constexpr (IT > 0) {
+#pragma unroll
+        for (int i = 0; i < IT; i++) place(t0 + 64 * i, keys[i]);
+    } else {
+        for (int i = 0; i < rounds; i++) place(t0 + 64 * i, t0 + 64 * i < n ? key_at(t0 + 64 * i) : 0u);
     }
 }
 
-// Moves the kept tokens of a sequence and key head to its front.  kept[i] >= i, so that a workgroup that reads its next tokens
-// before it writes the present ones, and goes from the front to the back, never overwrites what it has yet to read.
-// blockIdx.z: 0 the keys, their scales and the accounts, 1 the values and theirs.
-constexpr int kMoveTokens = 128;
+// Moves the kept tokens of a sequence and key head to its front, in place.  kept[i] >= i, so that a workgroup that reads its next
+// tokens before it writes the present ones, and goes from the front to the back, never overwrites what it has yet to read.
+// Workgroups share a head by what they move, not by tokens: blockIdx.z = 0 .. 3 the key codes of lanes 16 j .. 16 j + 15, then four
+// for every 64 values (the value codes of every fourth operand row's neighbours), and one for scales and accounts.
+constexpr int kMoveThreads = 256, kMoveTokens = 1024;
 
 // Every thread's loads are back: what the workgroup writes from here on is not what one of its wavefronts still reads.
 __device__ __forceinline__ void all_read() {
@@ -312,104 +405,137 @@ __device__ __forceinline__ void all_read() {
 }
 
 template <int D>
-__global__ __launch_bounds__(512) void kv_move_kernel(const KvCall kv, float *accounts, int keep, const int32_t *__restrict__ kept, int32_t *new_lengths) {
+__global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvCall kv, float *accounts, int keep, const int32_t *__restrict__ kept, int32_t *new_lengths) {
     typedef KvTile<D> T;
-    constexpr int G = T::G;
-    const int h = (int)blockIdx.x, b = (int)blockIdx.y, tid = (int)threadIdx.x;
+    constexpr int G = T::G, R = kMoveTokens / kMoveThreads;
+    __shared__ int64_t source[kMoveTokens];  // tile * 32 + token in it; -1: nothing comes
+    const int h = (int)blockIdx.x, b = (int)blockIdx.y, part = (int)blockIdx.z, tid = (int)threadIdx.x;
     const int32_t *list = kept + ((int64_t)b * kv.kv_heads + h) * keep;
     // (new_lengths may be kv.lengths: nobody else reads them in this launch)
-    if (h == 0 && blockIdx.z == 0 && tid == 0) new_lengths[b] = min(kv_seq(kv, b).length, keep);
+    if (h == 0 && part == 0 && tid == 0) new_lengths[b] = min(kv_seq(kv, b).length, keep);
     if (list[keep - 1] < keep) return;  // nothing to move: as many tokens as places, or fewer (-1)
-    if (blockIdx.z == 0) {
-        const int i_in = tid >> 2, j = tid & 3;
-        for (int i0 = 0; i0 < keep; i0 += kMoveTokens) {
-            const int i = i0 + i_in;
-            uint32_t code[G], scale = 0;
-            float account = 0.0f;
-            const bool live = i < keep;
-            const uint8_t *from = nullptr;
-            if (live) {
-                const int t = list[i];
-                from = kv_tile(kv, b, h, t >> 5, T::kBytes);
-                if (from) {
-                    const int in = t & 31, l = key_row(in) + 16 * j;
+    const int per_page = kv.page_tokens >> 5;
+    const auto tile_number = [&](int tile) -> int64_t {
+        const int slot = tile / per_page, page = kv.table[b * kv.table_stride + slot];
+        return (uint32_t)page < (uint32_t)kv.pages ? ((int64_t)page * kv.kv_heads + h) * per_page + (tile - slot * per_page) : -1;
+    };
+    for (int i0 = 0; i0 < keep; i0 += kMoveTokens) {
+        if (list[min(i0 + kMoveTokens, keep) - 1] == min(i0 + kMoveTokens, keep) - 1) continue;  // all of these stay where they are
 #pragma unroll
-                    for (int g = 0; g < G; g++) code[g] = *reinterpret_cast<const uint32_t *>(from + T::kKeys + T::code(key_half(in) * G + g, l));
-#pragma unroll
-                    for (int g = j; g < G; g += 4) scale |= (uint32_t)reinterpret_cast<const uint16_t *>(from + T::kKeyScales)[in * G + g] << (16 * (g >> 2));
-                    if (j == 0) {
-                        const float *p = kv_account(kv, accounts, b, h, t);
-                        account = p ? *p : 0.0f;
-                    }
-                }
-            }
-            all_read();
-            if (live && from) {
-                uint8_t *to = kv_tile(kv, b, h, i >> 5, T::kBytes);
-                if (to) {
-                    const int in = i & 31, l = key_row(in) + 16 * j;
-#pragma unroll
-                    for (int g = 0; g < G; g++) *reinterpret_cast<uint32_t *>(to + T::kKeys + T::code(key_half(in) * G + g, l)) = code[g];
-#pragma unroll
-                    for (int g = j; g < G; g += 4) reinterpret_cast<uint16_t *>(to + T::kKeyScales)[in * G + g] = (uint16_t)(scale >> (16 * (g >> 2)));
-                    if (j == 0) {
-                        float *p = kv_account(kv, accounts, b, h, i);
-                        if (p) *p = account;
-                    }
-                }
-            }
-            __syncthreads();
+        for (int n = 0; n < R; n++) {
+            const int i = i0 + n * kMoveThreads + tid;
+            const int t = i < keep ? list[i] : 0;
+            const int64_t tile = i < keep ? tile_number(t >> 5) : -1;
+            source[n * kMoveThreads + tid] = tile < 0 ? -1 : tile * 32 + (t & 31);
         }
-    } else {
-        // one thread: the dword of eight tokens for four values (64 lanes x D / 64 sets of them a tile), and the scales of one token
-        constexpr int kSets = D / 64, kTiles = 512 / (64 * kSets);
-        const int tile_in = tid / (64 * kSets), set = (tid >> 6) % kSets, lane = tid & 63, r = lane & 15, j = lane >> 4;
-        for (int i0 = 0; i0 < keep; i0 += kTiles * 32) {
-            const int i1 = i0 + tile_in * 32 + j * 8;  // the first of the eight
-            u4 word = {0, 0, 0, 0};
-            uint32_t mask = 0;
-            uint16_t scale[8] = {};
-            const int sg = set * 16 + r;  // (of the lanes, the first G of a value set's share move the scales)
+        __syncthreads();
+        if (part < 4) {  // one token a thread and round: its dwords of lane part
+            u4 code[R][(G + 3) / 4];
+            int64_t from[R];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int i = i1 + e;
-                if (i >= keep) continue;
-                const int t = list[i];
-                const uint8_t *from = kv_tile(kv, b, h, t >> 5, T::kBytes);
-                if (!from) continue;
-                const int in = t & 31, sh = nibble_shift(in & 7);
-                const u4 w = *reinterpret_cast<const u4 *>(from + T::kValues + ((set * 64) + r + 16 * (in >> 3)) * 16);
+            for (int n = 0; n < R; n++) {
+                from[n] = source[n * kMoveThreads + tid];
+                if (from[n] < 0) continue;
+                const int t = (int)from[n] & 31;
+                const uint8_t *at = kv.cache + (from[n] >> 5) * T::kBytes + T::kKeys + T::code(key_half(t) * G, key_row(t) + 16 * part);
+                if constexpr (G == 2) {
+                    const u2 w = *reinterpret_cast<const u2 *>(at);
+                    code[n][0] = u4{w.x, w.y, 0, 0};
+                } else {
 #pragma unroll
-                for (int c = 0; c < 4; c++) word[c] |= ((w[c] >> sh) & 15u) << nibble_shift(e);
-                mask |= 0xFu << nibble_shift(e);
-                if (sg < G) scale[e] = reinterpret_cast<const uint16_t *>(from + T::kValueScales)[sg * 32 + in];
-            }
-            all_read();
-            if (mask) {
-                uint8_t *to = kv_tile(kv, b, h, i1 >> 5, T::kBytes);
-                if (to) {
-                    u4 *at = reinterpret_cast<u4 *>(to + T::kValues + (set * 64 + lane) * 16);
-                    if (mask != 0xFFFFFFFFu) {
-                        const u4 old = *at;
-#pragma unroll
-                        for (int c = 0; c < 4; c++) word[c] |= old[c] & ~mask;
-                    }
-                    *at = word;
-                    if (sg < G) {
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if ((mask >> nibble_shift(e)) & 1u) reinterpret_cast<uint16_t *>(to + T::kValueScales)[sg * 32 + ((i1 + e) & 31)] = scale[e];
-                    }
+                    for (int c = 0; c < G / 4; c++) code[n][c] = *reinterpret_cast<const u4 *>(at + c * 1024);
                 }
             }
-            __syncthreads();
+            all_read();
+#pragma unroll
+            for (int n = 0; n < R; n++) {
+                const int i = i0 + n * kMoveThreads + tid;
+                const int64_t to = from[n] < 0 ? -1 : tile_number(i >> 5);
+                if (to < 0) continue;
+                const int t = i & 31;
+                uint8_t *at = kv.cache + to * T::kBytes + T::kKeys + T::code(key_half(t) * G, key_row(t) + 16 * part);
+                if constexpr (G == 2) {
+                    *reinterpret_cast<u2 *>(at) = u2{code[n][0].x, code[n][0].y};
+                } else {
+#pragma unroll
+                    for (int c = 0; c < G / 4; c++) *reinterpret_cast<u4 *>(at + c * 1024) = code[n][c];
+                }
+            }
+        } else if (part < 4 + D / 16) {  // a thread makes the dwords of eight tokens and four values: 16 threads a tile
+            constexpr int kRounds = kMoveTokens / 32 * 16 / kMoveThreads;
+            const int set = (part - 4) >> 2, r = ((part - 4) & 3) * 4 + (tid & 3), j = (tid >> 2) & 3;
+            u4 word[kRounds];
+            uint32_t mask[kRounds];
+#pragma unroll
+            for (int n = 0; n < kRounds; n++) {
+                const int i = (n * (kMoveThreads / 16) + (tid >> 4)) * 32 + j * 8;
+                word[n] = u4{0, 0, 0, 0};
+                mask[n] = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int64_t from = source[i + e];
+                    if (from < 0) continue;
+                    const int t = (int)from & 31, down = nibble_shift(t & 7);
+                    const u4 w = *reinterpret_cast<const u4 *>(kv.cache + (from >> 5) * T::kBytes + T::kValues + (set * 64 + r + 16 * (t >> 3)) * 16);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) word[n][c] |= ((w[c] >> down) & 15u) << nibble_shift(e);
+                    mask[n] |= 0xFu << nibble_shift(e);
+                }
+            }
+            all_read();
+#pragma unroll
+            for (int n = 0; n < kRounds; n++) {
+                const int i = i0 + (n * (kMoveThreads / 16) + (tid >> 4)) * 32;
+                const int64_t to = mask[n] ? tile_number(i >> 5) : -1;
+                if (to < 0) continue;
+                u4 *at = reinterpret_cast<u4 *>(kv.cache + to * T::kBytes + T::kValues + (set * 64 + r + 16 * j) * 16);
+                if (mask[n] != 0xFFFFFFFFu) {
+                    const u4 old = *at;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) word[n][c] |= old[c] & ~mask[n];
+                }
+                *at = word[n];
+            }
+        } else {
+            uint16_t ks[R][G], vs[R][G];
+            float account[R];
+            int64_t from[R];
+#pragma unroll
+            for (int n = 0; n < R; n++) {
+                from[n] = source[n * kMoveThreads + tid];
+                if (from[n] < 0) continue;
+                const int t = (int)from[n] & 31;
+                const uint8_t *at = kv.cache + (from[n] >> 5) * T::kBytes;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    ks[n][g] = reinterpret_cast<const uint16_t *>(at + T::kKeyScales)[t * G + g];
+                    vs[n][g] = reinterpret_cast<const uint16_t *>(at + T::kValueScales)[g * 32 + t];
+                }
+                account[n] = accounts[from[n]];  // (pages hold their tokens' accounts in the order of their tiles)
+            }
+            all_read();
+#pragma unroll
+            for (int n = 0; n < R; n++) {
+                const int i = i0 + n * kMoveThreads + tid;
+                const int64_t to = from[n] < 0 ? -1 : tile_number(i >> 5);
+                if (to < 0) continue;
+                const int t = i & 31;
+                uint8_t *at = kv.cache + to * T::kBytes;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    reinterpret_cast<uint16_t *>(at + T::kKeyScales)[t * G + g] = ks[n][g];
+                    reinterpret_cast<uint16_t *>(at + T::kValueScales)[g * 32 + t] = vs[n][g];
+                }
+                accounts[to * 32 + t] = account[n];
+            }
         }
     }
 }
 
-bool pairs_aligned(const HeadRows &h, int n) {
-    const int64_t size = (h.bf16 ? 2 : 4);
-    return ((reinterpret_cast<uintptr_t>(h.p) | (uintptr_t)(h.row * size) | (uintptr_t)(h.head * size)) & (uintptr_t)(n * size - 1)) == 0;
+// eight values with 16-byte loads
+bool wide_rows(const HeadRows &h) {
+    const int64_t size = h.bf16 ? 2 : 4;
+    return ((reinterpret_cast<uintptr_t>(h.p) | (uintptr_t)(h.row * size) | (uintptr_t)(h.head * size)) & 15) == 0;
 }
 
 template <int D> int append(const AppendArgs &a, bool bf16, hipStream_t s) {
@@ -427,8 +553,7 @@ template <int D> int read(const KvCall &kv, uint16_t *k, uint16_t *v, hipStream_
 
 int launch_kv_append(const KvCall &kv, const HeadRows &k, const HeadRows &v, float *accounts, hipStream_t s) {
     AppendArgs a{kv, k, v, accounts, (kv.max_new + 14) / 8, 0};
-    const int ne = kv.head_dim / 64;
-    a.wide = pairs_aligned(k, ne) && pairs_aligned(v, ne);
+    a.wide = wide_rows(k) && wide_rows(v);
     switch (kv.head_dim) {
     case 64: return append<64>(a, k.bf16, s);
     case 128: return append<128>(a, k.bf16, s);
@@ -444,14 +569,20 @@ int launch_kv_read(const KvCall &kv, uint16_t *k, uint16_t *v, hipStream_t s) {
     }
 }
 
+template <int D> static int move_kept(const KvCall &kv, float *accounts, int keep, const int32_t *kept, int32_t *new_lengths, hipStream_t s) {
+    return launch(kv_move_kernel<D>, dim3((unsigned)kv.kv_heads, (unsigned)kv.seqs, 4 + D / 16 + 1), dim3(kMoveThreads), 0, s, kv, accounts, keep, kept, new_lengths);
+}
+
 int launch_kv_evict(const KvCall &kv, float *accounts, int keep, int recent, int32_t *kept, int32_t *new_lengths, hipStream_t s) {
     const dim3 grid((unsigned)kv.kv_heads, (unsigned)kv.seqs);
-    if (int rc = launch(kv_select_kernel, grid, dim3(kSelectThreads), 0, s, kv, accounts, keep, recent, kept)) return rc;
-    const dim3 both((unsigned)kv.kv_heads, (unsigned)kv.seqs, 2);
+    const int64_t n = (int64_t)kv.max_pages * kv.page_tokens - recent;  // tokens to choose from, at most
+    // (32 keys a thread no longer fit the 128 registers of a workgroup of 1024)
+    const auto select = n <= 4 * kSelectThreads ? kv_select_kernel<4> : n <= 16 * kSelectThreads ? kv_select_kernel<16> : kv_select_kernel<0>;
+    if (int rc = launch(select, grid, dim3(kSelectThreads), 0, s, kv, accounts, keep, recent, kept)) return rc;
     switch (kv.head_dim) {
-    case 64: return launch(kv_move_kernel<64>, both, dim3(512), 0, s, kv, accounts, keep, kept, new_lengths);
-    case 128: return launch(kv_move_kernel<128>, both, dim3(512), 0, s, kv, accounts, keep, kept, new_lengths);
-    default: return launch(kv_move_kernel<256>, both, dim3(512), 0, s, kv, accounts, keep, kept, new_lengths);
+    case 64: return move_kept<64>(kv, accounts, keep, kept, new_lengths, s);
+    case 128: return move_kept<128>(kv, accounts, keep, kept, new_lengths, s);
+    default: return move_kept<256>(kv, accounts, keep, kept, new_lengths, s);
     }
 }
 

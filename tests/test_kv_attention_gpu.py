@@ -399,6 +399,52 @@ def test_evict(gpu, dim, page, keep, recent):
             assert np.array_equal(got[:len(want)], np.array([accounts[where[t][0], h, where[t][1]] for t in want], np.float32), equal_nan=True)
 
 
+@pytest.mark.parametrize("length", (4096, 4097, 16500, 40000))
+@pytest.mark.parametrize("kind", ("spread", "few", "same", "zeros", "signs"))
+def test_evict_long_sequences(gpu, length, kind):
+    """The selection alone over lengths that take each of its forms, and accounts that are hard on it."""
+    torch = gpu
+    from gomlx_amd import nn
+    rng = np.random.default_rng(length)
+    accounts = {"spread": np.exp(8 * rng.standard_normal(length)), "few": rng.integers(0, 3, length), "same": np.full(length, 0.7),
+                "zeros": np.where(rng.random(length) < 0.01, rng.random(length), 0), "signs": 1e30 * rng.standard_normal(length)}[kind].astype(np.float32)
+    if kind == "signs":
+        accounts[::50], accounts[1::50], accounts[2::50] = -0.0, np.inf, -np.inf
+    pages = -(-length // 64)
+    cache, table = nn.kv_cache(pages, 1, 64, 64), torch.randperm(pages, device="cuda").int().view(1, -1)
+    w = torch.zeros(pages, 1, 64, device="cuda")
+    padded = np.zeros(pages * 64, np.float32)
+    padded[:length] = accounts
+    w[table[0].long(), 0] = torch.from_numpy(padded).cuda().view(pages, 64)
+    n = torch.tensor([length], dtype=torch.int32, device="cuda")
+    for keep, recent in ((1, 0), (length // 3, 100), (length - 1, 0), (length // 2, length // 2)):
+        kept, _ = nn.kv_cache_evict(cache, w.clone(), table, n, keep, recent)
+        assert kept[0, 0].tolist() == ref.evict(accounts, keep, recent).tolist()
+
+
+def test_every_scale(gpu):
+    """The quotient that codes are rounded from, over every scale that there is and values around every code's border."""
+    torch = gpu
+    from gomlx_amd import nn
+    bits = np.arange(1, 0x7C00, dtype=np.uint16).view(np.float16).astype(np.float32)
+    scales = np.array([d for d in bits if d <= 8160 and ref._bf16(np.float32([d]))[0] == d], np.float32)
+    k = np.zeros((len(scales), 1, 64), np.float32)
+    for i, d in enumerate(scales):
+        border = (np.arange(-8, 8, dtype=np.float64) + 0.5) * d
+        near = np.concatenate([border, np.nextafter(border.astype(np.float32), np.float32(np.inf)), np.nextafter(border.astype(np.float32), np.float32(-np.inf)),
+                               border * (1 + 1e-6 * np.random.default_rng(i).standard_normal(16))]).astype(np.float32)
+        k[i, 0] = np.clip(near, -7.99 * d, 7.99 * d)
+        k[i, 0, [5, 40]] = -8 * d, 8 * d
+    cache = nn.kv_cache(-(-len(scales) // 256), 1, 64, 256)
+    table = torch.arange(cache.shape[0], dtype=torch.int32, device="cuda").view(1, -1)
+    n, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([len(scales)], [0, len(scales)]))
+    d = torch.from_numpy(k).cuda()
+    nn.kv_cache_append(cache, d, -d, table, n, starts=starts, max_new=len(scales))
+    got = nn.kv_cache_read(cache, table, n, starts=starts, max_new=len(scales), rows=len(scales))
+    for x, y in zip(got, ref.quantise(k, -k)):
+        assert np.array_equal(x.double().cpu().numpy(), y)
+
+
 def test_evict_writes_lengths_in_place_and_goes_on(gpu):
     """Serving: append, attend with accounts, evict into the same lengths, go on with the shorter sequences."""
     torch = gpu
@@ -592,6 +638,61 @@ def test_refusals(gpu):
     for bad in (dict(head_dim=80), dict(page_tokens=33), dict(kv_heads=0)):
         with pytest.raises((ValueError, _lib.NotImplementedByBackend)):
             nn.kv_cache(**{**dict(pages=1, kv_heads=1, head_dim=64, page_tokens=32), **bad})
+
+
+def test_native_host_path(gpu, monkeypatch):
+    """The native steps serve the calls of a decode loop, with the Python steps' results; what they do not know they leave alone."""
+    torch = gpu
+    from gomlx_amd import _lib, nn
+    c = Case(torch, [90, 33], 2, 64, 32, seed=1, wide_table=1).fill()
+    n, starts = c.ints([90, 33]), c.ints([0, 4, 6])
+    cos, sin = nn.rotary_table(100, 64)
+    x = torch.randn(2, 10, 64, device="cuda")
+    many = torch.randn(6, 4, 64, device="cuda").bfloat16()
+    gain = nn.RMSNorm(gain=torch.randn(64, device="cuda"), epsilon=1e-5, scale_offset=1.0)
+    fast = _lib.fast
+    assert fast is not None
+
+    def calls():
+        w = torch.zeros(c.pages, 2, 32, device="cuda")
+        cache = c.cache.clone()
+        q, k = nn.qk_norm_rope(x[:, :4], x[:, 4:6], n, cos, sin, gain, nn.RMSNorm(), True, torch.bfloat16)
+        out = [q, k, *nn.qk_norm_rope(x[:, :4], x[:, 4:6], n, cos, sin)]
+        out.append(nn.kv_cache_append(cache, k, x[:, 6:8].bfloat16(), c.d_table, n + 1, weights=w))
+        out.append(nn.kv_cache_append(cache, many[:, :2], many[:, 2:], c.d_table, n, starts=starts, max_new=4))
+        out += [cache.clone(), nn.cached_attention(q, cache, c.d_table, n + 1, weights=w), nn.cached_attention(many, cache, c.d_table, n, starts=starts, max_new=4, scale=0.3, window=9)]
+        out += [*nn.kv_cache_read(cache, c.d_table, n), *nn.kv_cache_read(cache, c.d_table, n, starts, 4, 6), *nn.kv_cache_evict(cache, w, c.d_table, n, 40, 3), w, cache]
+        return out
+
+    native = calls()
+    served = []
+
+    class Spy:
+        def __getattr__(self, name):
+            def call(*args):
+                result = getattr(fast, name)(*args)
+                served.append((name, result is not None))
+                return result
+            return call
+
+    monkeypatch.setattr(_lib, "fast", Spy())
+    spied = calls()
+    assert all(ok for _, ok in served) and {name for name, _ in served} == {"qk_norm_rope", "kv_append", "kv_read", "cached_attention", "kv_evict"}
+    monkeypatch.setattr(_lib, "fast", None)
+    plain = calls()
+    for a, b, d in zip(native, plain, spied):
+        assert (a is None and b is None and d is None) or (torch.equal(a, b) and torch.equal(a, d) and a.dtype == b.dtype and a.stride() == b.stride())
+    w = torch.zeros(c.pages, 2, 32, device="cuda")
+    q = x[:, :4]
+    for f, args in ((fast.cached_attention, (q.half(), c.cache, c.d_table, n, None, 1, None, 0, None)), (fast.cached_attention, (q[:, :3], c.cache, c.d_table, n, None, 1, None, 0, None)),
+                    (fast.cached_attention, (q, c.cache, c.d_table, n, None, 2, None, 0, None)), (fast.cached_attention, (q, c.cache, c.d_table.long(), n, None, 1, None, 0, None)),
+                    (fast.cached_attention, (q, c.cache, c.d_table, n, None, 1, None, -1, None)), (fast.cached_attention, (q, c.cache, c.d_table, n, None, 1, None, 0, w[:1])),
+                    (fast.cached_attention, (q.cpu(), c.cache, c.d_table, n, None, 1, None, 0, None)), (fast.kv_append, (c.cache, q[:, :2], q[:, :2].bfloat16(), c.d_table, n, None, 1, None)),
+                    (fast.kv_append, (c.cache, q[:1, :2], q[:1, :2], c.d_table, n, None, 1, None)), (fast.kv_read, (c.cache, c.d_table, n, starts, 4, None)),
+                    (fast.kv_evict, (c.cache, None, c.d_table, n, 4, 0)), (fast.kv_evict, (c.cache, w, c.d_table, n, 4, 5)),
+                    (fast.qk_norm_rope, (q, q[:1], n, cos, sin, None, None, False, None)), (fast.qk_norm_rope, (q, q, n, cos, sin[:3], None, None, False, None)),
+                    (fast.qk_norm_rope, (q, q, n, cos, sin, None, None, False, torch.float16)), (fast.qk_norm_rope, (q, q, n.long(), cos, sin, None, None, False, None))):
+        assert f(*args) is None
 
 
 def test_empty_calls(gpu):
