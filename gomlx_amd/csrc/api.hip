@@ -1333,9 +1333,11 @@ int gq_kv_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int
     if (!aligned_to(dOut, 16) || !aligned_to(dAccounts, 4)) return fail(GQ_ERR_INVALID, "%s: the output must be 16-byte aligned, accounts 4-byte", fn);
     // (grids are counted in 32 bits, threads included)
     if (call.rows > (INT32_MAX >> 7) / heads || call.max_new > INT32_MAX / 2 / heads) return fail(GQ_ERR_INVALID, "%s: %d rows of %d heads: too many", fn, call.rows, heads);
+    const int room = call.max_pages * call.page_tokens;
+    if ((int64_t)call.seqs * call.kv_heads > INT32_MAX / std::max(1, room / 32))
+        return fail(GQ_ERR_INVALID, "%s: %d sequences of up to %d tokens and %d key heads: more than 2^31 tiles (pass the page table's first columns)", fn, call.seqs, room, call.kv_heads);
     if (int rc = use_device()) return rc;
     CallScope scope;
-    const int room = call.max_pages * call.page_tokens;
     return launch_kv_attention(call, HeadRows{q->dX, q->row_stride, q->head_stride, dtype == GQ_BF16}, heads, scale, window >= room ? 0 : (int)window, dAccounts, dOut,
                                (hipStream_t)stream);
 }

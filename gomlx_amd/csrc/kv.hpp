@@ -37,6 +37,9 @@ __device__ __forceinline__ int key_half(int t) { return (t >> 2) & 1; }
 // What sequence b of a call has: `length` tokens, the last `news` of them new, their rows from `row0` on.
 struct KvSeq { int length, news, row0; };
 
+// A load that is the same for the whole wavefront, through the scalar cache (of what no kernel of this launch writes).
+__device__ __forceinline__ int32_t uniform_load(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
+
 // Lengths beyond the page table and rows beyond the call's are cut off, so that no device value leads a kernel out of its buffers.
 __device__ __forceinline__ KvSeq kv_seq(const KvCall &kv, int b) {
     KvSeq s;

@@ -13,6 +13,7 @@
 // where they lie.  The reference of a row's exponents is set so that its largest weight so far is 2^6, and moves only when a weight
 // would pass 2^14 (below fp16's largest number; small weights stay clear of its denormals): the lanes of the row then agree on a new one.
 #include "kv.hpp"
+#include "lds_dma.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -35,15 +36,20 @@ __device__ __forceinline__ h2 as_h2(uint32_t u) { return __builtin_bit_cast(h2, 
 __device__ __forceinline__ h2 both(float v) { h2 r = {(_Float16)v, (_Float16)v}; return r; }
 __device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) { h8 r = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y}; return r; }
 
-// Eight codes -> c - 8, exact: the nibbles become the low mantissa bits of 1024 (or, four places up, of 1024 + 16 c).
-__device__ __forceinline__ void unpack(uint32_t w, h2 (&v)[4]) {
-    const h2 sixteenth = both(0.0625f), low = both(-1032.0f), high = both(-72.0f);
-    const uint32_t x = w >> 8;
-    v[0] = as_h2((w & 0x000F000Fu) | 0x64006400u) + low;
-    v[1] = __builtin_elementwise_fma(as_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, high);
-    v[2] = as_h2((x & 0x000F000Fu) | 0x64006400u) + low;
-    v[3] = __builtin_elementwise_fma(as_h2((x & 0x00F000F0u) | 0x64006400u), sixteenth, high);
-}
+// Eight codes -> c - 8, exact: the nibbles become the low mantissa bits of 1024 (or, four places up, of 1024 + 16 c).  The constants
+// are kept out of the compiler's sight in registers, for an instruction that masks and sets in one takes no literals.
+struct Unpack {
+    uint32_t low = 0x000F000Fu, high = 0x00F000F0u, base = 0x64006400u;
+    __device__ __forceinline__ Unpack() { asm("" : "+s"(low), "+s"(high), "+v"(base)); }
+    __device__ __forceinline__ void operator()(uint32_t w, h2 (&v)[4]) const {
+        const h2 sixteenth = both(0.0625f), less = both(-1032.0f), less16 = both(-72.0f);
+        const uint32_t x = w >> 8;
+        v[0] = as_h2((w & low) | base) + less;
+        v[1] = __builtin_elementwise_fma(as_h2((w & high) | base), sixteenth, less16);
+        v[2] = as_h2((x & low) | base) + less;
+        v[3] = __builtin_elementwise_fma(as_h2((x & high) | base), sixteenth, less16);
+    }
+};
 
 struct AttendArgs {
     KvCall kv;
@@ -53,8 +59,11 @@ struct AttendArgs {
     void *out;               // [rows, heads, D]
     float *lse;              // [rows, heads], in powers of two; null where nobody asks
     float *part, *part_ml;   // chunks > 1: sums [rows * heads, chunks, D], (reference, sum) [rows * heads, chunks, 2]
-    int chunks;
+    int chunks, workgroups, rows;  // (rows: of a unit, at most)
+    int2 *pieces;            // per unit of kv_split_kernel: the first workgroup that works on it, and how many do
     float *accounts;
+    float *scores;           // of kv_split_kernel, in powers of two: [units, rows, score_tiles * 32] from the first tile that a unit sees; null: not kept
+    int score_tiles;
 };
 
 // The tiles that the rows of a row tile (sixteen neighbouring (new token, head of the group) pairs) see, and where its chunk of them lies.
@@ -154,7 +163,7 @@ template <int D> struct KeyWords {
         }
     }
     // operand of the sixteen tokens u for group g
-    __device__ __forceinline__ h8 operand(int u, int g) const {
+    __device__ __forceinline__ h8 operand(const Unpack &unpack, int u, int g) const {
         const int w = u * (D / 32) + g;
         h2 v[4];
         unpack(code[w >> 2][w & 3], v);
@@ -174,7 +183,7 @@ template <int D> struct ValueWords {
         for (int g = 0; g < D / 32; g++) scale[g] = *reinterpret_cast<const u4 *>(tile + KvTile<D>::kValueScales + g * 64 + j * 16);
     }
     // operand of the sixteen values 16 w ..
-    __device__ __forceinline__ h8 operand(int w) const {
+    __device__ __forceinline__ h8 operand(const Unpack &unpack, int w) const {
         h2 v[4];
         unpack(code[w >> 2][w & 3], v);
         const u4 d = scale[w >> 1];
@@ -186,13 +195,13 @@ __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_m
 
 // The scores of a tile's 32 tokens for sixteen rows: lane (r, j) gets those of the tokens 8 j + 0..7 for row r.
 template <int D, bool TWO>
-__device__ __forceinline__ void tile_scores(const KeyWords<D> &k, const h8 (&hi)[D / 32], const h8 (&lo)[TWO ? D / 32 : 1], float (&s)[8]) {
+__device__ __forceinline__ void tile_scores(const Unpack &unpack, const KeyWords<D> &k, const h8 (&hi)[D / 32], const h8 (&lo)[TWO ? D / 32 : 1], float (&s)[8]) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
         f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int g = 0; g < D / 32; g++) {
-            const h8 a = k.operand(u, g);
+            const h8 a = k.operand(unpack, u, g);
             acc = mfma(a, hi[g], acc);
             if constexpr (TWO) acc = mfma(a, lo[g], acc);
         }
@@ -203,10 +212,336 @@ __device__ __forceinline__ void tile_scores(const KeyWords<D> &k, const h8 (&hi)
 
 constexpr int kSplitWaves = 4;
 
+// The addresses of every `step`-th tile of a sequence and key head.
+struct TileWalk {
+    const uint8_t *cache;
+    const int32_t *table;
+    int per_page, slot, in, step, pages, heads, head, bytes;
+    __device__ __forceinline__ TileWalk(const KvCall &kv, int b, int h, int tile, int step_, int bytes_)
+        : cache(kv.cache), table(kv.table + b * kv.table_stride), per_page(kv.page_tokens >> 5), step(step_), pages(kv.pages), heads(kv.kv_heads), head(h), bytes(bytes_) {
+        slot = tile / per_page;
+        in = tile - slot * per_page;
+    }
+    __device__ __forceinline__ const uint8_t *next(bool is) {  // null where there is no tile, or none in the cache
+        const uint8_t *at = nullptr;
+        if (is) {
+            const int page = uniform_load(table + slot);
+            if ((uint32_t)page < (uint32_t)pages) at = cache + (((int64_t)page * heads + head) * per_page + in) * bytes;
+            in += step;
+            while (in >= per_page) { in -= per_page; slot++; }
+        }
+        return at;
+    }
+};
+
+// How the tiles of a call are shared out over its workgroups.  A unit is a sequence and key head (all rows of it: sixteen at most),
+// with the tiles that its rows see (one at least, so that rows that see nothing are written too).  Units are cut into pieces
+// of one length, of which all units together have about a.workgroups, one piece a workgroup: the lengths are known on the device only, so
+// every wavefront finds its place by a sum over them, 64 sequences at a time, one a lane.  (All tiles together: less than 2^31.)
+struct Piece {
+    int b, h, nth;       // sequence, key head, number of the piece in its unit; b < 0: there is none
+    int share, tiles;    // tiles of a piece, of the unit
+    KvSeq seq;
+    Span span;
+    __device__ __forceinline__ int pieces() const { return (tiles + share - 1) / share; }
+};
+__device__ __forceinline__ Span span_of(const AttendArgs &a, const KvSeq &seq) { return row_tile_span(seq, a.group, a.window, 0, 16); }
+__device__ __forceinline__ int tiles_of(const Span &span) { return span.rows ? max(1, ((span.hi + 31) >> 5) - (span.lo >> 5)) : 0; }
+
+// Sums over the lanes up to and with each, by data-parallel moves: 1, 2, 4, 8 lanes within rows of sixteen, then from the last lane of a
+// row into the next one, and of the first half into the second.
+__device__ __forceinline__ int lane_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
+__device__ __forceinline__ Piece piece_of(const AttendArgs &a, int index) {
+    const int lane = (int)threadIdx.x & 63, seqs = a.kv.seqs, heads = a.kv.kv_heads;
+    Piece p;
+    p.b = -1;
+    KvSeq mine{0, 0, 0};
+    int tiles = 0, total = 0;
+    for (int base = (seqs - 1) & ~63; base >= 0; base -= 64) {  // (the first 64 last: they stay)
+        mine = KvSeq{0, 0, 0};
+        if (base + lane < seqs) mine = kv_seq(a.kv, base + lane);
+        tiles = tiles_of(span_of(a, mine));
+        total += __builtin_amdgcn_readlane(lane_scan(tiles), 63) * heads;
+    }
+    // (a multiple of the wavefronts: each of them the same number of tiles)
+    const int least = (total + a.workgroups - 1) / a.workgroups;
+    p.share = max(1, (least + kSplitWaves - 1) / kSplitWaves) * kSplitWaves;
+    int front = 0;  // pieces in front
+    for (int base = 0; base < seqs; base += 64) {
+        if (base) {
+            mine = KvSeq{0, 0, 0};
+            if (base + lane < seqs) mine = kv_seq(a.kv, base + lane);
+            tiles = tiles_of(span_of(a, mine));
+        }
+        const int unit = (tiles + p.share - 1) / p.share;
+        const int upto = lane_scan(unit * heads);
+        const uint64_t past = __ballot(front + upto > index);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            p.b = base + l;
+            p.seq = KvSeq{__builtin_amdgcn_readlane(mine.length, l), __builtin_amdgcn_readlane(mine.news, l), __builtin_amdgcn_readlane(mine.row0, l)};
+            p.span = span_of(a, p.seq);
+            p.tiles = __builtin_amdgcn_readlane(tiles, l);
+            const int each = __builtin_amdgcn_readlane(unit, l), in = index - (front + __builtin_amdgcn_readlane(upto, l) - each * heads);
+            p.h = in / each;
+            p.nth = in - p.h * each;
+            break;
+        }
+        front += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return p;
+}
+
+template <bool BF16> __device__ __forceinline__ void store_result(void *out, int64_t at, f4 sum, float all) {
+    sum *= all == 0.0f ? 0.0f : 1.0f / all;  // (a row that has seen nothing)
+    if (all != all) sum = f4{all, all, all, all};
+    if constexpr (BF16) {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        const bf16x4 y = {(__bf16)sum.x, (__bf16)sum.y, (__bf16)sum.z, (__bf16)sum.w};
+        *reinterpret_cast<bf16x4 *>(static_cast<uint16_t *>(out) + at) = y;
+    } else {
+        *reinterpret_cast<f4 *>(static_cast<float *>(out) + at) = sum;
+    }
+}
+__device__ __forceinline__ float lse_of(float top, float all) { return all == 0.0f ? kNegInf : top + __builtin_amdgcn_logf(all); }
+
+constexpr int kSplitSlots = 2, kMostWorkgroups = 2048;
+
+template <int D> struct SplitLds {
+    static constexpr int kLoads = (KvTile<D>::kBytes + 1023) / 1024, kSlot = kLoads * 1024;  // DMA instructions of a tile
+    static constexpr int kSums = kSplitWaves * 16 * (D + 4) * 4, kJoin = kSums + 2 * kSplitWaves * 16 * 4;
+    static constexpr int kRing = kSplitWaves * kSplitSlots * kSlot, kBytes = kRing > kJoin ? kRing : kJoin;
+};
+
+// A tile to LDS, past the registers.  (The wait: nothing is read any more from where it goes; the s_nop: a vector instruction may have
+// written the descriptor's scalar registers just before.)
+template <int D> __device__ __forceinline__ void fetch_tile(uint32_t lds_at, const uint8_t *tile) {
+    const i32x4 rsrc = make_rsrc(tile, KvTile<D>::kBytes);  // (what the last instruction asks for behind the tile's end is not read)
+    const uint32_t lane = ((uint32_t)threadIdx.x & 63u) * 16u;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_nop 4" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < SplitLds<D>::kLoads; i++)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_at + (uint32_t)i * 1024u), "v"(lane), "s"(rsrc), "s"((uint32_t)i * 1024u) : "memory");
+}
+
+// A piece of a unit: up to sixteen rows, (new token, head) pairs, over `share` tiles.  Each wavefront takes every fourth tile, with a
+// maximum, sums and results of its own, and they meet in LDS.  A unit of one piece is finished here; the others leave their sums, by
+// workgroup, for kv_join_kernel.
+template <int D, bool BF16>
+__global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void kv_split_kernel(const AttendArgs a) {
+    constexpr bool TWO = !BF16;
+    constexpr int W = D / 16;
+    typedef SplitLds<D> Lds;
+    __shared__ __align__(16) uint8_t lds[Lds::kBytes];
+    // (the results take the place of the tiles once all of these are done with)
+    float(*sums)[16][D + 4] = reinterpret_cast<float(*)[16][D + 4]>(lds);
+    float(*refs)[16] = reinterpret_cast<float(*)[16]>(lds + Lds::kSums), (*totals)[16] = reinterpret_cast<float(*)[16]>(lds + Lds::kSums + kSplitWaves * 64);
+    const KvCall &kv = a.kv;
+    const int lane = (int)threadIdx.x & 63, r = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const Piece piece = piece_of(a, (int)blockIdx.x);
+    if (piece.b < 0) return;
+    const int b = piece.b, h = piece.h;
+    const KvSeq &seq = piece.seq;
+    const Span &span = piece.span;
+    const int tile0 = (span.lo >> 5) + piece.nth * piece.share, tile1 = (span.lo >> 5) + min((piece.nth + 1) * piece.share, piece.tiles);
+    const Unpack unpack;
+    {
+        const bool live = r < span.rows;
+        const int nth = live ? r / a.group : 0;              // new token of the row
+        const int head = h * a.group + (live ? r - nth * a.group : 0);
+        const int64_t row = seq.row0 + nth;
+        const int base = seq.length - seq.news, place = base + nth;  // its own token
+        const int see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
+        // tokens that every row sees (the operand rows that stand for none have scores of 0 and go nowhere)
+        const int all_hi = base + 1, all_lo = a.window ? base + (span.rows - 1) / a.group + 1 - a.window : 0;
+
+        f4 o[W];
+#pragma unroll
+        for (int w = 0; w < W; w++) o[w] = f4{0.f, 0.f, 0.f, 0.f};
+        float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
+
+        const int last = min(tile1, (span.hi + 31) >> 5);  // (a unit that sees nothing has a tile in name only)
+        TileWalk walk(kv, b, h, tile0 + wave, kSplitWaves, KvTile<D>::kBytes);
+        // the wavefront's ring of tiles: one is worked on while the next is on its way
+        uint8_t *ring = lds + wave * kSplitSlots * Lds::kSlot;
+        const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)ring);
+        const uint8_t *mem = walk.next(tile0 + wave < last);
+        if (mem) fetch_tile<D>(ring_at, mem);
+        h8 qh[D / 32], ql[TWO ? D / 32 : 1];
+        float back;
+        load_queries<D, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
+        const float to_log2 = back * a.scale_log2;
+        int turn = 0;
+        for (int tile = tile0 + wave; tile < last; tile += kSplitWaves) {
+            const uint8_t *mem_next = walk.next(tile + kSplitWaves < last);
+            if (mem_next) {
+                fetch_tile<D>(ring_at + (uint32_t)(turn ^ 1) * Lds::kSlot, mem_next);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Lds::kLoads) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            if (mem) {
+                KeyWords<D> k;
+                k.load(ring + turn * Lds::kSlot);
+                float s[8];
+                tile_scores<D, TWO>(unpack, k, qh, ql, s);
+                const int t0 = tile * 32;
+                float most = kNegInf;
+                if (t0 >= all_lo && t0 + 32 <= all_hi) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        s[e] *= to_log2;
+                        most = fmaxf(most, s[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int t = t0 + 8 * j + e;
+                        s[e] = t < see_hi && t >= see_lo ? s[e] * to_log2 : kNegInf;
+                        most = fmaxf(most, s[e]);
+                    }
+                }
+                if (a.scores && live) {
+                    float *to = a.scores + ((int64_t)(b * kv.kv_heads + h) * a.rows + r) * a.score_tiles * 32 + (t0 + 8 * j - (span.lo & ~31));
+                    *reinterpret_cast<f4 *>(to) = f4{s[0], s[1], s[2], s[3]};
+                    *reinterpret_cast<f4 *>(to + 4) = f4{s[4], s[5], s[6], s[7]};
+                }
+                if (__any(most > ref + kMostLog2)) {  // (the first score of a row among them: its reference is -infinity)
+                    most = fmaxf(most, __shfl_xor(most, 16));
+                    most = fmaxf(most, __shfl_xor(most, 32));
+                    const float next = fmaxf(ref, most - kHeadroom);
+                    const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
+                    ref = next;
+                    total *= shrink;
+#pragma unroll
+                    for (int w = 0; w < W; w++) o[w] *= shrink;
+                }
+                const float less = ref == kNegInf ? 0.0f : ref;
+                h8 ph, pl;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float p = __builtin_amdgcn_exp2f(s[e] - less);
+                    total += p;
+                    ph[e] = (_Float16)p;
+                    if constexpr (TWO) pl[e] = (_Float16)(p - (float)ph[e]);
+                }
+                ValueWords<D> v;
+                v.load(ring + turn * Lds::kSlot);
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    const h8 x = v.operand(unpack, w);
+                    o[w] = mfma(x, ph, o[w]);
+                    if constexpr (TWO) o[w] = mfma(x, pl, o[w]);
+                }
+            }
+            mem = mem_next;
+            turn ^= 1;
+        }
+        __syncthreads();
+        total += __shfl_xor(total, 16);
+        total += __shfl_xor(total, 32);
+#pragma unroll
+        for (int w = 0; w < W; w++) *reinterpret_cast<f4 *>(&sums[wave][r][16 * w + 4 * j]) = o[w];
+        if (j == 0) {
+            refs[wave][r] = ref;
+            totals[wave][r] = total;
+        }
+        __syncthreads();
+
+        const int pieces = piece.pieces();
+        if (a.pieces && piece.nth == 0 && threadIdx.x == 0) a.pieces[b * kv.kv_heads + h] = make_int2((int)blockIdx.x, pieces);
+        for (int i = (int)threadIdx.x; i < span.rows * (D / 4); i += 64 * kSplitWaves) {
+            const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4;
+            float top = kNegInf;
+#pragma unroll
+            for (int w = 0; w < kSplitWaves; w++) top = fmaxf(top, refs[w][rr]);
+            f4 sum = {0.f, 0.f, 0.f, 0.f};
+            float all = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kSplitWaves; w++) {
+                const float f = refs[w][rr] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(refs[w][rr] - top);
+                // (a wavefront without a reference has seen no number: its sum is zero, or NaN)
+                all += refs[w][rr] == kNegInf ? totals[w][rr] : totals[w][rr] * f;
+                sum += *reinterpret_cast<const f4 *>(&sums[w][rr][d]) * f;
+            }
+            if (pieces == 1) {
+                const int n = rr / a.group;
+                const int64_t out = (int64_t)(seq.row0 + n) * a.heads + h * a.group + (rr - n * a.group);
+                store_result<BF16>(a.out, out * D + d, sum, all);
+                if (a.lse && d == 0) a.lse[out] = lse_of(top, all);
+            } else {
+                *reinterpret_cast<f4 *>(a.part + ((int64_t)blockIdx.x * a.rows + rr) * D + d) = sum;
+                if (d == 0) {
+                    a.part_ml[((int64_t)blockIdx.x * a.rows + rr) * 2] = top;
+                    a.part_ml[((int64_t)blockIdx.x * a.rows + rr) * 2 + 1] = all;
+                }
+            }
+        }
+    }
+}
+
+
+// Joins the pieces of the units that more than one workgroup has worked on: one workgroup per unit and row.
+template <int D, bool BF16>
+__global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
+    constexpr int L = D / 4, S = 256 / L;  // lanes of a row's values, and the shares into which the pieces are divided
+    __shared__ f4 sums[S][L];
+    __shared__ float factors[kMostWorkgroups], tops[4], alls[4];
+    const int rr = (int)blockIdx.x, h = (int)blockIdx.y, b = (int)blockIdx.z, tid = (int)threadIdx.x;
+    const int2 piece = a.pieces[b * a.kv.kv_heads + h];
+    const KvSeq seq = kv_seq(a.kv, b);
+    if (rr >= span_of(a, seq).rows) return;  // (without rows nobody has written the unit's pieces)
+    const int first = piece.x, pieces = piece.y;
+    if (pieces == 1) return;
+    const auto line = [&](int i) { return (int64_t)(first + i) * a.rows + rr; };
+    float top = kNegInf;
+    for (int i = tid; i < pieces; i += 256) top = fmaxf(top, a.part_ml[line(i) * 2]);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    float all = 0.0f;
+    for (int i = tid; i < pieces; i += 256) {
+        const float ref = a.part_ml[line(i) * 2], t = a.part_ml[line(i) * 2 + 1];
+        const float f = ref == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
+        factors[i] = f;
+        all += ref == kNegInf ? t : t * f;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) all += __shfl_xor(all, m);
+    if ((tid & 63) == 0) alls[tid >> 6] = all;
+    __syncthreads();
+    all = (alls[0] + alls[1]) + (alls[2] + alls[3]);
+    const int l = tid % L, part = tid / L;
+    f4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = part; i < pieces; i += S) sum += *reinterpret_cast<const f4 *>(a.part + line(i) * D + l * 4) * factors[i];
+    sums[part][l] = sum;
+    __syncthreads();
+    if (part) return;
+    sum = sums[0][l];
+    for (int i = 1; i < S; i++) sum += sums[i][l];
+    const int n = rr / a.group;
+    const int64_t out = (int64_t)(seq.row0 + n) * a.heads + h * a.group + (rr - n * a.group);
+    store_result<BF16>(a.out, out * D + l * 4, sum, all);
+    if (a.lse && l == 0) a.lse[out] = lse_of(top, all);
+}
+
 // Sixteen rows of one key head over one chunk of the tokens that they see.  Each wavefront takes every fourth tile with a
 // maximum, sums and results of its own; they meet in LDS at the end.
 template <int D, bool BF16>
-__global__ __launch_bounds__(64 * kSplitWaves) void kv_split_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 1 : 2) void kv_rows_kernel(const AttendArgs a) {
     constexpr bool TWO = !BF16;
     constexpr int W = D / 16;
     __shared__ float sums[kSplitWaves][16][D + 4];
@@ -245,56 +580,69 @@ __global__ __launch_bounds__(64 * kSplitWaves) void kv_split_kernel(const Attend
     for (int w = 0; w < W; w++) o[w] = f4{0.f, 0.f, 0.f, 0.f};
     float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
 
-    for (int tile = tile0 + wave; tile < tile1; tile += kSplitWaves) {
-        const uint8_t *at = kv_tile(kv, b, h, tile, KvTile<D>::kBytes);
-        if (!at) continue;
-        KeyWords<D> k;
-        ValueWords<D> v;
+    const Unpack unpack;
+    TileWalk walk(kv, b, h, tile0 + wave, kSplitWaves, KvTile<D>::kBytes);
+    KeyWords<D> k, k_next;
+    ValueWords<D> v, v_next;
+    const uint8_t *at = walk.next(tile0 + wave < tile1);
+    if (at) {
         k.load(at);
         v.load(at);
-        float s[8];
-        tile_scores<D, TWO>(k, qh, ql, s);
-        const int t0 = tile * 32;
-        float most = kNegInf;
-        if (full_rows && t0 >= all_lo && t0 + 32 <= all_hi) {
+    }
+    for (int tile = tile0 + wave; tile < tile1; tile += kSplitWaves) {
+        const uint8_t *at_next = walk.next(tile + kSplitWaves < tile1);
+        if (at_next) {  // the next tile is on its way while this one is worked on
+            k_next.load(at_next);
+            v_next.load(at_next);
+        }
+        if (at) {
+            float s[8];
+            tile_scores<D, TWO>(unpack, k, qh, ql, s);
+            const int t0 = tile * 32;
+            float most = kNegInf;
+            if (full_rows && t0 >= all_lo && t0 + 32 <= all_hi) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    s[e] *= to_log2;
+                    most = fmaxf(most, s[e]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int t = t0 + 8 * j + e;
+                    s[e] = t < see_hi && t >= see_lo ? s[e] * to_log2 : kNegInf;
+                    most = fmaxf(most, s[e]);
+                }
+            }
+            if (__any(most > ref + kMostLog2)) {  // (the first score of a row among them: its reference is -infinity)
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                const float next = fmaxf(ref, most - kHeadroom);
+                const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
+                ref = next;
+                total *= shrink;
+#pragma unroll
+                for (int w = 0; w < W; w++) o[w] *= shrink;
+            }
+            const float from = ref == kNegInf ? 0.0f : ref;
+            h8 ph, pl;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                s[e] *= to_log2;
-                most = fmaxf(most, s[e]);
+                const float p = __builtin_amdgcn_exp2f(s[e] - from);
+                total += p;
+                ph[e] = (_Float16)p;
+                if constexpr (TWO) pl[e] = (_Float16)(p - (float)ph[e]);
             }
-        } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int t = t0 + 8 * j + e;
-                s[e] = t < see_hi && t >= see_lo ? s[e] * to_log2 : kNegInf;
-                most = fmaxf(most, s[e]);
+            for (int w = 0; w < W; w++) {
+                const h8 x = v.operand(unpack, w);
+                o[w] = mfma(x, ph, o[w]);
+                if constexpr (TWO) o[w] = mfma(x, pl, o[w]);
             }
         }
-        if (__any(most > ref + kMostLog2)) {  // (the first score of a row among them: its reference is -infinity)
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            const float next = fmaxf(ref, most - kHeadroom);
-            const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
-            ref = next;
-            total *= shrink;
-#pragma unroll
-            for (int w = 0; w < W; w++) o[w] *= shrink;
-        }
-        const float from = ref == kNegInf ? 0.0f : ref;
-        h8 ph, pl;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float p = __builtin_amdgcn_exp2f(s[e] - from);
-            total += p;
-            ph[e] = (_Float16)p;
-            if constexpr (TWO) pl[e] = (_Float16)(p - (float)ph[e]);
-        }
-#pragma unroll
-        for (int w = 0; w < W; w++) {
-            const h8 x = v.operand(w);
-            o[w] = mfma(x, ph, o[w]);
-            if constexpr (TWO) o[w] = mfma(x, pl, o[w]);
-        }
+        at = at_next;
+        k = k_next;
+        v = v_next;
     }
     total += __shfl_xor(total, 16);
     total += __shfl_xor(total, 32);
@@ -346,7 +694,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void kv_split_kernel(const Attend
 
 // Joins the chunks of a row: one workgroup per row and head.
 template <int D, bool BF16>
-__global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(256) void kv_rows_join_kernel(const AttendArgs a) {
     constexpr int L = D / 4, S = 256 / L;  // lanes of a row's values, and the shares into which the chunks are divided
     __shared__ f4 sums[S][L];
     __shared__ float refs[S], totals[S];
@@ -408,6 +756,32 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
     if (a.lse && l == 0) a.lse[to] = all == 0.0f ? kNegInf : top + __builtin_amdgcn_logf(all);
 }
 
+// The accounts from the scores that kv_split_kernel has kept: one thread a token, which adds up the unit's rows.
+__global__ __launch_bounds__(256) void kv_score_account_kernel(const AttendArgs a) {
+    __shared__ float lse[16];
+    const KvCall &kv = a.kv;
+    const int h = (int)blockIdx.y, b = (int)blockIdx.z, tid = (int)threadIdx.x;
+    const KvSeq seq = kv_seq(kv, b);
+    const Span span = span_of(a, seq);
+    const int first = span.lo & ~31, t = first + (int)blockIdx.x * 256 + tid;
+    if (span.rows == 0 || first + (int)blockIdx.x * 256 >= span.hi) return;
+    if (tid < span.rows) {
+        const int n = tid / a.group;
+        lse[tid] = a.lse[(int64_t)(seq.row0 + n) * a.heads + h * a.group + (tid - n * a.group)];
+    }
+    __syncthreads();
+    if (t < span.lo || t >= span.hi) return;
+    float *to = kv_account(kv, a.accounts, b, h, t);
+    if (!to) return;
+    const float *s = a.scores + (int64_t)(b * kv.kv_heads + h) * a.rows * a.score_tiles * 32 + (t - first);
+    float sum = 0.0f;
+    for (int r = 0; r < span.rows; r++) {
+        const float v = s[(int64_t)r * a.score_tiles * 32];
+        sum += v == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(v - lse[r]);  // (a token that the row does not see)
+    }
+    *to += sum;
+}
+
 // The accounts: a wavefront owns a tile of a sequence and key head and goes over all rows that see it, so that every account is
 // added to once, in one order.
 template <int D, bool BF16>
@@ -427,6 +801,7 @@ __global__ __launch_bounds__(256) void kv_account_kernel(const AttendArgs a) {
     const int lane = (int)threadIdx.x & 63, r = lane & 15, j = lane >> 4, t0 = tile * 32;
     // the new tokens that see one of the tile's
     const int n0 = max(0, t0 - base), n1 = a.window ? min(seq.news, t0 + 31 + a.window - base) : seq.news;
+    const Unpack unpack;
     float sum[8] = {};
     for (int i0 = n0 * a.group; i0 < n1 * a.group; i0 += 16) {
         const int idx = i0 + r;
@@ -438,7 +813,7 @@ __global__ __launch_bounds__(256) void kv_account_kernel(const AttendArgs a) {
         float back, s[8];
         load_queries<D, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
         const float lse = live ? a.lse[row * a.heads + head] : 0.0f;
-        tile_scores<D, TWO>(k, qh, ql, s);
+        tile_scores<D, TWO>(unpack, k, qh, ql, s);
         const float to_log2 = back * a.scale_log2;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -458,13 +833,30 @@ __global__ __launch_bounds__(256) void kv_account_kernel(const AttendArgs a) {
     }
 }
 
+// Scores that are kept for the accounts, at most; beyond, the keys are read a second time (16 sequences of up to 4096 tokens, 8 heads of 4
+// queries: 4 us from 10 MB of scores, 34 us from the keys).
+constexpr size_t kMostScoreBytes = (size_t)256 << 20;
+
+// Pieces that all units together are cut into.  Per CU at D = 64 / 128 / 256: four, three, two, as many as run there at a time by LDS or one
+// fewer.  (us a call at 1, 2, 3, 4, 6 a CU, D = 128: 32 sequences of up to 8192 tokens 65 55 52 53 50, one of 131072 39 38 39 39 42,
+// one of 16384 14 15 15 17 17; D = 64, 16 of up to 8192 28 22 20 19 20; D = 256, 8 of up to 8192 38 30 36 36 42.)
+int split_workgroups(int D) { return std::min(kMostWorkgroups, device_cu_count() * (D == 256 ? 2 : D == 128 ? 3 : 4)); }
+
 template <int D, bool BF16> int attend(const AttendArgs &a, int max_tiles, hipStream_t s) {
     const KvCall &kv = a.kv;
-    const dim3 grid((unsigned)(a.chunks * a.row_tiles), (unsigned)kv.kv_heads, (unsigned)kv.seqs);
-    if (int rc = launch(kv_split_kernel<D, BF16>, grid, dim3(64 * kSplitWaves), 0, s, a)) return rc;
-    if (a.chunks > 1)
-        if (int rc = launch(kv_join_kernel<D, BF16>, dim3((unsigned)((int64_t)kv.rows * a.heads)), dim3(256), 0, s, a)) return rc;
+    if (a.workgroups) {
+        const int grid = a.workgroups + kv.seqs * kv.kv_heads;  // (a unit's last piece may be short)
+        if (int rc = launch(kv_split_kernel<D, BF16>, dim3((unsigned)grid), dim3(64 * kSplitWaves), 0, s, a)) return rc;
+        if (a.part)
+            if (int rc = launch(kv_join_kernel<D, BF16>, dim3((unsigned)(kv.max_new * a.group), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a)) return rc;
+    } else {
+        const dim3 grid((unsigned)(a.chunks * a.row_tiles), (unsigned)kv.kv_heads, (unsigned)kv.seqs);
+        if (int rc = launch(kv_rows_kernel<D, BF16>, grid, dim3(64 * kSplitWaves), 0, s, a)) return rc;
+        if (a.chunks > 1)
+            if (int rc = launch(kv_rows_join_kernel<D, BF16>, dim3((unsigned)((int64_t)kv.rows * a.heads)), dim3(256), 0, s, a)) return rc;
+    }
     if (!a.accounts) return GQ_OK;
+    if (a.scores) return launch(kv_score_account_kernel, dim3((unsigned)((a.score_tiles + 7) / 8), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
     return launch(kv_account_kernel<D, BF16>, dim3((unsigned)((max_tiles + 3) / 4), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
 }
 
@@ -482,27 +874,45 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
     a.accounts = accounts;
     const int64_t size = q.bf16 ? 2 : 4;
     a.wide = ((reinterpret_cast<uintptr_t>(q.p) | (uintptr_t)(q.row * size) | (uintptr_t)(q.head * size)) & 15) == 0;
+    a.rows = kv.max_new * a.group;
     a.row_tiles = (int)(((int64_t)kv.max_new * a.group + 15) / 16);
     // tiles that a row tile's chunks have to cover, and those that see any of the new tokens
     const int64_t room = (int64_t)kv.max_pages * kv.page_tokens / 32;
     const int span_new = 15 / a.group + 1;  // new tokens of a row tile, less one
     const int64_t tiles = std::max<int64_t>(1, window ? std::min<int64_t>(room, ((int64_t)window + span_new + 31) / 32 + 1) : room);
     const int64_t max_tiles = std::max<int64_t>(1, window ? std::min<int64_t>(room, ((int64_t)window + kv.max_new + 31) / 32 + 1) : room);
-    const int64_t units = (int64_t)kv.seqs * kv.kv_heads * a.row_tiles;
-    // about 1024 workgroups, each with a tile per wavefront at least
-    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((1024 + units - 1) / units, (tiles + kSplitWaves - 1) / kSplitWaves));
-    a.chunk_tiles = (int)((tiles + chunks - 1) / chunks + kSplitWaves - 1) / kSplitWaves * kSplitWaves;
-    a.chunks = (int)((tiles + a.chunk_tiles - 1) / a.chunk_tiles);
     const size_t line = (size_t)kv.rows * heads;
-    const size_t lse_bytes = accounts ? (line * 4 + 255) / 256 * 256 : 0, ml_bytes = a.chunks > 1 ? (line * a.chunks * 8 + 255) / 256 * 256 : 0;
-    const size_t part_bytes = a.chunks > 1 ? line * a.chunks * (size_t)kv.head_dim * 4 : 0;
+    size_t lines = 0;  // of sums that are joined
+    if (a.row_tiles == 1) {
+        const int64_t all = (int64_t)kv.seqs * kv.kv_heads * tiles;
+        a.workgroups = (int)std::min<int64_t>(split_workgroups(kv.head_dim), (all + kSplitWaves - 1) / kSplitWaves);
+        if (tiles > kSplitWaves) lines = (size_t)(a.workgroups + kv.seqs * kv.kv_heads) * a.rows;
+    } else {
+        const int64_t units = (int64_t)kv.seqs * kv.kv_heads * a.row_tiles;
+        // about 1024 workgroups, each with a tile per wavefront at least
+        const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((1024 + units - 1) / units, (tiles + kSplitWaves - 1) / kSplitWaves));
+        a.chunk_tiles = (int)((tiles + chunks - 1) / chunks + kSplitWaves - 1) / kSplitWaves * kSplitWaves;
+        a.chunks = (int)((tiles + a.chunk_tiles - 1) / a.chunk_tiles);
+        if (a.chunks > 1) lines = line * a.chunks;
+    }
+    const size_t lse_bytes = accounts ? (line * 4 + 255) / 256 * 256 : 0, ml_bytes = (lines * 8 + 255) / 256 * 256;
+    const size_t score_bytes = a.workgroups && accounts ? (size_t)kv.seqs * kv.kv_heads * a.rows * tiles * 128 : 0;
+    const bool keep_scores = score_bytes > 0 && score_bytes <= kMostScoreBytes;
+    const size_t part_bytes = lines * (size_t)kv.head_dim * 4, piece_bytes = lines && a.workgroups ? (size_t)kv.seqs * kv.kv_heads * 8 : 0;
     if (lse_bytes + ml_bytes + part_bytes) {
         void *ws = nullptr;
-        if (int rc = stream_workspace(s, lse_bytes + ml_bytes + part_bytes, &ws)) return rc;
+        if (int rc = stream_workspace(s, lse_bytes + ml_bytes + part_bytes + (piece_bytes + 255) / 256 * 256 + (keep_scores ? score_bytes : 0), &ws)) return rc;
         unsigned char *p = static_cast<unsigned char *>(ws);
+        if (keep_scores) {
+            a.scores = reinterpret_cast<float *>(p + lse_bytes + ml_bytes + part_bytes + (piece_bytes + 255) / 256 * 256);
+            a.score_tiles = (int)tiles;
+        }
         if (lse_bytes) a.lse = reinterpret_cast<float *>(p);
-        a.part_ml = reinterpret_cast<float *>(p + lse_bytes);
-        a.part = reinterpret_cast<float *>(p + lse_bytes + ml_bytes);
+        if (lines) {
+            a.part_ml = reinterpret_cast<float *>(p + lse_bytes);
+            a.part = reinterpret_cast<float *>(p + lse_bytes + ml_bytes);
+            if (piece_bytes) a.pieces = reinterpret_cast<int2 *>(p + lse_bytes + ml_bytes + part_bytes);
+        }
     }
     switch (kv.head_dim) {
     case 64: return q.bf16 ? attend<64, true>(a, (int)max_tiles, s) : attend<64, false>(a, (int)max_tiles, s);
