@@ -25,6 +25,7 @@ namespace {
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
@@ -54,12 +55,12 @@ struct Unpack {
 struct AttendArgs {
     KvCall kv;
     HeadRows q;
-    int heads, group, window, chunk_tiles, row_tiles, wide;
+    int heads, group, window, row_tiles, wide;
     float scale_log2;        // scale * log2(e)
     void *out;               // [rows, heads, D]
     float *lse;              // [rows, heads], in powers of two; null where nobody asks
-    float *part, *part_ml;   // chunks > 1: sums [rows * heads, chunks, D], (reference, sum) [rows * heads, chunks, 2]
-    int chunks, workgroups, rows;  // (rows: of a unit, at most)
+    float *part, *part_ml;   // of kv_split_kernel's workgroups: sums [rows, D], (reference, sum) [rows, 2]
+    int workgroups, rows;    // of kv_split_kernel; (new token, head) pairs of a key head, at most
     int2 *pieces;            // per unit of kv_split_kernel: the first workgroup that works on it, and how many do
     float *accounts;
     float *scores;           // of kv_split_kernel, in powers of two: [units, rows, score_tiles * 32] from the first tile that a unit sees; null: not kept
@@ -85,16 +86,18 @@ __device__ __forceinline__ Span row_tile_span(const KvSeq &s, int group, int win
     return r;
 }
 
-// Sixteen query rows as operands: lane (r, j) gets the values 32 g + 8 j + 0..7 of row r, times 2^e with the largest of the row in
-// [2^11, 2^12); `back` is 2^-e.  TWO: a second operand with what the first has rounded off.
-template <int D, bool BF16, bool TWO>
-__device__ __forceinline__ void load_queries(const HeadRows &q, int64_t at, bool live, int wide, h8 (&hi)[D / 32], h8 (&lo)[TWO ? D / 32 : 1], float &back) {
-    const int j = ((int)threadIdx.x & 63) >> 4;
-    float x[D / 32][8];
+// ROWS (16 or 32) query rows as operands of the matrix instructions of that size: lane (r, j), r = lane % ROWS, gets the values
+// 8 (64 / ROWS) g + 8 j + 0..7 of row r for g = 0, 1, ..., times 2^e with the largest of the row in [2^11, 2^12); `back` is 2^-e.  TWO: a
+// second operand with what the first has rounded off.
+template <int D, int ROWS, bool BF16, bool TWO>
+__device__ __forceinline__ void load_queries(const HeadRows &q, int64_t at, bool live, int wide, h8 (&hi)[D * ROWS / 512], h8 (&lo)[TWO ? D * ROWS / 512 : 1], float &back) {
+    constexpr int N = D * ROWS / 512;
+    const int j = ((int)threadIdx.x & 63) / ROWS;
+    float x[N][8];
     float most = 0.0f;
 #pragma unroll
-    for (int g = 0; g < D / 32; g++) {
-        const int64_t p = at + 32 * g + 8 * j;
+    for (int g = 0; g < N; g++) {
+        const int64_t p = at + 512 / ROWS * g + 8 * j;
         if (!live) {
 #pragma unroll
             for (int e = 0; e < 8; e++) x[g][e] = 0.0f;
@@ -122,15 +125,15 @@ __device__ __forceinline__ void load_queries(const HeadRows &q, int64_t at, bool
 #pragma unroll
         for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(x[g][e]));
     }
-    most = fmaxf(most, __shfl_xor(most, 16));
-    most = fmaxf(most, __shfl_xor(most, 32));
+#pragma unroll
+    for (int m = ROWS; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
     int e = 0;
     if (most > 0.0f && most < __builtin_huge_valf()) e = 12 - __builtin_amdgcn_frexp_expf(most);
     e = e > 100 ? 100 : e;  // (below 2^-88 the scores of a row are nothing)
     const float up = ldexpf(1.0f, e);
     back = ldexpf(1.0f, -e);
 #pragma unroll
-    for (int g = 0; g < D / 32; g++) {
+    for (int g = 0; g < N; g++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const float v = x[g][i] * up;
@@ -379,7 +382,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
         if (mem) fetch_tile<D>(ring_at, mem);
         h8 qh[D / 32], ql[TWO ? D / 32 : 1];
         float back;
-        load_queries<D, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
+        load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
         const float to_log2 = back * a.scale_log2;
         int turn = 0;
         for (int tile = tile0 + wave; tile < last; tile += kSplitWaves) {
@@ -538,222 +541,236 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
     if (a.lse && l == 0) a.lse[out] = lse_of(top, all);
 }
 
-// Sixteen rows of one key head over one chunk of the tokens that they see.  Each wavefront takes every fourth tile with a
-// maximum, sums and results of its own; they meet in LDS at the end.
-template <int D, bool BF16>
-__global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 1 : 2) void kv_rows_kernel(const AttendArgs a) {
-    constexpr bool TWO = !BF16;
-    constexpr int W = D / 16;
-    __shared__ float sums[kSplitWaves][16][D + 4];
-    __shared__ float refs[kSplitWaves][16], totals[kSplitWaves][16];
-    const KvCall &kv = a.kv;
-    const int b = (int)blockIdx.z, h = (int)blockIdx.y;
-    const int row_tile = (int)blockIdx.x / a.chunks, chunk = (int)blockIdx.x - row_tile * a.chunks;
-    const KvSeq seq = kv_seq(kv, b);
-    const Span span = row_tile_span(seq, a.group, a.window, row_tile, 16);
-    if (span.rows == 0) return;
-    const int tile0 = (span.lo >> 5) + chunk * a.chunk_tiles, tiles_end = (span.hi + 31) >> 5;
-    if (chunk > 0 && tile0 >= tiles_end) return;
-    const int tile1 = min(tile0 + a.chunk_tiles, tiles_end);
+// Many rows: a workgroup takes 128 neighbouring (new token, head) pairs of a key head, 32 a wavefront, over all the tokens that they
+// see, and widens the cache's codes once for all of them: 64 tokens (D = 256: 32) at a time go through LDS as fp16 operands of
+// v_mfma_f32_32x32x16_f16, written in the order in which lanes read them, into the one of two buffers that is not worked on.
+// The instruction's results lie in a lane (r, half) as the operand rows 8 (i / 4) + 4 half + i % 4; operand row m is token m with bits 2
+// and 3 exchanged, so that a lane's results 8 s + 0..7 are the scores of tokens 16 s + 8 half + 0..7: the eight of one dword of value
+// codes, and its share of the second product's operand where they lie.
+//
+// Matrix instructions, exponentials and the widening run side by side, two workgroups a CU (2048 rows of 32 heads over 2049 to 4096
+// tokens, D = 128).  With a causal bound workgroups differ in length: the second half of them goes from short to long, so that the two of a CU
+// add up to the same.
+constexpr int kRowsWaves = 4, kRowsTile = 32 * kRowsWaves;
 
-    const int lane = (int)threadIdx.x & 63, r = lane & 15, j = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int idx = span.first_row + r;
-    const bool live = r < span.rows;
-    const int nth = live ? idx / a.group : 0;            // new token of the row
+template <int D> struct RowsLds {
+    static constexpr int kTiles = D == 256 ? 1 : 2;                // of the cache, at a time
+    static constexpr int kKeys = 64 * D, kTile = 2 * kKeys;        // bytes of a tile's key operands; of all its operands
+    static constexpr int kStage = kTiles * kTile;
+    static constexpr int kItems = kTiles * 2 * D / (64 * kRowsWaves);  // chunks of 16 bytes of codes that a thread widens
+};
+
+// The codes and scales that a thread widens, as loaded: chunk c (four dwords a lane) of a tile's keys or values.
+struct Chunk {
+    u4 code, scale[2];
+    template <int D> __device__ __forceinline__ void load(const uint8_t *tile, bool values, int c) {
+        constexpr int G = D / 32;
+        const int lane = c & 63, r = lane & 15, j = lane >> 4, w = (c >> 6) * 4;
+        code = *reinterpret_cast<const u4 *>(tile + (values ? KvTile<D>::kValues : KvTile<D>::kKeys) + c * 16);
+        if (values) {
+            const uint8_t *p = tile + KvTile<D>::kValueScales + (w >> 1) * 64 + j * 16;
+            scale[0] = *reinterpret_cast<const u4 *>(p);
+            scale[1] = *reinterpret_cast<const u4 *>(p + 64);
+        } else {
+            const uint8_t *p = tile + KvTile<D>::kKeyScales + (8 * (r >> 2) + (r & 3)) * (2 * G);  // of the first of the two tokens of row r
+            if constexpr (D == 64) {
+                scale[0].x = *reinterpret_cast<const uint32_t *>(p);
+                scale[0].y = *reinterpret_cast<const uint32_t *>(p + 4 * 2 * G);
+            } else {
+                const u2 v = *reinterpret_cast<const u2 *>(p + (w / G) * 4 * 2 * G + (w % G) * 2);
+                scale[0].x = v.x;
+                scale[0].y = v.y;
+            }
+        }
+    }
+    template <int D> __device__ __forceinline__ void widen(const Unpack &unpack, uint8_t *stage, bool values, int c) const {
+        constexpr int G = D / 32;
+        const int lane = c & 63, r = lane & 15, j = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int w = (c >> 6) * 4 + i;
+            h2 v[4];
+            unpack(code[i], v);
+            if (values) {
+                const u4 d = scale[i >> 1];
+                const h8 x = join(v[0] * as_h2(d[0]), v[1] * as_h2(d[1]), v[2] * as_h2(d[2]), v[3] * as_h2(d[3]));
+                // [32 values][tokens 16 s ..][lane]
+                *reinterpret_cast<h8 *>(stage + RowsLds<D>::kKeys + (((w >> 1) * 2 + (j >> 1)) * 64 + (w & 1) * 16 + r + 32 * (j & 1)) * 16) = x;
+            } else {
+                const h2 pair = as_h2((i >> 1) ? scale[0].y : scale[0].x);
+                const _Float16 one = (i & 1) ? pair.y : pair.x;
+                const h2 d = {one, one};
+                const h8 x = join(v[0] * d, v[1] * d, v[2] * d, v[3] * d);
+                const int g = w % G, u = w / G, m = (r >> 3) * 16 + u * 8 + ((r >> 2) & 1) * 4 + (r & 3);  // token 8 (r / 4) + 4 u + r % 4, bits 2 and 3 exchanged
+                *reinterpret_cast<h8 *>(stage + ((2 * g + (j >> 1)) * 64 + m + 32 * (j & 1)) * 16) = x;
+            }
+        }
+    }
+    template <int D> __device__ __forceinline__ static void clear(uint8_t *stage, bool values, int c) {  // (no such tile: numbers, which nobody sees)
+        const u4 zero = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; i++) *reinterpret_cast<u4 *>(stage + (values ? RowsLds<D>::kKeys : 0) + (c * 4 + i) * 16) = zero;
+    }
+};
+
+__device__ __forceinline__ f16 mfma32(h8 a, h8 b, f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+template <int D, bool BF16>
+__global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_kernel(const AttendArgs a) {
+    constexpr bool TWO = !BF16;
+    typedef RowsLds<D> Lds;
+    constexpr int KS = D / 16, VS = D / 32, T = Lds::kTiles, ITEMS = Lds::kItems;
+    __shared__ __align__(16) uint8_t stage[2][Lds::kStage];
+    const KvCall &kv = a.kv;
+    const int b = (int)blockIdx.y;
+    // (the key head goes round fastest: with eight of them, one to an XCD and its L2)
+    const int nth_tile = (int)blockIdx.x / kv.kv_heads, h = (int)blockIdx.x - nth_tile * kv.kv_heads;
+    const int row_tile = nth_tile < (a.row_tiles + 1) / 2 ? a.row_tiles - 1 - nth_tile : nth_tile - (a.row_tiles + 1) / 2;
+    const KvSeq seq = kv_seq(kv, b);
+    const Span span = row_tile_span(seq, a.group, a.window, row_tile, kRowsTile);
+    if (span.rows == 0) return;
+    const int tile0 = span.lo >> 5, tile1 = (span.hi + 31) >> 5;
+
+    const int tid = (int)threadIdx.x, lane = tid & 63, r = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int in = wave * 32 + r, idx = span.first_row + in;
+    const bool live = in < span.rows;
+    const int nth = live ? idx / a.group : 0;
     const int head = h * a.group + (live ? idx - nth * a.group : 0);
     const int64_t row = seq.row0 + nth;
-    const int place = seq.length - seq.news + nth;       // its own token
+    const int base = seq.length - seq.news, place = base + nth;
     const int see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
-    // tokens that every row of the tile sees
-    const int all_hi = __builtin_amdgcn_readfirstlane(seq.length - seq.news + span.first_row / a.group + 1);
-    const int all_lo = a.window ? seq.length - seq.news + (span.first_row + span.rows - 1) / a.group + 1 - a.window : 0;
-    const bool full_rows = span.rows == 16;
-
-    h8 qh[D / 32], ql[TWO ? D / 32 : 1];
-    float back;
-    load_queries<D, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
-    const float to_log2 = back * a.scale_log2;
-
-    f4 o[W];
-#pragma unroll
-    for (int w = 0; w < W; w++) o[w] = f4{0.f, 0.f, 0.f, 0.f};
-    float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
+    // what every row of the wavefront sees, and what one of them does
+    const int first_in = span.first_row + wave * 32, last_in = min(first_in + 31, span.first_row + span.rows - 1);
+    const int all_hi = base + first_in / a.group + 1, any_hi = wave * 32 < span.rows ? base + last_in / a.group + 1 : 0;
+    const int all_lo = a.window ? base + last_in / a.group + 1 - a.window : 0, any_lo = a.window ? all_hi - a.window : 0;
 
     const Unpack unpack;
-    TileWalk walk(kv, b, h, tile0 + wave, kSplitWaves, KvTile<D>::kBytes);
-    KeyWords<D> k, k_next;
-    ValueWords<D> v, v_next;
-    const uint8_t *at = walk.next(tile0 + wave < tile1);
-    if (at) {
-        k.load(at);
-        v.load(at);
-    }
-    for (int tile = tile0 + wave; tile < tile1; tile += kSplitWaves) {
-        const uint8_t *at_next = walk.next(tile + kSplitWaves < tile1);
-        if (at_next) {  // the next tile is on its way while this one is worked on
-            k_next.load(at_next);
-            v_next.load(at_next);
+    TileWalk walk(kv, b, h, tile0, 1, KvTile<D>::kBytes);
+    Chunk chunk[ITEMS];
+    uint32_t there = 0;  // tiles of the stage that the cache has, a bit each
+    const auto values_of = [&](int n) { return ITEMS == 1 ? tid >= 128 : n >= ITEMS / 2; };
+    const auto chunk_of = [&](int n) { return ITEMS == 1 ? tid & 127 : n % ((ITEMS + 1) / 2) * 256 + tid; };  // of the stage's keys or values
+    const auto load = [&](int tile) {  // the stage that begins with this tile
+        const uint8_t *mem[T];
+        there = 0;
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            mem[t] = walk.next(tile + t < tile1);
+            there |= mem[t] ? 1u << t : 0u;
         }
-        if (at) {
-            float s[8];
-            tile_scores<D, TWO>(unpack, k, qh, ql, s);
-            const int t0 = tile * 32;
-            float most = kNegInf;
-            if (full_rows && t0 >= all_lo && t0 + 32 <= all_hi) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    s[e] *= to_log2;
-                    most = fmaxf(most, s[e]);
-                }
-            } else {
+        for (int n = 0; n < ITEMS; n++) {
+            const int c = chunk_of(n);
+            const int t = __builtin_amdgcn_readfirstlane(c / D);  // (a wavefront's 64 chunks are of one tile)
+            const uint8_t *at = T == 2 && t ? mem[T - 1] : mem[0];
+            if (at) chunk[n].template load<D>(at, values_of(n), c % D);
+        }
+    };
+    const auto widen = [&](uint8_t *to) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int t = t0 + 8 * j + e;
-                    s[e] = t < see_hi && t >= see_lo ? s[e] * to_log2 : kNegInf;
-                    most = fmaxf(most, s[e]);
+        for (int n = 0; n < ITEMS; n++) {
+            const int c = chunk_of(n);
+            const int t = __builtin_amdgcn_readfirstlane(c / D);
+            if ((there >> t) & 1u) chunk[n].template widen<D>(unpack, to + t * Lds::kTile, values_of(n), c % D);
+            else Chunk::template clear<D>(to + t * Lds::kTile, values_of(n), c % D);
+        }
+    };
+
+    load(tile0);
+    h8 qh[KS], ql[TWO ? KS : 1];
+    float back;
+    load_queries<D, 32, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
+    const float to_log2 = back * a.scale_log2;
+
+    f16 o[VS];
+#pragma unroll
+    for (int w = 0; w < VS; w++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[w][i] = 0.0f;
+    float ref = kNegInf, total = 0.0f;
+
+    widen(stage[0]);
+    uint32_t now = there;
+    __syncthreads();
+    int turn = 0;
+    for (int tile = tile0; tile < tile1; tile += T) {
+        const bool more = tile + T < tile1;
+        if (more) load(tile + T);
+        const int t0 = tile * 32;
+        if (t0 < any_hi && t0 + 32 * T > any_lo) {
+            const uint8_t *from = stage[turn];
+            f16 s[T];
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    const h8 x = *reinterpret_cast<const h8 *>(from + t * Lds::kTile + (k * 64 + lane) * 16);
+                    s[t] = mfma32(x, qh[k], s[t]);
+                    if constexpr (TWO) s[t] = mfma32(x, ql[k], s[t]);
                 }
             }
-            if (__any(most > ref + kMostLog2)) {  // (the first score of a row among them: its reference is -infinity)
-                most = fmaxf(most, __shfl_xor(most, 16));
+            float most = kNegInf;
+            const bool open = t0 >= all_lo && t0 + 32 * T <= all_hi && now == (1u << T) - 1;
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    s[t][i] *= to_log2;
+                    if (!open) {
+                        const int token = t0 + 32 * t + 16 * (i >> 3) + 8 * half + (i & 7);
+                        s[t][i] = token < see_hi && token >= see_lo && ((now >> t) & 1u) ? s[t][i] : kNegInf;
+                    }
+                    most = fmaxf(most, s[t][i]);
+                }
+            }
+            if (__any(most > ref + kMostLog2)) {
                 most = fmaxf(most, __shfl_xor(most, 32));
                 const float next = fmaxf(ref, most - kHeadroom);
                 const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
                 ref = next;
                 total *= shrink;
 #pragma unroll
-                for (int w = 0; w < W; w++) o[w] *= shrink;
+                for (int w = 0; w < VS; w++) o[w] *= shrink;
             }
-            const float from = ref == kNegInf ? 0.0f : ref;
-            h8 ph, pl;
+            const float less = ref == kNegInf ? 0.0f : ref;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float p = __builtin_amdgcn_exp2f(s[e] - from);
-                total += p;
-                ph[e] = (_Float16)p;
-                if constexpr (TWO) pl[e] = (_Float16)(p - (float)ph[e]);
-            }
+            for (int t = 0; t < T; t++) {
 #pragma unroll
-            for (int w = 0; w < W; w++) {
-                const h8 x = v.operand(unpack, w);
-                o[w] = mfma(x, ph, o[w]);
-                if constexpr (TWO) o[w] = mfma(x, pl, o[w]);
+                for (int k = 0; k < 2; k++) {
+                    h8 ph, pl;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float p = __builtin_amdgcn_exp2f(s[t][8 * k + e] - less);
+                        total += p;
+                        ph[e] = (_Float16)p;
+                        if constexpr (TWO) pl[e] = (_Float16)(p - (float)ph[e]);
+                    }
+#pragma unroll
+                    for (int w = 0; w < VS; w++) {
+                        const h8 x = *reinterpret_cast<const h8 *>(from + t * Lds::kTile + Lds::kKeys + ((w * 2 + k) * 64 + lane) * 16);
+                        o[w] = mfma32(x, ph, o[w]);
+                        if constexpr (TWO) o[w] = mfma32(x, pl, o[w]);
+                    }
+                }
             }
         }
-        at = at_next;
-        k = k_next;
-        v = v_next;
+        if (more) widen(stage[turn ^ 1]);
+        now = there;
+        turn ^= 1;
+        __syncthreads();
     }
-    total += __shfl_xor(total, 16);
     total += __shfl_xor(total, 32);
+    if (!live) return;
+    const int64_t out = row * a.heads + head;
 #pragma unroll
-    for (int w = 0; w < W; w++) *reinterpret_cast<f4 *>(&sums[wave][r][16 * w + 4 * j]) = o[w];
-    if (j == 0) {
-        refs[wave][r] = ref;
-        totals[wave][r] = total;
-    }
-    __syncthreads();
-
-    for (int i = (int)threadIdx.x; i < span.rows * (D / 4); i += 64 * kSplitWaves) {
-        const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4;
-        float top = kNegInf;
+    for (int w = 0; w < VS; w++)
 #pragma unroll
-        for (int w = 0; w < kSplitWaves; w++) top = fmaxf(top, refs[w][rr]);
-        f4 sum = {0.f, 0.f, 0.f, 0.f};
-        float all = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kSplitWaves; w++) {
-            const float f = refs[w][rr] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(refs[w][rr] - top);
-            // (a wavefront without a reference has seen no number: its sum is zero, or NaN)
-            all += refs[w][rr] == kNegInf ? totals[w][rr] : totals[w][rr] * f;
-            sum += *reinterpret_cast<const f4 *>(&sums[w][rr][d]) * f;
-        }
-        const int ii = span.first_row + rr, n = ii / a.group;
-        const int64_t to = (int64_t)(seq.row0 + n) * a.heads + h * a.group + (ii - n * a.group);
-        if (a.chunks > 1) {
-            *reinterpret_cast<f4 *>(a.part + (to * a.chunks + chunk) * D + d) = sum;
-            if (d == 0) {
-                a.part_ml[(to * a.chunks + chunk) * 2] = top;
-                a.part_ml[(to * a.chunks + chunk) * 2 + 1] = all;
-            }
-        } else {
-            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-            sum *= inv;
-            if (all != all) sum = f4{all, all, all, all};
-            if constexpr (BF16) {
-                typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-                bf16x4 y = {(__bf16)sum.x, (__bf16)sum.y, (__bf16)sum.z, (__bf16)sum.w};
-                *reinterpret_cast<bf16x4 *>(static_cast<uint16_t *>(a.out) + to * D + d) = y;
-            } else {
-                *reinterpret_cast<f4 *>(static_cast<float *>(a.out) + to * D + d) = sum;
-            }
-            if (a.lse && d == 0) a.lse[to] = all == 0.0f ? kNegInf : top + __builtin_amdgcn_logf(all);
-        }
-    }
-}
-
-// Joins the chunks of a row: one workgroup per row and head.
-template <int D, bool BF16>
-__global__ __launch_bounds__(256) void kv_rows_join_kernel(const AttendArgs a) {
-    constexpr int L = D / 4, S = 256 / L;  // lanes of a row's values, and the shares into which the chunks are divided
-    __shared__ f4 sums[S][L];
-    __shared__ float refs[S], totals[S];
-    const int64_t row = blockIdx.x / a.heads;
-    const int head = (int)(blockIdx.x - row * a.heads);
-    int b = 0;
-    if (a.kv.starts) {  // the sequence of the row
-        int lo = 0, hi = a.kv.seqs - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (a.kv.starts[mid] <= row) lo = mid;
-            else hi = mid - 1;
-        }
-        b = lo;
-    } else {
-        b = (int)row;
-    }
-    const KvSeq seq = kv_seq(a.kv, b);
-    const int n = (int)row - seq.row0;
-    if (n < 0 || n >= seq.news) return;
-    const Span span = row_tile_span(seq, a.group, a.window, (n * a.group + head % a.group) >> 4, 16);
-    const int tiles = ((span.hi + 31) >> 5) - (span.lo >> 5);
-    const int used = max(1, min(a.chunks, (tiles + a.chunk_tiles - 1) / a.chunk_tiles));
-    const int l = (int)threadIdx.x % L, share = (int)threadIdx.x / L;
-    const int64_t to = row * a.heads + head;
-    float top = kNegInf, all = 0.0f;
-    f4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int c = share; c < used; c += S) {
-        const float ref = a.part_ml[(to * a.chunks + c) * 2], t = a.part_ml[(to * a.chunks + c) * 2 + 1];
-        const f4 v = *reinterpret_cast<const f4 *>(a.part + (to * a.chunks + c) * D + l * 4);
-        const float next = fmaxf(top, ref);
-        const float fo = top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - next), fn = ref == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ref - next);
-        sum = sum * fo + v * fn;
-        all = (top == kNegInf ? all : all * fo) + (ref == kNegInf ? t : t * fn);
-        top = next;
-    }
-    sums[share][l] = sum;
-    if (l == 0) { refs[share] = top; totals[share] = all; }
-    __syncthreads();
-    if (share) return;
-    top = kNegInf;
-    for (int i = 0; i < S; i++) top = fmaxf(top, refs[i]);
-    sum = f4{0.f, 0.f, 0.f, 0.f};
-    all = 0.0f;
-    for (int i = 0; i < S; i++) {
-        const float f = refs[i] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(refs[i] - top);
-        sum += sums[i][l] * f;
-        all += refs[i] == kNegInf ? totals[i] : totals[i] * f;
-    }
-    sum *= all == 0.0f ? 0.0f : 1.0f / all;
-    if (all != all) sum = f4{all, all, all, all};
-    if constexpr (BF16) {
-        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-        bf16x4 y = {(__bf16)sum.x, (__bf16)sum.y, (__bf16)sum.z, (__bf16)sum.w};
-        *reinterpret_cast<bf16x4 *>(static_cast<uint16_t *>(a.out) + to * D + l * 4) = y;
-    } else {
-        *reinterpret_cast<f4 *>(static_cast<float *>(a.out) + to * D + l * 4) = sum;
-    }
-    if (a.lse && l == 0) a.lse[to] = all == 0.0f ? kNegInf : top + __builtin_amdgcn_logf(all);
+        for (int i = 0; i < 16; i += 4)
+            store_result<BF16>(a.out, out * D + 32 * w + 2 * i + 4 * half, f4{o[w][i], o[w][i + 1], o[w][i + 2], o[w][i + 3]}, total);
+    if (a.lse && half == 0) a.lse[out] = lse_of(ref, total);
 }
 
 // The accounts from the scores that kv_split_kernel has kept: one thread a token, which adds up the unit's rows.
@@ -811,7 +828,7 @@ __global__ __launch_bounds__(256) void kv_account_kernel(const AttendArgs a) {
         const int place = base + nth, see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
         h8 qh[D / 32], ql[TWO ? D / 32 : 1];
         float back, s[8];
-        load_queries<D, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
+        load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
         const float lse = live ? a.lse[row * a.heads + head] : 0.0f;
         tile_scores<D, TWO>(unpack, k, qh, ql, s);
         const float to_log2 = back * a.scale_log2;
@@ -849,11 +866,8 @@ template <int D, bool BF16> int attend(const AttendArgs &a, int max_tiles, hipSt
         if (int rc = launch(kv_split_kernel<D, BF16>, dim3((unsigned)grid), dim3(64 * kSplitWaves), 0, s, a)) return rc;
         if (a.part)
             if (int rc = launch(kv_join_kernel<D, BF16>, dim3((unsigned)(kv.max_new * a.group), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a)) return rc;
-    } else {
-        const dim3 grid((unsigned)(a.chunks * a.row_tiles), (unsigned)kv.kv_heads, (unsigned)kv.seqs);
-        if (int rc = launch(kv_rows_kernel<D, BF16>, grid, dim3(64 * kSplitWaves), 0, s, a)) return rc;
-        if (a.chunks > 1)
-            if (int rc = launch(kv_rows_join_kernel<D, BF16>, dim3((unsigned)((int64_t)kv.rows * a.heads)), dim3(256), 0, s, a)) return rc;
+    } else if (int rc = launch(kv_rows_kernel<D, BF16>, dim3((unsigned)(a.row_tiles * kv.kv_heads), (unsigned)kv.seqs), dim3(64 * kRowsWaves), 0, s, a)) {
+        return rc;
     }
     if (!a.accounts) return GQ_OK;
     if (a.scores) return launch(kv_score_account_kernel, dim3((unsigned)((a.score_tiles + 7) / 8), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
@@ -875,25 +889,17 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
     const int64_t size = q.bf16 ? 2 : 4;
     a.wide = ((reinterpret_cast<uintptr_t>(q.p) | (uintptr_t)(q.row * size) | (uintptr_t)(q.head * size)) & 15) == 0;
     a.rows = kv.max_new * a.group;
-    a.row_tiles = (int)(((int64_t)kv.max_new * a.group + 15) / 16);
-    // tiles that a row tile's chunks have to cover, and those that see any of the new tokens
+    // tiles that a unit's rows see, at most, and those that see any of the new tokens
     const int64_t room = (int64_t)kv.max_pages * kv.page_tokens / 32;
-    const int span_new = 15 / a.group + 1;  // new tokens of a row tile, less one
-    const int64_t tiles = std::max<int64_t>(1, window ? std::min<int64_t>(room, ((int64_t)window + span_new + 31) / 32 + 1) : room);
-    const int64_t max_tiles = std::max<int64_t>(1, window ? std::min<int64_t>(room, ((int64_t)window + kv.max_new + 31) / 32 + 1) : room);
+    const int64_t tiles = std::max<int64_t>(1, window ? std::min<int64_t>(room, ((int64_t)window + kv.max_new + 31) / 32 + 1) : room);
     const size_t line = (size_t)kv.rows * heads;
     size_t lines = 0;  // of sums that are joined
-    if (a.row_tiles == 1) {
+    if (a.rows <= 16) {
         const int64_t all = (int64_t)kv.seqs * kv.kv_heads * tiles;
         a.workgroups = (int)std::min<int64_t>(split_workgroups(kv.head_dim), (all + kSplitWaves - 1) / kSplitWaves);
         if (tiles > kSplitWaves) lines = (size_t)(a.workgroups + kv.seqs * kv.kv_heads) * a.rows;
     } else {
-        const int64_t units = (int64_t)kv.seqs * kv.kv_heads * a.row_tiles;
-        // about 1024 workgroups, each with a tile per wavefront at least
-        const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((1024 + units - 1) / units, (tiles + kSplitWaves - 1) / kSplitWaves));
-        a.chunk_tiles = (int)((tiles + chunks - 1) / chunks + kSplitWaves - 1) / kSplitWaves * kSplitWaves;
-        a.chunks = (int)((tiles + a.chunk_tiles - 1) / a.chunk_tiles);
-        if (a.chunks > 1) lines = line * a.chunks;
+        a.row_tiles = (a.rows + kRowsTile - 1) / kRowsTile;
     }
     const size_t lse_bytes = accounts ? (line * 4 + 255) / 256 * 256 : 0, ml_bytes = (lines * 8 + 255) / 256 * 256;
     const size_t score_bytes = a.workgroups && accounts ? (size_t)kv.seqs * kv.kv_heads * a.rows * tiles * 128 : 0;
@@ -915,9 +921,9 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
         }
     }
     switch (kv.head_dim) {
-    case 64: return q.bf16 ? attend<64, true>(a, (int)max_tiles, s) : attend<64, false>(a, (int)max_tiles, s);
-    case 128: return q.bf16 ? attend<128, true>(a, (int)max_tiles, s) : attend<128, false>(a, (int)max_tiles, s);
-    default: return q.bf16 ? attend<256, true>(a, (int)max_tiles, s) : attend<256, false>(a, (int)max_tiles, s);
+    case 64: return q.bf16 ? attend<64, true>(a, (int)tiles, s) : attend<64, false>(a, (int)tiles, s);
+    case 128: return q.bf16 ? attend<128, true>(a, (int)tiles, s) : attend<128, false>(a, (int)tiles, s);
+    default: return q.bf16 ? attend<256, true>(a, (int)tiles, s) : attend<256, false>(a, (int)tiles, s);
     }
 }
 
