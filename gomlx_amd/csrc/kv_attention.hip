@@ -55,7 +55,7 @@ struct Unpack {
 struct AttendArgs {
     KvCall kv;
     HeadRows q;
-    int heads, group, window, row_tiles, wide;
+    int heads, group, window, wide;
     float scale_log2;        // scale * log2(e)
     void *out;               // [rows, heads, D]
     float *lse;              // [rows, heads], in powers of two; null where nobody asks
@@ -65,6 +65,10 @@ struct AttendArgs {
     float *accounts;
     float *scores;           // of kv_split_kernel, in powers of two: [units, rows, score_tiles * 32] from the first tile that a unit sees; null: not kept
     int score_tiles;
+    int row_pieces;          // of kv_rows_kernel: pieces that a row tile's tokens are cut into (> 1: sums [line, pieces, D], (reference, sum) [line, pieces, 2])
+    uint8_t *operands;       // of kv_rows_kernel, for the accounts: 32 rows' queries as it has them, [key heads, operand tiles]; null: not kept
+    float *row_scales;       // and what their scores are multiplied by, [key heads, operand tiles, 32]
+    int operand_tiles;
 };
 
 // The tiles that the rows of a row tile (sixteen neighbouring (new token, head of the group) pairs) see, and where its chunk of them lies.
@@ -87,10 +91,10 @@ __device__ __forceinline__ Span row_tile_span(const KvSeq &s, int group, int win
 }
 
 // ROWS (16 or 32) query rows as operands of the matrix instructions of that size: lane (r, j), r = lane % ROWS, gets the values
-// 8 (64 / ROWS) g + 8 j + 0..7 of row r for g = 0, 1, ..., times 2^e with the largest of the row in [2^11, 2^12); `back` is 2^-e.  TWO: a
-// second operand with what the first has rounded off.
+// 8 (64 / ROWS) g + 8 j + 0..7 of row r for g = 0, 1, ..., times 2^e with the largest of the row in [2^11, 2^12), and the sign of the scale, so that what is left to multiply scores by is not negative; `back` is 2^-e.
+// TWO: a second operand with what the first has rounded off.
 template <int D, int ROWS, bool BF16, bool TWO>
-__device__ __forceinline__ void load_queries(const HeadRows &q, int64_t at, bool live, int wide, h8 (&hi)[D * ROWS / 512], h8 (&lo)[TWO ? D * ROWS / 512 : 1], float &back) {
+__device__ __forceinline__ void load_queries(const HeadRows &q, int64_t at, bool live, int wide, float sign, h8 (&hi)[D * ROWS / 512], h8 (&lo)[TWO ? D * ROWS / 512 : 1], float &back) {
     constexpr int N = D * ROWS / 512;
     const int j = ((int)threadIdx.x & 63) / ROWS;
     float x[N][8];
@@ -130,7 +134,7 @@ __device__ __forceinline__ void load_queries(const HeadRows &q, int64_t at, bool
     int e = 0;
     if (most > 0.0f && most < __builtin_huge_valf()) e = 12 - __builtin_amdgcn_frexp_expf(most);
     e = e > 100 ? 100 : e;  // (below 2^-88 the scores of a row are nothing)
-    const float up = ldexpf(1.0f, e);
+    const float up = copysignf(ldexpf(1.0f, e), sign);
     back = ldexpf(1.0f, -e);
 #pragma unroll
     for (int g = 0; g < N; g++) {
@@ -382,8 +386,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
         if (mem) fetch_tile<D>(ring_at, mem);
         h8 qh[D / 32], ql[TWO ? D / 32 : 1];
         float back;
-        load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
-        const float to_log2 = back * a.scale_log2;
+        load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
+        const float to_log2 = back * fabsf(a.scale_log2);
         int turn = 0;
         for (int tile = tile0 + wave; tile < last; tile += kSplitWaves) {
             const uint8_t *mem_next = walk.next(tile + kSplitWaves < last);
@@ -615,21 +619,52 @@ struct Chunk {
 
 __device__ __forceinline__ f16 mfma32(h8 a, h8 b, f16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-template <int D, bool BF16>
+// The sequence and its row tile that number `index` of all row tiles is; b < 0: there is none.
+struct RowTile { int b, tile, tiles; KvSeq seq; };
+__device__ __forceinline__ RowTile row_tile_of(const AttendArgs &a, int index) {
+    const int lane = (int)threadIdx.x & 63, seqs = a.kv.seqs;
+    RowTile t;
+    t.b = -1;
+    int front = 0;
+    for (int base = 0; base < seqs; base += 64) {
+        KvSeq mine{0, 0, 0};
+        if (base + lane < seqs) mine = kv_seq(a.kv, base + lane);
+        const int tiles = (mine.news * a.group + kRowsTile - 1) / kRowsTile, upto = lane_scan(tiles);
+        const uint64_t past = __ballot(front + upto > index);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            t.b = base + l;
+            t.seq = KvSeq{__builtin_amdgcn_readlane(mine.length, l), __builtin_amdgcn_readlane(mine.news, l), __builtin_amdgcn_readlane(mine.row0, l)};
+            t.tiles = __builtin_amdgcn_readlane(tiles, l);
+            t.tile = index - (front + __builtin_amdgcn_readlane(upto, l) - t.tiles);
+            break;
+        }
+        front += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return t;
+}
+// The first operand tile of sequence b: tiles of 32 rows, of which no two sequences share one.
+__device__ __forceinline__ int first_operand_tile(const AttendArgs &a, const KvSeq &seq, int b) { return (int)((int64_t)seq.row0 * a.group / 32) + b; }
+
+template <int D, bool BF16, bool ACCOUNTS>
 __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_kernel(const AttendArgs a) {
     constexpr bool TWO = !BF16;
     typedef RowsLds<D> Lds;
     constexpr int KS = D / 16, VS = D / 32, T = Lds::kTiles, ITEMS = Lds::kItems;
     __shared__ __align__(16) uint8_t stage[2][Lds::kStage];
     const KvCall &kv = a.kv;
-    const int b = (int)blockIdx.y;
     // (the key head goes round fastest: with eight of them, one to an XCD and its L2)
-    const int nth_tile = (int)blockIdx.x / kv.kv_heads, h = (int)blockIdx.x - nth_tile * kv.kv_heads;
-    const int row_tile = nth_tile < (a.row_tiles + 1) / 2 ? a.row_tiles - 1 - nth_tile : nth_tile - (a.row_tiles + 1) / 2;
-    const KvSeq seq = kv_seq(kv, b);
+    const int rest = (int)blockIdx.x / kv.kv_heads, h = (int)blockIdx.x - rest * kv.kv_heads;
+    const int index = rest / a.row_pieces, piece = rest - index * a.row_pieces;
+    const RowTile unit = row_tile_of(a, index);
+    if (unit.b < 0) return;
+    const int b = unit.b;
+    const KvSeq &seq = unit.seq;
+    const int row_tile = unit.tile < (unit.tiles + 1) / 2 ? unit.tiles - 1 - unit.tile : unit.tile - (unit.tiles + 1) / 2;
     const Span span = row_tile_span(seq, a.group, a.window, row_tile, kRowsTile);
-    if (span.rows == 0) return;
-    const int tile0 = span.lo >> 5, tile1 = (span.hi + 31) >> 5;
+    const int stages = (((span.hi + 31) >> 5) - (span.lo >> 5) + T - 1) / T;
+    const int tile0 = (span.lo >> 5) + T * (int)((int64_t)stages * piece / a.row_pieces);
+    const int tile1 = min((span.hi + 31) >> 5, (span.lo >> 5) + T * (int)((int64_t)stages * (piece + 1) / a.row_pieces));
 
     const int tid = (int)threadIdx.x, lane = tid & 63, r = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -677,11 +712,11 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
         }
     };
 
-    load(tile0);
+    if (tile0 < tile1) load(tile0);
     h8 qh[KS], ql[TWO ? KS : 1];
     float back;
-    load_queries<D, 32, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
-    const float to_log2 = back * a.scale_log2;
+    load_queries<D, 32, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
+    const float to_log2 = fmaxf(back * fabsf(a.scale_log2), 1e-37f);  // (not 0, so that its product with -infinity stays that)
 
     f16 o[VS];
 #pragma unroll
@@ -690,7 +725,17 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
         for (int i = 0; i < 16; i++) o[w][i] = 0.0f;
     float ref = kNegInf, total = 0.0f;
 
-    widen(stage[0]);
+    if (ACCOUNTS && piece == 0 && wave * 32 < span.rows) {
+        const int64_t tile = (int64_t)h * a.operand_tiles + first_operand_tile(a, seq, b) + row_tile * kRowsWaves + wave;
+        h8 *to = reinterpret_cast<h8 *>(a.operands) + tile * (TWO ? 2 : 1) * KS * 64 + lane;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            to[k * 64] = qh[k];
+            if constexpr (TWO) to[(KS + k) * 64] = ql[k];
+        }
+        if (half == 0) a.row_scales[tile * 32 + r] = to_log2;
+    }
+    if (tile0 < tile1) widen(stage[0]);
     uint32_t now = there;
     __syncthreads();
     int turn = 0;
@@ -712,20 +757,21 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
                     if constexpr (TWO) s[t] = mfma32(x, ql[k], s[t]);
                 }
             }
-            float most = kNegInf;
-            const bool open = t0 >= all_lo && t0 + 32 * T <= all_hi && now == (1u << T) - 1;
+            float most = kNegInf;  // (scores as the products left them: what they are multiplied by is not negative)
+            if (!(t0 >= all_lo && t0 + 32 * T <= all_hi && now == (1u << T) - 1)) {
 #pragma unroll
-            for (int t = 0; t < T; t++) {
+                for (int t = 0; t < T; t++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    s[t][i] *= to_log2;
-                    if (!open) {
+                    for (int i = 0; i < 16; i++) {
                         const int token = t0 + 32 * t + 16 * (i >> 3) + 8 * half + (i & 7);
                         s[t][i] = token < see_hi && token >= see_lo && ((now >> t) & 1u) ? s[t][i] : kNegInf;
                     }
-                    most = fmaxf(most, s[t][i]);
-                }
             }
+#pragma unroll
+            for (int t = 0; t < T; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) most = fmaxf(most, s[t][i]);
+            if (most != kNegInf) most *= to_log2;
             if (__any(most > ref + kMostLog2)) {
                 most = fmaxf(most, __shfl_xor(most, 32));
                 const float next = fmaxf(ref, most - kHeadroom);
@@ -735,18 +781,28 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
 #pragma unroll
                 for (int w = 0; w < VS; w++) o[w] *= shrink;
             }
-            const float less = ref == kNegInf ? 0.0f : ref;
+            const float less = ref == kNegInf ? 0.0f : -ref;
 #pragma unroll
             for (int t = 0; t < T; t++) {
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     h8 ph, pl;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float p = __builtin_amdgcn_exp2f(s[t][8 * k + e] - less);
-                        total += p;
-                        ph[e] = (_Float16)p;
-                        if constexpr (TWO) pl[e] = (_Float16)(p - (float)ph[e]);
+                    for (int e = 0; e < 8; e += 2) {
+                        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e], to_log2, less)), p1 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e + 1], to_log2, less));
+                        ph[e] = (_Float16)p0;
+                        ph[e + 1] = (_Float16)p1;
+                        if constexpr (TWO) {
+                            pl[e] = (_Float16)(p0 - (float)ph[e]);
+                            pl[e + 1] = (_Float16)(p1 - (float)ph[e + 1]);
+                        }
+                        if constexpr (TWO || ACCOUNTS) {  // (accounts are kept to fp32's accuracy whatever the type)
+                            total += p0;
+                            total += p1;
+                        } else {  // the weights as they are used, two in one instruction
+                            const h2 pair = {ph[e], ph[e + 1]}, ones = {(_Float16)1.0f, (_Float16)1.0f};
+                            total = __builtin_amdgcn_fdot2(pair, ones, total, false);
+                        }
                     }
 #pragma unroll
                     for (int w = 0; w < VS; w++) {
@@ -765,12 +821,43 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     total += __shfl_xor(total, 32);
     if (!live) return;
     const int64_t out = row * a.heads + head;
+    if (a.row_pieces > 1) {
+        const int64_t line = out * a.row_pieces + piece;
+#pragma unroll
+        for (int w = 0; w < VS; w++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) *reinterpret_cast<f4 *>(a.part + line * D + 32 * w + 2 * i + 4 * half) = f4{o[w][i], o[w][i + 1], o[w][i + 2], o[w][i + 3]};
+        if (half == 0) {
+            a.part_ml[line * 2] = ref;
+            a.part_ml[line * 2 + 1] = total;
+        }
+        return;
+    }
 #pragma unroll
     for (int w = 0; w < VS; w++)
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
             store_result<BF16>(a.out, out * D + 32 * w + 2 * i + 4 * half, f4{o[w][i], o[w][i + 1], o[w][i + 2], o[w][i + 3]}, total);
-    if (a.lse && half == 0) a.lse[out] = lse_of(ref, total);
+    if (ACCOUNTS && half == 0) a.lse[out] = lse_of(ref, total);
+}
+
+// Joins the pieces of kv_rows_kernel: a thread makes four values of a line, (row, head).
+template <int D, bool BF16>
+__global__ __launch_bounds__(256) void kv_rows_join_kernel(const AttendArgs a) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, line = at / (D / 4);
+    const int d = (int)(at - line * (D / 4)) * 4, n = a.row_pieces;
+    if (line >= (int64_t)a.kv.rows * a.heads) return;
+    const float *ml = a.part_ml + line * n * 2;
+    float top = kNegInf, all = 0.0f;
+    for (int i = 0; i < n; i++) top = fmaxf(top, ml[2 * i]);
+    f4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < n; i++) {
+        const float f = ml[2 * i] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * i] - top);
+        all += ml[2 * i] == kNegInf ? ml[2 * i + 1] : ml[2 * i + 1] * f;
+        sum += *reinterpret_cast<const f4 *>(a.part + (line * n + i) * D + d) * f;
+    }
+    store_result<BF16>(a.out, line * D + d, sum, all);
+    if (a.lse && d == 0) a.lse[line] = lse_of(top, all);
 }
 
 // The accounts from the scores that kv_split_kernel has kept: one thread a token, which adds up the unit's rows.
@@ -799,53 +886,130 @@ __global__ __launch_bounds__(256) void kv_score_account_kernel(const AttendArgs 
     *to += sum;
 }
 
-// The accounts: a wavefront owns a tile of a sequence and key head and goes over all rows that see it, so that every account is
-// added to once, in one order.
+// The accounts of many rows: a workgroup owns a tile of a sequence and key head, its keys in registers as operands, and goes over all rows
+// that see it, as kv_rows_kernel has left them, 32 at a time and every fourth such tile a wavefront: every account is added to once, in
+// one order.  The way of the rows' operands from the other XCDs' memory side bounds it where there are few, matrix instructions
+// and one exponential a (row, token) where there are many.
+template <int D, bool BF16>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_account_kernel(const AttendArgs a) {
+    constexpr bool TWO = !BF16;
+    constexpr int KS = D / 16, G = D / 32, N = TWO ? 2 * KS : KS;
+    __shared__ float sums[4][32];
+    const KvCall &kv = a.kv;
+    const int h = (int)blockIdx.y, b = (int)blockIdx.z;
+    const KvSeq seq = kv_seq(kv, b);
+    const int base = seq.length - seq.news;
+    const int tile = (a.window ? max(0, base + 1 - a.window) >> 5 : 0) + (int)blockIdx.x, t0 = tile * 32;
+    if (t0 >= seq.length || seq.news == 0) return;
+    const uint8_t *mem = kv_tile(kv, b, h, tile, KvTile<D>::kBytes);
+    if (!mem) return;
+    const int lane = (int)threadIdx.x & 63, r = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    // the new tokens that see one of the tile's, and their operand tiles
+    const int n0 = max(0, t0 - base), n1 = a.window ? min(seq.news, t0 + 31 + a.window - base) : seq.news;
+    const int from = n0 * a.group / 32 + wave, to = (n1 * a.group + 31) / 32;
+    const int64_t first = (int64_t)h * a.operand_tiles + first_operand_tile(a, seq, b);
+    struct Rows {  // 32 rows
+        h8 q[N];
+        float scale, lse;
+        int place;  // -1: no row
+    };
+    const auto load = [&](int n, Rows &rows) {
+        const h8 *q = reinterpret_cast<const h8 *>(a.operands) + (first + n) * N * 64 + lane;
+#pragma unroll
+        for (int k = 0; k < N; k++) rows.q[k] = q[k * 64];
+        const int idx = n * 32 + r;
+        const bool live = idx < seq.news * a.group;
+        const int nth = live ? idx / a.group : 0, head = h * a.group + (live ? idx - nth * a.group : 0);
+        rows.place = live ? base + nth : -1;
+        rows.scale = a.row_scales[(first + n) * 32 + r];
+        rows.lse = a.lse[(int64_t)(seq.row0 + nth) * a.heads + head];
+    };
+    Rows now, next;
+    if (from < to) load(from, now);
+    // the tile's keys: operand row r is token r, values 16 k + 8 half + 0..7
+    h8 keys[KS];
+    {
+        const Unpack unpack;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const int g = k >> 1, j = 2 * (k & 1) + half;
+            h2 v[4];
+            unpack(*reinterpret_cast<const uint32_t *>(mem + KvTile<D>::kKeys + KvTile<D>::code(key_half(r) * G + g, key_row(r) + 16 * j)), v);
+            const _Float16 one = reinterpret_cast<const _Float16 *>(mem + KvTile<D>::kKeyScales)[r * G + g];
+            const h2 d = {one, one};
+            keys[k] = join(v[0] * d, v[1] * d, v[2] * d, v[3] * d);
+        }
+    }
+    float sum[16] = {};
+    for (int n = from; n < to; n += 4) {
+        if (n + 4 < to) load(n + 4, next);
+        f16 s;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            s = mfma32(keys[k], now.q[k], s);
+            if constexpr (TWO) s = mfma32(keys[k], now.q[KS + k], s);
+        }
+        const bool open = __all(now.place >= t0 + 31 && (!a.window || now.place - a.window < t0));
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int t = t0 + 8 * (i >> 2) + 4 * half + (i & 3);
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], now.scale, -now.lse));
+            sum[i] += open || (t <= now.place && (!a.window || t > now.place - a.window)) ? p : 0.0f;
+        }
+        now = next;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) sum[i] += __shfl_xor(sum[i], m);
+        if (r == 0) sums[wave][8 * (i >> 2) + 4 * half + (i & 3)] = sum[i];
+    }
+    __syncthreads();
+    const int t = t0 + (int)threadIdx.x;
+    if (threadIdx.x < 32 && t < seq.length) {
+        float *p = kv_account(kv, a.accounts, b, h, t);
+        if (p) *p += (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+    }
+}
+
+// The accounts of few rows over so many tokens that their scores are not kept: as above, by sixteen rows.
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void kv_account_kernel(const AttendArgs a) {
     constexpr bool TWO = !BF16;
     const KvCall &kv = a.kv;
     const int h = (int)blockIdx.y, b = (int)blockIdx.z;
     const KvSeq seq = kv_seq(kv, b);
-    const int base = seq.length - seq.news;
-    const int first_tile = a.window ? max(0, base + 1 - a.window) >> 5 : 0;
-    const int tile = __builtin_amdgcn_readfirstlane(first_tile + (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6));
-    if (tile * 32 >= seq.length || seq.news == 0) return;
-    const uint8_t *at = kv_tile(kv, b, h, tile, KvTile<D>::kBytes);
-    if (!at) return;
+    const Span span = span_of(a, seq);
+    const int tile = __builtin_amdgcn_readfirstlane((span.lo >> 5) + (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6));
+    if (span.rows == 0 || tile * 32 >= span.hi) return;
+    const uint8_t *mem = kv_tile(kv, b, h, tile, KvTile<D>::kBytes);
+    if (!mem) return;
     KeyWords<D> k;
-    k.load(at);
+    k.load(mem);
     const int lane = (int)threadIdx.x & 63, r = lane & 15, j = lane >> 4, t0 = tile * 32;
-    // the new tokens that see one of the tile's
-    const int n0 = max(0, t0 - base), n1 = a.window ? min(seq.news, t0 + 31 + a.window - base) : seq.news;
+    const bool live = r < span.rows;
+    const int nth = live ? r / a.group : 0, head = h * a.group + (live ? r - nth * a.group : 0);
+    const int64_t row = seq.row0 + nth;
+    const int place = seq.length - seq.news + nth, see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
     const Unpack unpack;
-    float sum[8] = {};
-    for (int i0 = n0 * a.group; i0 < n1 * a.group; i0 += 16) {
-        const int idx = i0 + r;
-        const bool live = idx < n1 * a.group;
-        const int nth = live ? idx / a.group : 0, head = h * a.group + (live ? idx - nth * a.group : 0);
-        const int64_t row = seq.row0 + nth;
-        const int place = base + nth, see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
-        h8 qh[D / 32], ql[TWO ? D / 32 : 1];
-        float back, s[8];
-        load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, qh, ql, back);
-        const float lse = live ? a.lse[row * a.heads + head] : 0.0f;
-        tile_scores<D, TWO>(unpack, k, qh, ql, s);
-        const float to_log2 = back * a.scale_log2;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int t = t0 + 8 * j + e;
-            sum[e] += t < see_hi && t >= see_lo ? __builtin_amdgcn_exp2f(s[e] * to_log2 - lse) : 0.0f;
-        }
-    }
+    h8 qh[D / 32], ql[TWO ? D / 32 : 1];
+    float back, s[8];
+    load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
+    const float lse = live ? a.lse[row * a.heads + head] : 0.0f;
+    tile_scores<D, TWO>(unpack, k, qh, ql, s);
+    const float to_log2 = back * fabsf(a.scale_log2);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-#pragma unroll
-        for (int m = 1; m < 16; m <<= 1) sum[e] += __shfl_xor(sum[e], m);
         const int t = t0 + 8 * j + e;
-        if (r == 0 && t < seq.length) {
+        float sum = t < see_hi && t >= see_lo ? __builtin_amdgcn_exp2f(s[e] * to_log2 - lse) : 0.0f;
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1) sum += __shfl_xor(sum, m);
+        if (r == 0 && t < span.hi) {
             float *p = kv_account(kv, a.accounts, b, h, t);
-            if (p) *p += sum[e];
+            if (p) *p += sum;
         }
     }
 }
@@ -859,6 +1023,9 @@ constexpr size_t kMostScoreBytes = (size_t)256 << 20;
 // one of 16384 14 15 15 17 17; D = 64, 16 of up to 8192 28 22 20 19 20; D = 256, 8 of up to 8192 38 30 36 36 42.)
 int split_workgroups(int D) { return std::min(kMostWorkgroups, device_cu_count() * (D == 256 ? 2 : D == 128 ? 3 : 4)); }
 
+// Row tiles that the sequences of a call have, at most.
+int64_t row_tiles_of(const AttendArgs &a) { return (int64_t)a.kv.rows * a.group / kRowsTile + a.kv.seqs; }
+
 template <int D, bool BF16> int attend(const AttendArgs &a, int max_tiles, hipStream_t s) {
     const KvCall &kv = a.kv;
     if (a.workgroups) {
@@ -866,12 +1033,15 @@ template <int D, bool BF16> int attend(const AttendArgs &a, int max_tiles, hipSt
         if (int rc = launch(kv_split_kernel<D, BF16>, dim3((unsigned)grid), dim3(64 * kSplitWaves), 0, s, a)) return rc;
         if (a.part)
             if (int rc = launch(kv_join_kernel<D, BF16>, dim3((unsigned)(kv.max_new * a.group), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a)) return rc;
-    } else if (int rc = launch(kv_rows_kernel<D, BF16>, dim3((unsigned)(a.row_tiles * kv.kv_heads), (unsigned)kv.seqs), dim3(64 * kRowsWaves), 0, s, a)) {
-        return rc;
+        if (!a.accounts) return GQ_OK;
+        if (a.scores) return launch(kv_score_account_kernel, dim3((unsigned)((a.score_tiles + 7) / 8), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
+        return launch(kv_account_kernel<D, BF16>, dim3((unsigned)((max_tiles + 3) / 4), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
     }
+    if (int rc = launch(a.accounts ? kv_rows_kernel<D, BF16, true> : kv_rows_kernel<D, BF16, false>, dim3((unsigned)(row_tiles_of(a) * kv.kv_heads * a.row_pieces)), dim3(64 * kRowsWaves), 0, s, a)) return rc;
+    if (a.row_pieces > 1)
+        if (int rc = launch(kv_rows_join_kernel<D, BF16>, dim3((unsigned)(((int64_t)kv.rows * a.heads * (D / 4) + 255) / 256)), dim3(256), 0, s, a)) return rc;
     if (!a.accounts) return GQ_OK;
-    if (a.scores) return launch(kv_score_account_kernel, dim3((unsigned)((a.score_tiles + 7) / 8), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
-    return launch(kv_account_kernel<D, BF16>, dim3((unsigned)((max_tiles + 3) / 4), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
+    return launch(kv_rows_account_kernel<D, BF16>, dim3((unsigned)max_tiles, (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -899,25 +1069,43 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
         a.workgroups = (int)std::min<int64_t>(split_workgroups(kv.head_dim), (all + kSplitWaves - 1) / kSplitWaves);
         if (tiles > kSplitWaves) lines = (size_t)(a.workgroups + kv.seqs * kv.kv_heads) * a.rows;
     } else {
-        a.row_tiles = (a.rows + kRowsTile - 1) / kRowsTile;
+        // two workgroups a CU, each with four stages of tokens or more
+        const int64_t units = std::max<int64_t>(1, row_tiles_of(a) * kv.kv_heads), stages = kv.head_dim == 256 ? tiles : (tiles + 1) / 2;
+        const int64_t enough = std::min<int64_t>((2 * device_cu_count() + units - 1) / units, std::max<int64_t>(1, stages / 4));
+        a.row_pieces = (int)enough;
+        if (a.row_pieces > 1) lines = line * a.row_pieces;
+        if (accounts) a.operand_tiles = (int)((int64_t)kv.rows * a.group / 32 + kv.seqs + 1);
     }
-    const size_t lse_bytes = accounts ? (line * 4 + 255) / 256 * 256 : 0, ml_bytes = (lines * 8 + 255) / 256 * 256;
+    // scratch memory, each part on a line of its own
+    size_t at = 0;
+    const auto part = [&at](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
     const size_t score_bytes = a.workgroups && accounts ? (size_t)kv.seqs * kv.kv_heads * a.rows * tiles * 128 : 0;
     const bool keep_scores = score_bytes > 0 && score_bytes <= kMostScoreBytes;
-    const size_t part_bytes = lines * (size_t)kv.head_dim * 4, piece_bytes = lines && a.workgroups ? (size_t)kv.seqs * kv.kv_heads * 8 : 0;
-    if (lse_bytes + ml_bytes + part_bytes) {
+    const size_t operand_tiles = (size_t)a.operand_tiles * kv.kv_heads;
+    const size_t lse = part(accounts ? line * 4 : 0), ml = part(lines * 8), sums = part(lines * (size_t)kv.head_dim * 4);
+    const size_t pieces = part(lines && a.workgroups ? (size_t)kv.seqs * kv.kv_heads * 8 : 0), scores = part(keep_scores ? score_bytes : 0);
+    const size_t operands = part(operand_tiles * 32 * kv.head_dim * (q.bf16 ? 2 : 4)), row_scales = part(operand_tiles * 128);
+    if (at) {
         void *ws = nullptr;
-        if (int rc = stream_workspace(s, lse_bytes + ml_bytes + part_bytes + (piece_bytes + 255) / 256 * 256 + (keep_scores ? score_bytes : 0), &ws)) return rc;
+        if (int rc = stream_workspace(s, at, &ws)) return rc;
         unsigned char *p = static_cast<unsigned char *>(ws);
+        if (accounts) a.lse = reinterpret_cast<float *>(p + lse);
+        if (lines) {
+            a.part_ml = reinterpret_cast<float *>(p + ml);
+            a.part = reinterpret_cast<float *>(p + sums);
+            a.pieces = reinterpret_cast<int2 *>(p + pieces);
+        }
         if (keep_scores) {
-            a.scores = reinterpret_cast<float *>(p + lse_bytes + ml_bytes + part_bytes + (piece_bytes + 255) / 256 * 256);
+            a.scores = reinterpret_cast<float *>(p + scores);
             a.score_tiles = (int)tiles;
         }
-        if (lse_bytes) a.lse = reinterpret_cast<float *>(p);
-        if (lines) {
-            a.part_ml = reinterpret_cast<float *>(p + lse_bytes);
-            a.part = reinterpret_cast<float *>(p + lse_bytes + ml_bytes);
-            if (piece_bytes) a.pieces = reinterpret_cast<int2 *>(p + lse_bytes + ml_bytes + part_bytes);
+        if (operand_tiles) {
+            a.operands = p + operands;
+            a.row_scales = reinterpret_cast<float *>(p + row_scales);
         }
     }
     switch (kv.head_dim) {
