@@ -219,25 +219,32 @@ __device__ __forceinline__ void tile_scores(const Unpack &unpack, const KeyWords
 
 constexpr int kSplitWaves = 4;
 
-// The addresses of every `step`-th tile of a sequence and key head.
-struct TileWalk {
-    const uint8_t *cache;
+// The addresses of every STEP-th tile of a sequence and key head.
+template <int BYTES, int STEP> struct TileWalk {
+    const KvCall &kv;
     const int32_t *table;
-    int per_page, slot, in, step, pages, heads, head, bytes;
-    __device__ __forceinline__ TileWalk(const KvCall &kv, int b, int h, int tile, int step_, int bytes_)
-        : cache(kv.cache), table(kv.table + b * kv.table_stride), per_page(kv.page_tokens >> 5), step(step_), pages(kv.pages), heads(kv.kv_heads), head(h), bytes(bytes_) {
+    const uint8_t *at;  // of the next tile; null: its page is none of the cache's
+    int per_page, slot, in, head;
+    __device__ __forceinline__ TileWalk(const KvCall &call, int b, int h, int tile, bool is) : kv(call), table(call.table + b * call.table_stride), at(nullptr), per_page(call.page_tokens >> 5), head(h) {
         slot = tile / per_page;
         in = tile - slot * per_page;
+        if (is) enter();
     }
-    __device__ __forceinline__ const uint8_t *next(bool is) {  // null where there is no tile, or none in the cache
-        const uint8_t *at = nullptr;
-        if (is) {
-            const int page = uniform_load(table + slot);
-            if ((uint32_t)page < (uint32_t)pages) at = cache + (((int64_t)page * heads + head) * per_page + in) * bytes;
-            in += step;
+    __device__ __forceinline__ void enter() {
+        const int page = uniform_load(table + slot);
+        at = (uint32_t)page < (uint32_t)kv.pages ? kv.cache + (((int64_t)page * kv.kv_heads + head) * per_page + in) * BYTES : nullptr;
+    }
+    // this tile's address, and on to the next one if `more` (it exists)
+    __device__ __forceinline__ const uint8_t *next(bool more) {
+        const uint8_t *here = at;
+        in += STEP;
+        if (in < per_page) {
+            at = at ? at + STEP * BYTES : nullptr;
+        } else {
             while (in >= per_page) { in -= per_page; slot++; }
+            if (more) enter();
         }
-        return at;
+        return here;
     }
 };
 
@@ -378,11 +385,11 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
         float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
 
         const int last = min(tile1, (span.hi + 31) >> 5);  // (a unit that sees nothing has a tile in name only)
-        TileWalk walk(kv, b, h, tile0 + wave, kSplitWaves, KvTile<D>::kBytes);
+        TileWalk<KvTile<D>::kBytes, kSplitWaves> walk(kv, b, h, tile0 + wave, tile0 + wave < last);
         // the wavefront's ring of tiles: one is worked on while the next is on its way
         uint8_t *ring = lds + wave * kSplitSlots * Lds::kSlot;
         const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)ring);
-        const uint8_t *mem = walk.next(tile0 + wave < last);
+        const uint8_t *mem = tile0 + wave < last ? walk.next(tile0 + wave + kSplitWaves < last) : nullptr;
         if (mem) fetch_tile<D>(ring_at, mem);
         h8 qh[D / 32], ql[TWO ? D / 32 : 1];
         float back;
@@ -390,7 +397,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
         const float to_log2 = back * fabsf(a.scale_log2);
         int turn = 0;
         for (int tile = tile0 + wave; tile < last; tile += kSplitWaves) {
-            const uint8_t *mem_next = walk.next(tile + kSplitWaves < last);
+            const uint8_t *mem_next = tile + kSplitWaves < last ? walk.next(tile + 2 * kSplitWaves < last) : nullptr;
             if (mem_next) {
                 fetch_tile<D>(ring_at + (uint32_t)(turn ^ 1) * Lds::kSlot, mem_next);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Lds::kLoads) : "memory");
@@ -546,7 +553,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
 }
 
 // Many rows: a workgroup takes 128 neighbouring (new token, head) pairs of a key head, 32 a wavefront, over all the tokens that they
-// see, and widens the cache's codes once for all of them: 64 tokens (D = 256: 32) at a time go through LDS as fp16 operands of
+// see, and widens the cache's codes once for all of them: 8192 values of keys and values each (64 tokens at D = 128) at a time go through LDS as fp16 operands of
 // v_mfma_f32_32x32x16_f16, written in the order in which lanes read them, into the one of two buffers that is not worked on.
 // The instruction's results lie in a lane (r, half) as the operand rows 8 (i / 4) + 4 half + i % 4; operand row m is token m with bits 2
 // and 3 exchanged, so that a lane's results 8 s + 0..7 are the scores of tokens 16 s + 8 half + 0..7: the eight of one dword of value
@@ -558,10 +565,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
 constexpr int kRowsWaves = 4, kRowsTile = 32 * kRowsWaves;
 
 template <int D> struct RowsLds {
-    static constexpr int kTiles = D == 256 ? 1 : 2;                // of the cache, at a time
+    static constexpr int kTiles = 256 / D;                         // of the cache, at a time: a chunk of codes of keys and one of values a thread
     static constexpr int kKeys = 64 * D, kTile = 2 * kKeys;        // bytes of a tile's key operands; of all its operands
     static constexpr int kStage = kTiles * kTile;
-    static constexpr int kItems = kTiles * 2 * D / (64 * kRowsWaves);  // chunks of 16 bytes of codes that a thread widens
 };
 
 // The codes and scales that a thread widens, as loaded: chunk c (four dwords a lane) of a tile's keys or values.
@@ -650,8 +656,10 @@ template <int D, bool BF16, bool ACCOUNTS>
 __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_kernel(const AttendArgs a) {
     constexpr bool TWO = !BF16;
     typedef RowsLds<D> Lds;
-    constexpr int KS = D / 16, VS = D / 32, T = Lds::kTiles, ITEMS = Lds::kItems;
+    constexpr int KS = D / 16, VS = D / 32, T = Lds::kTiles;
     __shared__ __align__(16) uint8_t stage[2][Lds::kStage];
+    __shared__ __align__(4) uint8_t there[2][4];  // which tiles of a stage's keys the cache has
+    constexpr uint32_t ALL = 0x01010101u >> (8 * (4 - T));
     const KvCall &kv = a.kv;
     // (the key head goes round fastest: with eight of them, one to an XCD and its L2)
     const int rest = (int)blockIdx.x / kv.kv_heads, h = (int)blockIdx.x - rest * kv.kv_heads;
@@ -681,50 +689,33 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     const int all_lo = a.window ? base + last_in / a.group + 1 - a.window : 0, any_lo = a.window ? all_hi - a.window : 0;
 
     const Unpack unpack;
-    TileWalk walk(kv, b, h, tile0, 1, KvTile<D>::kBytes);
-    Chunk chunk[ITEMS];
-    uint32_t there = 0;  // tiles of the stage that the cache has, a bit each
-    const auto values_of = [&](int n) { return ITEMS == 1 ? tid >= 128 : n >= ITEMS / 2; };
-    const auto chunk_of = [&](int n) { return ITEMS == 1 ? tid & 127 : n % ((ITEMS + 1) / 2) * 256 + tid; };  // of the stage's keys or values
-    const auto load = [&](int tile) {  // the stage that begins with this tile
-        const uint8_t *mem[T];
-        there = 0;
-#pragma unroll
-        for (int t = 0; t < T; t++) {
-            mem[t] = walk.next(tile + t < tile1);
-            there |= mem[t] ? 1u << t : 0u;
-        }
-#pragma unroll
-        for (int n = 0; n < ITEMS; n++) {
-            const int c = chunk_of(n);
-            const int t = __builtin_amdgcn_readfirstlane(c / D);  // (a wavefront's 64 chunks are of one tile)
-            const uint8_t *at = T == 2 && t ? mem[T - 1] : mem[0];
-            if (at) chunk[n].template load<D>(at, values_of(n), c % D);
-        }
+    // A wavefront widens the same tile of every stage, a thread one chunk of its keys and one of its values.
+    const int part = tid % D, tile_in = __builtin_amdgcn_readfirstlane(tid / D);
+    TileWalk<KvTile<D>::kBytes, T> walk(kv, b, h, tile0 + tile_in, tile0 + tile_in < tile1);
+    const auto locate = [&](int tile) __attribute__((always_inline)) { return tile + tile_in < tile1 ? walk.next(tile + tile_in + T < tile1) : nullptr; };
+    Chunk key_chunk, value_chunk;
+    const auto load = [&](const uint8_t *mem) __attribute__((always_inline)) {
+        key_chunk.template load<D>(mem, false, part);
+        value_chunk.template load<D>(mem, true, part);
     };
-    const auto widen = [&](uint8_t *to) {
-#pragma unroll
-        for (int n = 0; n < ITEMS; n++) {
-            const int c = chunk_of(n);
-            const int t = __builtin_amdgcn_readfirstlane(c / D);
-            if ((there >> t) & 1u) chunk[n].template widen<D>(unpack, to + t * Lds::kTile, values_of(n), c % D);
-            else Chunk::template clear<D>(to + t * Lds::kTile, values_of(n), c % D);
+    const auto widen = [&](const uint8_t *mem, int to) __attribute__((always_inline)) {
+        uint8_t *at = stage[to] + tile_in * Lds::kTile;
+        if (mem) {
+            key_chunk.template widen<D>(unpack, at, false, part);
+            value_chunk.template widen<D>(unpack, at, true, part);
+        } else {
+            Chunk::template clear<D>(at, false, part);
+            Chunk::template clear<D>(at, true, part);
         }
+        if (part == 0) there[to][tile_in] = mem ? 1 : 0;
     };
 
-    if (tile0 < tile1) load(tile0);
+    const uint8_t *first = locate(tile0);
+    if (first) load(first);
     h8 qh[KS], ql[TWO ? KS : 1];
     float back;
     load_queries<D, 32, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
     const float to_log2 = fmaxf(back * fabsf(a.scale_log2), 1e-37f);  // (not 0, so that its product with -infinity stays that)
-
-    f16 o[VS];
-#pragma unroll
-    for (int w = 0; w < VS; w++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[w][i] = 0.0f;
-    float ref = kNegInf, total = 0.0f;
-
     if (ACCOUNTS && piece == 0 && wave * 32 < span.rows) {
         const int64_t tile = (int64_t)h * a.operand_tiles + first_operand_tile(a, seq, b) + row_tile * kRowsWaves + wave;
         h8 *to = reinterpret_cast<h8 *>(a.operands) + tile * (TWO ? 2 : 1) * KS * 64 + lane;
@@ -735,88 +726,97 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
         }
         if (half == 0) a.row_scales[tile * 32 + r] = to_log2;
     }
-    if (tile0 < tile1) widen(stage[0]);
-    uint32_t now = there;
-    __syncthreads();
-    int turn = 0;
-    for (int tile = tile0; tile < tile1; tile += T) {
+
+    f16 o[VS];
+#pragma unroll
+    for (int w = 0; w < VS; w++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[w][i] = 0.0f;
+    float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
+
+    // One stage, from buffer `mine`; the next one goes into `other`.  (Making the next stage's scores in front of these weights, so that one wavefront has
+    // both kinds of work to issue, was no faster: the second workgroup of the CU does as well.)
+    const auto step = [&](int tile, int mine, int other) __attribute__((always_inline)) {
         const bool more = tile + T < tile1;
-        if (more) load(tile + T);
+        const uint8_t *next = more ? locate(tile + T) : nullptr;
+        if (next) load(next);
+        f16 s[T];
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const h8 x = *reinterpret_cast<const h8 *>(stage[mine] + t * Lds::kTile + (k * 64 + lane) * 16);
+                s[t] = mfma32(x, qh[k], s[t]);
+                if constexpr (TWO) s[t] = mfma32(x, ql[k], s[t]);
+            }
+        }
         const int t0 = tile * 32;
-        if (t0 < any_hi && t0 + 32 * T > any_lo) {
-            const uint8_t *from = stage[turn];
-            f16 s[T];
-#pragma unroll
-            for (int t = 0; t < T; t++) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    const h8 x = *reinterpret_cast<const h8 *>(from + t * Lds::kTile + (k * 64 + lane) * 16);
-                    s[t] = mfma32(x, qh[k], s[t]);
-                    if constexpr (TWO) s[t] = mfma32(x, ql[k], s[t]);
-                }
-            }
-            float most = kNegInf;  // (scores as the products left them: what they are multiplied by is not negative)
-            if (!(t0 >= all_lo && t0 + 32 * T <= all_hi && now == (1u << T) - 1)) {
-#pragma unroll
-                for (int t = 0; t < T; t++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int token = t0 + 32 * t + 16 * (i >> 3) + 8 * half + (i & 7);
-                        s[t][i] = token < see_hi && token >= see_lo && ((now >> t) & 1u) ? s[t][i] : kNegInf;
-                    }
-            }
+        const uint32_t known = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(there[mine])) & ALL;
+        if (!(t0 >= all_lo && t0 + 32 * T <= all_hi && known == ALL)) {
 #pragma unroll
             for (int t = 0; t < T; t++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) most = fmaxf(most, s[t][i]);
-            if (most != kNegInf) most *= to_log2;
-            if (__any(most > ref + kMostLog2)) {
-                most = fmaxf(most, __shfl_xor(most, 32));
-                const float next = fmaxf(ref, most - kHeadroom);
-                const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
-                ref = next;
-                total *= shrink;
+                for (int i = 0; i < 16; i++) {
+                    const int token = t0 + 32 * t + 16 * (i >> 3) + 8 * half + (i & 7);
+                    s[t][i] = token < see_hi && token >= see_lo && ((known >> (8 * t)) & 1u) ? s[t][i] : kNegInf;
+                }
+        }
+        float most = kNegInf;  // (scores as the products left them: what they are multiplied by is not negative)
 #pragma unroll
-                for (int w = 0; w < VS; w++) o[w] *= shrink;
-            }
-            const float less = ref == kNegInf ? 0.0f : -ref;
+        for (int t = 0; t < T; t++)
 #pragma unroll
-            for (int t = 0; t < T; t++) {
+            for (int i = 0; i < 16; i++) most = fmaxf(most, s[t][i]);
+        if (__any(most * to_log2 > ref + kMostLog2)) {
+            most *= to_log2;
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const float set = fmaxf(ref, most - kHeadroom);
+            const float shrink = set == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - set);
+            ref = set;
+            total *= shrink;
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    h8 ph, pl;
+            for (int w = 0; w < VS; w++) o[w] *= shrink;
+        }
+        const float less = ref == kNegInf ? 0.0f : -ref;
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e], to_log2, less)), p1 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e + 1], to_log2, less));
-                        ph[e] = (_Float16)p0;
-                        ph[e + 1] = (_Float16)p1;
-                        if constexpr (TWO) {
-                            pl[e] = (_Float16)(p0 - (float)ph[e]);
-                            pl[e + 1] = (_Float16)(p1 - (float)ph[e + 1]);
-                        }
-                        if constexpr (TWO || ACCOUNTS) {  // (accounts are kept to fp32's accuracy whatever the type)
-                            total += p0;
-                            total += p1;
-                        } else {  // the weights as they are used, two in one instruction
-                            const h2 pair = {ph[e], ph[e + 1]}, ones = {(_Float16)1.0f, (_Float16)1.0f};
-                            total = __builtin_amdgcn_fdot2(pair, ones, total, false);
-                        }
+        for (int t = 0; t < T; t++) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                h8 ph, pl;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e], to_log2, less)), p1 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e + 1], to_log2, less));
+                    ph[e] = (_Float16)p0;
+                    ph[e + 1] = (_Float16)p1;
+                    if constexpr (TWO) {
+                        pl[e] = (_Float16)(p0 - (float)ph[e]);
+                        pl[e + 1] = (_Float16)(p1 - (float)ph[e + 1]);
                     }
-#pragma unroll
-                    for (int w = 0; w < VS; w++) {
-                        const h8 x = *reinterpret_cast<const h8 *>(from + t * Lds::kTile + Lds::kKeys + ((w * 2 + k) * 64 + lane) * 16);
-                        o[w] = mfma32(x, ph, o[w]);
-                        if constexpr (TWO) o[w] = mfma32(x, pl, o[w]);
+                    if constexpr (TWO || ACCOUNTS) {  // (accounts are kept to fp32's accuracy whatever the type)
+                        total += p0;
+                        total += p1;
+                    } else {  // the weights as they are used, two in one instruction
+                        const h2 pair = {ph[e], ph[e + 1]}, ones = {(_Float16)1.0f, (_Float16)1.0f};
+                        total = __builtin_amdgcn_fdot2(pair, ones, total, false);
                     }
+                }
+#pragma unroll
+                for (int w = 0; w < VS; w++) {
+                    const h8 x = *reinterpret_cast<const h8 *>(stage[mine] + t * Lds::kTile + Lds::kKeys + ((w * 2 + k) * 64 + lane) * 16);
+                    o[w] = mfma32(x, ph, o[w]);
+                    if constexpr (TWO) o[w] = mfma32(x, pl, o[w]);
                 }
             }
         }
-        if (more) widen(stage[turn ^ 1]);
-        now = there;
-        turn ^= 1;
+        if (more) widen(next, other);
         __syncthreads();
+    };
+    if (tile0 < tile1) widen(first, 0);
+    __syncthreads();
+    for (int tile = tile0; tile < tile1; tile += 2 * T) {
+        step(tile, 0, 1);
+        if (tile + T < tile1) step(tile + T, 1, 0);
     }
     total += __shfl_xor(total, 32);
     if (!live) return;
@@ -1069,9 +1069,9 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
         a.workgroups = (int)std::min<int64_t>(split_workgroups(kv.head_dim), (all + kSplitWaves - 1) / kSplitWaves);
         if (tiles > kSplitWaves) lines = (size_t)(a.workgroups + kv.seqs * kv.kv_heads) * a.rows;
     } else {
-        // two workgroups a CU, each with four stages of tokens or more
-        const int64_t units = std::max<int64_t>(1, row_tiles_of(a) * kv.kv_heads), stages = kv.head_dim == 256 ? tiles : (tiles + 1) / 2;
-        const int64_t enough = std::min<int64_t>((2 * device_cu_count() + units - 1) / units, std::max<int64_t>(1, stages / 4));
+        // two workgroups a CU, each with 256 tokens or more
+        const int64_t units = std::max<int64_t>(1, row_tiles_of(a) * kv.kv_heads);
+        const int64_t enough = std::min<int64_t>((2 * device_cu_count() + units - 1) / units, std::max<int64_t>(1, tiles / 8));
         a.row_pieces = (int)enough;
         if (a.row_pieces > 1) lines = line * a.row_pieces;
         if (accounts) a.operand_tiles = (int)((int64_t)kv.rows * a.group / 32 + kv.seqs + 1);
