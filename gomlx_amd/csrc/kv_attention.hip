@@ -219,32 +219,26 @@ __device__ __forceinline__ void tile_scores(const Unpack &unpack, const KeyWords
 
 constexpr int kSplitWaves = 4;
 
-// The addresses of every STEP-th tile of a sequence and key head.
+// The addresses of every STEP-th tile of a sequence and key head from `tile` to `end`; the page of the next one is asked for a call ahead.
 template <int BYTES, int STEP> struct TileWalk {
     const KvCall &kv;
     const int32_t *table;
-    const uint8_t *at;  // of the next tile; null: its page is none of the cache's
-    int per_page, slot, in, head;
-    __device__ __forceinline__ TileWalk(const KvCall &call, int b, int h, int tile, bool is) : kv(call), table(call.table + b * call.table_stride), at(nullptr), per_page(call.page_tokens >> 5), head(h) {
+    int head, per_page, slot, in, left, page;
+    __device__ __forceinline__ TileWalk(const KvCall &call, int b, int h, int tile, int end)
+        : kv(call), table(call.table + b * call.table_stride), head(h), per_page(call.page_tokens >> 5), left(tile < end ? (end - tile + STEP - 1) / STEP : 0), page(-1) {
         slot = tile / per_page;
         in = tile - slot * per_page;
-        if (is) enter();
+        if (left) page = uniform_load(table + slot);
     }
-    __device__ __forceinline__ void enter() {
-        const int page = uniform_load(table + slot);
-        at = (uint32_t)page < (uint32_t)kv.pages ? kv.cache + (((int64_t)page * kv.kv_heads + head) * per_page + in) * BYTES : nullptr;
-    }
-    // this tile's address, and on to the next one if `more` (it exists)
-    __device__ __forceinline__ const uint8_t *next(bool more) {
-        const uint8_t *here = at;
+    // null behind the last one, and where the page is none of the cache's
+    __device__ __forceinline__ const uint8_t *next() {
+        if (left == 0) return nullptr;
+        const uint8_t *at = (uint32_t)page < (uint32_t)kv.pages ? kv.cache + (((int64_t)page * kv.kv_heads + head) * per_page + in) * BYTES : nullptr;
+        left--;
         in += STEP;
-        if (in < per_page) {
-            at = at ? at + STEP * BYTES : nullptr;
-        } else {
-            while (in >= per_page) { in -= per_page; slot++; }
-            if (more) enter();
-        }
-        return here;
+        while (in >= per_page) { in -= per_page; slot++; }
+        if (left) page = uniform_load(table + slot);
+        return at;
     }
 };
 
@@ -385,11 +379,11 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
         float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
 
         const int last = min(tile1, (span.hi + 31) >> 5);  // (a unit that sees nothing has a tile in name only)
-        TileWalk<KvTile<D>::kBytes, kSplitWaves> walk(kv, b, h, tile0 + wave, tile0 + wave < last);
+        TileWalk<KvTile<D>::kBytes, kSplitWaves> walk(kv, b, h, tile0 + wave, last);
         // the wavefront's ring of tiles: one is worked on while the next is on its way
         uint8_t *ring = lds + wave * kSplitSlots * Lds::kSlot;
         const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)ring);
-        const uint8_t *mem = tile0 + wave < last ? walk.next(tile0 + wave + kSplitWaves < last) : nullptr;
+        const uint8_t *mem = walk.next();
         if (mem) fetch_tile<D>(ring_at, mem);
         h8 qh[D / 32], ql[TWO ? D / 32 : 1];
         float back;
@@ -397,7 +391,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
         const float to_log2 = back * fabsf(a.scale_log2);
         int turn = 0;
         for (int tile = tile0 + wave; tile < last; tile += kSplitWaves) {
-            const uint8_t *mem_next = tile + kSplitWaves < last ? walk.next(tile + 2 * kSplitWaves < last) : nullptr;
+            const uint8_t *mem_next = walk.next();
             if (mem_next) {
                 fetch_tile<D>(ring_at + (uint32_t)(turn ^ 1) * Lds::kSlot, mem_next);
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Lds::kLoads) : "memory");
@@ -562,7 +556,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
 // Matrix instructions, exponentials and the widening run side by side, two workgroups a CU (2048 rows of 32 heads over 2049 to 4096
 // tokens, D = 128).  With a causal bound workgroups differ in length: the second half of them goes from short to long, so that the two of a CU
 // add up to the same.
-constexpr int kRowsWaves = 4, kRowsTile = 32 * kRowsWaves;
+constexpr int kRowsWaves = 4, kRowsTile = 32 * kRowsWaves, kRowsPiece = 12;  // rows of a workgroup; tiles of the cache, at least, in a piece of its tokens
 
 template <int D> struct RowsLds {
     static constexpr int kTiles = 256 / D;                         // of the cache, at a time: a chunk of codes of keys and one of values a thread
@@ -685,33 +679,38 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     const int see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
     // what every row of the wavefront sees, and what one of them does
     const int first_in = span.first_row + wave * 32, last_in = min(first_in + 31, span.first_row + span.rows - 1);
-    const int all_hi = base + first_in / a.group + 1, any_hi = wave * 32 < span.rows ? base + last_in / a.group + 1 : 0;
-    const int all_lo = a.window ? base + last_in / a.group + 1 - a.window : 0, any_lo = a.window ? all_hi - a.window : 0;
+    const int all_hi = __builtin_amdgcn_readfirstlane(base + first_in / a.group + 1);
+    const int all_lo = __builtin_amdgcn_readfirstlane(a.window ? base + last_in / a.group + 1 - a.window : 0);
 
     const Unpack unpack;
     // A wavefront widens the same tile of every stage, a thread one chunk of its keys and one of its values.
     const int part = tid % D, tile_in = __builtin_amdgcn_readfirstlane(tid / D);
-    TileWalk<KvTile<D>::kBytes, T> walk(kv, b, h, tile0 + tile_in, tile0 + tile_in < tile1);
-    const auto locate = [&](int tile) __attribute__((always_inline)) { return tile + tile_in < tile1 ? walk.next(tile + tile_in + T < tile1) : nullptr; };
-    Chunk key_chunk, value_chunk;
-    const auto load = [&](const uint8_t *mem) __attribute__((always_inline)) {
-        key_chunk.template load<D>(mem, false, part);
-        value_chunk.template load<D>(mem, true, part);
+    TileWalk<KvTile<D>::kBytes, T> walk(kv, b, h, tile0 + tile_in, tile1);
+    struct Fetched {  // of a stage, on its way
+        const uint8_t *mem;
+        Chunk keys, values;
+    } fetched[2];
+    const auto load = [&](Fetched &f) __attribute__((always_inline)) {
+        f.mem = walk.next();
+        if (f.mem) {
+            f.keys.template load<D>(f.mem, false, part);
+            f.values.template load<D>(f.mem, true, part);
+        }
     };
-    const auto widen = [&](const uint8_t *mem, int to) __attribute__((always_inline)) {
+    const auto widen = [&](const Fetched &f, int to) __attribute__((always_inline)) {
         uint8_t *at = stage[to] + tile_in * Lds::kTile;
-        if (mem) {
-            key_chunk.template widen<D>(unpack, at, false, part);
-            value_chunk.template widen<D>(unpack, at, true, part);
+        if (f.mem) {
+            f.keys.template widen<D>(unpack, at, false, part);
+            f.values.template widen<D>(unpack, at, true, part);
         } else {
             Chunk::template clear<D>(at, false, part);
             Chunk::template clear<D>(at, true, part);
         }
-        if (part == 0) there[to][tile_in] = mem ? 1 : 0;
+        if (part == 0) there[to][tile_in] = f.mem ? 1 : 0;
     };
 
-    const uint8_t *first = locate(tile0);
-    if (first) load(first);
+    load(fetched[0]);
+    load(fetched[1]);
     h8 qh[KS], ql[TWO ? KS : 1];
     float back;
     load_queries<D, 32, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
@@ -734,12 +733,10 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
         for (int i = 0; i < 16; i++) o[w][i] = 0.0f;
     float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
 
-    // One stage, from buffer `mine`; the next one goes into `other`.  (Making the next stage's scores in front of these weights, so that one wavefront has
+    // One stage, from buffer `mine`; the next one, which has been on its way for a stage, goes into `other`.  (Making the next stage's scores in front of these weights, so that one wavefront has
     // both kinds of work to issue, was no faster: the second workgroup of the CU does as well.)
     const auto step = [&](int tile, int mine, int other) __attribute__((always_inline)) {
-        const bool more = tile + T < tile1;
-        const uint8_t *next = more ? locate(tile + T) : nullptr;
-        if (next) load(next);
+        load(fetched[mine]);
         f16 s[T];
 #pragma unroll
         for (int t = 0; t < T; t++) {
@@ -752,6 +749,14 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
                 if constexpr (TWO) s[t] = mfma32(x, ql[k], s[t]);
             }
         }
+        // (operands are read four instructions ahead)
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < T * KS - 4; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, TWO ? 2 : 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, TWO ? 8 : 4, 0);
         const int t0 = tile * 32;
         const uint32_t known = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(there[mine])) & ALL;
         if (!(t0 >= all_lo && t0 + 32 * T <= all_hi && known == ALL)) {
@@ -809,10 +814,20 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
                 }
             }
         }
-        if (more) widen(next, other);
+        // (the weights of sixteen tokens are made while the products with those in front run)
+        __builtin_amdgcn_sched_group_barrier(0x002, 26, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+        for (int i = 0; i < 2 * T * VS - 4; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, TWO ? 2 : 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x002, 6, 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, TWO ? 8 : 4, 1);
+        if (tile + T < tile1) widen(fetched[other], other);
         __syncthreads();
     };
-    if (tile0 < tile1) widen(first, 0);
+    if (tile0 < tile1) widen(fetched[0], 0);
     __syncthreads();
     for (int tile = tile0; tile < tile1; tile += 2 * T) {
         step(tile, 0, 1);
@@ -1069,10 +1084,12 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
         a.workgroups = (int)std::min<int64_t>(split_workgroups(kv.head_dim), (all + kSplitWaves - 1) / kSplitWaves);
         if (tiles > kSplitWaves) lines = (size_t)(a.workgroups + kv.seqs * kv.kv_heads) * a.rows;
     } else {
-        // two workgroups a CU, each with 256 tokens or more
+        // As many workgroups as run at a time, each with enough tokens to be worth the 32 to 128 KB of sums that it leaves (us a call with 8, 12, 16, 32 tiles at
+        // least, D = 128: 512 tokens over 600 27 22 22 22, 64 of 4 sequences over 2000 31 29 30 36, 32 of 2 over 8000 36 34 35 40; D = 64, 301 of 5 over
+        // 1111 in a window 43 43 48 49)
         const int64_t units = std::max<int64_t>(1, row_tiles_of(a) * kv.kv_heads);
-        const int64_t enough = std::min<int64_t>((2 * device_cu_count() + units - 1) / units, std::max<int64_t>(1, tiles / 8));
-        a.row_pieces = (int)enough;
+        const int64_t enough = std::min<int64_t>((kv.head_dim == 256 ? 1 : 2) * device_cu_count() / units, std::max<int64_t>(1, tiles / kRowsPiece));
+        a.row_pieces = (int)std::max<int64_t>(1, enough);
         if (a.row_pieces > 1) lines = line * a.row_pieces;
         if (accounts) a.operand_tiles = (int)((int64_t)kv.rows * a.group / 32 + kv.seqs + 1);
     }
