@@ -1260,7 +1260,10 @@ int check_kv(const char *fn, const gq_kv_cache *kv, bool by_rows, KvCall *call) 
     }
     const bool starts = by_rows && kv->dStarts;
     *call = KvCall{static_cast<uint8_t *>(kv->dCache), (int)kv->pages, kv->kv_heads, kv->head_dim, kv->page_tokens, kv->dPageTable, kv->table_stride, kv->max_pages,
-                   kv->dLengths, starts ? kv->dStarts : nullptr, (int)kv->seqs, (int)rows, (int)(starts ? std::min(max_new, rows) : 1)};
+                   kv->dLengths, starts ? kv->dStarts : nullptr, (int)kv->seqs, (int)rows, (int)(starts ? std::min(max_new, rows) : 1), 0};
+    // ceil(2^32 / d) is over 2^32 / d by less than 1: exact for tiles below 2^32 / d
+    const uint64_t d = (uint64_t)kv->page_tokens / 32;
+    if (d > 1 && (uint64_t)kv->max_pages * d * d < (1ull << 32)) call->page_magic = (uint32_t)(((1ull << 32) + d - 1) / d);
     return GQ_OK;
 }
 }  // namespace

@@ -155,6 +155,7 @@ struct KvCall {
     int max_pages;
     const int32_t *lengths, *starts;  // starts null: row b is sequence b's one new token
     int seqs, rows, max_new;
+    uint32_t page_magic;  // tile / (page_tokens / 32) is the upper half of its product with this; 0: divide
 };
 // rows of head vectors, strides in elements, the values of a vector side by side
 struct HeadRows { const void *p; int64_t row, head; bool bf16; };

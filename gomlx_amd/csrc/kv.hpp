@@ -56,10 +56,15 @@ __device__ __forceinline__ KvSeq kv_seq(const KvCall &kv, int b) {
     return s;
 }
 
+// the place in the page table of a sequence's tile
+__device__ __forceinline__ int page_slot(const KvCall &kv, int tile) {
+    return kv.page_magic ? (int)__umulhi((uint32_t)tile, kv.page_magic) : tile / (kv.page_tokens >> 5);
+}
+
 // Tile `tile` of sequence b and key head h; null where the page table names no page of the cache.
 __device__ __forceinline__ uint8_t *kv_tile(const KvCall &kv, int b, int h, int tile, int tile_bytes) {
     const int per_page = kv.page_tokens >> 5;
-    const int slot = tile / per_page;
+    const int slot = page_slot(kv, tile);
     const int page = kv.table[b * kv.table_stride + slot];
     if ((uint32_t)page >= (uint32_t)kv.pages) return nullptr;
     return kv.cache + (((int64_t)page * kv.kv_heads + h) * per_page + (tile - slot * per_page)) * tile_bytes;
@@ -67,7 +72,7 @@ __device__ __forceinline__ uint8_t *kv_tile(const KvCall &kv, int b, int h, int 
 
 // The account of token p of sequence b and key head h; null as above.
 __device__ __forceinline__ float *kv_account(const KvCall &kv, float *accounts, int b, int h, int p) {
-    const int slot = p / kv.page_tokens;
+    const int slot = page_slot(kv, p >> 5);
     const int page = kv.table[b * kv.table_stride + slot];
     if ((uint32_t)page >= (uint32_t)kv.pages) return nullptr;
     return accounts + ((int64_t)page * kv.kv_heads + h) * kv.page_tokens + (p - slot * kv.page_tokens);

@@ -226,7 +226,7 @@ template <int BYTES, int STEP> struct TileWalk {
     int head, per_page, slot, in, left, page;
     __device__ __forceinline__ TileWalk(const KvCall &call, int b, int h, int tile, int end)
         : kv(call), table(call.table + b * call.table_stride), head(h), per_page(call.page_tokens >> 5), left(tile < end ? (end - tile + STEP - 1) / STEP : 0), page(-1) {
-        slot = tile / per_page;
+        slot = page_slot(call, tile);
         in = tile - slot * per_page;
         if (left) page = uniform_load(table + slot);
     }

@@ -92,29 +92,48 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
     const int b = (int)(unit / per);
     if (b >= kv.seqs) return;
     const int rest = (int)(unit - (int64_t)b * per), h = rest / a.blocks, nth = rest - h * a.blocks;
+    const int lane = (int)threadIdx.x & 63, l = lane % L, x = l * 8, mine = lane / L;  // the lane's values; its token of a round
+    const int g = x >> 5;
+    float k[ROUNDS][8], v[ROUNDS][8];
+    if (!kv.starts) {  // one row, which is known before the sequence's length is: whichever of the eight tokens it turns out to be
+        load8<BF16>(k[0], a.k.p, (int64_t)b * a.k.row + h * a.k.head + x, a.wide);
+        load8<BF16>(v[0], a.v.p, (int64_t)b * a.v.row + h * a.v.head + x, a.wide);
+    }
     const KvSeq s = kv_seq(kv, b);
     const int first = s.length - s.news, from = first < 0 ? 0 : first;
     const int block = (from >> 3) + nth, p0 = block * 8;
     if (p0 >= s.length || s.news == 0) return;
     uint8_t *tile = kv_tile(kv, b, h, p0 >> 5, T::kBytes);
     if (!tile) return;
-    const int lane = (int)threadIdx.x & 63, l = lane % L, x = l * 8, mine = lane / L;  // the lane's values; its token of a round
-    const int j = (p0 >> 3) & 3, g = x >> 5;
+    const int j = (p0 >> 3) & 3;
     const bool account = a.accounts && l == 0;
     const int live_from = from > p0 ? from - p0 : 0, live_to = s.length - p0 < 8 ? s.length - p0 : 8;  // new tokens of the block
-
-    float k[ROUNDS][8], v[ROUNDS][8];
+    uint32_t live_mask = 0;
+    for (int e = live_from; e < live_to; e++) live_mask |= 0xFu << nibble_shift(e);
+    // the dwords of value codes that the lane will finish, where other tokens share them
+    uint32_t *value_at[ROUNDS], old[ROUNDS];
 #pragma unroll
-    for (int n = 0; n < ROUNDS; n++) {
-        const int e = n * PER + mine;
-        if (e >= live_from && e < live_to) {
-            const int64_t row = s.row0 + (p0 + e - first);
+    for (int i = 0; i < ROUNDS; i++) {
+        const int c = x + mine * ROUNDS + i;
+        value_at[i] = reinterpret_cast<uint32_t *>(tile + T::kValues + T::code(c >> 4, (c & 15) + 16 * j));
+        old[i] = live_mask == 0xFFFFFFFFu ? 0u : *value_at[i];
+    }
+    if (kv.starts) {
+#pragma unroll
+        for (int n = 0; n < ROUNDS; n++) {
+            const int e = n * PER + mine;
+            const int64_t row = s.row0 + min(max(p0 + e - first, 0), s.news - 1);
             load8<BF16>(k[n], a.k.p, row * a.k.row + h * a.k.head + x, a.wide);
             load8<BF16>(v[n], a.v.p, row * a.v.row + h * a.v.head + x, a.wide);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) k[n][i] = v[n][i] = 0.0f;
         }
+    } else {
+#pragma unroll
+        for (int n = 1; n < ROUNDS; n++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                k[n][i] = k[0][i];
+                v[n][i] = v[0][i];
+            }
     }
     uint32_t bits[8] = {};
 #pragma unroll
@@ -152,8 +171,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
             }
         }
     }
-    // lanes of equal values, L, 2 L, ... apart, pass each other the dwords that the other one finishes
-    int count = 8, base = 0;
+    // Lanes of equal values, L, 2 L, ... apart, pass each other the dwords that the other one finishes: lane `mine` of them those from mine * ROUNDS on.
+    int count = 8;
 #pragma unroll
     for (int m = 32; m >= L; m >>= 1) {
         count >>= 1;
@@ -164,16 +183,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
             const uint32_t give = upper ? bits[i] : bits[i + count], keep = upper ? bits[i + count] : bits[i];
             bits[i] = keep | (uint32_t)__shfl_xor((int)give, m);
         }
-        base += upper ? count : 0;
     }
-    uint32_t live_mask = 0;
-    for (int e = live_from; e < live_to; e++) live_mask |= 0xFu << nibble_shift(e);
 #pragma unroll
-    for (int i = 0; i < ROUNDS; i++) {
-        const int c = x + base + i;
-        uint32_t *at = reinterpret_cast<uint32_t *>(tile + T::kValues + T::code(c >> 4, (c & 15) + 16 * j));
-        *at = live_mask == 0xFFFFFFFFu ? bits[i] : (*at & ~live_mask) | bits[i];
-    }
+    for (int i = 0; i < ROUNDS; i++) *value_at[i] = (old[i] & ~live_mask) | bits[i];
 }
 
 // What the cache stands for at the last tokens of every sequence, in the fp16 numbers that it holds; zeros in front of a
@@ -239,7 +251,7 @@ __device__ __forceinline__ uint32_t account_key(float f) {
 }
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
-constexpr int kBins = 2048;
+constexpr int kBins = 2048, kFew = 512;
 
 // The sum of v over the threads in front, and over all.
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *waves, uint32_t &total) {
@@ -267,11 +279,11 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *waves, uint
 // One workgroup per sequence and key head.  A wavefront owns a run of neighbouring tokens, 64 at a time, and holds their keys in
 // registers where IT rounds of them suffice (IT = 0: reads them again for every pass).  The smallest kept key is found digit by
 // digit, eleven bits at a time of its distance from the smallest key there is, so that keys of similar size spread over the
-// histogram (those that equal the smallest, zeros mostly, are left out of it); a wavefront then counts what it keeps, and
+// histogram (those that equal the smallest, zeros mostly, are left out of it), until so few are left that each is held against all of them; a wavefront then counts what it keeps, and
 // writes its tokens behind those of the wavefronts in front.
 template <int IT>
 __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall kv, const float *__restrict__ accounts, int keep, int recent, int32_t *__restrict__ kept) {
-    __shared__ uint32_t hist[kBins], waves[kSelectWaves], found[2], ends[2][kSelectWaves];
+    __shared__ uint32_t hist[kBins], waves[kSelectWaves], found[2], ends[2][kSelectWaves], few[kFew], count;
     const int h = (int)blockIdx.x, b = (int)blockIdx.y, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const KvSeq s = kv_seq(kv, b);
     int32_t *out = kept + ((int64_t)b * kv.kv_heads + h) * keep;
@@ -292,8 +304,18 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall 
     };
     uint32_t keys[IT ? IT : 1];
     if constexpr (IT > 0) {
+        // (loads without branches between them, of the last token where there is none: they go out together)
+        int64_t at[IT];
 #pragma unroll
-        for (int i = 0; i < IT; i++) keys[i] = t0 + 64 * i < n ? key_at(t0 + 64 * i) : 0u;
+        for (int i = 0; i < IT; i++) {
+            const int t = min(t0 + 64 * i, n - 1), slot = page_slot(kv, t >> 5), page = kv.table[b * kv.table_stride + slot];
+            at[i] = (uint32_t)page < (uint32_t)kv.pages ? ((int64_t)page * kv.kv_heads + h) * kv.page_tokens + (t - slot * kv.page_tokens) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < IT; i++) {
+            const uint32_t u = kv.pages ? account_key(accounts[max(at[i], (int64_t)0)]) : 0u;
+            keys[i] = at[i] < 0 ? 0u : u;
+        }
     }
     const auto each = [&](auto f) {  // f(token, key) for the thread's tokens
         if constexpr (IT > 0) {
@@ -353,6 +375,27 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall 
         }
         key += digit << shift;
         width = shift;
+        if (width == 0 || hist[digit] > kFew) continue;
+        // few are left: each against all of them
+        if (tid == 0) count = 0;
+        __syncthreads();
+        each([&](int, uint32_t u) {
+            if (u > low && u >= key && u - key < (1u << width)) few[atomicAdd(&count, 1u)] = u;
+        });
+        __syncthreads();
+        const uint32_t all = count, mine = (uint32_t)tid < all ? few[tid] : 0;
+        if ((uint32_t)tid < all) {
+            uint32_t above = 0, same = 0;
+            for (uint32_t i = 0; i < all; i++) {
+                above += few[i] > mine;
+                same += few[i] == mine;
+            }
+            if (above < want && want <= above + same) { found[0] = mine; found[1] = want - above; }  // (all that equal it write the same)
+        }
+        __syncthreads();
+        key = found[0];
+        want = found[1];
+        break;
     }
     // u > key stay, and the first `want` that equal it
     uint32_t more = 0, same = 0;
@@ -408,36 +451,59 @@ template <int D>
 __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvCall kv, float *accounts, int keep, const int32_t *__restrict__ kept, int32_t *new_lengths) {
     typedef KvTile<D> T;
     constexpr int G = T::G, R = kMoveTokens / kMoveThreads;
-    __shared__ int64_t source[kMoveTokens];  // tile * 32 + token in it; -1: nothing comes
+    __shared__ int64_t sources[2][kMoveTokens];  // tile * 32 + token in it
     const int h = (int)blockIdx.x, b = (int)blockIdx.y, part = (int)blockIdx.z, tid = (int)threadIdx.x;
     const int32_t *list = kept + ((int64_t)b * kv.kv_heads + h) * keep;
     // (new_lengths may be kv.lengths: nobody else reads them in this launch)
     if (h == 0 && part == 0 && tid == 0) new_lengths[b] = min(kv_seq(kv, b).length, keep);
-    if (list[keep - 1] < keep) return;  // nothing to move: as many tokens as places, or fewer (-1)
+    if (list[keep - 1] < keep || kv.pages == 0) return;  // nothing to move: as many tokens as places, or fewer (-1)
     const int per_page = kv.page_tokens >> 5;
     const auto tile_number = [&](int tile) -> int64_t {
-        const int slot = tile / per_page, page = kv.table[b * kv.table_stride + slot];
+        const int slot = page_slot(kv, tile), page = kv.table[b * kv.table_stride + slot];
         return (uint32_t)page < (uint32_t)kv.pages ? ((int64_t)page * kv.kv_heads + h) * per_page + (tile - slot * per_page) : -1;
     };
-    for (int i0 = 0; i0 < keep; i0 += kMoveTokens) {
-        if (list[min(i0 + kMoveTokens, keep) - 1] == min(i0 + kMoveTokens, keep) - 1) continue;  // all of these stay where they are
+    // Where the tokens of a step come from, found out a step ahead.  (-1 behind the last one, and where the page table names no page: nothing is written there;
+    // what is read for it is the cache's first tile, so that loads need no branches between them and go out together.)
+    int entry[R];
+    bool stay;  // the thread's tokens of the step are where they belong
+    const auto ask = [&](int i0) {
 #pragma unroll
         for (int n = 0; n < R; n++) {
             const int i = i0 + n * kMoveThreads + tid;
-            const int t = i < keep ? list[i] : 0;
-            const int64_t tile = i < keep ? tile_number(t >> 5) : -1;
-            source[n * kMoveThreads + tid] = tile < 0 ? -1 : tile * 32 + (t & 31);
+            entry[n] = i < keep ? list[i] : -1;
         }
-        __syncthreads();
+    };
+    const auto found = [&](int64_t *to, int at) {
+        int64_t tile[R];
+#pragma unroll
+        for (int n = 0; n < R; n++) tile[n] = tile_number(max(entry[n], 0) >> 5);
+#pragma unroll
+        for (int n = 0; n < R; n++) to[n * kMoveThreads + tid] = entry[n] < 0 || tile[n] < 0 ? -1 : tile[n] * 32 + (entry[n] & 31);
+        stay = true;
+#pragma unroll
+        for (int n = 0; n < R; n++) stay = stay && (entry[n] < 0 || entry[n] == at + n * kMoveThreads + tid);
+    };
+    ask(0);
+    found(sources[0], 0);
+    for (int i0 = 0, turn = 0; i0 < keep; i0 += kMoveTokens, turn ^= 1) {
+        const int64_t *source = sources[turn];
+        const bool all_stay = __syncthreads_and(stay);
+        ask(i0 + kMoveTokens);
+        if (all_stay) {
+            found(sources[turn ^ 1], i0 + kMoveTokens);
+            continue;
+        }
         if (part < 4) {  // one token a thread and round: its dwords of lane part
             u4 code[R][(G + 3) / 4];
-            int64_t from[R];
+            int64_t from[R], to[R];
+#pragma unroll
+            for (int n = 0; n < R; n++) to[n] = tile_number(min(i0 + n * kMoveThreads + tid, keep - 1) >> 5);
 #pragma unroll
             for (int n = 0; n < R; n++) {
                 from[n] = source[n * kMoveThreads + tid];
-                if (from[n] < 0) continue;
-                const int t = (int)from[n] & 31;
-                const uint8_t *at = kv.cache + (from[n] >> 5) * T::kBytes + T::kKeys + T::code(key_half(t) * G, key_row(t) + 16 * part);
+                const int64_t some = max(from[n], (int64_t)0);
+                const int t = (int)some & 31;
+                const uint8_t *at = kv.cache + (some >> 5) * T::kBytes + T::kKeys + T::code(key_half(t) * G, key_row(t) + 16 * part);
                 if constexpr (G == 2) {
                     const u2 w = *reinterpret_cast<const u2 *>(at);
                     code[n][0] = u4{w.x, w.y, 0, 0};
@@ -446,14 +512,14 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvCall kv, 
                     for (int c = 0; c < G / 4; c++) code[n][c] = *reinterpret_cast<const u4 *>(at + c * 1024);
                 }
             }
+            found(sources[turn ^ 1], i0 + kMoveTokens);
             all_read();
 #pragma unroll
             for (int n = 0; n < R; n++) {
                 const int i = i0 + n * kMoveThreads + tid;
-                const int64_t to = from[n] < 0 ? -1 : tile_number(i >> 5);
-                if (to < 0) continue;
+                if (from[n] < 0 || to[n] < 0) continue;
                 const int t = i & 31;
-                uint8_t *at = kv.cache + to * T::kBytes + T::kKeys + T::code(key_half(t) * G, key_row(t) + 16 * part);
+                uint8_t *at = kv.cache + to[n] * T::kBytes + T::kKeys + T::code(key_half(t) * G, key_row(t) + 16 * part);
                 if constexpr (G == 2) {
                     *reinterpret_cast<u2 *>(at) = u2{code[n][0].x, code[n][0].y};
                 } else {
@@ -466,29 +532,36 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvCall kv, 
             const int set = (part - 4) >> 2, r = ((part - 4) & 3) * 4 + (tid & 3), j = (tid >> 2) & 3;
             u4 word[kRounds];
             uint32_t mask[kRounds];
+            int64_t to[kRounds];
+#pragma unroll
+            for (int n = 0; n < kRounds; n++) to[n] = tile_number(min(i0 + (n * (kMoveThreads / 16) + (tid >> 4)) * 32, keep - 1) >> 5);
 #pragma unroll
             for (int n = 0; n < kRounds; n++) {
                 const int i = (n * (kMoveThreads / 16) + (tid >> 4)) * 32 + j * 8;
                 word[n] = u4{0, 0, 0, 0};
                 mask[n] = 0;
+                u4 w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int64_t some = max(source[i + e], (int64_t)0);
+                    w[e] = *reinterpret_cast<const u4 *>(kv.cache + (some >> 5) * T::kBytes + T::kValues + (set * 64 + r + 16 * (((int)some & 31) >> 3)) * 16);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int64_t from = source[i + e];
-                    if (from < 0) continue;
-                    const int t = (int)from & 31, down = nibble_shift(t & 7);
-                    const u4 w = *reinterpret_cast<const u4 *>(kv.cache + (from >> 5) * T::kBytes + T::kValues + (set * 64 + r + 16 * (t >> 3)) * 16);
+                    const int down = nibble_shift((int)from & 7);
+                    const uint32_t here = from < 0 ? 0u : 15u;
 #pragma unroll
-                    for (int c = 0; c < 4; c++) word[n][c] |= ((w[c] >> down) & 15u) << nibble_shift(e);
-                    mask[n] |= 0xFu << nibble_shift(e);
+                    for (int c = 0; c < 4; c++) word[n][c] |= ((w[e][c] >> down) & here) << nibble_shift(e);
+                    mask[n] |= here << nibble_shift(e);
                 }
             }
+            found(sources[turn ^ 1], i0 + kMoveTokens);
             all_read();
 #pragma unroll
             for (int n = 0; n < kRounds; n++) {
-                const int i = i0 + (n * (kMoveThreads / 16) + (tid >> 4)) * 32;
-                const int64_t to = mask[n] ? tile_number(i >> 5) : -1;
-                if (to < 0) continue;
-                u4 *at = reinterpret_cast<u4 *>(kv.cache + to * T::kBytes + T::kValues + (set * 64 + r + 16 * j) * 16);
+                if (!mask[n] || to[n] < 0) continue;
+                u4 *at = reinterpret_cast<u4 *>(kv.cache + to[n] * T::kBytes + T::kValues + (set * 64 + r + 16 * j) * 16);
                 if (mask[n] != 0xFFFFFFFFu) {
                     const u4 old = *at;
 #pragma unroll
@@ -499,34 +572,36 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvCall kv, 
         } else {
             uint16_t ks[R][G], vs[R][G];
             float account[R];
-            int64_t from[R];
+            int64_t from[R], to[R];
+#pragma unroll
+            for (int n = 0; n < R; n++) to[n] = tile_number(min(i0 + n * kMoveThreads + tid, keep - 1) >> 5);
 #pragma unroll
             for (int n = 0; n < R; n++) {
                 from[n] = source[n * kMoveThreads + tid];
-                if (from[n] < 0) continue;
-                const int t = (int)from[n] & 31;
-                const uint8_t *at = kv.cache + (from[n] >> 5) * T::kBytes;
+                const int64_t some = max(from[n], (int64_t)0);
+                const int t = (int)some & 31;
+                const uint8_t *at = kv.cache + (some >> 5) * T::kBytes;
 #pragma unroll
                 for (int g = 0; g < G; g++) {
                     ks[n][g] = reinterpret_cast<const uint16_t *>(at + T::kKeyScales)[t * G + g];
                     vs[n][g] = reinterpret_cast<const uint16_t *>(at + T::kValueScales)[g * 32 + t];
                 }
-                account[n] = accounts[from[n]];  // (pages hold their tokens' accounts in the order of their tiles)
+                account[n] = accounts[some];  // (pages hold their tokens' accounts in the order of their tiles)
             }
+            found(sources[turn ^ 1], i0 + kMoveTokens);
             all_read();
 #pragma unroll
             for (int n = 0; n < R; n++) {
                 const int i = i0 + n * kMoveThreads + tid;
-                const int64_t to = from[n] < 0 ? -1 : tile_number(i >> 5);
-                if (to < 0) continue;
+                if (from[n] < 0 || to[n] < 0) continue;
                 const int t = i & 31;
-                uint8_t *at = kv.cache + to * T::kBytes;
+                uint8_t *at = kv.cache + to[n] * T::kBytes;
 #pragma unroll
                 for (int g = 0; g < G; g++) {
                     reinterpret_cast<uint16_t *>(at + T::kKeyScales)[t * G + g] = ks[n][g];
                     reinterpret_cast<uint16_t *>(at + T::kValueScales)[g * 32 + t] = vs[n][g];
                 }
-                accounts[to * 32 + t] = account[n];
+                accounts[to[n] * 32 + t] = account[n];
             }
         }
     }
