@@ -37,6 +37,21 @@ __device__ __forceinline__ int key_half(int t) { return (t >> 2) & 1; }
 // What sequence b of a call has: `length` tokens, the last `news` of them new, their rows from `row0` on.
 struct KvSeq { int length, news, row0; };
 
+// The lanes' values up to and with each, combined by f, by data-parallel moves: 1, 2, 4, 8 lanes within rows of sixteen, then from the last lane
+// of a row into the next one, and of the first half into the second.  `none` combines to nothing.
+template <class F> __device__ __forceinline__ int lane_scan(int v, int none, F f) {
+    v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xF, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xA, 0xF, false));
+    v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xC, 0xF, false));
+    return v;
+}
+__device__ __forceinline__ int lane_scan(int v) {
+    return lane_scan(v, 0, [](int a, int b) { return a + b; });
+}
+
 // A load that is the same for the whole wavefront, through the scalar cache (of what no kernel of this launch writes).
 __device__ __forceinline__ int32_t uniform_load(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
 

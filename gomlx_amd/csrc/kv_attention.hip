@@ -256,18 +256,6 @@ struct Piece {
 __device__ __forceinline__ Span span_of(const AttendArgs &a, const KvSeq &seq) { return row_tile_span(seq, a.group, a.window, 0, 16); }
 __device__ __forceinline__ int tiles_of(const Span &span) { return span.rows ? max(1, ((span.hi + 31) >> 5) - (span.lo >> 5)) : 0; }
 
-// Sums over the lanes up to and with each, by data-parallel moves: 1, 2, 4, 8 lanes within rows of sixteen, then from the last lane of a
-// row into the next one, and of the first half into the second.
-__device__ __forceinline__ int lane_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
-
 __device__ __forceinline__ Piece piece_of(const AttendArgs &a, int index) {
     const int lane = (int)threadIdx.x & 63, seqs = a.kv.seqs, heads = a.kv.kv_heads;
     Piece p;

@@ -256,12 +256,7 @@ constexpr int kBins = 2048, kFew = 512;
 // The sum of v over the threads in front, and over all.
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *waves, uint32_t &total) {
     const int lane = (int)threadIdx.x & 63, w = (int)threadIdx.x >> 6;
-    uint32_t inc = v;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_up((int)inc, s);
-        if (lane >= s) inc += o;
-    }
+    const uint32_t inc = (uint32_t)lane_scan((int)v);
     __syncthreads();  // (the previous use of `waves` is over)
     if (lane == 63) waves[w] = inc;
     __syncthreads();
@@ -283,7 +278,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *waves, uint
 // writes its tokens behind those of the wavefronts in front.
 template <int IT>
 __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall kv, const float *__restrict__ accounts, int keep, int recent, int32_t *__restrict__ kept) {
-    __shared__ uint32_t hist[kBins], waves[kSelectWaves], found[2], ends[2][kSelectWaves], few[kFew], count;
+    __shared__ uint32_t hist[kBins], waves[kSelectWaves], found[2], ends[3][kSelectWaves], few[kFew], count;
     const int h = (int)blockIdx.x, b = (int)blockIdx.y, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const KvSeq s = kv_seq(kv, b);
     int32_t *out = kept + ((int64_t)b * kv.kv_heads + h) * keep;
@@ -327,27 +322,33 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall 
                 if (t0 + 64 * i < n) f(t0 + 64 * i, key_at(t0 + 64 * i));
         }
     };
-    uint32_t low = 0xFFFFFFFFu, high = 0;
+    // the smallest key, the smallest but for accounts of 0, and the largest
+    uint32_t low = 0xFFFFFFFFu, next = 0xFFFFFFFFu, high = 0;
+    const uint32_t zero = account_key(0.0f);
     each([&](int, uint32_t u) {
         low = min(low, u);
+        next = min(next, u == zero ? 0xFFFFFFFFu : u);
         high = max(high, u);
     });
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        low = min(low, (uint32_t)__shfl_xor((int)low, m));
-        high = max(high, (uint32_t)__shfl_xor((int)high, m));
-    }
-    if (lane == 0) { ends[0][wave] = low; ends[1][wave] = high; }
+    const auto least = [](int a, int b) { return (int)min((uint32_t)a, (uint32_t)b); };
+    const auto most = [](int a, int b) { return (int)max((uint32_t)a, (uint32_t)b); };
+    low = (uint32_t)lane_scan((int)low, -1, least);
+    next = (uint32_t)lane_scan((int)next, -1, least);
+    high = (uint32_t)lane_scan((int)high, 0, most);
+    if (lane == 63) { ends[0][wave] = low; ends[1][wave] = high; ends[2][wave] = next; }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kSelectWaves; i++) {
-        low = min(low, ends[0][i]);
-        high = max(high, ends[1][i]);
+        low = i ? min(low, ends[0][i]) : ends[0][0];
+        high = i ? max(high, ends[1][i]) : ends[1][0];
+        next = i ? min(next, ends[2][i]) : ends[2][0];
     }
     __syncthreads();
-    // digits of u - low; `want` counts down to how many of the tokens that equal the key are kept
-    int width = 32 - __clz(high - low);  // bits that are open (0: every key is the same)
-    uint32_t key = low;                  // the smallest key that the open bits allow
+    // Digits of the distance from the smallest key (zeros, which many are, lie far below the others: from the next one then); `want` counts down to
+    // how many of the tokens that equal the key are kept.
+    uint32_t key = low == zero && next != 0xFFFFFFFFu ? next : low;  // the smallest key that the open bits allow
+    int width = 32 - __clz(high - min(key, high));  // bits that are open (0: every key is the same, or one more than the smallest)
+    if (key != low && width == 0) width = 1;
     while (width > 0) {
         const int shift = width > 11 ? width - 11 : 0;
         const uint32_t top = width < 32 ? 1u << width : 0u;  // keys from key to key + top - 1 are looked at (0: all)
@@ -366,16 +367,16 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall 
         else if (before + first < want && want <= before + first + second) { found[0] = (uint32_t)bin - 1; found[1] = want - before - first; }
         if (tid == 0 && want > total) { found[0] = 0xFFFFFFFFu; found[1] = want - total; }  // down to those that equal the smallest
         __syncthreads();
-        const uint32_t digit = found[0];
+        const uint32_t digit = found[0], left = digit == 0xFFFFFFFFu ? 0u : hist[digit];
         want = found[1];
-        __syncthreads();
+        __syncthreads();  // (from here on the next pass may clear hist and set found)
         if (digit == 0xFFFFFFFFu) {
             key = low;
             break;
         }
         key += digit << shift;
         width = shift;
-        if (width == 0 || hist[digit] > kFew) continue;
+        if (width == 0 || left > kFew) continue;
         // few are left: each against all of them
         if (tid == 0) count = 0;
         __syncthreads();
@@ -403,13 +404,8 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall 
         more += u > key;
         same += u == key;
     });
-    uint32_t mores = more, sames = same;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        mores += (uint32_t)__shfl_xor((int)mores, m);
-        sames += (uint32_t)__shfl_xor((int)sames, m);
-    }
-    if (lane == 0) { ends[0][wave] = mores; ends[1][wave] = sames; }
+    const uint32_t mores = (uint32_t)lane_scan((int)more), sames = (uint32_t)lane_scan((int)same);
+    if (lane == 63) { ends[0][wave] = mores; ends[1][wave] = sames; }
     __syncthreads();
     uint32_t at = 0, equal = 0;  // kept, and equal to the key, in front
     for (int i = 0; i < wave; i++) {
@@ -459,8 +455,8 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvCall kv, 
     if (list[keep - 1] < keep || kv.pages == 0) return;  // nothing to move: as many tokens as places, or fewer (-1)
     const int per_page = kv.page_tokens >> 5;
     const auto tile_number = [&](int tile) -> int64_t {
-        const int slot = page_slot(kv, tile), page = kv.table[b * kv.table_stride + slot];
-        return (uint32_t)page < (uint32_t)kv.pages ? ((int64_t)page * kv.kv_heads + h) * per_page + (tile - slot * per_page) : -1;
+        const int slot = min(page_slot(kv, tile), kv.max_pages - 1), page = kv.table[b * kv.table_stride + slot];
+        return (uint32_t)page < (uint32_t)kv.pages && tile - slot * per_page < per_page ? ((int64_t)page * kv.kv_heads + h) * per_page + (tile - slot * per_page) : -1;
     };
     // Where the tokens of a step come from, found out a step ahead.  (-1 behind the last one, and where the page table names no page: nothing is written there;
     // what is read for it is the cache's first tile, so that loads need no branches between them and go out together.)

@@ -400,16 +400,18 @@ def test_evict(gpu, dim, page, keep, recent):
 
 
 @pytest.mark.parametrize("length", (4096, 4097, 16500, 40000))
-@pytest.mark.parametrize("kind", ("spread", "few", "same", "zeros", "signs"))
+@pytest.mark.parametrize("kind", ("spread", "few", "same", "zeros", "signs", "crowded"))
 def test_evict_long_sequences(gpu, length, kind):
     """The selection alone over lengths that take each of its forms, and accounts that are hard on it."""
     torch = gpu
     from gomlx_amd import nn
     rng = np.random.default_rng(length)
     accounts = {"spread": np.exp(8 * rng.standard_normal(length)), "few": rng.integers(0, 3, length), "same": np.full(length, 0.7),
-                "zeros": np.where(rng.random(length) < 0.01, rng.random(length), 0), "signs": 1e30 * rng.standard_normal(length)}[kind].astype(np.float32)
+                "zeros": np.where(rng.random(length) < 0.01, rng.random(length), 0), "crowded": 1 + 1e-4 * rng.random(length), "signs": 1e30 * rng.standard_normal(length)}[kind].astype(np.float32)
     if kind == "signs":
         accounts[::50], accounts[1::50], accounts[2::50] = -0.0, np.inf, -np.inf
+    if kind == "crowded":  # thousands share every digit but the last
+        accounts[::1000], accounts[7::1000] = 1e30, 1e-30
     pages = -(-length // 64)
     cache, table = nn.kv_cache(pages, 1, 64, 64), torch.randperm(pages, device="cuda").int().view(1, -1)
     w = torch.zeros(pages, 1, 64, device="cuda")
