@@ -332,6 +332,10 @@ template <int D> __device__ __forceinline__ void fetch_tile(uint32_t lds_at, con
 // A piece of a unit: up to sixteen rows, (new token, head) pairs, over `share` tiles.  Each wavefront takes every fourth tile, with a
 // maximum, sums and results of its own, and they meet in LDS.  A unit of one piece is finished here; the others leave their sums, by
 // workgroup, for kv_join_kernel.
+//
+// One pass over the cache bounds it: 32 sequences of 2048 to 8192 tokens, 8 heads of D = 128, 193 MB: 42 us, 4.5 TB/s (a copy reaches 4.8).  One
+// sequence of 2047 tokens, 2.4 MB: 6.2 us, most of it the way from lengths to table to tiles, each a load that waits for the one in front.
+// Tiles by DMA because two of them a wavefront in flight would take a third of its registers (through registers the call took 48 to 55 us, one sequence of 131072 tokens 40 instead of 38).
 template <int D, bool BF16>
 __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void kv_split_kernel(const AttendArgs a) {
     constexpr bool TWO = !BF16;
@@ -351,143 +355,141 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
     const Span &span = piece.span;
     const int tile0 = (span.lo >> 5) + piece.nth * piece.share, tile1 = (span.lo >> 5) + min((piece.nth + 1) * piece.share, piece.tiles);
     const Unpack unpack;
-    {
-        const bool live = r < span.rows;
-        const int nth = live ? r / a.group : 0;              // new token of the row
-        const int head = h * a.group + (live ? r - nth * a.group : 0);
-        const int64_t row = seq.row0 + nth;
-        const int base = seq.length - seq.news, place = base + nth;  // its own token
-        const int see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
-        // tokens that every row sees (the operand rows that stand for none have scores of 0 and go nowhere)
-        const int all_hi = base + 1, all_lo = a.window ? base + (span.rows - 1) / a.group + 1 - a.window : 0;
+    const bool live = r < span.rows;
+    const int nth = live ? r / a.group : 0;              // new token of the row
+    const int head = h * a.group + (live ? r - nth * a.group : 0);
+    const int64_t row = seq.row0 + nth;
+    const int base = seq.length - seq.news, place = base + nth;  // its own token
+    const int see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
+    // tokens that every row sees (the operand rows that stand for none have scores of 0 and go nowhere)
+    const int all_hi = base + 1, all_lo = a.window ? base + (span.rows - 1) / a.group + 1 - a.window : 0;
 
-        f4 o[W];
+    f4 o[W];
 #pragma unroll
-        for (int w = 0; w < W; w++) o[w] = f4{0.f, 0.f, 0.f, 0.f};
-        float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
+    for (int w = 0; w < W; w++) o[w] = f4{0.f, 0.f, 0.f, 0.f};
+    float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
 
-        const int last = min(tile1, (span.hi + 31) >> 5);  // (a unit that sees nothing has a tile in name only)
-        TileWalk<KvTile<D>::kBytes, kSplitWaves> walk(kv, b, h, tile0 + wave, last);
-        // the wavefront's ring of tiles: one is worked on while the next is on its way
-        uint8_t *ring = lds + wave * kSplitSlots * Lds::kSlot;
-        const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)ring);
-        const uint8_t *mem = walk.next();
-        if (mem) fetch_tile<D>(ring_at, mem);
-        h8 qh[D / 32], ql[TWO ? D / 32 : 1];
-        float back;
-        load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
-        const float to_log2 = back * fabsf(a.scale_log2);
-        int turn = 0;
-        for (int tile = tile0 + wave; tile < last; tile += kSplitWaves) {
-            const uint8_t *mem_next = walk.next();
-            if (mem_next) {
-                fetch_tile<D>(ring_at + (uint32_t)(turn ^ 1) * Lds::kSlot, mem_next);
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Lds::kLoads) : "memory");
-            } else {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
-            if (mem) {
-                KeyWords<D> k;
-                k.load(ring + turn * Lds::kSlot);
-                float s[8];
-                tile_scores<D, TWO>(unpack, k, qh, ql, s);
-                const int t0 = tile * 32;
-                float most = kNegInf;
-                if (t0 >= all_lo && t0 + 32 <= all_hi) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        s[e] *= to_log2;
-                        most = fmaxf(most, s[e]);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int t = t0 + 8 * j + e;
-                        s[e] = t < see_hi && t >= see_lo ? s[e] * to_log2 : kNegInf;
-                        most = fmaxf(most, s[e]);
-                    }
-                }
-                if (a.scores && live) {
-                    float *to = a.scores + ((int64_t)(b * kv.kv_heads + h) * a.rows + r) * a.score_tiles * 32 + (t0 + 8 * j - (span.lo & ~31));
-                    *reinterpret_cast<f4 *>(to) = f4{s[0], s[1], s[2], s[3]};
-                    *reinterpret_cast<f4 *>(to + 4) = f4{s[4], s[5], s[6], s[7]};
-                }
-                if (__any(most > ref + kMostLog2)) {  // (the first score of a row among them: its reference is -infinity)
-                    most = fmaxf(most, __shfl_xor(most, 16));
-                    most = fmaxf(most, __shfl_xor(most, 32));
-                    const float next = fmaxf(ref, most - kHeadroom);
-                    const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
-                    ref = next;
-                    total *= shrink;
-#pragma unroll
-                    for (int w = 0; w < W; w++) o[w] *= shrink;
-                }
-                const float less = ref == kNegInf ? 0.0f : ref;
-                h8 ph, pl;
+    const int last = min(tile1, (span.hi + 31) >> 5);  // (a unit that sees nothing has a tile in name only)
+    TileWalk<KvTile<D>::kBytes, kSplitWaves> walk(kv, b, h, tile0 + wave, last);
+    // the wavefront's ring of tiles: one is worked on while the next is on its way
+    uint8_t *ring = lds + wave * kSplitSlots * Lds::kSlot;
+    const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)ring);
+    const uint8_t *mem = walk.next();
+    if (mem) fetch_tile<D>(ring_at, mem);
+    h8 qh[D / 32], ql[TWO ? D / 32 : 1];
+    float back;
+    load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
+    const float to_log2 = back * fabsf(a.scale_log2);
+    int turn = 0;
+    for (int tile = tile0 + wave; tile < last; tile += kSplitWaves) {
+        const uint8_t *mem_next = walk.next();
+        if (mem_next) {
+            fetch_tile<D>(ring_at + (uint32_t)(turn ^ 1) * Lds::kSlot, mem_next);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Lds::kLoads) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (mem) {
+            KeyWords<D> k;
+            k.load(ring + turn * Lds::kSlot);
+            float s[8];
+            tile_scores<D, TWO>(unpack, k, qh, ql, s);
+            const int t0 = tile * 32;
+            float most = kNegInf;
+            if (t0 >= all_lo && t0 + 32 <= all_hi) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float p = __builtin_amdgcn_exp2f(s[e] - less);
-                    total += p;
-                    ph[e] = (_Float16)p;
-                    if constexpr (TWO) pl[e] = (_Float16)(p - (float)ph[e]);
+                    s[e] *= to_log2;
+                    most = fmaxf(most, s[e]);
                 }
-                ValueWords<D> v;
-                v.load(ring + turn * Lds::kSlot);
-#pragma unroll
-                for (int w = 0; w < W; w++) {
-                    const h8 x = v.operand(unpack, w);
-                    o[w] = mfma(x, ph, o[w]);
-                    if constexpr (TWO) o[w] = mfma(x, pl, o[w]);
-                }
-            }
-            mem = mem_next;
-            turn ^= 1;
-        }
-        __syncthreads();
-        total += __shfl_xor(total, 16);
-        total += __shfl_xor(total, 32);
-#pragma unroll
-        for (int w = 0; w < W; w++) *reinterpret_cast<f4 *>(&sums[wave][r][16 * w + 4 * j]) = o[w];
-        if (j == 0) {
-            refs[wave][r] = ref;
-            totals[wave][r] = total;
-        }
-        __syncthreads();
-
-        const int pieces = piece.pieces();
-        if (a.pieces && piece.nth == 0 && threadIdx.x == 0) a.pieces[b * kv.kv_heads + h] = make_int2((int)blockIdx.x, pieces);
-        for (int i = (int)threadIdx.x; i < span.rows * (D / 4); i += 64 * kSplitWaves) {
-            const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4;
-            float top = kNegInf;
-#pragma unroll
-            for (int w = 0; w < kSplitWaves; w++) top = fmaxf(top, refs[w][rr]);
-            f4 sum = {0.f, 0.f, 0.f, 0.f};
-            float all = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kSplitWaves; w++) {
-                const float f = refs[w][rr] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(refs[w][rr] - top);
-                // (a wavefront without a reference has seen no number: its sum is zero, or NaN)
-                all += refs[w][rr] == kNegInf ? totals[w][rr] : totals[w][rr] * f;
-                sum += *reinterpret_cast<const f4 *>(&sums[w][rr][d]) * f;
-            }
-            if (pieces == 1) {
-                const int n = rr / a.group;
-                const int64_t out = (int64_t)(seq.row0 + n) * a.heads + h * a.group + (rr - n * a.group);
-                store_result<BF16>(a.out, out * D + d, sum, all);
-                if (a.lse && d == 0) a.lse[out] = lse_of(top, all);
             } else {
-                *reinterpret_cast<f4 *>(a.part + ((int64_t)blockIdx.x * a.rows + rr) * D + d) = sum;
-                if (d == 0) {
-                    a.part_ml[((int64_t)blockIdx.x * a.rows + rr) * 2] = top;
-                    a.part_ml[((int64_t)blockIdx.x * a.rows + rr) * 2 + 1] = all;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int t = t0 + 8 * j + e;
+                    s[e] = t < see_hi && t >= see_lo ? s[e] * to_log2 : kNegInf;
+                    most = fmaxf(most, s[e]);
                 }
+            }
+            if (a.scores && live) {
+                float *to = a.scores + ((int64_t)(b * kv.kv_heads + h) * a.rows + r) * a.score_tiles * 32 + (t0 + 8 * j - (span.lo & ~31));
+                *reinterpret_cast<f4 *>(to) = f4{s[0], s[1], s[2], s[3]};
+                *reinterpret_cast<f4 *>(to + 4) = f4{s[4], s[5], s[6], s[7]};
+            }
+            if (__any(most > ref + kMostLog2)) {  // (the first score of a row among them: its reference is -infinity)
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                const float next = fmaxf(ref, most - kHeadroom);
+                const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
+                ref = next;
+                total *= shrink;
+#pragma unroll
+                for (int w = 0; w < W; w++) o[w] *= shrink;
+            }
+            const float less = ref == kNegInf ? 0.0f : ref;
+            h8 ph, pl;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float p = __builtin_amdgcn_exp2f(s[e] - less);
+                total += p;
+                ph[e] = (_Float16)p;
+                if constexpr (TWO) pl[e] = (_Float16)(p - (float)ph[e]);
+            }
+            ValueWords<D> v;
+            v.load(ring + turn * Lds::kSlot);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const h8 x = v.operand(unpack, w);
+                o[w] = mfma(x, ph, o[w]);
+                if constexpr (TWO) o[w] = mfma(x, pl, o[w]);
+            }
+        }
+        mem = mem_next;
+        turn ^= 1;
+    }
+    __syncthreads();
+    total += __shfl_xor(total, 16);
+    total += __shfl_xor(total, 32);
+#pragma unroll
+    for (int w = 0; w < W; w++) *reinterpret_cast<f4 *>(&sums[wave][r][16 * w + 4 * j]) = o[w];
+    if (j == 0) {
+        refs[wave][r] = ref;
+        totals[wave][r] = total;
+    }
+    __syncthreads();
+
+    const int pieces = piece.pieces();
+    if (a.pieces && piece.nth == 0 && threadIdx.x == 0) a.pieces[b * kv.kv_heads + h] = make_int2((int)blockIdx.x, pieces);
+    for (int i = (int)threadIdx.x; i < span.rows * (D / 4); i += 64 * kSplitWaves) {
+        const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4;
+        float top = kNegInf;
+#pragma unroll
+        for (int w = 0; w < kSplitWaves; w++) top = fmaxf(top, refs[w][rr]);
+        f4 sum = {0.f, 0.f, 0.f, 0.f};
+        float all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kSplitWaves; w++) {
+            const float f = refs[w][rr] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(refs[w][rr] - top);
+            // (a wavefront without a reference has seen no number: its sum is zero, or NaN)
+            all += refs[w][rr] == kNegInf ? totals[w][rr] : totals[w][rr] * f;
+            sum += *reinterpret_cast<const f4 *>(&sums[w][rr][d]) * f;
+        }
+        if (pieces == 1) {
+            const int n = rr / a.group;
+            const int64_t out = (int64_t)(seq.row0 + n) * a.heads + h * a.group + (rr - n * a.group);
+            store_result<BF16>(a.out, out * D + d, sum, all);
+            if (a.lse && d == 0) a.lse[out] = lse_of(top, all);
+        } else {
+            *reinterpret_cast<f4 *>(a.part + ((int64_t)blockIdx.x * a.rows + rr) * D + d) = sum;
+            if (d == 0) {
+                a.part_ml[((int64_t)blockIdx.x * a.rows + rr) * 2] = top;
+                a.part_ml[((int64_t)blockIdx.x * a.rows + rr) * 2 + 1] = all;
             }
         }
     }
 }
 
-
-// Joins the pieces of the units that more than one workgroup has worked on: one workgroup per unit and row.
+// Joins the pieces of the units that more than one workgroup has worked on: one workgroup per unit and row.  4 to 5 us, the chain from the
+// unit's pieces to their references to their sums.
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
     constexpr int L = D / 4, S = 256 / L;  // lanes of a row's values, and the shares into which the pieces are divided
@@ -543,7 +545,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
 //
 // Matrix instructions, exponentials and the widening run side by side, two workgroups a CU (2048 rows of 32 heads over 2049 to 4096
 // tokens, D = 128).  With a causal bound workgroups differ in length: the second half of them goes from short to long, so that the two of a CU
-// add up to the same.
+// add up to the same.  That call: 122 us in bfloat16, 845 TFLOP/s (a library product of 8192^3: 1193).
 constexpr int kRowsWaves = 4, kRowsTile = 32 * kRowsWaves, kRowsPiece = 12;  // rows of a workgroup; tiles of the cache, at least, in a piece of its tokens
 
 template <int D> struct RowsLds {
@@ -1018,7 +1020,7 @@ __global__ __launch_bounds__(256) void kv_account_kernel(const AttendArgs a) {
 }
 
 // Scores that are kept for the accounts, at most; beyond, the keys are read a second time (16 sequences of up to 4096 tokens, 8 heads of 4
-// queries: 4 us from 10 MB of scores, 34 us from the keys).
+// queries: 5.8 us from 10 MB of scores, 34 us from the keys).
 constexpr size_t kMostScoreBytes = (size_t)256 << 20;
 
 // Pieces that all units together are cut into.  Per CU at D = 64 / 128 / 256: four, three, two, as many as run there at a time by LDS or one

@@ -8,6 +8,8 @@
 //
 // A lane holds four neighbouring values, D / 4 lanes a head, so that a wavefront reads and writes whole lines; the partner of a
 // value in the other half of the rotation is a lane exchange away.  All arithmetic in 32 bits, one rounding at the store.
+//
+// HBM bounds it: 2048 rows of 32 + 8 heads of D = 128, float32 to bfloat16, 64 MB: 16.7 us a call, 3.8 TB/s; one row: 3.2 us, a launch and two loads.
 #include "common.hpp"
 
 namespace gq {

@@ -511,7 +511,8 @@ def cached_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
     neighbouring query heads share one.  ``scale`` defaults to head_dim^-1/2.  A token sees itself and the tokens in front of it in its
     sequence, with a ``window`` the last that many; one that sees nothing gets zeros.  ``weights``: float32 [pages, kv_heads, page_tokens],
     to which the softmax weights that every cached token receives are added (summed over rows and the query heads of a key head): what
-    ``kv_cache_evict`` goes by.  Every row of q belongs to a sequence.  Returns [rows, heads, head_dim] of q's type, contiguous."""
+    ``kv_cache_evict`` goes by.  Sequences may share pages (a common beginning, say), with ``weights`` they must not.  Every row of q belongs to a
+    sequence.  Returns [rows, heads, head_dim] of q's type, contiguous."""
     if _lib.fast is not None and (out := _lib.fast.cached_attention(q, cache, page_table, lengths, starts, max_new, scale, window, weights)) is not None:
         return out
     import ctypes
@@ -536,7 +537,7 @@ def kv_cache_evict(cache: torch.Tensor, weights: torch.Tensor, page_table: torch
     """Shrinks every sequence of more than ``keep`` tokens to ``keep``: for each key head the last ``recent`` tokens and the keep - recent
     others of largest accumulated weight stay (ties: the earlier token), moved to the front of the sequence's pages in their order,
     with their weights.  Returns (kept, lengths): int32 [sequences, kv_heads, keep] former places of the kept tokens (-1 behind the last), and
-    the new lengths, min(length, keep); ``lengths`` itself is left as it is."""
+    the new lengths, min(length, keep); ``lengths`` itself is left as it is.  Sequences must not share pages."""
     if _lib.fast is not None and (out := _lib.fast.kv_evict(cache, weights, page_table, lengths, keep, recent)) is not None:
         return out
     import ctypes
