@@ -666,8 +666,9 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     const int head = h * a.group + (live ? idx - nth * a.group : 0);
     const int64_t row = seq.row0 + nth;
     const int base = seq.length - seq.news, place = base + nth;
-    const int see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
-    // what every row of the wavefront sees, and what one of them does
+    const int own = live ? place : -1;  // (a row that is none, or without tokens, sees nothing)
+    const uint32_t most_behind = a.window ? (uint32_t)a.window : 0x80000000u;
+    // what every row of the wavefront sees
     const int first_in = span.first_row + wave * 32, last_in = min(first_in + 31, span.first_row + span.rows - 1);
     const int all_hi = __builtin_amdgcn_readfirstlane(base + first_in / a.group + 1);
     const int all_lo = __builtin_amdgcn_readfirstlane(a.window ? base + last_in / a.group + 1 - a.window : 0);
@@ -751,12 +752,12 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
         const uint32_t known = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(there[mine])) & ALL;
         if (!(t0 >= all_lo && t0 + 32 * T <= all_hi && known == ALL)) {
 #pragma unroll
-            for (int t = 0; t < T; t++)
+            for (int t = 0; t < T; t++) {
+                const uint32_t window = (known >> (8 * t)) & 1u ? most_behind : 0u;
+                const int behind = own - t0 - 32 * t - 8 * half;  // the tokens from the lane's first one to the row's own
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int token = t0 + 32 * t + 16 * (i >> 3) + 8 * half + (i & 7);
-                    s[t][i] = token < see_hi && token >= see_lo && ((known >> (8 * t)) & 1u) ? s[t][i] : kNegInf;
-                }
+                for (int i = 0; i < 16; i++) s[t][i] = (uint32_t)(behind - 16 * (i >> 3) - (i & 7)) < window ? s[t][i] : kNegInf;
+            }
         }
         float most = kNegInf;  // (scores as the products left them: what they are multiplied by is not negative)
 #pragma unroll
@@ -854,8 +855,10 @@ __global__ __launch_bounds__(256) void kv_rows_join_kernel(const AttendArgs a) {
     if (line >= (int64_t)a.kv.rows * a.heads) return;
     const float *ml = a.part_ml + line * n * 2;
     float top = kNegInf, all = 0.0f;
+#pragma unroll 8
     for (int i = 0; i < n; i++) top = fmaxf(top, ml[2 * i]);
     f4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int i = 0; i < n; i++) {
         const float f = ml[2 * i] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[2 * i] - top);
         all += ml[2 * i] == kNegInf ? ml[2 * i + 1] : ml[2 * i + 1] * f;
@@ -891,27 +894,31 @@ __global__ __launch_bounds__(256) void kv_score_account_kernel(const AttendArgs 
     *to += sum;
 }
 
-// The accounts of many rows: a workgroup owns a tile of a sequence and key head, its keys in registers as operands, and goes over all rows
-// that see it, as kv_rows_kernel has left them, 32 at a time and every fourth such tile a wavefront: every account is added to once, in
+// The accounts of many rows: a workgroup owns one or two neighbouring tiles of a sequence and key head, their keys in registers as operands, and goes over
+// all rows that see them, as kv_rows_kernel has left them, 32 at a time and every fourth such tile a wavefront: every account is added to once, in
 // one order.  The way of the rows' operands from the other XCDs' memory side bounds it where there are few, matrix instructions
-// and one exponential a (row, token) where there are many.
+// and one exponential a (row, token) where there are many: 78 us for 2048 rows of 32 heads over 2049 to 4096 tokens, D = 128, bfloat16, 12 for 301 rows and
+// fewer of 5 sequences, 12 heads of D = 64, float32, 500 tokens in a window.
+//
+// Two tiles where their operands fit the registers of two wavefronts a SIMD, for the rows' operands are then read half as often (the first of these calls with its
+// attention 200 us, with one tile a workgroup 223; at D = 64 a third wavefront does more than the second tile: the other call 38 us, with two tiles 44 to 50).
+template <int D, bool BF16> constexpr int account_tiles() { return D == 128 && BF16 ? 2 : 1; }
 template <int D, bool BF16>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_account_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void kv_rows_account_kernel(const AttendArgs a) {
     constexpr bool TWO = !BF16;
-    constexpr int KS = D / 16, G = D / 32, N = TWO ? 2 * KS : KS;
-    __shared__ float sums[4][32];
+    constexpr int AHEAD = 2;  // row tiles of a wavefront on their way or worked on
+    constexpr int KS = D / 16, G = D / 32, N = TWO ? 2 * KS : KS, NT = account_tiles<D, BF16>();
+    __shared__ float sums[4][32 * NT];
     const KvCall &kv = a.kv;
     const int h = (int)blockIdx.y, b = (int)blockIdx.z;
     const KvSeq seq = kv_seq(kv, b);
     const int base = seq.length - seq.news;
-    const int tile = (a.window ? max(0, base + 1 - a.window) >> 5 : 0) + (int)blockIdx.x, t0 = tile * 32;
+    const int tile = (a.window ? max(0, base + 1 - a.window) >> 5 : 0) + (int)blockIdx.x * NT, t0 = tile * 32;
     if (t0 >= seq.length || seq.news == 0) return;
-    const uint8_t *mem = kv_tile(kv, b, h, tile, KvTile<D>::kBytes);
-    if (!mem) return;
     const int lane = (int)threadIdx.x & 63, r = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    // the new tokens that see one of the tile's, and their operand tiles
-    const int n0 = max(0, t0 - base), n1 = a.window ? min(seq.news, t0 + 31 + a.window - base) : seq.news;
+    // the new tokens that see one of the tiles', and their operand tiles
+    const int n0 = max(0, t0 - base), n1 = a.window ? min(seq.news, t0 + 32 * NT - 1 + a.window - base) : seq.news;
     const int from = n0 * a.group / 32 + wave, to = (n1 * a.group + 31) / 32;
     const int64_t first = (int64_t)h * a.operand_tiles + first_operand_tile(a, seq, b);
     struct Rows {  // 32 rows
@@ -919,7 +926,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_account_kernel(
         float scale, lse;
         int place;  // -1: no row
     };
-    const auto load = [&](int n, Rows &rows) {
+    const auto load = [&](int n, Rows &rows) __attribute__((always_inline)) {
         const h8 *q = reinterpret_cast<const h8 *>(a.operands) + (first + n) * N * 64 + lane;
 #pragma unroll
         for (int k = 0; k < N; k++) rows.q[k] = q[k * 64];
@@ -930,53 +937,90 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_account_kernel(
         rows.scale = a.row_scales[(first + n) * 32 + r];
         rows.lse = a.lse[(int64_t)(seq.row0 + nth) * a.heads + head];
     };
-    Rows now, next;
-    if (from < to) load(from, now);
-    // the tile's keys: operand row r is token r, values 16 k + 8 half + 0..7
-    h8 keys[KS];
+    Rows ring[AHEAD];
+#pragma unroll
+    for (int p = 0; p < AHEAD; p++)
+        if (from + 4 * p < to) load(from + 4 * p, ring[p]);
+    // the tiles' keys: operand row r is token r, values 16 k + 8 half + 0..7 (of a tile that the cache does not have: zeros)
+    h8 keys[NT][KS];
     {
         const Unpack unpack;
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const int g = k >> 1, j = 2 * (k & 1) + half;
-            h2 v[4];
-            unpack(*reinterpret_cast<const uint32_t *>(mem + KvTile<D>::kKeys + KvTile<D>::code(key_half(r) * G + g, key_row(r) + 16 * j)), v);
-            const _Float16 one = reinterpret_cast<const _Float16 *>(mem + KvTile<D>::kKeyScales)[r * G + g];
-            const h2 d = {one, one};
-            keys[k] = join(v[0] * d, v[1] * d, v[2] * d, v[3] * d);
+        for (int t = 0; t < NT; t++) {
+            const uint8_t *mem = t0 + 32 * t < seq.length ? kv_tile(kv, b, h, tile + t, KvTile<D>::kBytes) : nullptr;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const int g = k >> 1, j = 2 * (k & 1) + half;
+                uint32_t code = 0x88888888u;
+                _Float16 one = (_Float16)0.0f;
+                if (mem) {
+                    code = *reinterpret_cast<const uint32_t *>(mem + KvTile<D>::kKeys + KvTile<D>::code(key_half(r) * G + g, key_row(r) + 16 * j));
+                    one = reinterpret_cast<const _Float16 *>(mem + KvTile<D>::kKeyScales)[r * G + g];
+                }
+                h2 v[4];
+                unpack(code, v);
+                const h2 d = {one, one};
+                keys[t][k] = join(v[0] * d, v[1] * d, v[2] * d, v[3] * d);
+            }
         }
     }
-    float sum[16] = {};
-    for (int n = from; n < to; n += 4) {
-        if (n + 4 < to) load(n + 4, next);
-        f16 s;
+    const uint32_t window = a.window ? (uint32_t)a.window : 0x80000000u;
+    float sum[NT][16] = {};
+    for (int n = from; n < to; n += 4 * AHEAD) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+        for (int p = 0; p < AHEAD; p++) {
+            if (n + 4 * p >= to) break;
+            Rows &now = ring[p];
+            const bool open = __all(now.place >= t0 + 32 * NT - 1 && (!a.window || now.place - a.window < t0));
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-            s = mfma32(keys[k], now.q[k], s);
-            if constexpr (TWO) s = mfma32(keys[k], now.q[KS + k], s);
+            for (int t = 0; t < NT; t++) {
+                f16 s;
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    s = mfma32(keys[t][k], now.q[k], s);
+                    if constexpr (TWO) s = mfma32(keys[t][k], now.q[KS + k], s);
+                }
+                if (open) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sum[t][i] += __builtin_amdgcn_exp2f(fmaf(s[i], now.scale, -now.lse));
+                } else {
+                    const int behind = now.place - t0 - 32 * t - 4 * half;  // tokens of the tile's first for the lane to the row's own
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float w = __builtin_amdgcn_exp2f(fmaf(s[i], now.scale, -now.lse));
+                        sum[t][i] += (uint32_t)(behind - 8 * (i >> 2) - (i & 3)) < window ? w : 0.0f;
+                    }
+                }
+            }
+            if (n + 4 * (p + AHEAD) < to) load(n + 4 * (p + AHEAD), now);
         }
-        const bool open = __all(now.place >= t0 + 31 && (!a.window || now.place - a.window < t0));
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int t = t0 + 8 * (i >> 2) + 4 * half + (i & 3);
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], now.scale, -now.lse));
-            sum[i] += open || (t <= now.place && (!a.window || t > now.place - a.window)) ? p : 0.0f;
-        }
-        now = next;
     }
+    // over the 32 rows: lanes that differ in one bit pass each other half of what they have left, until each pair of lanes has one token's sum
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
+    for (int t = 0; t < NT; t++) {
+        int count = 16;
 #pragma unroll
-        for (int m = 1; m < 32; m <<= 1) sum[i] += __shfl_xor(sum[i], m);
-        if (r == 0) sums[wave][8 * (i >> 2) + 4 * half + (i & 3)] = sum[i];
+        for (int m = 16; m > 1; m >>= 1) {
+            count >>= 1;
+            const bool upper = lane & m;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (i >= count) break;
+                const float give = upper ? sum[t][i] : sum[t][i + count], keep = upper ? sum[t][i + count] : sum[t][i];
+                sum[t][i] = keep + __shfl_xor(give, m);
+            }
+        }
+        const float all = sum[t][0] + __shfl_xor(sum[t][0], 1);
+        const int i = r >> 1;
+        if (!(r & 1)) sums[wave][32 * t + 8 * (i >> 2) + 4 * half + (i & 3)] = all;
     }
     __syncthreads();
-    const int t = t0 + (int)threadIdx.x;
-    if (threadIdx.x < 32 && t < seq.length) {
-        float *p = kv_account(kv, a.accounts, b, h, t);
-        if (p) *p += (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+    const int i = (int)threadIdx.x, token = t0 + i;
+    if (i < 32 * NT && token < seq.length) {
+        float *p = kv_account(kv, a.accounts, b, h, token);
+        if (p) *p += (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
     }
 }
 
@@ -1046,7 +1090,8 @@ template <int D, bool BF16> int attend(const AttendArgs &a, int max_tiles, hipSt
     if (a.row_pieces > 1)
         if (int rc = launch(kv_rows_join_kernel<D, BF16>, dim3((unsigned)(((int64_t)kv.rows * a.heads * (D / 4) + 255) / 256)), dim3(256), 0, s, a)) return rc;
     if (!a.accounts) return GQ_OK;
-    return launch(kv_rows_account_kernel<D, BF16>, dim3((unsigned)max_tiles, (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
+    constexpr int NT = account_tiles<D, BF16>();
+    return launch(kv_rows_account_kernel<D, BF16>, dim3((unsigned)((max_tiles + NT - 1) / NT), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
 }
 
 }  // namespace
