@@ -60,7 +60,8 @@ struct AttendArgs {
     void *out;               // [rows, heads, D]
     float *lse;              // [rows, heads], in powers of two; null where nobody asks
     float *part, *part_ml;   // of kv_split_kernel's workgroups: sums [rows, D], (reference, sum) [rows, 2]
-    int workgroups, rows;    // of kv_split_kernel; (new token, head) pairs of a key head, at most
+    int workgroups, rows;    // of kv_split_kernel; (new token, head) pairs of a key head that it has, at most
+    int few;                 // sequences of so many such pairs or fewer are kv_split_kernel's, the others kv_rows_kernel's
     int2 *pieces;            // per unit of kv_split_kernel: the first workgroup that works on it, and how many do
     float *accounts;
     float *scores;           // of kv_split_kernel, in powers of two: [units, rows, score_tiles * 32] from the first tile that a unit sees; null: not kept
@@ -217,7 +218,7 @@ __device__ __forceinline__ void tile_scores(const Unpack &unpack, const KeyWords
     }
 }
 
-constexpr int kSplitWaves = 4;
+constexpr int kSplitWaves = 4, kSplitRows = 16;
 
 // The addresses of every STEP-th tile of a sequence and key head from `tile` to `end`; the page of the next one is asked for a call ahead.
 template <int BYTES, int STEP> struct TileWalk {
@@ -253,7 +254,12 @@ struct Piece {
     Span span;
     __device__ __forceinline__ int pieces() const { return (tiles + share - 1) / share; }
 };
-__device__ __forceinline__ Span span_of(const AttendArgs &a, const KvSeq &seq) { return row_tile_span(seq, a.group, a.window, 0, 16); }
+// (a sequence of more rows than `few` has none here)
+__device__ __forceinline__ Span span_of(const AttendArgs &a, const KvSeq &seq) {
+    Span span = row_tile_span(seq, a.group, a.window, 0, kSplitRows);
+    if (seq.news * a.group > a.few) span.rows = 0;
+    return span;
+}
 __device__ __forceinline__ int tiles_of(const Span &span) { return span.rows ? max(1, ((span.hi + 31) >> 5) - (span.lo >> 5)) : 0; }
 
 __device__ __forceinline__ Piece piece_of(const AttendArgs &a, int index) {
@@ -619,7 +625,7 @@ __device__ __forceinline__ RowTile row_tile_of(const AttendArgs &a, int index) {
     for (int base = 0; base < seqs; base += 64) {
         KvSeq mine{0, 0, 0};
         if (base + lane < seqs) mine = kv_seq(a.kv, base + lane);
-        const int tiles = (mine.news * a.group + kRowsTile - 1) / kRowsTile, upto = lane_scan(tiles);
+        const int rows = mine.news * a.group, tiles = rows > a.few ? (rows + kRowsTile - 1) / kRowsTile : 0, upto = lane_scan(tiles);
         const uint64_t past = __ballot(front + upto > index);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
@@ -847,7 +853,8 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     if (ACCOUNTS && half == 0) a.lse[out] = lse_of(ref, total);
 }
 
-// Joins the pieces of kv_rows_kernel: a thread makes four values of a line, (row, head).
+// Joins the pieces of kv_rows_kernel: a thread makes four values of a line, (row, head).  (Rows of sequences that kv_split_kernel has get what was in the
+// scratch memory, until that kernel writes them.)
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void kv_rows_join_kernel(const AttendArgs a) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, line = at / (D / 4);
@@ -914,7 +921,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void kv_rows_
     const KvSeq seq = kv_seq(kv, b);
     const int base = seq.length - seq.news;
     const int tile = (a.window ? max(0, base + 1 - a.window) >> 5 : 0) + (int)blockIdx.x * NT, t0 = tile * 32;
-    if (t0 >= seq.length || seq.news == 0) return;
+    if (t0 >= seq.length || seq.news * a.group <= a.few) return;
     const int lane = (int)threadIdx.x & 63, r = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     // the new tokens that see one of the tiles', and their operand tiles
@@ -1072,26 +1079,37 @@ constexpr size_t kMostScoreBytes = (size_t)256 << 20;
 // one of 16384 14 15 15 17 17; D = 64, 16 of up to 8192 28 22 20 19 20; D = 256, 8 of up to 8192 38 30 36 36 42.)
 int split_workgroups(int D) { return std::min(kMostWorkgroups, device_cu_count() * (D == 256 ? 2 : D == 128 ? 3 : 4)); }
 
+// One call may hold prompts beside single tokens: where its sequences have on average, but for the longest, under half of the largest number of new tokens,
+// and the page table has room for this many tiles, those of few rows are taken by the kernel for them, in launches of their own.  (us a call with one kernel and with
+// both, D = 128: 512 new tokens beside 31 single ones over 2000 to 8192, 8192 tiles: 185 75; 300 beside one over 131072: 585 59; 256 beside 31 over 1500, 1536
+// tiles: 46 36; beside 31 over 500, 512 tiles: 23 30; 512 beside 7 over 1000, 256 tiles: 36 42.)
+constexpr int64_t kMixedTiles = 1024;
+
 // Row tiles that the sequences of a call have, at most.
 int64_t row_tiles_of(const AttendArgs &a) { return (int64_t)a.kv.rows * a.group / kRowsTile + a.kv.seqs; }
 
 template <int D, bool BF16> int attend(const AttendArgs &a, int max_tiles, hipStream_t s) {
     const KvCall &kv = a.kv;
+    const unsigned heads = (unsigned)kv.kv_heads, seqs = (unsigned)kv.seqs;
+    if (a.row_pieces) {
+        constexpr int NT = account_tiles<D, BF16>();
+        const unsigned grid = (unsigned)(row_tiles_of(a) * kv.kv_heads * a.row_pieces);
+        if (int rc = launch(a.accounts ? kv_rows_kernel<D, BF16, true> : kv_rows_kernel<D, BF16, false>, dim3(grid), dim3(64 * kRowsWaves), 0, s, a)) return rc;
+        if (a.row_pieces > 1)
+            if (int rc = launch(kv_rows_join_kernel<D, BF16>, dim3((unsigned)(((int64_t)kv.rows * a.heads * (D / 4) + 255) / 256)), dim3(256), 0, s, a)) return rc;
+        if (a.accounts)
+            if (int rc = launch(kv_rows_account_kernel<D, BF16>, dim3((unsigned)((max_tiles + NT - 1) / NT), heads, seqs), dim3(256), 0, s, a)) return rc;
+    }
     if (a.workgroups) {
         const int grid = a.workgroups + kv.seqs * kv.kv_heads;  // (a unit's last piece may be short)
         if (int rc = launch(kv_split_kernel<D, BF16>, dim3((unsigned)grid), dim3(64 * kSplitWaves), 0, s, a)) return rc;
-        if (a.part)
-            if (int rc = launch(kv_join_kernel<D, BF16>, dim3((unsigned)(kv.max_new * a.group), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a)) return rc;
+        if (a.pieces)
+            if (int rc = launch(kv_join_kernel<D, BF16>, dim3((unsigned)a.rows, heads, seqs), dim3(256), 0, s, a)) return rc;
         if (!a.accounts) return GQ_OK;
-        if (a.scores) return launch(kv_score_account_kernel, dim3((unsigned)((a.score_tiles + 7) / 8), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
-        return launch(kv_account_kernel<D, BF16>, dim3((unsigned)((max_tiles + 3) / 4), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
+        if (a.scores) return launch(kv_score_account_kernel, dim3((unsigned)((a.score_tiles + 7) / 8), heads, seqs), dim3(256), 0, s, a);
+        return launch(kv_account_kernel<D, BF16>, dim3((unsigned)((max_tiles + 3) / 4), heads, seqs), dim3(256), 0, s, a);
     }
-    if (int rc = launch(a.accounts ? kv_rows_kernel<D, BF16, true> : kv_rows_kernel<D, BF16, false>, dim3((unsigned)(row_tiles_of(a) * kv.kv_heads * a.row_pieces)), dim3(64 * kRowsWaves), 0, s, a)) return rc;
-    if (a.row_pieces > 1)
-        if (int rc = launch(kv_rows_join_kernel<D, BF16>, dim3((unsigned)(((int64_t)kv.rows * a.heads * (D / 4) + 255) / 256)), dim3(256), 0, s, a)) return rc;
-    if (!a.accounts) return GQ_OK;
-    constexpr int NT = account_tiles<D, BF16>();
-    return launch(kv_rows_account_kernel<D, BF16>, dim3((unsigned)((max_tiles + NT - 1) / NT), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a);
+    return GQ_OK;
 }
 
 }  // namespace
@@ -1108,26 +1126,32 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
     a.accounts = accounts;
     const int64_t size = q.bf16 ? 2 : 4;
     a.wide = ((reinterpret_cast<uintptr_t>(q.p) | (uintptr_t)(q.row * size) | (uintptr_t)(q.head * size)) & 15) == 0;
-    a.rows = kv.max_new * a.group;
     // tiles that a unit's rows see, at most, and those that see any of the new tokens
     const int64_t room = (int64_t)kv.max_pages * kv.page_tokens / 32;
     const int64_t tiles = std::max<int64_t>(1, window ? std::min<int64_t>(room, ((int64_t)window + kv.max_new + 31) / 32 + 1) : room);
+    const int64_t most_rows = (int64_t)kv.max_new * a.group;
+    const bool many = most_rows > kSplitRows;
     const size_t line = (size_t)kv.rows * heads;
-    size_t lines = 0;  // of sums that are joined
-    if (a.rows <= 16) {
-        const int64_t all = (int64_t)kv.seqs * kv.kv_heads * tiles;
-        a.workgroups = (int)std::min<int64_t>(split_workgroups(kv.head_dim), (all + kSplitWaves - 1) / kSplitWaves);
-        if (tiles > kSplitWaves) lines = (size_t)(a.workgroups + kv.seqs * kv.kv_heads) * a.rows;
-    } else {
+    size_t row_lines = 0, split_lines = 0;  // of sums that are joined
+    a.few = many ? 0 : kSplitRows;
+    if (many) {
+        if (kv.starts && kv.seqs * tiles >= kMixedTiles && 2 * ((int64_t)kv.rows - kv.max_new) < (int64_t)(kv.seqs - 1) * kv.max_new) a.few = kSplitRows;
         // As many workgroups as run at a time, each with enough tokens to be worth the 32 to 128 KB of sums that it leaves (us a call with 8, 12, 16, 32 tiles at
         // least, D = 128: 512 tokens over 600 27 22 22 22, 64 of 4 sequences over 2000 31 29 30 36, 32 of 2 over 8000 36 34 35 40; D = 64, 301 of 5 over
         // 1111 in a window 43 43 48 49)
         const int64_t units = std::max<int64_t>(1, row_tiles_of(a) * kv.kv_heads);
         const int64_t enough = std::min<int64_t>((kv.head_dim == 256 ? 1 : 2) * device_cu_count() / units, std::max<int64_t>(1, tiles / kRowsPiece));
         a.row_pieces = (int)std::max<int64_t>(1, enough);
-        if (a.row_pieces > 1) lines = line * a.row_pieces;
+        if (a.row_pieces > 1) row_lines = line * a.row_pieces;
         if (accounts) a.operand_tiles = (int)((int64_t)kv.rows * a.group / 32 + kv.seqs + 1);
     }
+    if (a.few) {
+        a.rows = (int)std::min<int64_t>(most_rows, kSplitRows);
+        const int64_t all = (int64_t)kv.seqs * kv.kv_heads * tiles;
+        a.workgroups = (int)std::min<int64_t>(split_workgroups(kv.head_dim), (all + kSplitWaves - 1) / kSplitWaves);
+        if (tiles > kSplitWaves) split_lines = (size_t)(a.workgroups + kv.seqs * kv.kv_heads) * a.rows;
+    }
+    const size_t lines = std::max(row_lines, split_lines);  // (kv_split_kernel runs when the others' sums are done with)
     // scratch memory, each part on a line of its own
     size_t at = 0;
     const auto part = [&at](size_t bytes) {
@@ -1139,7 +1163,7 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
     const bool keep_scores = score_bytes > 0 && score_bytes <= kMostScoreBytes;
     const size_t operand_tiles = (size_t)a.operand_tiles * kv.kv_heads;
     const size_t lse = part(accounts ? line * 4 : 0), ml = part(lines * 8), sums = part(lines * (size_t)kv.head_dim * 4);
-    const size_t pieces = part(lines && a.workgroups ? (size_t)kv.seqs * kv.kv_heads * 8 : 0), scores = part(keep_scores ? score_bytes : 0);
+    const size_t pieces = part(split_lines ? (size_t)kv.seqs * kv.kv_heads * 8 : 0), scores = part(keep_scores ? score_bytes : 0);
     const size_t operands = part(operand_tiles * 32 * kv.head_dim * (q.bf16 ? 2 : 4)), row_scales = part(operand_tiles * 128);
     if (at) {
         void *ws = nullptr;
@@ -1149,8 +1173,8 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
         if (lines) {
             a.part_ml = reinterpret_cast<float *>(p + ml);
             a.part = reinterpret_cast<float *>(p + sums);
-            a.pieces = reinterpret_cast<int2 *>(p + pieces);
         }
+        if (split_lines) a.pieces = reinterpret_cast<int2 *>(p + pieces);
         if (keep_scores) {
             a.scores = reinterpret_cast<float *>(p + scores);
             a.score_tiles = (int)tiles;

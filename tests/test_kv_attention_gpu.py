@@ -241,6 +241,16 @@ def test_several_tokens(gpu, dtype, dim, kv_heads, heads, window):
 
 
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("dim,heads,window", ((64, 8, 0), (128, 8, 0), (256, 8, 0), (128, 2, 700), (64, 32, 50)))
+def test_prompts_beside_single_tokens(gpu, dtype, dim, heads, window):
+    """One call whose sequences differ in new tokens, so that some have few rows over many tokens and some many: at two key heads of `heads` queries,
+    5 and 4 new tokens lie on either side of sixteen rows."""
+    c = Case(gpu, [2100, 300, 40, 1000, 33, 1, 900] + [5] * 40, dim=dim, page=96, seed=dim + heads, wide_table=30).fill()
+    c.check([1, 70, 0, 4, 5, 1, 3] + [1] * 40, heads, dtype, window, with_accounts=True)
+    c.check([2, 0, 1, 1, 1, 0, 45] + [0, 1] * 20, heads, dtype, window)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
 def test_prompt_of_a_thousand_tokens(gpu, dtype):
     c = Case(gpu, [1217], 1, 128, 128, seed=9).fill()
     c.check([1001], 4, dtype, with_accounts=True)
