@@ -551,7 +551,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
 //
 // Matrix instructions, exponentials and the widening run side by side, two workgroups a CU (2048 rows of 32 heads over 2049 to 4096
 // tokens, D = 128).  With a causal bound workgroups differ in length: the second half of them goes from short to long, so that the two of a CU
-// add up to the same.  That call: 122 us in bfloat16, 845 TFLOP/s (a library product of 8192^3: 1193).
+// add up to the same.  That call: 121 us in bfloat16, 850 TFLOP/s (a library product of 8192^3: 1193): a stage of 64 tokens
+// has 1024 cycles of matrix instructions a wavefront and 1270 of others, which overlap little, and takes 2600.
 constexpr int kRowsWaves = 4, kRowsTile = 32 * kRowsWaves, kRowsPiece = 12;  // rows of a workgroup; tiles of the cache, at least, in a piece of its tokens
 
 template <int D> struct RowsLds {
