@@ -272,11 +272,13 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *waves, uint
 }
 
 // One workgroup per sequence and key head.  A wavefront owns a run of neighbouring tokens, 64 at a time, and holds their keys in
-// registers where IT rounds of them suffice (IT = 0: reads them again for every pass).  The smallest kept key is found digit by
+// registers where IT rounds of them suffice, in LDS where kLdsRounds do (IT = kInLds; IT = 0: reads them again for every pass).  The smallest kept key is found digit by
 // digit, eleven bits at a time of its distance from the smallest key there is, so that keys of similar size spread over the
 // histogram (those that equal the smallest, zeros mostly, are left out of it), until so few are left that each is held against all of them; a wavefront then counts what it keeps, and
 // writes its tokens behind those of the wavefronts in front.
-// The passes' barriers bound it, one behind the other: 10 us for 8 heads of one sequence of 4096 tokens, 28 us for those of 16 sequences of 4096 to 16384.
+// The passes' barriers bound it, one behind the other: 10 us for 8 heads of one sequence of 4096 tokens, 28 us for those of 16 sequences of 4096 to 16384.  20
+// heads of 7000 to 28000 tokens: the keys in LDS 40 us, read again for every pass 71.
+constexpr int kInLds = -1, kLdsRounds = 32;
 template <int IT>
 __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall kv, const float *__restrict__ accounts, int keep, int recent, int32_t *__restrict__ kept) {
     __shared__ uint32_t hist[kBins], waves[kSelectWaves], found[2], ends[3][kSelectWaves], few[kFew], count;
@@ -291,14 +293,15 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall 
     uint32_t want = (uint32_t)(keep - recent);  // of the first n tokens (n > want)
     for (int i = tid; i < recent; i += kSelectThreads) out[want + i] = n + i;
     if (want == 0) return;
-    const int rounds = IT ? IT : (n + kSelectThreads - 1) / kSelectThreads;
+    const int rounds = IT > 0 ? IT : (n + kSelectThreads - 1) / kSelectThreads;
     const int t0 = wave * rounds * 64 + lane;
     // (an account without a page counts as the smallest)
     const auto key_at = [&](int t) {
         const float *p = kv_account(kv, const_cast<float *>(accounts), b, h, t);
         return p ? account_key(*p) : 0u;
     };
-    uint32_t keys[IT ? IT : 1];
+    uint32_t keys[IT > 0 ? IT : 1];
+    extern __shared__ uint32_t lds_keys[];  // [round][thread]: a thread reads what it has written
     if constexpr (IT > 0) {
         // (loads without branches between them, of the last token where there is none: they go out together)
         int64_t at[IT];
@@ -312,12 +315,25 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall 
             const uint32_t u = kv.pages ? account_key(accounts[max(at[i], (int64_t)0)]) : 0u;
             keys[i] = at[i] < 0 ? 0u : u;
         }
+    } else if constexpr (IT == kInLds) {
+#pragma unroll 8
+        for (int i = 0; i < rounds; i++) {
+            const int t = min(t0 + 64 * i, n - 1), slot = page_slot(kv, t >> 5), page = kv.table[b * kv.table_stride + slot];
+            const bool there = (uint32_t)page < (uint32_t)kv.pages;
+            const int64_t at = there ? ((int64_t)page * kv.kv_heads + h) * kv.page_tokens + (t - slot * kv.page_tokens) : 0;
+            const uint32_t u = kv.pages ? account_key(accounts[at]) : 0u;
+            lds_keys[i * kSelectThreads + tid] = there ? u : 0u;
+        }
     }
     const auto each = [&](auto f) {  // f(token, key) for the thread's tokens
         if constexpr (IT > 0) {
 #pragma unroll
             for (int i = 0; i < IT; i++)
                 if (t0 + 64 * i < n) f(t0 + 64 * i, keys[i]);
+        } else if constexpr (IT == kInLds) {
+#pragma unroll 4
+            for (int i = 0; i < rounds; i++)
+                if (t0 + 64 * i < n) f(t0 + 64 * i, lds_keys[i * kSelectThreads + tid]);
         } else {
             for (int i = 0; i < rounds; i++)
                 if (t0 + 64 * i < n) f(t0 + 64 * i, key_at(t0 + 64 * i));
@@ -428,7 +444,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvCall 
 #pragma unroll
         for (int i = 0; i < IT; i++) place(t0 + 64 * i, keys[i]);
     } else {
-        for (int i = 0; i < rounds; i++) place(t0 + 64 * i, t0 + 64 * i < n ? key_at(t0 + 64 * i) : 0u);
+        for (int i = 0; i < rounds; i++) place(t0 + 64 * i, IT == kInLds ? lds_keys[i * kSelectThreads + tid] : t0 + 64 * i < n ? key_at(t0 + 64 * i) : 0u);
     }
 }
 
@@ -651,8 +667,15 @@ int launch_kv_evict(const KvCall &kv, float *accounts, int keep, int recent, int
     const dim3 grid((unsigned)kv.kv_heads, (unsigned)kv.seqs);
     const int64_t n = (int64_t)kv.max_pages * kv.page_tokens - recent;  // tokens to choose from, at most
     // (32 keys a thread no longer fit the 128 registers of a workgroup of 1024)
-    const auto select = n <= 4 * kSelectThreads ? kv_select_kernel<4> : n <= 16 * kSelectThreads ? kv_select_kernel<16> : kv_select_kernel<0>;
-    if (int rc = launch(select, grid, dim3(kSelectThreads), 0, s, kv, accounts, keep, recent, kept)) return rc;
+    if (n > 16 * kSelectThreads && n <= kLdsRounds * kSelectThreads) {
+        constexpr int bytes = kLdsRounds * kSelectThreads * 4;
+        static const bool lds_ok = hipFuncSetAttribute(reinterpret_cast<const void *>(kv_select_kernel<kInLds>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+        if (!lds_ok) return fail(GQ_ERR_HIP, "kv_evict: cannot reserve %d bytes of LDS", bytes);
+        if (int rc = launch(kv_select_kernel<kInLds>, grid, dim3(kSelectThreads), bytes, s, kv, accounts, keep, recent, kept)) return rc;
+    } else {
+        const auto select = n <= 4 * kSelectThreads ? kv_select_kernel<4> : n <= 16 * kSelectThreads ? kv_select_kernel<16> : kv_select_kernel<0>;
+        if (int rc = launch(select, grid, dim3(kSelectThreads), 0, s, kv, accounts, keep, recent, kept)) return rc;
+    }
     switch (kv.head_dim) {
     case 64: return move_kept<64>(kv, accounts, keep, kept, new_lengths, s);
     case 128: return move_kept<128>(kv, accounts, keep, kept, new_lengths, s);

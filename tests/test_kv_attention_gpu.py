@@ -434,6 +434,24 @@ def test_evict_long_sequences(gpu, length, kind):
         assert kept[0, 0].tolist() == ref.evict(accounts, keep, recent).tolist()
 
 
+@pytest.mark.parametrize("choose", (4096, 16384, 16416, 32768, 32800))
+def test_evict_at_the_ends_of_the_selections_forms(gpu, choose):
+    """As many tokens to choose from as one form takes and the next: kept in registers, in LDS, or read again.  Ties among them."""
+    torch = gpu
+    from gomlx_amd import nn
+    rng = np.random.default_rng(choose)
+    length, recent = choose + 32, 32
+    accounts = np.round(4 * rng.standard_normal((2, length))).astype(np.float32)
+    pages = length // 32
+    cache, table = nn.kv_cache(pages, 2, 64, 32), torch.arange(pages, device="cuda").int().view(1, -1)
+    w = torch.from_numpy(accounts).cuda().view(2, pages, 32).transpose(0, 1).contiguous()
+    n = torch.tensor([length], dtype=torch.int32, device="cuda")
+    for keep in (recent + 1, length // 2, length - 1):
+        kept, _ = nn.kv_cache_evict(cache, w.clone(), table, n, keep, recent)
+        for h in range(2):
+            assert kept[0, h].tolist() == ref.evict(accounts[h], keep, recent).tolist()
+
+
 def test_every_scale(gpu):
     """The quotient that codes are rounded from, over every scale that there is and values around every code's border."""
     torch = gpu
