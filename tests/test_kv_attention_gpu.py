@@ -251,6 +251,15 @@ def test_prompts_beside_single_tokens(gpu, dtype, dim, heads, window):
 
 
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("dim", (64, 128, 256))
+def test_accounts_where_scores_have_no_room(gpu, dtype, dim):
+    """A page table of 15000 columns: the scores of the rows that it has room for would be more than 256 MB, so the accounts are made from the keys."""
+    c = Case(gpu, [1, 0, 33, 500, 64, 130, 31, 90, 700], 2, dim, 64, seed=dim, wide_table=15000).fill()
+    c.check([1] * 9, 8, dtype, with_accounts=True)
+    c.check([1, 0, 2, 4, 3, 1, 1, 4, 2], 6, dtype, with_accounts=True)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
 def test_prompt_of_a_thousand_tokens(gpu, dtype):
     c = Case(gpu, [1217], 1, 128, 128, seed=9).fill()
     c.check([1001], 4, dtype, with_accounts=True)
