@@ -759,8 +759,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
 
     // One stage, from buffer `mine`; the next one, which has been on its way for a stage, goes into `other`.  (Making the next stage's scores in front of these weights, so that one wavefront has
     // both kinds of work to issue, was no faster: the second workgroup of the CU does as well.)
-    const auto step = [&](int tile, int mine, int other) __attribute__((always_inline)) {
-        load(fetched[mine]);
+    const auto attend_stage = [&](int tile, int mine) __attribute__((always_inline)) {
         f16 s[T];
 #pragma unroll
         for (int t = 0; t < T; t++) {
@@ -852,6 +851,12 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, TWO ? 8 : 4, 1);
+    };
+    // (a wavefront without rows widens for the others; at D = 256 the branch would move accumulators about: 56 us become 65)
+    const bool rows_here = D == 256 || wave * 32 < span.rows;
+    const auto step = [&](int tile, int mine, int other) __attribute__((always_inline)) {
+        load(fetched[mine]);
+        if (rows_here) attend_stage(tile, mine);
         if (tile + T < tile1) widen(fetched[other], other);
         __syncthreads();
     };
@@ -1167,12 +1172,15 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
     a.few = many ? 0 : kSplitRows;
     if (many) {
         if (kv.starts && kv.seqs * tiles >= kMixedTiles && 2 * ((int64_t)kv.rows - kv.max_new) < (int64_t)(kv.seqs - 1) * kv.max_new) a.few = kSplitRows;
-        // As many workgroups as run at a time, each with enough tokens to be worth the 32 to 128 KB of sums that it leaves (us a call with 8, 12, 16, 32 tiles at
-        // least, D = 128: 512 tokens over 600 27 22 22 22, 64 of 4 sequences over 2000 31 29 30 36, 32 of 2 over 8000 36 34 35 40; D = 64, 301 of 5 over
-        // 1111 in a window 43 43 48 49)
-        const int64_t units = std::max<int64_t>(1, row_tiles_of(a) * kv.kv_heads);
-        const int64_t enough = std::min<int64_t>((kv.head_dim == 256 ? 1 : 2) * device_cu_count() / units, std::max<int64_t>(1, tiles / kRowsPiece));
-        a.row_pieces = (int)std::max<int64_t>(1, enough);
+        // Pieces of a row tile's tokens: as many workgroups as run at a time (row tiles as if sequences had the same number of new tokens), each with enough
+        // tokens for its start (us a call with 8, 12, 16, 32 tiles at least, D = 128: 512 tokens over 600 27 22 22 22, 64 of 4 sequences over 2000 31 29 30 36, 32 of
+        // 2 over 8000 36 34 35 40; D = 64, 301 of 5 over 1111 in a window 43 43 48 49), and no more than pay for a launch and for the sums' way to memory and back: at
+        // two pieces 8 tokens of 32 sequences over 4000 take 56 us for 94, 300 of 4 over 1000 59 for 52.
+        const int64_t units = (((int64_t)kv.rows * a.group + kv.seqs - 1) / kv.seqs + kRowsTile - 1) / kRowsTile * kv.seqs * kv.kv_heads;
+        const double tile_us = (kv.head_dim == 64 ? 0.5 : kv.head_dim == 128 ? 0.62 : 1.3) * (q.bf16 ? 1.0 : 1.6), sums_us = 2.0 * line * kv.head_dim * 4 / 4.5e6;  // (as measured, two workgroups a CU where they fit)
+        int64_t pieces = std::min<int64_t>((kv.head_dim == 256 ? 1 : 2) * device_cu_count() / units, tiles / kRowsPiece);
+        while (pieces > 1 && tiles * tile_us * (pieces - 1) < (4.0 + sums_us * pieces) * pieces) pieces--;
+        a.row_pieces = (int)std::max<int64_t>(1, pieces);
         if (a.row_pieces > 1) row_lines = line * a.row_pieces;
         if (accounts) a.operand_tiles = (int)((int64_t)kv.rows * a.group / 32 + kv.seqs + 1);
     }
