@@ -4,7 +4,7 @@
 //     o_i  = sum_j P_ij v_j,  P_i = softmax(s_i);  a row that sees nothing gets zeros
 //     account_j += sum of P_ij over the rows and the query heads of the key head (where asked for)
 //
-// Both products run on v_mfma_f32_16x16x32_f16.  Keys and values are fp16 numbers as they stand (kv.hpp), q is scaled by a power
+// Both products run on the fp16 matrix instructions (16x16x32 for few rows, 32x32x16 for many).  Keys and values are fp16 numbers as they stand (kv.hpp), q is scaled by a power
 // of two per row and taken as one fp16 number (bf16: exact) or as the sum of two (fp32: 22 bits), P likewise as one (bf16) or
 // two; scores, running maximum, sums and results are fp32.
 //
