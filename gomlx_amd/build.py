@@ -119,7 +119,7 @@ def build_binding(verbose: bool = True) -> str:
     inc = [os.path.join(T, "include"), os.path.join(T, "include", "torch", "csrc", "api", "include"), "/opt/rocm/include", sysconfig.get_paths()["include"]]
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(x for i in inc for x in ("-isystem", i)),
-           os.path.join(CSRC, "binding.cpp"), "-o", BINDING, "-L" + os.path.join(T, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+           os.path.join(CSRC, "binding.cpp"), "-o", BINDING, "-L" + os.path.join(T, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"binding build failed:\n{r.stdout}\n{r.stderr}")
