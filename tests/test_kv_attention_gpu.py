@@ -280,6 +280,18 @@ def test_large_and_small_scores(gpu, dtype, news):
 
 
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("dim,news", ((64, 1), (64, 40), (256, 1), (256, 40), (256, 130)))
+def test_scores_that_grow_along_the_sequence(gpu, dtype, dim, news):
+    """What a row has summed is scaled down again and again: later keys are larger, and queries so large that every tile has a new largest score."""
+    c = Case(gpu, [420], 2, dim, 64, seed=dim + news, scale=2.0)
+    c.k[0] *= np.linspace(0.1, 1.5, 420, dtype=np.float32)[:, None, None]
+    c.fill()
+    q = gpu.randn(news, 4, dim, device="cuda", generator=gpu.Generator("cuda").manual_seed(news))
+    for factor in (2.0, 25.0):
+        c.check([news], 4, dtype, q=q * factor, with_accounts=True)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
 def test_tiny_keys_and_values_are_exact_operands(gpu, dtype):
     """Values whose scales are fp16 denormals: the matrix instructions must not flush them."""
     c = Case(gpu, [100], 1, 64, 32, seed=5)
