@@ -83,8 +83,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const RopeArgs a) {
     const bool known = (uint32_t)pos < (uint64_t)a.table_rows;
     const int64_t at = known ? (int64_t)pos * half : 0;
     float4 y = x;
+    const bool turns = known && d < a.rot;  // (nothing is read for a position that the table does not have: it may have none, and no memory)
     if constexpr (INTERLEAVED) {
-        if (d < a.rot) {
+        if (turns) {
             const float2 c = *reinterpret_cast<const float2 *>(a.cos + at + (d >> 1)), s = *reinterpret_cast<const float2 *>(a.sin + at + (d >> 1));
             y.x = fmaf(x.x, c.x, -(x.y * s.x));
             y.y = fmaf(x.x, s.x, x.y * c.x);
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const RopeArgs a) {
         const int step = half >> 2;  // lanes to the partner
         const int from = ((int)threadIdx.x & 63) + (d < a.rot ? (upper ? -step : step) : 0);
         const float4 o = make_float4(__shfl(x.x, from), __shfl(x.y, from), __shfl(x.z, from), __shfl(x.w, from));
-        if (d < a.rot) {
+        if (turns) {
             const int i = upper ? d - half : d;
             const float4 c = *reinterpret_cast<const float4 *>(a.cos + at + i);
             float4 s = *reinterpret_cast<const float4 *>(a.sin + at + i);

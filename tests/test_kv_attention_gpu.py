@@ -570,6 +570,23 @@ def test_qk_norm_rope_rows_off_every_vector(gpu):
     assert torch.equal(a, zero)
 
 
+@pytest.mark.parametrize("dim", (64, 128, 256))
+@pytest.mark.parametrize("interleaved", (False, True))
+@pytest.mark.parametrize("kind", ("f32", "bf16"))
+def test_qk_norm_rope_without_a_table(gpu, dim, interleaved, kind):
+    """A table of no rows, which has no memory, and one cut to no rows: every position lies outside, every row is NaN."""
+    torch = gpu
+    from gomlx_amd import nn
+    q, k = (torch.randn(5, h, dim, device="cuda").to({"f32": torch.float32, "bf16": torch.bfloat16}[kind]) for h in (3, 1))
+    pos = torch.tensor([0, 1, -1, 7, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    full = nn.rotary_table(8, dim)
+    for cos, sin in (nn.rotary_table(0, dim), [t[:0] for t in full], nn.rotary_table(0, 8)):
+        for y in nn.qk_norm_rope(q, k, pos, cos, sin, q_norm=nn.RMSNorm(), interleaved=interleaved):
+            assert y.isnan().all()
+    for y in nn.qk_norm_rope(q, k, pos, *full, interleaved=interleaved):
+        assert y.isnan().all(-1).all(-1).tolist() == [False, False, True, False, True] and y.isnan().any(-1).any(-1).tolist() == [False, False, True, False, True]
+
+
 # ---- together -----------------------------------------------------------------------------------------------------------
 
 
