@@ -34,8 +34,9 @@ template <int D> struct KvTile {
 __device__ __forceinline__ int key_row(int t) { return (t >> 3) * 4 + (t & 3); }
 __device__ __forceinline__ int key_half(int t) { return (t >> 2) & 1; }
 
-// What sequence b of a call has: `length` tokens, the last `news` of them new, their rows from `row0` on.
-struct KvSeq { int length, news, row0; };
+// What sequence b of a call has: tokens 0 .. length - 1 that its pages have room for, and `news` rows from `row0` on, of which row n is token first + n
+// (a negative one, or one from `length` on, is absent).
+struct KvSeq { int length, news, row0, first; };
 
 // The lanes' values up to and with each, combined by f, by data-parallel moves: 1, 2, 4, 8 lanes within rows of sixteen, then from the last lane
 // of a row into the next one, and of the first half into the second.  `none` combines to nothing.
@@ -55,7 +56,8 @@ __device__ __forceinline__ int lane_scan(int v) {
 // A load that is the same for the whole wavefront, through the scalar cache (of what no kernel of this launch writes).
 __device__ __forceinline__ int32_t uniform_load(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
 
-// Lengths beyond the page table and rows beyond the call's are cut off, so that no device value leads a kernel out of its buffers.
+// Tokens beyond the page table and rows beyond the call's are left out, so that no device value leads a kernel out of its buffers.  The places of
+// the others go by the length and the starts as they are.
 __device__ __forceinline__ KvSeq kv_seq(const KvCall &kv, int b) {
     KvSeq s;
     const int64_t room = (int64_t)kv.max_pages * kv.page_tokens;
@@ -65,9 +67,12 @@ __device__ __forceinline__ KvSeq kv_seq(const KvCall &kv, int b) {
     int from = b, to = b + 1;
     if (kv.starts) { from = kv.starts[b]; to = kv.starts[b + 1]; }
     from = from < 0 ? 0 : from > kv.rows ? kv.rows : from;
-    to = to < from ? from : to > kv.rows ? kv.rows : to;
+    to = to < from ? from : to;
+    const int first = length - (to - from);
+    to = to > kv.rows ? kv.rows : to;
     s.row0 = from;
     s.news = to - from > kv.max_new ? kv.max_new : to - from;
+    s.first = first < -s.news ? -s.news : first;  // (every place is in front of the sequence either way)
     return s;
 }
 

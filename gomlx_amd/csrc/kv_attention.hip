@@ -82,11 +82,9 @@ __device__ __forceinline__ Span row_tile_span(const KvSeq &s, int group, int win
     r.rows = r.rows < 0 ? 0 : r.rows > tile_rows ? tile_rows : r.rows;
     r.lo = r.hi = 0;
     if (r.rows > 0) {
-        const int base = s.length - s.news;
-        const int hi = base + (r.first_row + r.rows - 1) / group + 1;
-        const int lo = window ? base + r.first_row / group + 1 - window : 0;
-        r.hi = hi < 0 ? 0 : hi;
-        r.lo = lo < 0 ? 0 : lo;
+        const int hi = s.first + (r.first_row + r.rows - 1) / group + 1, first = s.first + r.first_row / group + 1;
+        r.hi = hi < 0 ? 0 : min(hi, s.length);
+        r.lo = window && first > window ? min(first - window, r.hi) : 0;
     }
     return r;
 }
@@ -243,6 +241,11 @@ template <int BYTES, int STEP> struct TileWalk {
     }
 };
 
+__device__ __forceinline__ KvSeq seq_of_lane(const KvSeq &s, int lane) {
+    return KvSeq{__builtin_amdgcn_readlane(s.length, lane), __builtin_amdgcn_readlane(s.news, lane), __builtin_amdgcn_readlane(s.row0, lane),
+                 __builtin_amdgcn_readlane(s.first, lane)};
+}
+
 // How the tiles of a call are shared out over its workgroups.  A unit is a sequence and key head (all rows of it: sixteen at most),
 // with the tiles that its rows see (one at least, so that rows that see nothing are written too).  Units are cut into pieces
 // of one length, of which all units together have about a.workgroups, one piece a workgroup: the lengths are known on the device only, so
@@ -266,10 +269,10 @@ __device__ __forceinline__ Piece piece_of(const AttendArgs &a, int index) {
     const int lane = (int)threadIdx.x & 63, seqs = a.kv.seqs, heads = a.kv.kv_heads;
     Piece p;
     p.b = -1;
-    KvSeq mine{0, 0, 0};
+    KvSeq mine{};
     int tiles = 0, total = 0;
     for (int base = (seqs - 1) & ~63; base >= 0; base -= 64) {  // (the first 64 last: they stay)
-        mine = KvSeq{0, 0, 0};
+        mine = KvSeq{};
         if (base + lane < seqs) mine = kv_seq(a.kv, base + lane);
         tiles = tiles_of(span_of(a, mine));
         total += __builtin_amdgcn_readlane(lane_scan(tiles), 63) * heads;
@@ -280,7 +283,7 @@ __device__ __forceinline__ Piece piece_of(const AttendArgs &a, int index) {
     int front = 0;  // pieces in front
     for (int base = 0; base < seqs; base += 64) {
         if (base) {
-            mine = KvSeq{0, 0, 0};
+            mine = KvSeq{};
             if (base + lane < seqs) mine = kv_seq(a.kv, base + lane);
             tiles = tiles_of(span_of(a, mine));
         }
@@ -290,7 +293,7 @@ __device__ __forceinline__ Piece piece_of(const AttendArgs &a, int index) {
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             p.b = base + l;
-            p.seq = KvSeq{__builtin_amdgcn_readlane(mine.length, l), __builtin_amdgcn_readlane(mine.news, l), __builtin_amdgcn_readlane(mine.row0, l)};
+            p.seq = seq_of_lane(mine, l);
             p.span = span_of(a, p.seq);
             p.tiles = __builtin_amdgcn_readlane(tiles, l);
             const int each = __builtin_amdgcn_readlane(unit, l), in = index - (front + __builtin_amdgcn_readlane(upto, l) - each * heads);
@@ -365,7 +368,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
     const int nth = live ? r / a.group : 0;              // new token of the row
     const int head = h * a.group + (live ? r - nth * a.group : 0);
     const int64_t row = seq.row0 + nth;
-    const int base = seq.length - seq.news, place = base + nth;  // its own token
+    const int base = seq.first, place = base + nth;  // its own token
     const int see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
     // tokens that every row sees (the operand rows that stand for none have scores of 0 and go nowhere)
     const int all_hi = base + 1, all_lo = a.window ? base + (span.rows - 1) / a.group + 1 - a.window : 0;
@@ -624,14 +627,14 @@ __device__ __forceinline__ RowTile row_tile_of(const AttendArgs &a, int index) {
     t.b = -1;
     int front = 0;
     for (int base = 0; base < seqs; base += 64) {
-        KvSeq mine{0, 0, 0};
+        KvSeq mine{};
         if (base + lane < seqs) mine = kv_seq(a.kv, base + lane);
         const int rows = mine.news * a.group, tiles = rows > a.few ? (rows + kRowsTile - 1) / kRowsTile : 0, upto = lane_scan(tiles);
         const uint64_t past = __ballot(front + upto > index);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             t.b = base + l;
-            t.seq = KvSeq{__builtin_amdgcn_readlane(mine.length, l), __builtin_amdgcn_readlane(mine.news, l), __builtin_amdgcn_readlane(mine.row0, l)};
+            t.seq = seq_of_lane(mine, l);
             t.tiles = __builtin_amdgcn_readlane(tiles, l);
             t.tile = index - (front + __builtin_amdgcn_readlane(upto, l) - t.tiles);
             break;
@@ -691,7 +694,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     const int nth = live ? idx / a.group : 0;
     const int head = h * a.group + (live ? idx - nth * a.group : 0);
     const int64_t row = seq.row0 + nth;
-    const int base = seq.length - seq.news, place = base + nth;
+    const int base = seq.first, place = base + nth;
     const int own = live ? place : -1;  // (a row that is none, or without tokens, sees nothing)
     const uint32_t most_behind = a.window ? (uint32_t)a.window : 0x80000000u;
     // what every row of the wavefront sees
@@ -955,13 +958,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void kv_rows_
     const KvCall &kv = a.kv;
     const int h = (int)blockIdx.y, b = (int)blockIdx.z;
     const KvSeq seq = kv_seq(kv, b);
-    const int base = seq.length - seq.news;
-    const int tile = (a.window ? max(0, base + 1 - a.window) >> 5 : 0) + (int)blockIdx.x * NT, t0 = tile * 32;
-    if (t0 >= seq.length || seq.news * a.group <= a.few) return;
+    const int base = seq.first;
+    const int tile = (a.window && base + 1 > a.window ? (base + 1 - a.window) >> 5 : 0) + (int)blockIdx.x * NT;
+    if (tile >= (seq.length + 31) >> 5 || seq.news * a.group <= a.few) return;
+    const int t0 = tile * 32;
     const int lane = (int)threadIdx.x & 63, r = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     // the new tokens that see one of the tiles', and their operand tiles
-    const int n0 = max(0, t0 - base), n1 = a.window ? min(seq.news, t0 + 32 * NT - 1 + a.window - base) : seq.news;
+    const int n0 = max(0, t0 - base), n1 = a.window ? (int)min((int64_t)seq.news, (int64_t)t0 + 32 * NT - 1 + a.window - base) : seq.news;
     const int from = n0 * a.group / 32 + wave, to = (n1 * a.group + 31) / 32;
     const int64_t first = (int64_t)h * a.operand_tiles + first_operand_tile(a, seq, b);
     struct Rows {  // 32 rows
@@ -1085,7 +1089,7 @@ __global__ __launch_bounds__(256) void kv_account_kernel(const AttendArgs a) {
     const bool live = r < span.rows;
     const int nth = live ? r / a.group : 0, head = h * a.group + (live ? r - nth * a.group : 0);
     const int64_t row = seq.row0 + nth;
-    const int place = seq.length - seq.news + nth, see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
+    const int place = seq.first + nth, see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
     const Unpack unpack;
     h8 qh[D / 32], ql[TWO ? D / 32 : 1];
     float back, s[8];

@@ -100,14 +100,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
         load8<BF16>(v[0], a.v.p, (int64_t)b * a.v.row + h * a.v.head + x, a.wide);
     }
     const KvSeq s = kv_seq(kv, b);
-    const int first = s.length - s.news, from = first < 0 ? 0 : first;
-    const int block = (from >> 3) + nth, p0 = block * 8;
-    if (p0 >= s.length || s.news == 0) return;
+    const int first = s.first, from = first < 0 ? 0 : first, end = min(first + s.news, s.length);  // new tokens that have a place: from .. end - 1
+    if (nth * 8 >= end - (from & ~7) || from >= end) return;
+    const int p0 = (from & ~7) + nth * 8;
     uint8_t *tile = kv_tile(kv, b, h, p0 >> 5, T::kBytes);
     if (!tile) return;
     const int j = (p0 >> 3) & 3;
     const bool account = a.accounts && l == 0;
-    const int live_from = from > p0 ? from - p0 : 0, live_to = s.length - p0 < 8 ? s.length - p0 : 8;  // new tokens of the block
+    const int live_from = from > p0 ? from - p0 : 0, live_to = end - p0 < 8 ? end - p0 : 8;  // new tokens of the block
     uint32_t live_mask = 0;
     for (int e = live_from; e < live_to; e++) live_mask |= 0xFu << nibble_shift(e);
     // the dwords of value codes that the lane will finish, where other tokens share them
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
 }
 
 // What the cache stands for at the last tokens of every sequence, in the fp16 numbers that it holds; zeros in front of a
-// sequence's first token and where the page table names no page.  Bytes bound it: 7.3 us for the tokens of the 7 prompts above.
+// sequence's first token, behind the page table's end and where it names no page.  Bytes bound it: 7.3 us for the tokens of the 7 prompts above.
 template <int D>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvCall kv, uint16_t *__restrict__ K, uint16_t *__restrict__ V, int blocks) {
     typedef KvTile<D> T;
@@ -200,10 +200,10 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvCall kv, uint16_t 
     if (b >= kv.seqs) return;
     const int rest = (int)(unit - (int64_t)b * per), h = rest / blocks, nth = rest - h * blocks;
     const KvSeq s = kv_seq(kv, b);
-    const int first = s.length - s.news;
-    const int p0 = (first >> 3) * 8 + nth * 8;  // (an arithmetic shift: blocks of eight also in front of the first token)
-    if (p0 >= s.length) return;
-    const uint8_t *tile = p0 >= 0 ? kv_tile(kv, b, h, p0 >> 5, T::kBytes) : nullptr;
+    const int first = s.first, end = first + s.news;
+    if (nth * 8 >= end - (first & ~7)) return;
+    const int p0 = (first & ~7) + nth * 8;  // (blocks of eight also in front of the first token)
+    const uint8_t *tile = p0 >= 0 && p0 < s.length ? kv_tile(kv, b, h, p0 >> 5, T::kBytes) : nullptr;
     const int lane = (int)threadIdx.x & 63, x = lane * NE, j = (p0 >> 3) & 3, g = x >> 5;
     uint32_t vw[NE] = {};
     if (tile) {
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvCall kv, uint16_t 
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         const int p = p0 + e;
-        if (p < first || p >= s.length) continue;
+        if (p < first || p >= end) continue;
         uint16_t k[NE] = {}, v[NE] = {};
         if (tile) {
             const int t = p & 31, w = key_half(t) * G + g, l = key_row(t) + 16 * ((x >> 3) & 3);

@@ -460,7 +460,7 @@ def kv_cache(pages: int, kv_heads: int, head_dim: int, page_tokens: int = 64, de
     may hold anything.  The calls below take it with ``lengths``, int32 [sequences], the tokens of each sequence with the call's new ones.
     A call's rows are one new token per sequence, or, with ``starts`` (int32 [sequences + 1]), rows ``starts[b]`` to ``starts[b + 1]`` the
     new tokens of sequence b, at most ``max_new``: in either case the last tokens of the sequence.  Table, lengths and starts are read
-    on the device.  A table may be a slice of the first columns of a wider one: its width bounds the work that is laid out."""
+    on the device; a token that the table has no page for is absent: not written, not attended to.  A table may be a slice of the first columns of a wider one: its width bounds the work that is laid out."""
     if head_dim not in _HEAD_DIMS:
         raise _lib.NotImplementedByBackend(_lib.ERR_NOT_IMPLEMENTED, f"kv_cache: head_dim {head_dim} is not implemented (64, 128, 256)")
     if pages < 0 or kv_heads < 1 or page_tokens < 1 or page_tokens % 32:
@@ -492,7 +492,7 @@ def kv_cache_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_
 def kv_cache_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, max_new: int = 1,
                   rows: int | None = None) -> tuple:
     """(keys, values) float16 [rows, kv_heads, head_dim] that the cache stands for at the last tokens of every sequence, exact.  Rows in
-    front of a sequence's first token are zero."""
+    front of a sequence's first token and rows of absent tokens are zero; rows that belong to no sequence hold anything."""
     if _lib.fast is not None and (out := _lib.fast.kv_read(cache, page_table, lengths, starts, max_new, rows)) is not None:
         return out
     import ctypes

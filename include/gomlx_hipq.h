@@ -241,8 +241,9 @@ int gq_embedding_lookup(int type, const void *dTable, int64_t vocab, int64_t K,
  * dLengths[b] counts the tokens of sequence b with its new ones.  The rows dStarts[b] to dStarts[b + 1] of a call's row
  * arguments are its new tokens, the last ones of it (at most max_new); dStarts == NULL: row b is the one new token of sequence b.
  * These arrays lie on the device, so that a recorded graph replays over growing sequences.  Device values that lead out of the
- * buffers are not followed: lengths are cut at the page table's end, rows at `rows`, and a token whose page is none of the
- * cache's is taken as absent. ---- */
+ * buffers are not followed: a token behind the page table's end, or whose page is none of the cache's, is absent (not written, not
+ * seen, read as zeros; the others keep their places), as are rows beyond `rows` and, of more than max_new rows of a sequence, those
+ * behind the first max_new.  Outputs of rows of no sequence hold anything. ---- */
 typedef struct {
     void *dCache;
     int64_t pages;
@@ -272,7 +273,8 @@ int gq_qk_norm_rope(int dtype, const gq_head_rows *q, int q_heads, const gq_head
  * head's key or value, a NaN among them, is kept as one that makes every row that attends to it NaN (its key reads as NaN, its
  * value as 0).  dAccounts (may be NULL): [pages, kv_heads, page_tokens], set to 0 for the new tokens. */
 int gq_kv_append(const gq_kv_cache *kv, int dtype, const gq_head_rows *k, const gq_head_rows *v, float *dAccounts, void *stream);
-/* What the cache stands for at the new (last) tokens: fp16 [rows, kv_heads, head_dim], exact; zeros in front of a sequence's first token. */
+/* What the cache stands for at the new (last) tokens: fp16 [rows, kv_heads, head_dim], exact; zeros in front of a sequence's first token
+ * and for absent ones. */
 int gq_kv_read(const gq_kv_cache *kv, uint16_t *dK, uint16_t *dV, void *stream);
 /* Attention of the new tokens over their sequences, o = softmax(scale q . k) v: a token sees itself and the tokens in front of
  * it, with window > 0 the last `window` of them.  heads is a multiple of kv_heads; neighbouring query heads share a key head.
@@ -285,7 +287,7 @@ int gq_kv_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int
 /* Eviction by account: of every sequence longer than `keep` and every key head stay the last `recent` tokens and the
  * keep - recent others of largest account (ties: the lower token; NaN counts as the largest), moved to the front of its pages
  * in their order, with their accounts.  dKept[seqs, kv_heads, keep]: their former places, -1 behind the last one;
- * dNewLengths[seqs] (may be dLengths itself): min(length, keep).  dStarts, rows and max_new are not used.  Sequences must not share pages. */
+ * dNewLengths[seqs] (may be dLengths itself): min(length, keep).  A length beyond the page table is taken as one that ends with it.  dStarts, rows and max_new are not used.  Sequences must not share pages. */
 int gq_kv_evict(const gq_kv_cache *kv, float *dAccounts, int64_t keep, int64_t recent, int32_t *dKept, int32_t *dNewLengths, void *stream);
 
 /* ---- Executable.Execute of a compiled graph (core/graph/graph.go:669): a sequence of

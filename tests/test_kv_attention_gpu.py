@@ -373,6 +373,93 @@ def test_device_values_that_lead_nowhere(gpu):
     torch.cuda.synchronize()
 
 
+def absent_case(torch, length, rows, heads, room, dim, seed):
+    """Two sequences of `room` cached tokens, of which the first says that it has `length` with `rows` new ones; a plain copy of everything."""
+    c = Case(torch, [room, room], 2, dim, 32, seed=seed).fill()
+    accounts = torch.from_numpy(c.rng.random((c.pages, 2, 32)).astype(np.float32)).cuda()
+    k, v, q = (torch.from_numpy(c.rng.standard_normal((rows, h, dim)).astype(np.float32)).cuda() for h in (2, 2, heads))
+    return c, accounts, k, v, q
+
+
+@pytest.mark.parametrize("dim", (64, 128, 256))
+@pytest.mark.parametrize("length,rows,max_new", ((130, 4, 4), (150, 60, 60), (129, 1, 1), (300, 40, 40), (100, 10, 6), (100, 70, 30), (150, 70, 40), (50, 90, 60)))
+def test_tokens_without_a_place(gpu, dim, length, rows, max_new):
+    """A sequence that has outgrown its page table, and rows behind the first max_new: new tokens lie where the length says, those without a place are
+    absent, and nothing else moves: not the cached tokens in front, their accounts, nor other pages."""
+    torch, room, heads = gpu, 128, 4
+    c, accounts, k, v, q = absent_case(torch, length, rows, heads, room, dim, length + rows)
+    nn, place = c.nn, [length - rows + n for n in range(min(rows, max_new))]
+    stored = [n for n, p in enumerate(place) if 0 <= p < room]
+    lengths, starts = c.ints([length, room]), c.ints([0, rows, rows])
+    before, w0 = c.host().copy(), accounts.cpu().numpy()
+    nn.kv_cache_append(c.cache, k, v, c.d_table, lengths, starts=starts, max_new=max_new, weights=accounts)
+    host, w1 = c.host(), accounts.cpu().numpy()
+    new = ref.quantise(k.cpu().numpy(), v.cpu().numpy())
+    expect = w0.copy()
+    for n in stored:
+        expect[c.table[0, place[n] // 32], :, place[n] % 32] = 0
+    assert np.array_equal(w1, expect)
+    for h in range(2):
+        for i, (x, y) in enumerate(zip(ref.decode(before, c.table[0], room, h), ref.decode(host, c.table[0], room, h))):
+            for n in stored:
+                x[place[n]] = new[i][n, h]
+            assert np.array_equal(x, y)
+    others = sorted(set(range(c.pages)) - set(c.table[0].tolist()))
+    assert np.array_equal(before[others], host[others])
+    got = nn.kv_cache_read(c.cache, c.d_table, lengths, starts=starts, max_new=max_new, rows=rows)
+    for i, x in enumerate(got):
+        x = x.double().cpu().numpy()
+        for n, p in enumerate(place):
+            want = np.zeros((2, dim)) if not 0 <= p < room else np.stack([ref.decode(host, c.table[0], room, h)[i][p] for h in range(2)])
+            assert np.array_equal(x[n], want)
+    for dtype in ("f32", "bf16"):
+        for window in (0, 45):
+            w = torch.from_numpy(w0).cuda()
+            qd = q.to({"f32": torch.float32, "bf16": torch.bfloat16}[dtype])
+            out = nn.cached_attention(qd, c.cache, c.d_table, lengths, starts=starts, max_new=max_new, window=window, weights=w).double().cpu().numpy()
+            total, slack = w0.astype(np.float64), np.abs(w0.astype(np.float64)) * 2 * EPS
+            for h in range(2):
+                keys, values = ref.decode(host, c.table[0], room, h)
+                for n, p in enumerate(place):
+                    lo, hi = max(0, p + 1 - window if window else 0), min(p + 1, room)
+                    y = out[n, 2 * h:2 * h + 2]
+                    if lo >= hi:
+                        assert np.all(y == 0)
+                        continue
+                    x = qd[n:n + 1, 2 * h:2 * h + 2].double().cpu().numpy()
+                    want, share, s, seen = ref.attention(x, keys[lo:hi], values[lo:hi], dim ** -0.5, 0)
+                    bound, eps_p = attention_bound(x, keys[lo:hi], values[lo:hi], dim ** -0.5, share, s, seen, dtype)
+                    assert np.all(np.abs(y - want[0]) <= bound[0] + np.abs(want[0]) * (2.0 ** -8 if dtype == "bf16" else 2 * EPS))
+                    t = np.arange(lo, hi)
+                    total[c.table[0, t // 32], h, t % 32] += share[0].sum(0)
+                    slack[c.table[0, t // 32], h, t % 32] += (share[0] * (eps_p[0][:, None] + (2 * len(place) + 4) * EPS)).sum(0) + total[c.table[0, t // 32], h, t % 32] * EPS
+            assert np.all(np.abs(w.cpu().numpy() - total) <= slack)
+    kept, left = nn.kv_cache_evict(c.cache, accounts, c.d_table, lengths, 300, 20)  # a length beyond the table ends with it
+    assert left.tolist() == [min(length, room), room] and kept[0, 0].tolist() == [t if t < min(length, room) else -1 for t in range(300)]
+
+
+@pytest.mark.parametrize("dim", (64, 128))
+def test_single_tokens_past_the_page_table(gpu, dim):
+    """Steps of one token each that go on past the table's end leave the cache alone, and attend to what there is."""
+    torch = gpu
+    c = Case(torch, [64, 40], 2, dim, 32, seed=dim).fill()
+    before = c.host().copy()
+    w = torch.ones(c.pages, 2, 32, device="cuda")
+    q = torch.randn(2, 4, dim, device="cuda")
+    want = c.nn.cached_attention(q, c.cache, c.d_table, c.ints([64, 40]))
+    for step in range(1, 4):
+        lengths = c.ints([64 + step, 40])
+        c.nn.kv_cache_append(c.cache, q[:, :2], q[:, 2:], c.d_table, lengths, weights=w)
+        c.lengths = [64, 40]
+        host = c.host()
+        for h in range(2):
+            for x, y in zip(ref.decode(before, c.table[0], 64, h), ref.decode(host, c.table[0], 64, h)):
+                assert np.array_equal(x, y)
+        assert torch.equal(c.nn.cached_attention(q, c.cache, c.d_table, lengths)[0], want[0])
+    gone = sorted(set(range(c.pages)) - set(c.table[1].tolist()))
+    assert np.array_equal(host[gone], before[gone]) and np.all(w.cpu().numpy()[gone] == 1)
+
+
 def test_cache_past_four_gigabytes(gpu):
     """Pages whose bytes lie beyond 2^32."""
     torch = gpu
