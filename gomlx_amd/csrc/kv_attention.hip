@@ -5,7 +5,7 @@
 //     account_j += sum of P_ij over the rows and the query heads of the key head (where asked for)
 //
 // Both products run on the fp16 matrix instructions (16x16x32 for few rows, 32x32x16 for many).  Keys and values are fp16 numbers as they stand (kv.hpp), q is scaled by a power
-// of two per row and taken as one fp16 number (bf16: exact) or as the sum of two (fp32: 22 bits), P likewise as one (bf16) or
+// of two per row (fp32: and by the scale's mantissa) and taken as one fp16 number (bf16: exact) or as the sum of two (fp32: 22 bits), P likewise as one (bf16) or
 // two; scores, running maximum, sums and results are fp32.
 //
 // The first product is formed transposed, S^T = K Q^T: a lane holds one query (its column) and eight neighbouring tokens of the
@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace gq {
 
@@ -32,6 +33,10 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kHeadroom = 6.0f;   // a row's largest weight is 2^6 when its reference is set ...
 constexpr float kMostLog2 = 14.0f;  // ... and stays under 2^14
+// With many rows a weight comes from a score's exact product with the scale, less a reference that is a rounded one: one instruction, and from references of
+// this size on an error of a 2^-8 th and more of a factor of 2 (at 2^27, of more than fp16 numbers have room for).  There the product is rounded as the reference was.
+// (bfloat16 alone: float32 queries take all of the scale but a power of two, by which products are exact.)
+constexpr float kCoarse = 65536.0f;
 
 __device__ __forceinline__ h2 as_h2(uint32_t u) { return __builtin_bit_cast(h2, u); }
 __device__ __forceinline__ h2 both(float v) { h2 r = {(_Float16)v, (_Float16)v}; return r; }
@@ -90,10 +95,10 @@ __device__ __forceinline__ Span row_tile_span(const KvSeq &s, int group, int win
 }
 
 // ROWS (16 or 32) query rows as operands of the matrix instructions of that size: lane (r, j), r = lane % ROWS, gets the values
-// 8 (64 / ROWS) g + 8 j + 0..7 of row r for g = 0, 1, ..., times 2^e with the largest of the row in [2^11, 2^12), and the sign of the scale, so that what is left to multiply scores by is not negative; `back` is 2^-e.
-// TWO: a second operand with what the first has rounded off.
+// 8 (64 / ROWS) g + 8 j + 0..7 of row r for g = 0, 1, ..., times 2^e with the largest of the row in [2^11, 2^12), and the sign of the scale, so that what is left to multiply scores by, to_log2, is
+// not negative.  TWO: a second operand with what the first has rounded off; both with the scale's mantissa (1/2 to 1; a rounding in 24 bits), so that to_log2 is a power of two.
 template <int D, int ROWS, bool BF16, bool TWO>
-__device__ __forceinline__ void load_queries(const HeadRows &q, int64_t at, bool live, int wide, float sign, h8 (&hi)[D * ROWS / 512], h8 (&lo)[TWO ? D * ROWS / 512 : 1], float &back) {
+__device__ __forceinline__ void load_queries(const HeadRows &q, int64_t at, bool live, int wide, float scale_log2, h8 (&hi)[D * ROWS / 512], h8 (&lo)[TWO ? D * ROWS / 512 : 1], float &to_log2) {
     constexpr int N = D * ROWS / 512;
     const int j = ((int)threadIdx.x & 63) / ROWS;
     float x[N][8];
@@ -133,13 +138,14 @@ __device__ __forceinline__ void load_queries(const HeadRows &q, int64_t at, bool
     int e = 0;
     if (most > 0.0f && most < __builtin_huge_valf()) e = 12 - __builtin_amdgcn_frexp_expf(most);
     e = e > 100 ? 100 : e;  // (below 2^-88 the scores of a row are nothing)
-    const float up = copysignf(ldexpf(1.0f, e), sign);
-    back = ldexpf(1.0f, -e);
+    const float up = TWO ? ldexpf(__builtin_amdgcn_frexp_mantf(scale_log2), e) : copysignf(ldexpf(1.0f, e), scale_log2);
+    to_log2 = TWO ? ldexpf(1.0f, __builtin_amdgcn_frexp_expf(scale_log2) - e) : ldexpf(1.0f, -e) * fabsf(scale_log2);
 #pragma unroll
     for (int g = 0; g < N; g++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float v = x[g][i] * up;
+            float v = x[g][i] * up;
+            if constexpr (TWO) asm("" : "+v"(v));  // (or the first operand may be made of the product before its rounding, and what is left of it after)
             const _Float16 a = (_Float16)v;
             hi[g][i] = a;
             if constexpr (TWO) lo[g][i] = (_Float16)(v - (float)a);
@@ -224,8 +230,13 @@ template <int BYTES, int STEP> struct TileWalk {
     const int32_t *table;
     int head, per_page, slot, in, left, page;
     __device__ __forceinline__ TileWalk(const KvCall &call, int b, int h, int tile, int end)
-        : kv(call), table(call.table + b * call.table_stride), head(h), per_page(call.page_tokens >> 5), left(tile < end ? (end - tile + STEP - 1) / STEP : 0), page(-1) {
-        slot = page_slot(call, tile);
+        : kv(call), table(call.table + b * call.table_stride), head(h), per_page(call.page_tokens >> 5) {
+        start(tile, end);
+    }
+    __device__ __forceinline__ void start(int tile, int end) {
+        left = tile < end ? (end - tile + STEP - 1) / STEP : 0;
+        page = -1;
+        slot = page_slot(kv, tile);
         in = tile - slot * per_page;
         if (left) page = uniform_load(table + slot);
     }
@@ -386,9 +397,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
     const uint8_t *mem = walk.next();
     if (mem) fetch_tile<D>(ring_at, mem);
     h8 qh[D / 32], ql[TWO ? D / 32 : 1];
-    float back;
-    load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
-    const float to_log2 = back * fabsf(a.scale_log2);
+    float to_log2;
+    load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, to_log2);
     int turn = 0;
     for (int tile = tile0 + wave; tile < last; tile += kSplitWaves) {
         const uint8_t *mem_next = walk.next();
@@ -732,8 +742,9 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     load(fetched[0]);
     load(fetched[1]);
     h8 qh[KS], ql[TWO ? KS : 1];
-    float back;
-    load_queries<D, 32, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
+    float to_log2;
+    load_queries<D, 32, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, to_log2);
+    to_log2 = fmaxf(to_log2, 0x1p-122f);  // (not 0, so that its product with -infinity stays that)
     if constexpr (D == 256) {  // (512 registers: the rows' operands in accumulation registers, beside the results)
 #pragma unroll
         for (int k = 0; k < KS; k++) {
@@ -741,7 +752,6 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
             if constexpr (TWO) asm("" : "+a"(ql[k]));
         }
     }
-    const float to_log2 = fmaxf(back * fabsf(a.scale_log2), 1e-37f);  // (not 0, so that its product with -infinity stays that)
     if (ACCOUNTS && piece == 0 && wave * 32 < span.rows) {
         const int64_t tile = (int64_t)h * a.operand_tiles + first_operand_tile(a, seq, b) + row_tile * kRowsWaves + wave;
         h8 *to = reinterpret_cast<h8 *>(a.operands) + tile * (TWO ? 2 : 1) * KS * 64 + lane;
@@ -754,15 +764,14 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     }
 
     f16 o[VS];
-#pragma unroll
-    for (int w = 0; w < VS; w++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[w][i] = 0.0f;
-    float ref = kNegInf, total = 0.0f;  // the row's reference, and the lane's share of its sum
+    float ref, total;     // the row's reference, and the lane's share of its sum
+    bool coarse = false;  // one of the wavefront's references has been large
 
     // One stage, from buffer `mine`; the next one, which has been on its way for a stage, goes into `other`.  (Making the next stage's scores in front of these weights, so that one wavefront has
     // both kinds of work to issue, was no faster: the second workgroup of the CU does as well.)
-    const auto attend_stage = [&](int tile, int mine) __attribute__((always_inline)) {
+    const auto attend_stage = [&](auto mode, int tile, int mine) __attribute__((always_inline)) {
+        constexpr bool COARSE = decltype(mode)::value;  // (the rows' scores may be large: they are multiplied first)
+        const float by = COARSE ? 1.0f : to_log2;
         f16 s[T];
 #pragma unroll
         for (int t = 0; t < T; t++) {
@@ -783,6 +792,12 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, TWO ? 8 : 4, 0);
+        if constexpr (COARSE) {
+#pragma unroll
+            for (int t = 0; t < T; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[t][i] *= to_log2;
+        }
         const int t0 = tile * 32;
         const uint32_t known = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t *>(there[mine])) & ALL;
         if (!(t0 >= all_lo && t0 + 32 * T <= all_hi && known == ALL)) {
@@ -799,12 +814,13 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
         for (int t = 0; t < T; t++)
 #pragma unroll
             for (int i = 0; i < 16; i++) most = fmaxf(most, s[t][i]);
-        if (__any(most * to_log2 > ref + kMostLog2)) {
-            most *= to_log2;
+        if (__any(most * by > ref + kMostLog2)) {
+            most *= by;
             most = fmaxf(most, __shfl_xor(most, 32));
             const float set = fmaxf(ref, most - kHeadroom);
             const float shrink = set == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - set);
             ref = set;
+            if constexpr (!TWO && !COARSE) coarse = coarse || __any(fabsf(ref) >= kCoarse && ref != kNegInf);
             total *= shrink;
             if constexpr (D == 256) {
                 scale_accumulators(o, shrink);
@@ -821,7 +837,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
                 h8 ph, pl;
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e], to_log2, less)), p1 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e + 1], to_log2, less));
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e], by, less)), p1 = __builtin_amdgcn_exp2f(fmaf(s[t][8 * k + e + 1], by, less));
                     ph[e] = (_Float16)p0;
                     ph[e + 1] = (_Float16)p1;
                     if constexpr (TWO) {
@@ -857,17 +873,36 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     };
     // (a wavefront without rows widens for the others; at D = 256 the branch would move accumulators about: 56 us become 65)
     const bool rows_here = D == 256 || wave * 32 < span.rows;
-    const auto step = [&](int tile, int mine, int other) __attribute__((always_inline)) {
+    const auto step = [&](auto mode, int tile, int mine, int other) __attribute__((always_inline)) {
         load(fetched[mine]);
-        if (rows_here) attend_stage(tile, mine);
+        if (rows_here) attend_stage(mode, tile, mine);
         if (tile + T < tile1) widen(fetched[other], other);
         __syncthreads();
     };
-    if (tile0 < tile1) widen(fetched[0], 0);
-    __syncthreads();
-    for (int tile = tile0; tile < tile1; tile += 2 * T) {
-        step(tile, 0, 1);
-        if (tile + T < tile1) step(tile + T, 1, 0);
+    const auto attend_all = [&](auto mode) __attribute__((always_inline)) {
+#pragma unroll
+        for (int w = 0; w < VS; w++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[w][i] = 0.0f;
+        ref = kNegInf;
+        total = 0.0f;
+        if (tile0 < tile1) widen(fetched[0], 0);
+        __syncthreads();
+        for (int tile = tile0; tile < tile1; tile += 2 * T) {
+            step(mode, tile, 0, 1);
+            if (tile + T < tile1) step(mode, tile + T, 1, 0);
+        }
+    };
+    attend_all(std::false_type{});
+    // Again from the start with scores that are large: what was summed is not theirs.  (A branch for them in the stage would cost all others: at D = 256, 1714
+    // rows of 2 sequences over themselves 81 us, with it 90.)
+    if constexpr (!TWO) {
+        if (__syncthreads_or(coarse)) {
+            walk.start(tile0 + tile_in, tile1);
+            load(fetched[0]);
+            load(fetched[1]);
+            attend_all(std::true_type{});
+        }
     }
     total += __shfl_xor(total, 32);
     if (!live) return;
@@ -974,15 +1009,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void kv_rows_
         int place;  // -1: no row
     };
     const auto load = [&](int n, Rows &rows) __attribute__((always_inline)) {
-        const h8 *q = reinterpret_cast<const h8 *>(a.operands) + (first + n) * N * 64 + lane;
-#pragma unroll
-        for (int k = 0; k < N; k++) rows.q[k] = q[k * 64];
         const int idx = n * 32 + r;
         const bool live = idx < seq.news * a.group;
         const int nth = live ? idx / a.group : 0, head = h * a.group + (live ? idx - nth * a.group : 0);
         rows.place = live ? base + nth : -1;
-        rows.scale = a.row_scales[(first + n) * 32 + r];
         rows.lse = a.lse[(int64_t)(seq.row0 + nth) * a.heads + head];
+        rows.scale = a.row_scales[(first + n) * 32 + r];
+        const h8 *q = reinterpret_cast<const h8 *>(a.operands) + (first + n) * N * 64 + lane;
+#pragma unroll
+        for (int k = 0; k < N; k++) rows.q[k] = q[k * 64];
     };
     Rows ring[AHEAD];
 #pragma unroll
@@ -1018,7 +1053,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void kv_rows_
         for (int p = 0; p < AHEAD; p++) {
             if (n + 4 * p >= to) break;
             Rows &now = ring[p];
-            const bool open = __all(now.place >= t0 + 32 * NT - 1 && (!a.window || now.place - a.window < t0));
+            const bool open = __all(now.place >= t0 + 32 * NT - 1 && (!a.window || now.place - a.window < t0) && (TWO || fabsf(now.lse) < kCoarse));
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 f16 s;
@@ -1036,7 +1071,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 2 : 3) void kv_rows_
                     const int behind = now.place - t0 - 32 * t - 4 * half;  // tokens of the tile's first for the lane to the row's own
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float w = __builtin_amdgcn_exp2f(fmaf(s[i], now.scale, -now.lse));
+                        const float w = __builtin_amdgcn_exp2f(s[i] * now.scale - now.lse);
                         sum[t][i] += (uint32_t)(behind - 8 * (i >> 2) - (i & 3)) < window ? w : 0.0f;
                     }
                 }
@@ -1092,11 +1127,10 @@ __global__ __launch_bounds__(256) void kv_account_kernel(const AttendArgs a) {
     const int place = seq.first + nth, see_hi = live ? place + 1 : 0, see_lo = a.window ? place + 1 - a.window : 0;
     const Unpack unpack;
     h8 qh[D / 32], ql[TWO ? D / 32 : 1];
-    float back, s[8];
-    load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, back);
+    float to_log2, s[8];
+    load_queries<D, 16, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, to_log2);
     const float lse = live ? a.lse[row * a.heads + head] : 0.0f;
     tile_scores<D, TWO>(unpack, k, qh, ql, s);
-    const float to_log2 = back * fabsf(a.scale_log2);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         const int t = t0 + 8 * j + e;

@@ -292,6 +292,32 @@ def test_scores_that_grow_along_the_sequence(gpu, dtype, dim, news):
 
 
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("dim", (64, 128, 256))
+@pytest.mark.parametrize("news", (1, 40))
+def test_scores_past_the_whole_numbers_of_float32(gpu, dtype, dim, news):
+    """Scores of 10^4 to 10^23, whose rounding in float32 is far more than the room of an exponent: the largest takes all the weight.  (Keys are
+    multiples of a vector of ones, so that scores are the exact products of few bits, rounded with the scale alone.)"""
+    torch = gpu
+    c = Case(torch, [300], 2, dim, 64, seed=dim)
+    c.k[0][:] = (1 + np.arange(300) % 7 / 8).astype(np.float32)[:, None, None]
+    c.k[0][33] = 2.0
+    c.fill()
+    q = torch.ones(news, 4, dim, device="cuda")
+    value = np.stack([ref.decode(c.host(), c.table[0], 300, h)[1][33] for h in (0, 0, 1, 1)])
+    weights = np.zeros((c.pages, 2, 64))
+    weights[c.table[0, 0], :, 33] = 2 * news
+    for scale in (100.0, 3e3, 1e5, 7.7e5, 3e6, 1.23e7, 1e8, 3.3e9, 1e12, 1.7e20, -1e8):
+        got = torch.zeros(c.pages, 2, 64, device="cuda")
+        sign = -1 if scale < 0 else 1
+        _, out = c.attend([news], 4, dtype, q=sign * q, scale=scale, accounts=got)
+        _, again = c.attend([news], 4, dtype, q=sign * q, scale=scale)
+        for y in (out, again):  # the weight's rounding as an operand (its sum may be of unrounded ones) and the output's
+            assert np.all(np.abs(y - value) <= np.abs(value) * (2.0 ** -8 + 2.0 ** -10 if dtype == "bf16" else 2.0 ** -20)), scale
+        # a weight of one: the sum's logarithm is rounded as the score is, and both are equal but for that
+        assert np.all(np.abs(got.cpu().numpy() - weights) <= weights * 2.0 ** -6), scale
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
 def test_tiny_keys_and_values_are_exact_operands(gpu, dtype):
     """Values whose scales are fp16 denormals: the matrix instructions must not flush them."""
     c = Case(gpu, [100], 1, 64, 32, seed=5)
