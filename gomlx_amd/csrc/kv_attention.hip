@@ -10,8 +10,9 @@
 //
 // The first product is formed transposed, S^T = K Q^T: a lane holds one query (its column) and eight neighbouring tokens of the
 // tile, so that maximum and sum are plain lane arithmetic and the weights are the second product's operand, O^T = V^T P^T,
-// where they lie.  The reference of a row's exponents is set so that its largest weight so far is 2^6, and moves only when a weight
-// would pass 2^14 (below fp16's largest number; small weights stay clear of its denormals): the lanes of the row then agree on a new one.
+// where they lie.  The reference of a row's exponents is set so that its largest weight so far is 2^6 (fp32: 2^12, 2^9 at D = 256), and moves only when
+// a weight would pass 2^14 (2^15.5; fp16's largest number is 2^16): the lanes of the row then agree on a new one.  fp16 numbers are 2^-24 apart at least, so that a
+// weight is rounded to 2^-31 (2^-37, 2^-34) of its row's largest where that is more than its 11 (22) bits: of 100000 weights that small together 5e-5 (7e-7, 6e-6) may be lost.
 #include "kv.hpp"
 #include "lds_dma.hpp"
 
@@ -31,8 +32,17 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kHeadroom = 6.0f;   // a row's largest weight is 2^6 when its reference is set ...
-constexpr float kMostLog2 = 14.0f;  // ... and stays under 2^14
+// A row's largest weight when its reference is set, and what it stays under, as powers of two.  (fp32: little room to spare, for the sake of the smallest weights; a
+// reference that moves more often costs 1 % up to D = 128.  At D = 256, where results have to leave the accumulation registers for it, 64 rows of 5 sequences over
+// 4000 to 16000 tokens take 105 108 112 123 us with 2^6 2^9 2^10 2^12.)
+template <int D, bool TWO> struct Weights { static constexpr float kSet = !TWO ? 6.0f : D == 256 ? 9.0f : 12.0f, kMost = TWO ? 15.5f : 14.0f; };
+// Whether a score asks for a new reference: by their difference, for a sum with the reference is rounded where scores are large.
+template <int D, bool TWO> __device__ __forceinline__ bool passes(float score, float ref) { return score - ref > Weights<D, TWO>::kMost; }
+// The reference that a row's largest score asks for.  (From scores of 2^26 on the difference can round to more than there is room for.)
+template <int D, bool TWO> __device__ __forceinline__ float reference(float most) {
+    const float set = most - Weights<D, TWO>::kSet;
+    return passes<D, TWO>(most, set) ? most : set;
+}
 // With many rows a weight comes from a score's exact product with the scale, less a reference that is a rounded one: one instruction, and from references of
 // this size on an error of a 2^-8 th and more of a factor of 2 (at 2^27, of more than fp16 numbers have room for).  There the product is rounded as the reference was.
 // (bfloat16 alone: float32 queries take all of the scale but a power of two, by which products are exact.)
@@ -434,10 +444,10 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 2 : BF16 ? 4 : 3) void
                 *reinterpret_cast<f4 *>(to) = f4{s[0], s[1], s[2], s[3]};
                 *reinterpret_cast<f4 *>(to + 4) = f4{s[4], s[5], s[6], s[7]};
             }
-            if (__any(most > ref + kMostLog2)) {  // (the first score of a row among them: its reference is -infinity)
+            if (__any(passes<D, TWO>(most, ref))) {  // (the first score of a row among them: its reference is -infinity)
                 most = fmaxf(most, __shfl_xor(most, 16));
                 most = fmaxf(most, __shfl_xor(most, 32));
-                const float next = fmaxf(ref, most - kHeadroom);
+                const float next = fmaxf(ref, reference<D, TWO>(most));
                 const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
                 ref = next;
                 total *= shrink;
@@ -814,10 +824,10 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
         for (int t = 0; t < T; t++)
 #pragma unroll
             for (int i = 0; i < 16; i++) most = fmaxf(most, s[t][i]);
-        if (__any(most * by > ref + kMostLog2)) {
+        if (__any(passes<D, TWO>(most * by, ref))) {
             most *= by;
             most = fmaxf(most, __shfl_xor(most, 32));
-            const float set = fmaxf(ref, most - kHeadroom);
+            const float set = fmaxf(ref, reference<D, TWO>(most));
             const float shrink = set == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref - set);
             ref = set;
             if constexpr (!TWO && !COARSE) coarse = coarse || __any(fabsf(ref) >= kCoarse && ref != kNegInf);

@@ -278,8 +278,9 @@ int gq_kv_append(const gq_kv_cache *kv, int dtype, const gq_head_rows *k, const 
 int gq_kv_read(const gq_kv_cache *kv, uint16_t *dK, uint16_t *dV, void *stream);
 /* Attention of the new tokens over their sequences, o = softmax(scale q . k) v: a token sees itself and the tokens in front of
  * it, with window > 0 the last `window` of them.  heads is a multiple of kv_heads; neighbouring query heads share a key head.
- * q and the output [rows, heads, head_dim] (16-byte aligned) are of one type, GQ_F32 (products in 22 bits and more) or GQ_BF16
- * (weights rounded to 11 bits); all sums in fp32.  A row that sees nothing gets zeros.  dAccounts (may be NULL): every token's
+ * q and the output [rows, heads, head_dim] (16-byte aligned) are of one type, GQ_F32 (queries in 22 bits of their row's largest, weights
+ * in 22 bits) or GQ_BF16 (weights in 11 bits); a weight is off by up to 2^-37 (head_dim 256: 2^-34; GQ_BF16:
+ * 2^-31) of its row's largest where that is more.  All sums in fp32.  A row that sees nothing gets zeros.  dAccounts (may be NULL): every token's
  * account grows by the weights that the call's rows gave it, summed over the query heads of a key head.  Sequences may share pages (a
  * common beginning, say), with dAccounts they must not.  May use a per-stream workspace, as the dense entry points: make one call outside a recording first. */
 int gq_kv_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int heads, float scale, int64_t window, float *dAccounts, void *dOut,

@@ -318,6 +318,32 @@ def test_scores_past_the_whole_numbers_of_float32(gpu, dtype, dim, news):
 
 
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("dim", (64, 128, 256))
+@pytest.mark.parametrize("news", (1, 9, 70, 4200))
+@pytest.mark.parametrize("accounts", (False, True))
+def test_one_large_weight_beside_many_small_ones(gpu, dtype, dim, news, accounts):
+    """60000 tokens, of which the first has 2^18 to 2^36 times the weight of every other: what these add up to is not lost.  The first one's value is 0 and
+    the others' 1, so that a result is the others' share.  A weight is off by 2^-31 (bfloat16) or 2^-37 (float32; 2^-34 at head_dim 256) of the row's largest at most, half
+    the spacing of the smallest operands, beside the relative errors: of sixty thousand additions in float32, of the exponent, of the output."""
+    torch = gpu
+    n = 60000
+    c = Case(torch, [n], 1, dim, 256, seed=news)
+    c.k[0][:], c.v[0][:] = 0.0, 1.0
+    c.k[0][0], c.v[0][0] = 1.0, 0.0
+    c.fill()
+    heads = 8 if news == 4200 else 2  # (4200 rows of 8 heads: every row goes over all the tokens in one piece)
+    q = torch.ones(news, heads, dim, device="cuda")
+    others = np.arange(n - news, n, dtype=np.float64)  # in front of a row's own token, and that one
+    for octaves in (18, 20, 21, 22, 23, 26, 29, 32, 34, 36):
+        w = torch.zeros(c.pages, 1, 256, device="cuda") if accounts else None
+        _, out = c.attend([news], heads, dtype, q=q, scale=octaves * np.log(2.0) / dim, accounts=w)
+        share = others * 2.0 ** -octaves
+        want = (share / (1 + share))[:, None, None]
+        bound = n * 2.0 ** (-31 if dtype == "bf16" else -34 if dim == 256 else -37) + want * (n * EPS + octaves * 2.0 ** -21 + (2.0 ** -8 + 2.0 ** -11 if dtype == "bf16" else 2.0 ** -21))
+        assert np.all(np.abs(out - want) <= bound), (octaves, np.abs(out - want).max(), bound.max())
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
 def test_tiny_keys_and_values_are_exact_operands(gpu, dtype):
     """Values whose scales are fp16 denormals: the matrix instructions must not flush them."""
     c = Case(gpu, [100], 1, 64, 32, seed=5)
