@@ -1304,7 +1304,6 @@ int gq_kv_append(const gq_kv_cache *kv, int dtype, const gq_head_rows *k, const 
     if (int rc = check_head_rows(fn, "v", v, dtype, call.rows, call.kv_heads)) return rc;
     if (!aligned_to(dAccounts, 4)) return fail(GQ_ERR_INVALID, "%s: accounts must be 4-byte aligned", fn);
     if (call.seqs == 0 || call.rows == 0 || call.max_new == 0 || call.max_pages == 0 || call.pages == 0) return GQ_OK;
-    if ((int64_t)call.seqs * call.kv_heads > kMaxGrid / ((call.max_new + 14) / 8)) return fail(GQ_ERR_INVALID, "%s: too many sequences, heads and new tokens", fn);
     if (int rc = use_device()) return rc;
     const bool bf16 = dtype == GQ_BF16;
     return launch_kv_append(call, HeadRows{k->dX, k->row_stride, k->head_stride, bf16}, HeadRows{v->dX, v->row_stride, v->head_stride, bf16}, dAccounts, (hipStream_t)stream);
@@ -1317,7 +1316,6 @@ int gq_kv_read(const gq_kv_cache *kv, uint16_t *dK, uint16_t *dV, void *stream) 
     if (call.seqs == 0 || call.rows == 0 || call.max_new == 0) return GQ_OK;
     if (!dK || !dV) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
     if (!aligned_to(dK, 16) || !aligned_to(dV, 16)) return fail(GQ_ERR_INVALID, "%s: outputs must be 16-byte aligned", fn);
-    if ((int64_t)call.seqs * call.kv_heads > kMaxGrid / ((call.max_new + 14) / 8)) return fail(GQ_ERR_INVALID, "%s: too many sequences, heads and new tokens", fn);
     if (int rc = use_device()) return rc;
     return launch_kv_read(call, dK, dV, (hipStream_t)stream);
 }

@@ -76,6 +76,11 @@ __device__ __forceinline__ KvSeq kv_seq(const KvCall &kv, int b) {
     return s;
 }
 
+__device__ __forceinline__ KvSeq seq_of_lane(const KvSeq &s, int lane) {
+    return KvSeq{__builtin_amdgcn_readlane(s.length, lane), __builtin_amdgcn_readlane(s.news, lane), __builtin_amdgcn_readlane(s.row0, lane),
+                 __builtin_amdgcn_readlane(s.first, lane)};
+}
+
 // the place in the page table of a sequence's tile
 __device__ __forceinline__ int page_slot(const KvCall &kv, int tile) {
     return kv.page_magic ? (int)__umulhi((uint32_t)tile, kv.page_magic) : tile / (kv.page_tokens >> 5);

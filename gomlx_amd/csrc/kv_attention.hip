@@ -262,11 +262,6 @@ template <int BYTES, int STEP> struct TileWalk {
     }
 };
 
-__device__ __forceinline__ KvSeq seq_of_lane(const KvSeq &s, int lane) {
-    return KvSeq{__builtin_amdgcn_readlane(s.length, lane), __builtin_amdgcn_readlane(s.news, lane), __builtin_amdgcn_readlane(s.row0, lane),
-                 __builtin_amdgcn_readlane(s.first, lane)};
-}
-
 // How the tiles of a call are shared out over its workgroups.  A unit is a sequence and key head (all rows of it: sixteen at most),
 // with the tiles that its rows see (one at least, so that rows that see nothing are written too).  Units are cut into pieces
 // of one length, of which all units together have about a.workgroups, one piece a workgroup: the lengths are known on the device only, so

@@ -68,6 +68,62 @@ __device__ __forceinline__ uint32_t code_of(float v, float d, float inv) {
     return (uint32_t)fminf(fmaxf(floorf(quotient + 8.5f), 0.0f), 15.0f);
 }
 
+// How the writer and the reader share out a call: a wavefront takes a block of eight tokens of a sequence and key head.  They are laid out for the longest of a call's
+// sequences, `blocks` a sequence; or, `together`, `blocks` a key head for all sequences, as many as the rows can need, which wavefronts look up by a sum over the
+// sequences, 64 at a time, one a lane.  That is taken where the first layout would be more than run at a time, and more than the second by what the sums cost.  (us a call of
+// the writer with either, 8 heads of D = 128, new tokens: 512 beside 31 single ones 8.4 6.1, beside 7 6.0 6.0; 8192 beside 255 365 19; 128 beside 255 14 7.9; 100
+// beside 2047 60 47; 32 beside 1023 22 27; 300 of 4 sequences 6.3 6.6.  The reader 4.8 4.5, 4.6 4.4, 295 12, 7.9 5.3, 39 32, 11 18, 4.7 4.9.)
+struct Layout { int blocks, together; };
+Layout layout_of(const KvCall &kv) {
+    // blocks that a sequence's rows touch at most, and all rows: one row one, up to nine two, ...
+    const int64_t each = (kv.max_new + 14) / 8, all = std::min<int64_t>(kv.rows, 2 * (int64_t)kv.seqs) + kv.rows / 8;
+    const bool together = kv.starts && kv.seqs * each * kv.kv_heads > 32 * device_cu_count() && kv.seqs * each > all * (256 + kv.seqs) / 256;
+    return Layout{(int)(together ? all : each), together};
+}
+// Threads of a launch are counted in 32 bits.
+int wavefronts_of(const char *fn, const KvCall &kv, const Layout &layout, unsigned *workgroups) {
+    const int64_t units = (int64_t)kv.kv_heads * layout.blocks * (layout.together ? 1 : kv.seqs);
+    if (units >= (int64_t)1 << 26) return fail(GQ_ERR_INVALID, "%s: %d rows of %d sequences and %d key heads: too many", fn, kv.rows, kv.seqs, kv.kv_heads);
+    *workgroups = (unsigned)((units + 3) / 4);
+    return GQ_OK;
+}
+
+struct Block { int b, h, nth; KvSeq s; };  // of the sequence's blocks; b < 0: there is none
+// COUNT(sequence): the blocks that its rows touch
+template <class COUNT> __device__ __forceinline__ Block block_of(const KvCall &kv, const Layout &layout, int unit, COUNT count) {
+    Block r;
+    if (!layout.together) {
+        const int per = kv.kv_heads * layout.blocks;
+        r.b = unit / per;
+        if (r.b >= kv.seqs) { r.b = -1; return r; }
+        const int rest = unit - r.b * per;
+        r.h = rest / layout.blocks;
+        r.nth = rest - r.h * layout.blocks;
+        r.s = kv_seq(kv, r.b);
+        if (r.nth >= count(r.s)) r.b = -1;
+        return r;
+    }
+    const int index = unit / kv.kv_heads, lane = (int)threadIdx.x & 63;
+    r.h = unit - index * kv.kv_heads;
+    r.b = -1;
+    int front = 0;
+    for (int base = 0; base < kv.seqs; base += 64) {
+        KvSeq mine{};
+        if (base + lane < kv.seqs) mine = kv_seq(kv, base + lane);
+        const int blocks = count(mine), upto = lane_scan(blocks);
+        const uint64_t past = __ballot(front + upto > index);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            r.b = base + l;
+            r.s = seq_of_lane(mine, l);
+            r.nth = index - (front + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(blocks, l));
+            break;
+        }
+        front += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return r;
+}
+
 // Eight tokens of one block (a lane's share of a value operand: their codes share dwords) per wavefront, key head and sequence.
 // A lane takes eight values of a token, D / 8 lanes a token, and D / 64 rounds the block: a lane's key codes are one dword.  Its
 // value codes are eight dwords that other lanes hold other tokens of; the lanes of equal values exchange halves until each has
@@ -79,7 +135,8 @@ struct AppendArgs {
     KvCall kv;
     HeadRows k, v;
     float *accounts;
-    int blocks, wide;  // blocks of eight tokens that the new ones of a sequence can touch
+    Layout layout;
+    int wide;
 };
 
 template <int D, bool BF16>
@@ -87,22 +144,25 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
     typedef KvTile<D> T;
     constexpr int G = T::G, L = D / 8, ROUNDS = D / 64, PER = 8 / ROUNDS;  // lanes of a token, rounds, tokens of a round
     const KvCall &kv = a.kv;
-    const int64_t unit = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    const int per = kv.kv_heads * a.blocks;
-    const int b = (int)(unit / per);
-    if (b >= kv.seqs) return;
-    const int rest = (int)(unit - (int64_t)b * per), h = rest / a.blocks, nth = rest - h * a.blocks;
+    const int unit = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
     const int lane = (int)threadIdx.x & 63, l = lane % L, x = l * 8, mine = lane / L;  // the lane's values; its token of a round
     const int g = x >> 5;
     float k[ROUNDS][8], v[ROUNDS][8];
     if (!kv.starts) {  // one row, which is known before the sequence's length is: whichever of the eight tokens it turns out to be
+        const int b = unit / kv.kv_heads, h = unit - b * kv.kv_heads;
+        if (b >= kv.seqs) return;
         load8<BF16>(k[0], a.k.p, (int64_t)b * a.k.row + h * a.k.head + x, a.wide);
         load8<BF16>(v[0], a.v.p, (int64_t)b * a.v.row + h * a.v.head + x, a.wide);
     }
-    const KvSeq s = kv_seq(kv, b);
-    const int first = s.first, from = first < 0 ? 0 : first, end = min(first + s.news, s.length);  // new tokens that have a place: from .. end - 1
-    if (nth * 8 >= end - (from & ~7) || from >= end) return;
-    const int p0 = (from & ~7) + nth * 8;
+    const Block block = block_of(kv, a.layout, unit, [](const KvSeq &s) {
+        const int from = max(s.first, 0), end = min(s.first + s.news, s.length);
+        return end > from ? ((end + 7) >> 3) - (from >> 3) : 0;
+    });
+    if (block.b < 0) return;
+    const KvSeq &s = block.s;
+    const int b = block.b, h = block.h;
+    const int first = s.first, from = max(first, 0), end = min(first + s.news, s.length);  // new tokens that have a place: from .. end - 1
+    const int p0 = (from & ~7) + block.nth * 8;
     uint8_t *tile = kv_tile(kv, b, h, p0 >> 5, T::kBytes);
     if (!tile) return;
     const int j = (p0 >> 3) & 3;
@@ -191,18 +251,17 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
 // What the cache stands for at the last tokens of every sequence, in the fp16 numbers that it holds; zeros in front of a
 // sequence's first token, behind the page table's end and where it names no page.  Bytes bound it: 7.3 us for the tokens of the 7 prompts above.
 template <int D>
-__global__ __launch_bounds__(256) void kv_read_kernel(const KvCall kv, uint16_t *__restrict__ K, uint16_t *__restrict__ V, int blocks) {
+__global__ __launch_bounds__(256) void kv_read_kernel(const KvCall kv, uint16_t *__restrict__ K, uint16_t *__restrict__ V, const Layout layout) {
     typedef KvTile<D> T;
     constexpr int NE = D / 64, G = T::G;
-    const int64_t unit = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    const int per = kv.kv_heads * blocks;
-    const int b = (int)(unit / per);
-    if (b >= kv.seqs) return;
-    const int rest = (int)(unit - (int64_t)b * per), h = rest / blocks, nth = rest - h * blocks;
-    const KvSeq s = kv_seq(kv, b);
+    // (blocks of eight also in front of the first token)
+    const Block block = block_of(kv, layout, __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6))),
+                                 [](const KvSeq &s) { return s.news ? ((s.first + s.news + 7) >> 3) - (s.first >> 3) : 0; });
+    if (block.b < 0) return;
+    const KvSeq &s = block.s;
+    const int b = block.b, h = block.h;
     const int first = s.first, end = first + s.news;
-    if (nth * 8 >= end - (first & ~7)) return;
-    const int p0 = (first & ~7) + nth * 8;  // (blocks of eight also in front of the first token)
+    const int p0 = (first & ~7) + block.nth * 8;
     const uint8_t *tile = p0 >= 0 && p0 < s.length ? kv_tile(kv, b, h, p0 >> 5, T::kBytes) : nullptr;
     const int lane = (int)threadIdx.x & 63, x = lane * NE, j = (p0 >> 3) & 3, g = x >> 5;
     uint32_t vw[NE] = {};
@@ -629,20 +688,22 @@ bool wide_rows(const HeadRows &h) {
 }
 
 template <int D> int append(const AppendArgs &a, bool bf16, hipStream_t s) {
-    const int64_t units = (int64_t)a.kv.seqs * a.kv.kv_heads * a.blocks;
-    const dim3 grid((unsigned)((units + 3) / 4)), block(256);
+    unsigned workgroups;
+    if (int rc = wavefronts_of("kv_append", a.kv, a.layout, &workgroups)) return rc;
+    const dim3 grid(workgroups), block(256);
     return bf16 ? launch(kv_append_kernel<D, true>, grid, block, 0, s, a) : launch(kv_append_kernel<D, false>, grid, block, 0, s, a);
 }
 template <int D> int read(const KvCall &kv, uint16_t *k, uint16_t *v, hipStream_t s) {
-    const int blocks = (kv.max_new + 14) / 8;
-    const int64_t units = (int64_t)kv.seqs * kv.kv_heads * blocks;
-    return launch(kv_read_kernel<D>, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, kv, k, v, blocks);
+    const Layout layout = layout_of(kv);
+    unsigned workgroups;
+    if (int rc = wavefronts_of("kv_read", kv, layout, &workgroups)) return rc;
+    return launch(kv_read_kernel<D>, dim3(workgroups), dim3(256), 0, s, kv, k, v, layout);
 }
 
 }  // namespace
 
 int launch_kv_append(const KvCall &kv, const HeadRows &k, const HeadRows &v, float *accounts, hipStream_t s) {
-    AppendArgs a{kv, k, v, accounts, (kv.max_new + 14) / 8, 0};
+    AppendArgs a{kv, k, v, accounts, layout_of(kv), 0};
     a.wide = wide_rows(k) && wide_rows(v);
     switch (kv.head_dim) {
     case 64: return append<64>(a, k.bf16, s);

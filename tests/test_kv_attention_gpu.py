@@ -219,6 +219,67 @@ def test_read_in_front_of_the_first_token_and_absent_pages(gpu):
         assert np.all(got[12:20] == 0) and np.array_equal(got[20:52], w1[i][:32]) and np.all(got[52:84] == 0) and np.array_equal(got[84:], w1[i][64:])
 
 
+@pytest.mark.parametrize("dim", (64, 128, 256))
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+def test_one_prompt_beside_many_sequences(gpu, dim, dtype):
+    """A call whose sequences differ widely in new tokens, none among them, some of more rows than tokens and some past their page table: every token lies where it belongs,
+    and is read back."""
+    torch = gpu
+    rng = np.random.default_rng(dim)
+    news = [int(n) for n in rng.integers(0, 3, 200)]
+    news[70], news[131], news[199] = 700, 33, 5
+    room = 768
+    lengths = [n + int(x) for n, x in zip(news, rng.integers(0, 60, 200))]
+    lengths[131], lengths[199], lengths[3] = 20, room + 2, 0
+    news[3] = 2
+    c = Case(torch, [min(n, room) for n in lengths], 2, dim, 96, seed=dim)
+    assert c.table.shape[1] * 96 == room
+    rows, starts = sum(news), np.concatenate([[0], np.cumsum(news)])
+    k, v = (torch.from_numpy(rng.standard_normal((rows, 2, dim)).astype(np.float32)).cuda().to({"f32": torch.float32, "bf16": torch.bfloat16}[dtype]) for _ in range(2))
+    accounts = torch.ones(c.pages, 2, 96, device="cuda")
+    how = dict(starts=c.ints(starts), max_new=700)
+    c.nn.kv_cache_append(c.cache, k, v, c.d_table, c.ints(lengths), weights=accounts, **how)
+    want = ref.quantise(k.float().cpu().numpy(), v.float().cpu().numpy())
+    got = [x.double().cpu().numpy() for x in c.nn.kv_cache_read(c.cache, c.d_table, c.ints(lengths), rows=rows, **how)]
+    host, left = c.host(), np.ones((c.pages, 2, 96), np.float32)
+    for b, n in enumerate(news):
+        place = np.arange(lengths[b] - n, lengths[b])
+        there = (place >= 0) & (place < room)
+        for h in range(2):
+            for i, x in enumerate(ref.decode(host, c.table[b], min(lengths[b], room), h)):
+                new = want[i][starts[b]:starts[b + 1], h]
+                assert np.array_equal(x[place[there]], new[there])
+                assert np.array_equal(got[i][starts[b]:starts[b + 1], h], np.where(there[:, None], new, 0))
+        left[c.table[b, place[there] // 96], :, place[there] % 96] = 0
+    assert np.array_equal(accounts.cpu().numpy(), left)
+
+
+def test_a_very_long_prompt_beside_many_single_tokens(gpu):
+    """131072 new tokens of one sequence and one of each of 511: more blocks of eight tokens a sequence, key head and sequences than a launch has threads for."""
+    torch = gpu
+    from gomlx_amd import nn
+    n, others, heads, dim, page = 131072, 511, 8, 64, 256
+    k, v = (torch.randn(n + others, heads, dim, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    table = torch.full((others + 1, n // page), -1, dtype=torch.int32, device="cuda")
+    table[200] = torch.arange(n // page, dtype=torch.int32, device="cuda")
+    rest = [b for b in range(others + 1) if b != 200]
+    table[rest, 0] = torch.arange(n // page, n // page + others, dtype=torch.int32, device="cuda")
+    lengths = torch.full((others + 1,), 9, dtype=torch.int32, device="cuda")
+    lengths[200] = n
+    starts = torch.tensor([b if b <= 200 else b + n - 1 for b in range(others + 2)], dtype=torch.int32, device="cuda")
+    caches = [nn.kv_cache(n // page + others, heads, dim, page) for _ in range(2)]
+    nn.kv_cache_append(caches[0], k, v, table, lengths, starts=starts, max_new=n)
+    nn.kv_cache_append(caches[1], k[200:200 + n], v[200:200 + n], table[200:201], lengths[200:201], starts=torch.tensor([0, n], dtype=torch.int32, device="cuda"), max_new=n)
+    single = [torch.cat([x[:200], x[200 + n:]]) for x in (k, v)]
+    nn.kv_cache_append(caches[1], *single, table[rest].contiguous(), lengths[rest].contiguous())
+    assert torch.equal(*caches)
+    got = nn.kv_cache_read(caches[0], table, lengths, starts=starts, max_new=n, rows=n + others)
+    want = nn.kv_cache_read(caches[0], table[200:201], lengths[200:201], starts=torch.tensor([0, n], dtype=torch.int32, device="cuda"), max_new=n, rows=n)
+    alone = nn.kv_cache_read(caches[0], table[rest].contiguous(), lengths[rest].contiguous())
+    for x, y, z in zip(got, want, alone):
+        assert torch.equal(x[200:200 + n], y) and torch.equal(torch.cat([x[:200], x[200 + n:]]), z)
+
+
 # ---- attention --------------------------------------------------------------------------------------------------------
 
 
