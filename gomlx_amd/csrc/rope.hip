@@ -12,6 +12,8 @@
 // HBM bounds it: 2048 rows of 32 + 8 heads of D = 128, float32 to bfloat16, 64 MB: 16.7 us a call, 3.8 TB/s; one row: 3.2 us, a launch and two loads.
 #include "common.hpp"
 
+#include <algorithm>
+
 namespace gq {
 
 namespace {
@@ -19,7 +21,7 @@ namespace {
 struct RopeArgs {
     HeadRows q, k;
     int q_heads, heads;  // heads: of queries and keys together
-    int64_t rows, table_rows;
+    int64_t rows, table_rows, first;  // first: workgroups of the call in front of the launch's
     const int32_t *positions;
     const float *cos, *sin;
     int rot;
@@ -53,7 +55,7 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 template <int D, bool BF16, bool OUT_BF16, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const RopeArgs a) {
     constexpr int L = D / 4;  // lanes of a head
-    const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
+    const int64_t unit = ((a.first + blockIdx.x) * 256 + threadIdx.x) / L;
     const int lane = (int)threadIdx.x & (L - 1);
     const int64_t row = unit / a.heads;
     if (row >= a.rows) return;  // (whole heads leave together: the exchanges below stay inside one head)
@@ -115,11 +117,16 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const RopeArgs a) {
     }
 }
 
-template <int D, bool BF16, bool OUT_BF16> int launch_rope(const RopeArgs &a, bool interleaved, hipStream_t s) {
+template <int D, bool BF16, bool OUT_BF16> int launch_rope(RopeArgs a, bool interleaved, hipStream_t s) {
     const int64_t per = 256 / (D / 4), blocks = (a.rows * a.heads + per - 1) / per;
-    const dim3 grid((unsigned)blocks), block(256);
-    return interleaved ? launch(qk_norm_rope_kernel<D, BF16, OUT_BF16, true>, grid, block, 0, s, a)
-                       : launch(qk_norm_rope_kernel<D, BF16, OUT_BF16, false>, grid, block, 0, s, a);
+    constexpr int64_t kMost = ((int64_t)1 << 24) - 1;  // (a launch has fewer than 2^32 threads: 2^26 heads of 256 values, 2^28 of 64)
+    for (a.first = 0; a.first < blocks; a.first += kMost) {
+        const dim3 grid((unsigned)std::min(blocks - a.first, kMost)), block(256);
+        if (int rc = interleaved ? launch(qk_norm_rope_kernel<D, BF16, OUT_BF16, true>, grid, block, 0, s, a)
+                                 : launch(qk_norm_rope_kernel<D, BF16, OUT_BF16, false>, grid, block, 0, s, a))
+            return rc;
+    }
+    return GQ_OK;
 }
 template <int D> int launch_rope(const RopeArgs &a, bool interleaved, bool bf16, bool out_bf16, hipStream_t s) {
     if (bf16) return out_bf16 ? launch_rope<D, true, true>(a, interleaved, s) : launch_rope<D, true, false>(a, interleaved, s);

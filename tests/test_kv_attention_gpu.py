@@ -787,6 +787,24 @@ def test_qk_norm_rope_without_a_table(gpu, dim, interleaved, kind):
         assert y.isnan().all(-1).all(-1).tolist() == [False, False, True, False, True] and y.isnan().any(-1).any(-1).tolist() == [False, False, True, False, True]
 
 
+def test_qk_norm_rope_of_more_heads_than_a_launch_has_threads_for(gpu):
+    """2^26 and some heads of 256 values, one head over and over (34 GB of results)."""
+    torch = gpu
+    from gomlx_amd import nn
+    rows, heads, dim = (1 << 20) + 3, 64, 256
+    one = torch.randn(1, heads, dim, device="cuda", dtype=torch.bfloat16)
+    cos, sin = nn.rotary_table(16, dim)
+    pos = (torch.arange(rows, device="cuda") % 16).int()
+    q, k = nn.qk_norm_rope(one.expand(rows, heads, dim), one[:, :0].expand(rows, 0, dim), pos, cos, sin)
+    want, _ = nn.qk_norm_rope(one.expand(1024, heads, dim), one[:, :0].expand(1024, 0, dim), pos[:1024].contiguous(), cos, sin)
+    assert k.shape == (rows, 0, dim)
+    for at in range(0, rows, 1024):
+        n = min(1024, rows - at)
+        assert torch.equal(q[at:at + n], want[:n]), at
+    del q
+    torch.cuda.empty_cache()
+
+
 # ---- together -----------------------------------------------------------------------------------------------------------
 
 
