@@ -1332,10 +1332,11 @@ int gq_kv_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int
     if (call.seqs == 0 || call.rows == 0 || call.max_new == 0) return GQ_OK;
     if (!dOut) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
     if (!aligned_to(dOut, 16) || !aligned_to(dAccounts, 4)) return fail(GQ_ERR_INVALID, "%s: the output must be 16-byte aligned, accounts 4-byte", fn);
-    // (grids are counted in 32 bits, threads included)
-    if (call.rows > (INT32_MAX >> 7) / heads || call.max_new > INT32_MAX / 2 / heads) return fail(GQ_ERR_INVALID, "%s: %d rows of %d heads: too many", fn, call.rows, heads);
+    // (threads of a launch are counted in 32 bits: fewer than 2^24 workgroups, of which a key head of a sequence has one and its rows one for every 128)
+    if (call.rows > INT32_MAX / 2 / heads || (int64_t)call.rows * heads / 128 + (int64_t)call.seqs * call.kv_heads > (1 << 24) - 4096)
+        return fail(GQ_ERR_INVALID, "%s: %d rows of %d heads, %d sequences of %d key heads: too many", fn, call.rows, heads, call.seqs, call.kv_heads);
     const int room = call.max_pages * call.page_tokens;
-    if ((int64_t)call.seqs * call.kv_heads > INT32_MAX / std::max(1, room / 32))
+    if ((int64_t)call.seqs * call.kv_heads > (INT32_MAX - 4096) / std::max(1, room / 32))
         return fail(GQ_ERR_INVALID, "%s: %d sequences of up to %d tokens and %d key heads: more than 2^31 tiles (pass the page table's first columns)", fn, call.seqs, room, call.kv_heads);
     if (int rc = use_device()) return rc;
     CallScope scope;

@@ -1170,8 +1170,11 @@ int64_t row_tiles_of(const AttendArgs &a) { return (int64_t)a.kv.rows * a.group 
 template <int D, bool BF16> int attend(const AttendArgs &a, int max_tiles, hipStream_t s) {
     const KvCall &kv = a.kv;
     const unsigned heads = (unsigned)kv.kv_heads, seqs = (unsigned)kv.seqs;
+    constexpr int NT = account_tiles<D, BF16>();
+    // (workgroups for the accounts are laid out by the page table's width; a launch has fewer than 2^24 of them)
+    if (a.accounts && ((a.row_pieces && (max_tiles + NT - 1) / NT >= 1 << 24) || (a.workgroups && !a.scores && (max_tiles + 3) / 4 >= 1 << 24)))
+        return fail(GQ_ERR_INVALID, "kv_attention: accounts of up to %d tiles of a sequence: too many (pass the page table's first columns)", max_tiles);
     if (a.row_pieces) {
-        constexpr int NT = account_tiles<D, BF16>();
         const unsigned grid = (unsigned)(row_tiles_of(a) * kv.kv_heads * a.row_pieces);
         if (int rc = launch(a.accounts ? kv_rows_kernel<D, BF16, true> : kv_rows_kernel<D, BF16, false>, dim3(grid), dim3(64 * kRowsWaves), 0, s, a)) return rc;
         if (a.row_pieces > 1)

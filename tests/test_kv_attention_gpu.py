@@ -573,6 +573,55 @@ def test_single_tokens_past_the_page_table(gpu, dim):
     assert np.array_equal(host[gone], before[gone]) and np.all(w.cpu().numpy()[gone] == 1)
 
 
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+def test_more_rows_than_a_launch_has_threads_for_one_by_one(gpu, dtype):
+    """131072 new tokens of 128 heads, 2^24 rows, in one call: every one of them over its window."""
+    torch = gpu
+    from gomlx_amd import nn
+    n, heads, dim, window = 131072, 128, 64, 64
+    kind = {"f32": torch.float32, "bf16": torch.bfloat16}[dtype]
+    gen = torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn(n, 1, dim, device="cuda", dtype=torch.bfloat16, generator=gen) for _ in range(2))
+    table = torch.arange(n // 256, dtype=torch.int32, device="cuda").view(1, -1)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = nn.kv_cache(n // 256, 1, dim, 256)
+    nn.kv_cache_append(cache, k, v, table, ints(n), starts=ints(0, n), max_new=n)
+    q = torch.randn(1, heads, dim, device="cuda", generator=gen).to(kind)
+    out = nn.cached_attention(q.expand(n, heads, dim), cache, table, ints(n), starts=ints(0, n), max_new=n, window=window)
+    keys, values = (x[:, 0].double().cpu().numpy() for x in nn.kv_cache_read(cache, table, ints(n), starts=ints(0, n), max_new=n, rows=n))
+    x = q.double().cpu().numpy()
+    for p in [0, 1, 62, 63, 64, 65, 4095, 65535, 65536, 99999, 131008, 131071] + list(range(500, n, 9973)):
+        lo = max(0, p + 1 - window)
+        want, share, scores, seen = ref.attention(x, keys[lo:p + 1], values[lo:p + 1], dim ** -0.5, 0)
+        bound, _ = attention_bound(x, keys[lo:p + 1], values[lo:p + 1], dim ** -0.5, share, scores, seen, dtype)
+        assert np.all(np.abs(out[p].double().cpu().numpy() - want[0]) <= bound[0] + np.abs(want[0]) * (2.0 ** -8 if dtype == "bf16" else 2 * EPS)), p
+
+
+@pytest.mark.parametrize("news", (1, 40))
+def test_a_page_table_wider_than_a_launch(gpu, news):
+    """A table with room for 2^29 tokens: attention goes by the tokens that there are; accounts, whose workgroups are laid out by its width, ask for a slice of it
+    where they are too many."""
+    torch = gpu
+    from gomlx_amd import _lib
+    c = Case(torch, [100], 2, 64, 64, seed=news).fill()
+    wide = torch.full((1, 1 << 23), -1, dtype=torch.int32, device="cuda")
+    wide[:, :c.table.shape[1]] = c.d_table
+    q = torch.randn(news, 4, 64, device="cuda")
+    how = dict(starts=c.ints([0, news]), max_new=news)
+    want, got = (c.nn.cached_attention(q, c.cache, t, c.ints([100]), **how).double() for t in (c.d_table, wide))
+    assert (got - want).abs().max() <= 2.0 ** -18 * want.abs().max()
+    weights = [torch.zeros(c.pages, 2, 64, device="cuda") for _ in range(2)]
+    c.nn.cached_attention(q, c.cache, c.d_table, c.ints([100]), weights=weights[0], **how)
+    if news == 1:  # (16 rows and fewer: four tiles a workgroup)
+        c.nn.cached_attention(q, c.cache, wide, c.ints([100]), weights=weights[1], **how)
+        assert (weights[0] - weights[1]).abs().max() <= 2.0 ** -18
+    else:
+        with pytest.raises(_lib.HipqError, match="first columns"):
+            c.nn.cached_attention(q, c.cache, wide, c.ints([100]), weights=weights[1], **how)
+        c.nn.cached_attention(q, c.cache, wide[:, :1 << 22], c.ints([100]), weights=weights[1], **how)
+        assert (weights[0] - weights[1]).abs().max() <= 2.0 ** -18 * news
+
+
 def test_cache_past_four_gigabytes(gpu):
     """Pages whose bytes lie beyond 2^32."""
     torch = gpu
