@@ -1159,7 +1159,8 @@ constexpr size_t kMostScoreBytes = (size_t)256 << 20;
 int split_workgroups(int D) { return std::min(kMostWorkgroups, device_cu_count() * (D == 256 ? 2 : D == 128 ? 3 : 4)); }
 
 // One call may hold prompts beside single tokens: where its sequences have on average, but for the longest, under half of the largest number of new tokens,
-// and the page table has room for this many tiles, those of few rows are taken by the kernel for them, in launches of their own.  (us a call with one kernel and with
+// and the page table has room for this many tiles, those of few rows are taken by the kernel for them, in launches of their own.  (With more than sixteen query heads a
+// key head even single tokens have too many rows for it.)  (us a call with one kernel and with
 // both, D = 128: 512 new tokens beside 31 single ones over 2000 to 8192, 8192 tiles: 185 75; 300 beside one over 131072: 585 59; 256 beside 31 over 1500, 1536
 // tiles: 46 36; beside 31 over 500, 512 tiles: 23 30; 512 beside 7 over 1000, 256 tiles: 36 42.)
 constexpr int64_t kMixedTiles = 1024;
@@ -1217,7 +1218,7 @@ int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float sc
     size_t row_lines = 0, split_lines = 0;  // of sums that are joined
     a.few = many ? 0 : kSplitRows;
     if (many) {
-        if (kv.starts && kv.seqs * tiles >= kMixedTiles && 2 * ((int64_t)kv.rows - kv.max_new) < (int64_t)(kv.seqs - 1) * kv.max_new) a.few = kSplitRows;
+        if (a.group <= kSplitRows && kv.starts && kv.seqs * tiles >= kMixedTiles && 2 * ((int64_t)kv.rows - kv.max_new) < (int64_t)(kv.seqs - 1) * kv.max_new) a.few = kSplitRows;
         // Pieces of a row tile's tokens: as many workgroups as run at a time (row tiles as if sequences had the same number of new tokens), each with enough
         // tokens for its start (us a call with 8, 12, 16, 32 tiles at least, D = 128: 512 tokens over 600 27 22 22 22, 64 of 4 sequences over 2000 31 29 30 36, 32 of
         // 2 over 8000 36 34 35 40; D = 64, 301 of 5 over 1111 in a window 43 43 48 49), and no more than pay for a launch and for the sums' way to memory and back: at

@@ -312,6 +312,25 @@ def test_prompts_beside_single_tokens(gpu, dtype, dim, heads, window):
 
 
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("heads", (17, 40))
+def test_prompts_beside_single_tokens_at_many_heads_a_key_head(gpu, dtype, heads):
+    """More than sixteen query heads a key head: single tokens are many rows as well, and no launch goes out for sequences of few."""
+    torch = gpu
+    import ctypes
+    from gomlx_amd import _lib
+    c = Case(torch, [900, 300, 40, 700] + [9] * 30, kv_heads=1, dim=64, page=64, seed=heads, wide_table=30).fill()
+    news = [1, 70, 0, 2] + [1] * 30
+    c.check(news, heads, dtype, with_accounts=True)
+    c.check(news, heads, dtype, window=33)
+    for accounts in (None, torch.zeros(c.pages, 1, 64, device="cuda")):
+        launches = ctypes.c_int()
+        _lib.check(_lib.lib().gq_profile_begin())
+        c.attend(news, heads, dtype, accounts=accounts)
+        _lib.check(_lib.lib().gq_profile_end(ctypes.byref(launches), None))
+        assert launches.value <= (2 if accounts is None else 3)
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
 @pytest.mark.parametrize("dim", (64, 128, 256))
 def test_accounts_where_scores_have_no_room(gpu, dtype, dim):
     """A page table of 15000 columns: the scores of the rows that it has room for would be more than 256 MB, so the accounts are made from the keys."""
