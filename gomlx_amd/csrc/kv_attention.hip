@@ -749,7 +749,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, D == 256 ? 1 : 2) void kv_rows_ker
     h8 qh[KS], ql[TWO ? KS : 1];
     float to_log2;
     load_queries<D, 32, BF16, TWO>(a.q, row * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, to_log2);
-    to_log2 = fmaxf(to_log2, 0x1p-122f);  // (not 0, so that its product with -infinity stays that)
+    to_log2 = to_log2 < 0x1p-122f ? 0x1p-122f : to_log2;  // (not 0, so that its product with -infinity stays that; a scale of NaN stays one)
     if constexpr (D == 256) {  // (512 registers: the rows' operands in accumulation registers, beside the results)
 #pragma unroll
         for (int k = 0; k < KS; k++) {

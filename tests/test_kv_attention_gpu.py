@@ -424,6 +424,16 @@ def test_one_large_weight_beside_many_small_ones(gpu, dtype, dim, news, accounts
 
 
 @pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("dim", (64, 128, 256))
+@pytest.mark.parametrize("news", (1, 40))
+def test_a_scale_of_nan(gpu, dtype, dim, news):
+    """Rows that see a token are NaN, whichever kernel they take."""
+    c = Case(gpu, [90], 2, dim, 64, seed=dim).fill()
+    _, out = c.attend([news], 4, dtype, scale=float("nan"))
+    assert np.isnan(out).all()
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
 def test_tiny_keys_and_values_are_exact_operands(gpu, dtype):
     """Values whose scales are fp16 denormals: the matrix instructions must not flush them."""
     c = Case(gpu, [100], 1, 64, 32, seed=5)
