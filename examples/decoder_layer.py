@@ -70,8 +70,9 @@ def main() -> None:
     p.add_argument("--budget", type=int, default=512)
     p.add_argument("--shape", type=int, nargs=4, default=(4096, 32, 8, 14336), metavar=("HIDDEN", "HEADS", "KV_HEADS", "FFN"))
     a = p.parse_args()
-    layer = Layer(*a.shape)
-    caches = Caches(layer, a.seqs, a.prompt + a.tokens + 2)
+    most = a.prompt + a.tokens + 2  # (two steps warm up)
+    layer = Layer(*a.shape, positions=most)
+    caches = Caches(layer, a.seqs, most)
     news = [max(1, a.prompt - 37 * b) for b in range(a.seqs)]
     starts = torch.tensor([0] + torch.tensor(news).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
     caches.lengths += torch.tensor(news, dtype=torch.int32, device="cuda")

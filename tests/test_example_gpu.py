@@ -83,3 +83,10 @@ def test_example_runs(gpu, monkeypatch, capsys):
     monkeypatch.setattr("sys.argv", ["decoder_layer.py", "--tokens", "6", "--seqs", "3", "--prompt", "100", "--budget", "64", "--shape", "512", "4", "2", "768"])
     ex.main()
     assert "us a step" in capsys.readouterr().out
+
+
+def test_example_runs_past_the_layers_usual_positions(gpu, monkeypatch, capsys):
+    ex = _example()
+    monkeypatch.setattr("sys.argv", ["decoder_layer.py", "--tokens", "3", "--seqs", "2", "--prompt", "4095", "--budget", "100", "--shape", "256", "4", "2", "512"])
+    ex.main()
+    assert "us a step" in capsys.readouterr().out
