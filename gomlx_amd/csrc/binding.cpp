@@ -374,7 +374,7 @@ struct Cache {
     }
 };
 
-// (past the dispatcher, which costs 0.4 us a tensor: norms and rotation of one row, whose call the host bounds, 5.4 -> 4.5 us)
+// (past the dispatcher, which costs 0.4 us a tensor: norms and rotation of one row, whose call the host bounds, 6.7 -> 5.5 us)
 at::Tensor fresh(const at::Tensor &like, at::IntArrayRef shape, at::ScalarType type) { return at::Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt)); }
 
 PyObject *pair(at::Tensor &&a, at::Tensor &&b) {

@@ -569,7 +569,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const AttendArgs a) {
 //
 // Matrix instructions, exponentials and the widening run side by side, two workgroups a CU (2048 rows of 32 heads over 2049 to 4096
 // tokens, D = 128).  With a causal bound workgroups differ in length: the second half of them goes from short to long, so that the two of a CU
-// add up to the same.  That call: 121 us in bfloat16, 850 TFLOP/s (a library product of 8192^3: 1193): a stage of 64 tokens
+// add up to the same.  That call: 121 us in bfloat16 (float32: 199), 850 TFLOP/s (a library product of 8192^3: 1193): a stage of 64 tokens
 // has 1024 cycles of matrix instructions a wavefront and 1270 of others, which overlap little, and takes 2600.
 constexpr int kRowsWaves = 4, kRowsTile = 32 * kRowsWaves, kRowsPiece = 12;  // rows of a workgroup; tiles of the cache, at least, in a piece of its tokens
 
@@ -662,8 +662,8 @@ __device__ __forceinline__ RowTile row_tile_of(const AttendArgs &a, int index) {
 __device__ __forceinline__ int first_operand_tile(const AttendArgs &a, const KvSeq &seq, int b) { return (int)((int64_t)seq.row0 * a.group / 32) + b; }
 
 // Results that live in accumulation registers, in which nothing but matrix instructions computes.  Written out, because the compiler would copy all of them to
-// ordinary registers and back in every stage for a multiplication that next to none of them needs.  (us a call, D = 256: 64 rows of 5 sequences over 4000 to
-// 16000 tokens in float32 320 260, 1714 rows of 2 over themselves in bfloat16 98 84.)  (The waits: it does not know what matrix instruction
+// ordinary registers and back in every stage for a multiplication that next to none of them needs.  (us a call, D = 256, 8 heads of 2 key heads: 64 rows
+// of 5 sequences over 4000 to 16000 tokens in float32 117 108, 1714 rows of 2 over themselves in bfloat16 95 82.)  (The waits: it does not know what matrix instruction
 // the reads are behind and the writes in front of.)
 template <int N> __device__ __forceinline__ void scale_accumulators(f16 (&v)[N], float by) {
     asm volatile("s_nop 15\n\ts_nop 15");
