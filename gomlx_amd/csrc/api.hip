@@ -1340,7 +1340,7 @@ int gq_kv_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int
         return fail(GQ_ERR_INVALID, "%s: %d sequences of up to %d tokens and %d key heads: more than 2^31 tiles (pass the page table's first columns)", fn, call.seqs, room, call.kv_heads);
     if (int rc = use_device()) return rc;
     CallScope scope;
-    return launch_kv_attention(call, HeadRows{q->dX, q->row_stride, q->head_stride, dtype == GQ_BF16}, heads, scale, window >= room ? 0 : (int)window, dAccounts, dOut,
+    return launch_kv_attention(call, HeadRows{q->dX, q->row_stride, q->head_stride, dtype == GQ_BF16}, heads, scale, (int)std::min<int64_t>(window, INT32_MAX), dAccounts, dOut,
                                (hipStream_t)stream);
 }
 

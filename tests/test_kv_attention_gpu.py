@@ -580,6 +580,35 @@ def test_tokens_without_a_place(gpu, dim, length, rows, max_new):
     assert left.tolist() == [min(length, room), room] and kept[0, 0].tolist() == [t if t < min(length, room) else -1 for t in range(300)]
 
 
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("rows", (1, 3, 40))
+def test_windows_of_sequences_past_the_page_table(gpu, dtype, rows):
+    """A window wider than the table still ends where it ends for rows whose places lie behind it; one wider than anything sees all there is."""
+    torch, room, heads, dim = gpu, 128, 4, 64
+    c, accounts, _, _, q = absent_case(torch, 300, rows, heads, room, dim, rows)
+    q = q.to({"f32": torch.float32, "bf16": torch.bfloat16}[dtype])
+    host, lengths, starts = c.host(), c.ints([300, room]), c.ints([0, rows, rows])
+    for window in (128, 200, 255, 290, 400, 2 ** 31 - 1, 2 ** 40):
+        w = torch.zeros_like(accounts)
+        out = c.nn.cached_attention(q, c.cache, c.d_table, lengths, starts=starts, max_new=rows, window=window, weights=w).double().cpu().numpy()
+        total = np.zeros(accounts.shape)
+        for h in range(2):
+            keys, values = ref.decode(host, c.table[0], room, h)
+            for n in range(rows):
+                lo = max(0, 300 - rows + n + 1 - window)
+                y = out[n, 2 * h:2 * h + 2]
+                if lo >= room:
+                    assert np.all(y == 0)
+                    continue
+                x = q[n:n + 1, 2 * h:2 * h + 2].double().cpu().numpy()
+                want, share, s, seen = ref.attention(x, keys[lo:], values[lo:], dim ** -0.5, 0)
+                bound, _ = attention_bound(x, keys[lo:], values[lo:], dim ** -0.5, share, s, seen, dtype)
+                assert np.all(np.abs(y - want[0]) <= bound[0] + np.abs(want[0]) * (2.0 ** -8 if dtype == "bf16" else 2 * EPS)), window
+                t = np.arange(lo, room)
+                total[c.table[0, t // 32], h, t % 32] += share[0].sum(0)
+        assert np.all(np.abs(w.cpu().numpy() - total) <= 1e-4 * total)
+
+
 @pytest.mark.parametrize("dim", (64, 128))
 def test_single_tokens_past_the_page_table(gpu, dim):
     """Steps of one token each that go on past the table's end leave the cache alone, and attend to what there is."""
