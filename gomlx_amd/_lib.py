@@ -61,6 +61,10 @@ SIGNATURES = [
     ("gq_kv_read", _int, [_vp, _vp, _vp, _vp]),
     ("gq_kv_attention", _int, [_vp, _int, _vp, _int, ctypes.c_float, _i64, _vp, _vp, _vp]),
     ("gq_kv_evict", _int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    ("gq_draft_tree", _int, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    ("gq_kv_tree_attention", _int, [_vp, _int, _vp, _int, ctypes.c_float, _i64, _vp, _i64, _vp, _vp]),
+    ("gq_sample", _int, [_int, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    ("gq_kv_accept", _int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp]),
     ("gq_graph_begin", _int, [_vp]),
     ("gq_graph_end", _int, [_vp, ctypes.POINTER(_vp)]),
     ("gq_graph_launch", _int, [_vp, _vp]),
@@ -94,6 +98,12 @@ class HeadRowsDesc(ctypes.Structure):
     _fields_ = [("dX", _vp), ("row_stride", _i64), ("head_stride", _i64)]
 
 
+class SamplingDesc(ctypes.Structure):
+    """gq_sampling of include/gomlx_hipq.h."""
+    _fields_ = [("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("top_k", _i64),
+                ("dTemperature", _vp), ("dTopP", _vp), ("dMinP", _vp), ("dTopK", _vp)]
+
+
 class HipqError(RuntimeError):
     """A hard failure reported by the library (anything but NOT_IMPLEMENTED)."""
 
@@ -115,7 +125,8 @@ _fast_tried = False
 # Entry points the native host path calls, in the order in which csrc/binding.cpp takes them.
 _BOUND = ("gq_qdense_check", "gq_qdense_f32", "gq_qdense_bf16", "gq_qdense_block_f32", "gq_qdense_block_bf16", "gq_qdense_gated_f32",
           "gq_qdense_gated_bf16", "gq_qdense_f32_batch", "gq_qdense_norm_f32_batch", "gq_qdense_norm_bf16_batch", "gq_dequantize",
-          "gq_embedding_lookup", "gq_bytes_per_block", "gq_values_per_block", "gq_qk_norm_rope", "gq_kv_append", "gq_kv_read", "gq_kv_attention", "gq_kv_evict")
+          "gq_embedding_lookup", "gq_bytes_per_block", "gq_values_per_block", "gq_qk_norm_rope", "gq_kv_append", "gq_kv_read", "gq_kv_attention", "gq_kv_evict",
+          "gq_draft_tree", "gq_kv_tree_attention", "gq_sample", "gq_kv_accept")
 
 
 def lib() -> ctypes.CDLL:

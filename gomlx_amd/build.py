@@ -26,7 +26,7 @@ WORKSPACE_TEST = os.path.join(HOST, "build", "workspace_test")
 
 # (the units that take longest to compile come first: they are the critical path of the parallel build)
 SOURCES = ["gemm_wreg.hip", "gemm.hip", "gemm_dma.hip", "mmv.hip", "mlp.hip", "gemv_ks.hip", "api.hip", "dequant.hip", "gemv.hip", "gemv_xs.hip", "mmq.hip",
-           "kv_attention.hip", "kv_cache.hip", "rope.hip"]
+           "kv_attention.hip", "kv_cache.hip", "rope.hip", "kv_tree.hip", "kv_draft.hip", "sample.hip"]
 
 # -packed-fp32-ops (note the minus): keep hipcc from forming v_pk_*_f32 instructions.
 # -ffp-contract=off: dequantisation must round every fp32 operation on its own; fused

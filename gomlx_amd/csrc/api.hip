@@ -1357,6 +1357,99 @@ int gq_kv_evict(const gq_kv_cache *kv, float *dAccounts, int64_t keep, int64_t r
     return launch_kv_evict(call, dAccounts, (int)keep, (int)recent, dKept, dNewLengths, (hipStream_t)stream);
 }
 
+namespace {
+// What a tree of drafted tokens has to fit: the nodes that a kernel holds of a sequence, and a bit for each of them.
+int check_nodes(const char *fn, int64_t nodes) {
+    return nodes <= kMostNodes ? GQ_OK : fail(GQ_ERR_NOT_IMPLEMENTED, "%s: up to %lld drafted tokens of a sequence: more than %d are not implemented", fn, (long long)nodes, kMostNodes);
+}
+int check_words(const char *fn, int64_t words, int64_t nodes) {
+    if (words < 1 || words > INT32_MAX / 32) return fail(GQ_ERR_INVALID, "%s: masks of %lld words", fn, (long long)words);
+    return words * 32 >= nodes ? GQ_OK : fail(GQ_ERR_INVALID, "%s: masks of %lld words have no bits for %lld rows of a sequence", fn, (long long)words, (long long)nodes);
+}
+struct Int32Range { const int32_t *p; int64_t n; };
+bool overlap(const Int32Range &a, const Int32Range &b) { return a.p && b.p && a.n > 0 && b.n > 0 && a.p < b.p + b.n && b.p < a.p + a.n; }
+}  // namespace
+
+int gq_draft_tree(const int32_t *dParents, const int32_t *dFirst, const int32_t *dStarts, int64_t seqs, int64_t rows, int64_t max_new, int32_t *dTree,
+                  int64_t words, int32_t *dPositions, void *stream) {
+    const char *fn = "gq_draft_tree";
+    if (seqs < 0 || rows < 0 || max_new < 0 || rows > INT32_MAX || max_new > INT32_MAX) return fail(GQ_ERR_INVALID, "%s: %lld sequences, rows=%lld, max_new=%lld", fn, (long long)seqs, (long long)rows, (long long)max_new);
+    if (seqs > (1 << 24) - 1) return fail(GQ_ERR_INVALID, "%s: %lld sequences: too many", fn, (long long)seqs);
+    if (!dStarts && (rows != seqs || max_new < 1))
+        return fail(GQ_ERR_INVALID, "%s: without dStarts every sequence has one row (%lld rows, %lld sequences, max_new %lld)", fn, (long long)rows, (long long)seqs, (long long)max_new);
+    const int64_t most = dStarts ? std::min(max_new, rows) : 1;
+    if (int rc = check_nodes(fn, most)) return rc;
+    if (int rc = check_words(fn, words, most)) return rc;
+    if (seqs == 0 || rows == 0 || most == 0) return GQ_OK;
+    if (!dParents || !dFirst || !dTree || !dPositions) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
+    if (!aligned_to(dParents, 4) || !aligned_to(dFirst, 4) || !aligned_to(dStarts, 4) || !aligned_to(dTree, 4) || !aligned_to(dPositions, 4)) return fail(GQ_ERR_INVALID, "%s: arrays must be 4-byte aligned", fn);
+    if (int rc = use_device()) return rc;
+    return launch_draft_tree(TreeCall{dParents, dFirst, dStarts, (int)seqs, (int)rows, (int)most}, dTree, (int)words, dPositions, (hipStream_t)stream);
+}
+
+int gq_kv_tree_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int heads, float scale, int64_t window, const int32_t *dTree, int64_t words,
+                         void *dOut, void *stream) {
+    const char *fn = "gq_kv_tree_attention";
+    KvCall call;
+    if (int rc = check_kv(fn, kv, true, &call)) return rc;
+    if (int rc = check_float_type(fn, dtype)) return rc;
+    if (heads <= 0 || heads % call.kv_heads) return fail(GQ_ERR_INVALID, "%s: %d query heads are not a multiple of %d key heads", fn, heads, call.kv_heads);
+    if (window < 0) return fail(GQ_ERR_INVALID, "%s: negative window", fn);
+    if (int rc = check_head_rows(fn, "q", q, dtype, call.rows, heads)) return rc;
+    if (int rc = check_words(fn, words, call.max_new)) return rc;
+    if (call.seqs == 0 || call.rows == 0 || call.max_new == 0) return GQ_OK;
+    if (!dOut || !dTree) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
+    if (!aligned_to(dOut, 16) || !aligned_to(dTree, 4)) return fail(GQ_ERR_INVALID, "%s: the output must be 16-byte aligned, masks 4-byte", fn);
+    if (call.rows > INT32_MAX / 2 / heads) return fail(GQ_ERR_INVALID, "%s: %d rows of %d heads: too many", fn, call.rows, heads);
+    const int span = (int)std::min<int64_t>(window, INT32_MAX);
+    if (int rc = check_kv_tree_attention(fn, call, heads, span)) return rc;
+    if (int rc = use_device()) return rc;
+    CallScope scope;
+    return launch_kv_tree_attention(call, HeadRows{q->dX, q->row_stride, q->head_stride, dtype == GQ_BF16}, heads, scale, span, dTree, (int)words,
+                                    dOut, (hipStream_t)stream);
+}
+
+int gq_sample(int dtype, const void *dLogits, int64_t rows, int64_t vocab, int64_t row_stride, const float *dUniform, const gq_sampling *how, int32_t *dTokens,
+              float *dProbabilities, void *stream) {
+    const char *fn = "gq_sample";
+    if (int rc = check_float_type(fn, dtype)) return rc;
+    if (rows < 0 || vocab < 1 || row_stride < 0) return fail(GQ_ERR_INVALID, "%s: %lld rows of %lld logits, %lld apart", fn, (long long)rows, (long long)vocab, (long long)row_stride);
+    if (!how) return fail(GQ_ERR_INVALID, "%s: null settings", fn);
+    if (rows == 0) return GQ_OK;
+    if (!dLogits || !dUniform || !dTokens) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
+    if (!aligned_to(dLogits, dtype == GQ_BF16 ? 2 : 4)) return fail(GQ_ERR_INVALID, "%s: logits are not aligned to their elements", fn);
+    for (const void *p : {(const void *)dUniform, (const void *)dTokens, (const void *)dProbabilities, (const void *)how->dTemperature, (const void *)how->dTopP, (const void *)how->dMinP, (const void *)how->dTopK})
+        if (!aligned_to(p, 4)) return fail(GQ_ERR_INVALID, "%s: arrays must be 4-byte aligned", fn);
+    if (int rc = use_device()) return rc;
+    CallScope scope;
+    const Sampling s{how->temperature, how->top_p, how->min_p, (int)std::max<int64_t>(0, std::min<int64_t>(how->top_k, INT32_MAX)), how->dTemperature, how->dTopP, how->dMinP, how->dTopK};
+    return launch_sample(dLogits, dtype == GQ_BF16, rows, vocab, row_stride, dUniform, s, dTokens, dProbabilities, (hipStream_t)stream);
+}
+
+int gq_kv_accept(const gq_kv_cache *kv, const int32_t *dParents, const int32_t *dTokens, const int32_t *dSampled, float *dAccounts, int32_t *dPath,
+                 int64_t path_columns, int32_t *dNext, int32_t *dNewLengths, void *stream) {
+    const char *fn = "gq_kv_accept";
+    KvCall call;
+    if (int rc = check_kv(fn, kv, true, &call)) return rc;
+    if (int rc = check_nodes(fn, call.max_new)) return rc;
+    if (path_columns < call.max_new || path_columns > INT32_MAX) return fail(GQ_ERR_INVALID, "%s: %lld columns for paths of up to %d rows", fn, (long long)path_columns, call.max_new);
+    if (call.seqs == 0) return GQ_OK;
+    if ((call.rows > 0 && (!dParents || !dTokens || !dSampled)) || (path_columns > 0 && !dPath) || !dNext || !dNewLengths) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
+    const Int32Range in[] = {{dParents, call.rows}, {dTokens, call.rows}, {dSampled, call.rows}, {call.lengths, call.seqs}, {call.starts, (int64_t)call.seqs + 1},
+                             {call.table, call.max_pages ? (call.seqs - 1) * call.table_stride + call.max_pages : 0}};
+    const Int32Range out[] = {{dPath, call.seqs * path_columns}, {dNext, call.seqs}, {dNewLengths, call.seqs}};
+    for (const Int32Range &o : out) {
+        if (!aligned_to(o.p, 4)) return fail(GQ_ERR_INVALID, "%s: arrays must be 4-byte aligned", fn);
+        for (const Int32Range &i : in)
+            if (overlap(o, i)) return fail(GQ_ERR_INVALID, "%s: an output overlaps an input", fn);
+    }
+    for (const Int32Range &i : in)
+        if (!aligned_to(i.p, 4)) return fail(GQ_ERR_INVALID, "%s: arrays must be 4-byte aligned", fn);
+    if (!aligned_to(dAccounts, 4)) return fail(GQ_ERR_INVALID, "%s: accounts must be 4-byte aligned", fn);
+    if (int rc = use_device()) return rc;
+    return launch_kv_accept(call, dParents, dTokens, dSampled, dAccounts, dPath, (int)path_columns, dNext, dNewLengths, (hipStream_t)stream);
+}
+
 int gq_graph_begin(void *stream) {
     if (!stream) return fail(GQ_ERR_INVALID, "gq_graph_begin: recording needs an explicit stream");
     if (profile_state().active) return fail(GQ_ERR_INVALID, "gq_graph_begin: kernel timing is active on this thread");

@@ -18,6 +18,7 @@
 #include <climits>
 #include <cmath>
 #include <initializer_list>
+#include <limits>
 
 #include "../../include/gomlx_hipq.h"
 
@@ -43,8 +44,12 @@ struct Entry {
     decltype(&gq_kv_read) kv_read;
     decltype(&gq_kv_attention) kv_attention;
     decltype(&gq_kv_evict) kv_evict;
+    decltype(&gq_draft_tree) draft_tree;
+    decltype(&gq_kv_tree_attention) tree_attention;
+    decltype(&gq_sample) sample;
+    decltype(&gq_kv_accept) kv_accept;
 } g;
-constexpr int kEntries = 19;
+constexpr int kEntries = 23;
 bool g_bound = false;
 PyTypeObject *g_activation = nullptr;  // nn.Activation
 PyObject *s_scheme, *s_ggml_type, *s_gain, *s_epsilon, *s_scale_offset;
@@ -490,6 +495,123 @@ PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
+// ---- decoding with drafted tokens ------------------------------------------------------------------------------------------
+
+// draft_tree(parents, first, starts, max_new)
+PyObject *draft_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        int64_t most;
+        if (n != 4 || !THPVariable_CheckExact(a[0]) || !THPVariable_CheckExact(a[1]) || !to_i64(a[3], most) || most < 1 || most > INT_MAX) return none();
+        const at::Tensor &up = THPVariable_Unpack(a[0]), &fi = THPVariable_Unpack(a[1]);
+        if (!up.is_cuda() || up.dim() != 1 || fi.dim() != 1 || up.size(0) < 1 || fi.size(0) < 1) return none();
+        const int64_t rows = up.size(0), seqs = fi.size(0), words = (most + 31) / 32;
+        const c10::DeviceIndex device = up.get_device();
+        const int32_t *pp = int32_vector(a[0], rows, device), *fp = int32_vector(a[1], seqs, device), *sp = nullptr;
+        if (!pp || !fp || (a[2] == Py_None ? rows != seqs || most != 1 : !(sp = int32_vector(a[2], seqs + 1, device)))) return none();
+        at::Tensor tree = fresh(up, {rows, words}, at::kInt), positions = fresh(up, {rows}, at::kInt);
+        int32_t *tp = tree.mutable_data_ptr<int32_t>(), *op = positions.mutable_data_ptr<int32_t>();
+        void *s = stream_of(up);
+        const int rc = without_gil([&] { return g.draft_tree(pp, fp, sp, seqs, rows, most, tp, words, op, s); });
+        return rc == GQ_OK ? pair(std::move(tree), std::move(positions)) : none();
+    });
+}
+
+// tree_attention(q, cache, page_table, lengths, tree, starts, max_new, scale | None, window)
+PyObject *tree_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        HeadRows q;
+        Cache c;
+        int64_t window;
+        if (n != 9 || !q.read(a[0]) || !c.read(a[1], a[2], a[3], a[5], a[6], q.t->size(0), Py_None) || !to_i64(a[8], window)) return none();
+        if (q.t->size(2) != c.d.head_dim || q.t->size(1) < 1 || q.t->size(1) % c.d.kv_heads || q.t->size(1) > INT_MAX || q.t->get_device() != c.t->get_device()) return none();
+        const at::Tensor *t = gpu_tensor(a[4]);
+        if (!t || t->scalar_type() != at::kInt || t->dim() != 2 || t->size(0) != c.d.rows || t->size(1) < 1 || t->get_device() != c.t->get_device()) return none();
+        double scale;
+        if (a[7] == Py_None) scale = 1.0 / std::sqrt((double)c.d.head_dim);
+        else if (PyFloat_Check(a[7])) scale = PyFloat_AS_DOUBLE(a[7]);
+        else return none();
+        at::Tensor out = fresh(*q.t, q.t->sizes(), q.t->scalar_type());
+        const int32_t *tp = t->const_data_ptr<int32_t>();
+        void *op = out.mutable_data_ptr(), *s = stream_of(*c.t);
+        const int rc = without_gil([&] {
+            return g.tree_attention(&c.d, element_type(q.t->scalar_type()), &q.d, (int)q.t->size(1), (float)scale, window, tp, t->size(1), op, s);
+        });
+        return rc == GQ_OK ? THPVariable_Wrap(std::move(out)) : none();
+    });
+}
+
+// One setting of `sample`: a number in its range, or a vector with one for each row.
+template <class T> bool setting(PyObject *o, at::ScalarType type, int64_t rows, c10::DeviceIndex device, double most, double &value, const T *&vector) {
+    if (PyFloat_Check(o)) value = PyFloat_AS_DOUBLE(o);
+    else if (PyLong_Check(o)) {
+        int64_t v;
+        if (!to_i64(o, v)) return false;
+        value = (double)v;
+    } else {
+        const at::Tensor *t = gpu_tensor(o);
+        if (!t || t->scalar_type() != type || t->dim() != 1 || t->size(0) != rows || t->get_device() != device) return false;
+        vector = t->const_data_ptr<T>();
+        return true;
+    }
+    return value >= 0.0 && value <= most;
+}
+
+// sample(logits, uniform, temperature, top_k, top_p, min_p, probabilities)
+PyObject *sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        if (n != 7 || !THPVariable_CheckExact(a[0]) || !PyBool_Check(a[6])) return none();
+        const at::Tensor &x = THPVariable_Unpack(a[0]);
+        if (!x.is_cuda() || x.layout() != at::kStrided || x.dim() != 2 || x.size(0) < 1 || x.size(1) < 1 || element_type(x.scalar_type()) < 0 || (x.size(1) > 1 && x.stride(1) != 1)) return none();
+        const int64_t rows = x.size(0);
+        const c10::DeviceIndex device = x.get_device();
+        const at::Tensor *u = gpu_tensor(a[1]);
+        if (!u || u->scalar_type() != at::kFloat || u->dim() != 1 || u->size(0) != rows || u->get_device() != device) return none();
+        gq_sampling d{};
+        double k = 0.0;
+        const double any = std::numeric_limits<double>::infinity();
+        if (PyFloat_Check(a[3]) || !setting(a[2], at::kFloat, rows, device, any, d.temperature, d.dTemperature) || !setting(a[3], at::kInt, rows, device, 2147483647.0, k, d.dTopK) ||
+            !setting(a[4], at::kFloat, rows, device, 1.0, d.top_p, d.dTopP) || !setting(a[5], at::kFloat, rows, device, 1.0, d.min_p, d.dMinP))
+            return none();
+        d.top_k = (int64_t)k;
+        at::Tensor tokens = fresh(x, {rows}, at::kInt), shares;
+        int32_t *tp = tokens.mutable_data_ptr<int32_t>();
+        float *sp = nullptr;
+        if (a[6] == Py_True) {
+            shares = fresh(x, {rows}, at::kFloat);
+            sp = shares.mutable_data_ptr<float>();
+        }
+        const void *xp = x.const_data_ptr();
+        const float *up = u->const_data_ptr<float>();
+        void *s = stream_of(x);
+        const int rc = without_gil([&] { return g.sample(element_type(x.scalar_type()), xp, rows, x.size(1), x.stride(0), up, &d, tp, sp, s); });
+        if (rc != GQ_OK) return none();
+        return sp ? pair(std::move(tokens), std::move(shares)) : THPVariable_Wrap(std::move(tokens));
+    });
+}
+
+// kv_accept(cache, page_table, lengths, parents, tokens, sampled, starts, max_new, weights)
+PyObject *kv_accept(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Cache c;
+        if (n != 9 || !THPVariable_CheckExact(a[3]) || THPVariable_Unpack(a[3]).dim() != 1 || !c.read(a[0], a[1], a[2], a[6], a[7], THPVariable_Unpack(a[3]).size(0), a[8])) return none();
+        const c10::DeviceIndex device = c.t->get_device();
+        const int32_t *in[3];
+        for (int i = 0; i < 3; i++)
+            if (!(in[i] = int32_vector(a[3 + i], c.d.rows, device))) return none();
+        at::Tensor path = fresh(*c.t, {c.d.seqs, c.d.max_new}, at::kInt), token = fresh(*c.t, {c.d.seqs}, at::kInt), left = fresh(*c.t, {c.d.seqs}, at::kInt);
+        int32_t *pp = path.mutable_data_ptr<int32_t>(), *tp = token.mutable_data_ptr<int32_t>(), *lp = left.mutable_data_ptr<int32_t>();
+        void *s = stream_of(*c.t);
+        const int rc = without_gil([&] { return g.kv_accept(&c.d, in[0], in[1], in[2], c.accounts, pp, c.d.max_new, tp, lp, s); });
+        if (rc != GQ_OK) return none();
+        PyObject *out = PyTuple_New(3);
+        if (!out) return nullptr;
+        PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(path)));
+        PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(token)));
+        PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(left)));
+        return out;
+    });
+}
+
 // bind(Activation, address, ...): the enumeration of nn.py, the entry points in the order of Entry
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != kEntries + 1 || !PyType_Check(a[0])) { PyErr_Format(PyExc_TypeError, "bind takes a type and %d addresses", kEntries); return nullptr; }
@@ -522,6 +644,10 @@ PyMethodDef methods[] = {
     {"kv_read", (PyCFunction)(void (*)(void))kv_read, METH_FASTCALL, nullptr},
     {"cached_attention", (PyCFunction)(void (*)(void))cached_attention, METH_FASTCALL, nullptr},
     {"kv_evict", (PyCFunction)(void (*)(void))kv_evict, METH_FASTCALL, nullptr},
+    {"draft_tree", (PyCFunction)(void (*)(void))draft_tree, METH_FASTCALL, nullptr},
+    {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL, nullptr},
+    {"sample", (PyCFunction)(void (*)(void))sample, METH_FASTCALL, nullptr},
+    {"kv_accept", (PyCFunction)(void (*)(void))kv_accept, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -166,6 +166,34 @@ int launch_kv_append(const KvCall &kv, const HeadRows &k, const HeadRows &v, flo
 int launch_kv_read(const KvCall &kv, uint16_t *k, uint16_t *v, hipStream_t s);
 int launch_kv_attention(const KvCall &kv, const HeadRows &q, int heads, float scale, int window, float *accounts, void *out, hipStream_t s);
 int launch_kv_evict(const KvCall &kv, float *accounts, int keep, int recent, int32_t *kept, int32_t *new_lengths, hipStream_t s);
+// Trees of drafted tokens: the nodes of a sequence are its rows, of which a kernel holds so many at most.
+constexpr int kMostNodes = 1024;
+struct TreeCall {
+    const int32_t *parents, *first, *starts;  // starts null: row b is sequence b's one node
+    int seqs, rows, max_new;
+    // the rows of sequence b; those beyond the call's, and behind the first max_new of a sequence, are left out
+    __device__ __forceinline__ void rows_of(int b, int &row0, int &news) const {
+        int from = b, to = b + 1;
+        if (starts) { from = starts[b]; to = starts[b + 1]; }
+        row0 = from < 0 ? 0 : from > rows ? rows : from;
+        to = to < row0 ? row0 : to > rows ? rows : to;
+        news = to - row0 > max_new ? max_new : to - row0;
+    }
+};
+int launch_draft_tree(const TreeCall &c, int32_t *tree, int words, int32_t *positions, hipStream_t s);
+int check_kv_tree_attention(const char *fn, const KvCall &kv, int heads, int window);  // (sizes that a launch takes; no sequences and no rows are none)
+int launch_kv_tree_attention(const KvCall &kv, const HeadRows &q, int heads, float scale, int window, const int32_t *tree, int words, void *out, hipStream_t s);
+int launch_kv_accept(const KvCall &kv, const int32_t *parents, const int32_t *tokens, const int32_t *sampled, float *accounts, int32_t *path, int path_columns, int32_t *next,
+                     int32_t *new_lengths, hipStream_t s);
+// A token for every row of logits (sample.hip).  Settings: where a pointer is not null it has one for each row.
+struct Sampling {
+    double temperature, top_p, min_p;
+    int top_k;
+    const float *temperatures, *top_ps, *min_ps;
+    const int32_t *top_ks;
+};
+int launch_sample(const void *logits, bool bf16, int64_t rows, int64_t vocab, int64_t row_stride, const float *uniform, const Sampling &how, int32_t *tokens,
+                  float *probabilities, hipStream_t s);
 
 int launch_gemm(int type, bool x_is_bf16, const void *x, int64_t M, int64_t K, const uint8_t *W, int64_t N,
                 const float *bias, int act, float *y, hipStream_t s);

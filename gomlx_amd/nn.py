@@ -17,6 +17,7 @@ returns None for whatever it does not take, and the Python steps below then run 
 from __future__ import annotations
 
 import enum
+import math
 from dataclasses import dataclass
 
 import torch
@@ -551,3 +552,146 @@ def kv_cache_evict(cache: torch.Tensor, weights: torch.Tensor, page_table: torch
     new_lengths = torch.empty_like(lengths)
     _lib.check(_lib.lib().gq_kv_evict(ctypes.byref(d), weights.data_ptr(), keep, recent, kept.data_ptr(), new_lengths.data_ptr(), _stream_ptr(cache)))
     return kept, new_lengths
+
+
+# ---- decoding with drafted tokens: a tree of them goes through the model at once, and the path that the model's own samples follow is kept
+
+
+def _tree_rows(parents, starts, max_new: int, first):
+    """(sequences, rows) of a call on trees, and the checks that need no look at the device."""
+    if parents.dim() != 1 or first.dim() != 1:
+        raise ValueError("parents must be an int32 [rows], first an int32 [sequences] tensor")
+    rows, seqs = parents.shape[0], first.shape[0]
+    _int32("parents", parents, (rows,))
+    _int32("first", first, (seqs,))
+    if starts is not None:
+        _int32("starts", starts, (seqs + 1,))
+    elif rows != seqs or max_new != 1:
+        raise ValueError(f"without starts every sequence has one row: got {rows} rows of {seqs} sequences, max_new {max_new}")
+    if max_new < 1:
+        raise ValueError(f"max_new must be at least 1, got {max_new}")
+    for name, t in (("first", first), ("starts", starts)):
+        if t is not None and t.device != parents.device:
+            raise ValueError(f"{name} is on {t.device}, parents on {parents.device}")
+    return seqs, rows
+
+
+def draft_tree(parents: torch.Tensor, first: torch.Tensor, starts: torch.Tensor | None = None, max_new: int = 1) -> tuple:
+    """What the nodes of every sequence's tree of drafted tokens see, and where they stand: (tree, positions).
+
+    Rows ``starts[b]`` to ``starts[b + 1]`` (at most ``max_new``, 1024 of them at most; without ``starts`` one row a sequence) are the nodes of sequence b, as in the calls on a
+    cache.  The first is the root: the token that the last step sampled, at position ``first[b]`` (int32 [sequences]).  ``parents``, int32 [rows]: the parent of
+    each, counted from the sequence's first row and in front of its child; anything else is none, -1 for the root's.  ``tree``, int32 [rows, max_new / 32 rounded up], has
+    bit j % 32 of word j / 32 set where a row sees the sequence's row j, itself and its ancestors: what ``tree_attention`` takes.  ``positions``, int32 [rows]: for
+    ``qk_norm_rope``.  Rows that belong to no sequence hold anything."""
+    if _lib.fast is not None and (out := _lib.fast.draft_tree(parents, first, starts, max_new)) is not None:
+        return out
+    seqs, rows = _tree_rows(parents, starts, max_new, first)
+    words = -(-max_new // 32)
+    _init(parents.device.index or 0)
+    tree = torch.empty((rows, words), dtype=torch.int32, device=parents.device)
+    positions = torch.empty(rows, dtype=torch.int32, device=parents.device)
+    _lib.check(_lib.lib().gq_draft_tree(parents.data_ptr(), first.data_ptr(), None if starts is None else starts.data_ptr(), seqs, rows, max_new, tree.data_ptr(), words,
+                                        positions.data_ptr(), _stream_ptr(parents)))
+    return tree, positions
+
+
+def tree_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, tree: torch.Tensor, starts: torch.Tensor | None = None,
+                   max_new: int = 1, scale: float | None = None, window: int = 0) -> torch.Tensor:
+    """``cached_attention`` of drafted tokens (which the cache already holds, in the order of their rows): each sees the tokens in front of its sequence's new
+    ones, and of these the ones whose bits are set in its row of ``tree``, int32 [rows, words] (``draft_tree``; any other masks will do, bits from the sequence's
+    number of rows on are not looked at).  With a ``window`` it sees the last that many of all these.  A row that sees nothing gets zeros.  No accounts are kept:
+    which of the tokens stay is known only after ``kv_cache_accept``."""
+    if _lib.fast is not None and (out := _lib.fast.tree_attention(q, cache, page_table, lengths, tree, starts, max_new, scale, window)) is not None:
+        return out
+    import ctypes
+    xd = _float_type("tree_attention", q)
+    d = _kv_desc(cache, page_table, lengths, starts, max_new, q.shape[0] if q.dim() else None)
+    dq = _head_rows("q", q, dim=d.head_dim)
+    heads = q.shape[1]
+    if heads < 1 or heads % d.kv_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {d.kv_heads} key heads")
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    _require_cuda("tree", tree)
+    if tree.dtype != torch.int32 or tree.dim() != 2 or tree.shape[0] != d.rows or 32 * tree.shape[1] < min(max_new, d.rows) or tree.shape[1] < 1:
+        raise ValueError(f"tree must be an int32 [{d.rows}, a bit for each of up to {max_new} rows of a sequence] tensor, got {tree.dtype} {tuple(tree.shape)}")
+    if q.device != cache.device or tree.device != cache.device:
+        raise ValueError("q, tree and the cache must be on one device")
+    _init(cache.device.index or 0)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _lib.check(_lib.lib().gq_kv_tree_attention(ctypes.byref(d), xd, ctypes.byref(dq), heads, d.head_dim ** -0.5 if scale is None else scale, window, tree.data_ptr(),
+                                               tree.shape[1], out.data_ptr(), _stream_ptr(cache)))
+    return out
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, probabilities: bool = False):
+    """A token for every row of logits [rows, vocabulary] (float32 or bfloat16, strided rows allowed) from a given number of [0, 1) for each, ``uniform`` (float32 [rows]).
+
+    With weights exp((x - max x) / temperature) and tokens in order of their logits, equal ones by index, stay: the first ``top_k``; of these the shortest
+    beginning that weighs at least ``top_p`` of them, one token at least; of these those that weigh ``min_p`` of the largest and more.  The token is the lowest index up
+    to which what stays weighs more than ``uniform`` of it all.  A temperature of 0 asks for the first in order; ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0 are no bounds.  Each
+    of the four is one number, or a tensor with one for each row (float32, ``top_k`` int32; values outside their range count as the nearest in it, NaN as no bound, a temperature of NaN as 0).
+    A NaN logit counts as minus infinity; a row without a number above that gets token -1.  Weights and sums are formed in 64 bits: the same arguments give the same token.
+
+    Returns int32 [rows]; with ``probabilities`` also float32 [rows], what share of the weight that stays the token has."""
+    if _lib.fast is not None and (out := _lib.fast.sample(logits, uniform, temperature, top_k, top_p, min_p, probabilities)) is not None:
+        return out
+    import ctypes
+    xd = _float_type("sample", logits)
+    if not logits.is_cuda:
+        raise ValueError("logits must be a GPU tensor: this backend has no CPU path")
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"logits must be [rows, vocabulary] with the values of a row side by side, got {tuple(logits.shape)}")
+    rows = logits.shape[0]
+    _require_cuda("uniform", uniform)
+    if uniform.dtype != torch.float32 or tuple(uniform.shape) != (rows,):
+        raise ValueError(f"uniform must be a float32 [{rows}] tensor, got {uniform.dtype} {tuple(uniform.shape)}")
+    d = _lib.SamplingDesc(1.0, 1.0, 0.0, 0)
+    for name, field, value, least, most in (("temperature", "dTemperature", temperature, 0.0, math.inf), ("top_k", "dTopK", top_k, 0, math.inf),
+                                            ("top_p", "dTopP", top_p, 0.0, 1.0), ("min_p", "dMinP", min_p, 0.0, 1.0)):
+        if isinstance(value, torch.Tensor):
+            dtype = torch.int32 if name == "top_k" else torch.float32
+            _require_cuda(name, value)
+            if value.dtype != dtype or tuple(value.shape) != (rows,) or value.device != logits.device:
+                raise ValueError(f"{name} must be a number or a {dtype} [{rows}] tensor on {logits.device}, got {value.dtype} {tuple(value.shape)} on {value.device}")
+            setattr(d, field, value.data_ptr())
+        elif not least <= value <= most:
+            raise ValueError(f"{name} must be between {least} and {most}, got {value}")
+        else:
+            setattr(d, name, min(int(value), 2 ** 31 - 1) if name == "top_k" else float(value))
+    if uniform.device != logits.device:
+        raise ValueError("uniform and logits must be on one device")
+    _init(logits.device.index or 0)
+    tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    shares = torch.empty(rows, dtype=torch.float32, device=logits.device) if probabilities else None
+    _lib.check(_lib.lib().gq_sample(xd, logits.data_ptr(), rows, logits.shape[1], logits.stride(0), uniform.data_ptr(), ctypes.byref(d), tokens.data_ptr(),
+                                    None if shares is None else shares.data_ptr(), _stream_ptr(logits)))
+    return (tokens, shares) if probabilities else tokens
+
+
+def kv_cache_accept(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, sampled: torch.Tensor,
+                    starts: torch.Tensor | None = None, max_new: int = 1, weights: torch.Tensor | None = None) -> tuple:
+    """Keeps of every sequence's drafted tokens, its last ones in the cache, the path that the model's samples follow, and drops the others.
+
+    ``parents``: as in ``draft_tree``.  ``tokens``, int32 [rows]: the drafted tokens (the root's is not looked at); ``sampled``, int32 [rows]: what the model samples behind
+    each of them (``sample`` of its logits).  From the root on the path goes to the first child whose token is the sample of the path's end, until there is none.  Its keys
+    and values move behind one another, with their accounts where ``weights`` is given.  Returns (path, token, lengths): int32 [sequences, max_new], the path's
+    rows counted from the sequence's first, -1 behind the last; int32 [sequences], the sample at its end, the next step's root (-1 for a sequence without rows); and the new lengths (``lengths`` itself is
+    left as it is).  Each layer has a call of its own for its cache, all with the same answer.  Sequences must not share the pages of their drafted tokens."""
+    if _lib.fast is not None and (out := _lib.fast.kv_accept(cache, page_table, lengths, parents, tokens, sampled, starts, max_new, weights)) is not None:
+        return out
+    import ctypes
+    if parents.dim() != 1:
+        raise ValueError("parents must be an int32 [rows] tensor")
+    d = _kv_desc(cache, page_table, lengths, starts, max_new, parents.shape[0], weights)
+    for name, t in (("parents", parents), ("tokens", tokens), ("sampled", sampled)):
+        _int32(name, t, (d.rows,))
+        if t.device != cache.device:
+            raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+    _init(cache.device.index or 0)
+    path = torch.empty((d.seqs, max_new), dtype=torch.int32, device=cache.device)
+    token, new_lengths = torch.empty_like(lengths), torch.empty_like(lengths)
+    _lib.check(_lib.lib().gq_kv_accept(ctypes.byref(d), parents.data_ptr(), tokens.data_ptr(), sampled.data_ptr(), None if weights is None else weights.data_ptr(),
+                                       path.data_ptr(), max_new, token.data_ptr(), new_lengths.data_ptr(), _stream_ptr(cache)))
+    return path, token, new_lengths

@@ -291,6 +291,47 @@ int gq_kv_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int
  * dNewLengths[seqs] (may be dLengths itself): min(length, keep).  A length beyond the page table is taken as one that ends with it.  dStarts, rows and max_new are not used.  Sequences must not share pages. */
 int gq_kv_evict(const gq_kv_cache *kv, float *dAccounts, int64_t keep, int64_t recent, int32_t *dKept, int32_t *dNewLengths, void *stream);
 
+/* ---- Decoding with drafted tokens: a step takes a tree of them for every sequence through the model at once and keeps the path that the model's own
+ * samples follow, so that it gives the same tokens as decoding one by one, several a step.  (The reference decodes token by token.)
+ *
+ * The drafted tokens of a sequence are the new ones of the calls above: rows dStarts[b] to dStarts[b + 1], appended to the cache in the order of the rows.
+ * Its first row is the tree's root, the token that the last step sampled.  dParents[row]: the parent of each, counted from the sequence's first row, in front
+ * of its child; anything else is none (the root's, and that of a row which then sees only the context and itself and is never accepted).  At most 1024 a sequence
+ * (gq_kv_tree_attention: any number).
+ *
+ * gq_draft_tree: dTree[rows, words], bit j % 32 of word j / 32 set where the row sees the sequence's row j, itself and its ancestors (words at
+ * least max_new / 32), and dPositions = dFirst[b], the position of the root, plus the number of ancestors.  Rows of no sequence are left as they are. */
+int gq_draft_tree(const int32_t *dParents, const int32_t *dFirst, const int32_t *dStarts, int64_t seqs, int64_t rows, int64_t max_new, int32_t *dTree,
+                  int64_t words, int32_t *dPositions, void *stream);
+/* gq_kv_attention of rows that see, instead of all new tokens up to their own, those whose bits are set in dTree[rows, words] (any masks; bits from the sequence's
+ * number of rows on are not looked at), and the tokens in front of the new ones; with window > 0 the last `window` of all these.  No accounts: which rows
+ * will stay is not known yet.  May use a per-stream workspace: make one call outside a recording first. */
+int gq_kv_tree_attention(const gq_kv_cache *kv, int dtype, const gq_head_rows *q, int heads, float scale, int64_t window, const int32_t *dTree, int64_t words,
+                         void *dOut, void *stream);
+/* A token for every row of logits (GQ_F32 or GQ_BF16, rows row_stride elements apart) and a number u of [0, 1) for each, dUniform[rows].  With weights
+ * exp((x - max x) / temperature) and the tokens in order of their logits, equal ones by index, stay: the first top_k; of these the shortest beginning that weighs at
+ * least top_p of them, one token at least; of these those of weight min_p and more.  The token is the lowest index up to which what stays weighs more than u of it all.
+ * temperature <= 0 (or NaN): the first in order.  top_k <= 0, top_p >= 1, min_p <= 0 (NaN among them): no bound; top_p <= 0: the first in order; min_p > 1 counts as 1.  Weights
+ * and sums are formed in 64 bits and do not depend on any order of execution.  A NaN counts as minus infinity; a row without a number above it gets token -1 and probability 0.  Where a
+ * pointer is not NULL every row has a setting of its own.  dProbabilities (may be NULL): what share of the weight that stays the token has.  At most 2^21 - 7 tokens.
+ * Uses a per-stream workspace: make one call outside a recording first. */
+typedef struct {
+    double temperature, top_p, min_p;
+    int64_t top_k;
+    const float *dTemperature, *dTopP, *dMinP;  /* [rows] or NULL */
+    const int32_t *dTopK;                       /* [rows] or NULL */
+} gq_sampling;
+int gq_sample(int dtype, const void *dLogits, int64_t rows, int64_t vocab, int64_t row_stride, const float *dUniform, const gq_sampling *how, int32_t *dTokens,
+              float *dProbabilities, void *stream);
+/* The end of a step.  dTokens[rows]: the drafted tokens (the root's is not looked at); dSampled[rows]: what the model samples behind each of them.  From the root on
+ * the path goes to the first child whose token is the sample of the path's end, until there is none (a negative sample has none).  dPath[seqs, path_columns]: its rows, counted
+ * from the sequence's first, -1 behind the last (path_columns at least the rows of a sequence); dNext[seqs]: the sample at its end, the next step's root (-1 for a sequence
+ * without rows).  The path's keys and values move behind one another in the cache, with their accounts (dAccounts may be NULL), to where the sequence's new
+ * rows begin; dNewLengths[seqs]: the tokens up to its end.  A call per layer's cache, all with the same answer.  No output may overlap an input (dNewLengths is not
+ * dLengths).  Sequences must not share the pages of their new tokens. */
+int gq_kv_accept(const gq_kv_cache *kv, const int32_t *dParents, const int32_t *dTokens, const int32_t *dSampled, float *dAccounts, int32_t *dPath,
+                 int64_t path_columns, int32_t *dNext, int32_t *dNewLengths, void *stream);
+
 /* ---- Executable.Execute of a compiled graph (core/graph/graph.go:669): a sequence of
  * launches recorded once and replayed with one submission (HIP graph).  Between begin
  * and end, entry points called with this stream are recorded, not run.  A graph replays on
