@@ -12,9 +12,10 @@
 // Weights are formed in 64 bits: next to a border, of which a vocabulary has as many as tokens, 32 would give another token once in some hundred rows.  Where order must
 // not matter (histograms, sums that several threads add to) they are whole numbers of 2^-42 of the largest.  The same arguments always give the same token.
 //
-// Two launches.  The first reads the logits once: a wavefront a chunk, which leaves its maximum, its sum and its largest keys (32 at least, some 45, complete from
+// The first launch reads the logits once: a wavefront a chunk, which leaves its maximum, its sum and its largest keys (32 at least, some 45, complete from
 // a level on).  In the second a workgroup a row finds the cut among the keys that the chunks have left, and reads a single chunk again.  Where the cut lies
-// below what they have left (a flat distribution under top-p) it goes over the row again, three times or more.
+// below what they have left (a flat distribution under top-p) the row is gone over twice more, by all its chunks at a time in launches that find nothing to do otherwise; where the
+// call's settings make that unlikely these launches are left out, and the second one does it by itself.
 #include "common.hpp"
 
 #include <algorithm>
@@ -27,7 +28,8 @@ namespace {
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kChunk = 2048, kChunkKeys = 128, kMostChunks = 1024;
-constexpr int kPickThreads = 512, kPickWaves = kPickThreads / 64, kBins = 2048, kListMost = 6144;
+constexpr int kPickThreads = 512, kPickWaves = kPickThreads / 64, kBins = 2048, kListBins = 512, kListMost = 6144, kFew = 64;
+constexpr int kWideRows = 128;  // flat rows that the launches for them have room for; the others are gone over in the second launch
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -39,6 +41,19 @@ struct Chunk {
     int count;
 };
 
+// A flat row on its way through the launches for it: the weights of its tokens by bins of 1/32 in powers of two, the keys of the bin with the cut in it, what the chunks weigh above it.
+struct Wide {
+    int64_t row;
+    float most;
+    uint32_t floor_key;
+    uint32_t listed;
+    uint64_t weights[kBins];
+    uint32_t counts[kBins];
+    uint64_t chunk_weight[kMostChunks];
+    uint32_t keys[kListMost];
+    uint16_t chunks[kListMost];
+};
+
 struct SampleArgs {
     const uint8_t *logits;
     int64_t row_bytes;
@@ -47,6 +62,9 @@ struct SampleArgs {
     const float *uniform;
     Chunk *chunk;      // [rows, chunks]
     uint32_t *keys;    // [rows, chunks, kChunkKeys]
+    Wide *wide;        // [wide_rows]; null: there are no launches for them
+    uint32_t *wides;   // how many there are (or would be)
+    int wide_rows;
     int32_t *tokens;
     float *probabilities;  // may be null
 };
@@ -56,6 +74,7 @@ struct Settings {
     int k;                 // 0: all
     bool first;            // the first of the order
     __device__ __forceinline__ bool cuts() const { return k || top_p < 1.0 || min_p > 0.0; }
+    __device__ __forceinline__ bool orders() const { return k || top_p < 1.0; }
 };
 __device__ __forceinline__ Settings settings_of(const SampleArgs &a, int64_t row) {
     Settings s;
@@ -72,36 +91,37 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs &a, int64_t row
 }
 
 // Logits in order as whole numbers; a NaN counts as minus infinity, -0 as 0.
-__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : kNegInf; }
+__device__ __forceinline__ float clean(float x) { return x == x ? x : kNegInf; }
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t u = __float_as_uint(x);
+    const uint32_t u = __float_as_uint(x + 0.0f);
     return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
-// 2^y for y <= 0, to 1e-11 of itself: the series of exp(f ln 2) for |f| <= 1/2 up to its ninth power.
+// 2^y for -1010 <= y <= 0, to 1e-12 of itself: the nearest whole number to the exponent, for the rest, at most 1/2 either way, 1 + c1 f + ... + c8 f^8 that is nearest
+// to 2^f there (a weighted least-squares fit, to 8.2e-13).
 __device__ __forceinline__ double power_of_two(double y) {
-    y = fmax(y, -1100.0);  // (a NaN too: 0)
-    const double n = __builtin_rint(y), f = y - n;
-    double p = 1.01780860092396997e-7;   // ln(2)^k / k!, k = 9, 8, ...
-    p = fma(p, f, 1.32154867901443095e-6);
-    p = fma(p, f, 1.52527338040598403e-5);
-    p = fma(p, f, 1.54035303933816099e-4);
-    p = fma(p, f, 1.33335581464284434e-3);
-    p = fma(p, f, 9.61812910762847716e-3);
-    p = fma(p, f, 5.55041086648215800e-2);
-    p = fma(p, f, 2.40226506959100712e-1);
-    p = fma(p, f, 6.93147180559945309e-1);
+    const double whole = y + 6755399441055744.0;  // 1.5 * 2^52: the last bits of the sum are the whole number
+    const double f = y - (whole - 6755399441055744.0);
+    double p = 1.3178930833147116e-06;
+    p = fma(p, f, 1.530915726184116e-05);
+    p = fma(p, f, 1.5403825484862121e-04);
+    p = fma(p, f, 1.333345485557617e-03);
+    p = fma(p, f, 9.61812861606663e-03);
+    p = fma(p, f, 5.5504109352728245e-02);
+    p = fma(p, f, 2.4022650698111078e-01);
+    p = fma(p, f, 6.931471805482102e-01);
     p = fma(p, f, 1.0);
-    return ldexp(p, (int)n);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(whole) << 20), __double2loint(p));
 }
-__device__ __forceinline__ double weight(float x, float most, double rate) { return x == most ? 1.0 : power_of_two(((double)x - (double)most) * rate); }
+// (what weighs 2^-1000 of the largest, minus infinity and NaN among it, is nothing in any sum)
+__device__ __forceinline__ double weight(float x, float most, double rate) { return x == most ? 1.0 : power_of_two(fmax(((double)x - (double)most) * rate, -1000.0)); }
 constexpr double kUnit = 4398046511104.0;  // 2^42: a vocabulary of 2^21 tokens of the same weight sums to 2^63
 __device__ __forceinline__ uint64_t units(double w) { return (uint64_t)__builtin_rint(w * kUnit); }
 
 // A row as 16-byte blocks, aligned: `lead` places in front of its first logit are no part of it.
 template <bool BF16> struct Row {
-    static constexpr int kSize = BF16 ? 2 : 4, kBlock = 16 / kSize, kLoads = kChunk / 64 / kBlock;
+    static constexpr int kSize = BF16 ? 2 : 4, kBlock = 16 / kSize;
     const uint8_t *base;
     int lead, end;  // logits lie in places lead to end
     __device__ __forceinline__ Row(const SampleArgs &a, int64_t row) {
@@ -113,35 +133,60 @@ template <bool BF16> struct Row {
     __device__ __forceinline__ int chunks() const { return (end + kChunk - 1) / kChunk; }
     __device__ __forceinline__ float one(int place) const {
         if (place < lead || place >= end) return kNegInf;
-        if constexpr (BF16) return clean(__uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(base)[place] << 16));
-        else return clean(reinterpret_cast<const float *>(base)[place]);
+        if constexpr (BF16) return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(base)[place] << 16);
+        else return reinterpret_cast<const float *>(base)[place];
     }
     // where value i of lane `lane` of a chunk lies
     __device__ __forceinline__ static int place(int chunk, int lane, int i) { return chunk * kChunk + ((i / kBlock) * 64 + lane) * kBlock + i % kBlock; }
-    __device__ __forceinline__ void load(int chunk, int lane, float (&x)[32]) const {
+    // values `from` on of a lane, N of them (a multiple of eight)
+    template <int N> __device__ __forceinline__ void load(int chunk, int lane, float (&x)[N], int from = 0) const {
         if (chunk * kChunk >= lead && (chunk + 1) * kChunk <= end) {
-            u4 w[kLoads];
+            constexpr int LOADS = N / kBlock;
+            u4 w[LOADS];
 #pragma unroll
-            for (int i = 0; i < kLoads; i++) w[i] = *reinterpret_cast<const u4 *>(base + (int64_t)place(chunk, lane, i * kBlock) * kSize);
+            for (int i = 0; i < LOADS; i++) w[i] = *reinterpret_cast<const u4 *>(base + (int64_t)place(chunk, lane, from + i * kBlock) * kSize);
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
+            for (int i = 0; i < N; i++) {
                 if constexpr (BF16) {
                     const uint32_t u = w[i / 8][i % 8 / 2];
-                    x[i] = clean(__uint_as_float(i & 1 ? u & 0xFFFF0000u : u << 16));
+                    x[i] = __uint_as_float(i & 1 ? u & 0xFFFF0000u : u << 16);
                 } else {
-                    x[i] = clean(__uint_as_float(w[i / 4][i % 4]));
+                    x[i] = __uint_as_float(w[i / 4][i % 4]);
                 }
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; i++) x[i] = one(place(chunk, lane, i));
+            for (int i = 0; i < N; i++) x[i] = one(place(chunk, lane, from + i));
         }
     }
 };
 
-template <class T, class F> __device__ __forceinline__ T over_lanes(T v, F f) {
+// The lanes' values up to and with each, by data-parallel moves: 1, 2, 4, 8 lanes within rows of sixteen, then from the last lane of a row into the next one, and of
+// the first half into the second.  `none` combines to nothing.  (Through LDS, as shuffles go, a scan of 64 bits takes three times as long, and the second launch is a chain of them.)
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t moved(uint32_t v, uint32_t none) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t moved(uint64_t v, uint64_t none) {
+    return (uint64_t)moved<CTRL, ROWS>((uint32_t)(v >> 32), (uint32_t)(none >> 32)) << 32 | moved<CTRL, ROWS>((uint32_t)v, (uint32_t)none);
+}
+template <class T, class F> __device__ __forceinline__ T scan_lanes(T v, T none, F f) {
+    v = f(v, moved<0x111, 0xF>(v, none));
+    v = f(v, moved<0x112, 0xF>(v, none));
+    v = f(v, moved<0x114, 0xF>(v, none));
+    v = f(v, moved<0x118, 0xF>(v, none));
+    v = f(v, moved<0x142, 0xA>(v, none));
+    v = f(v, moved<0x143, 0xC>(v, none));
+    return v;
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) { return (uint64_t)last_lane((uint32_t)(v >> 32)) << 32 | last_lane((uint32_t)v); }
+struct Sum { template <class T> static constexpr T none = 0; template <class T> __device__ __forceinline__ T operator()(T p, T q) const { return p + q; } };
+struct Most { template <class T> static constexpr T none = 0; template <class T> __device__ __forceinline__ T operator()(T p, T q) const { return max(p, q); } };
+struct Least { template <class T> static constexpr T none = ~(T)0; template <class T> __device__ __forceinline__ T operator()(T p, T q) const { return min(p, q); } };
+template <class F, class T> __device__ __forceinline__ T over_lanes(T v, F f) { return last_lane(scan_lanes(v, F::template none<T>, f)); }
+__device__ __forceinline__ double sum_of_lanes(double v) {
 #pragma unroll
-    for (int m = 32; m; m >>= 1) v = f(v, __shfl_xor(v, m));
+    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
     return v;
 }
 
@@ -158,35 +203,45 @@ template <bool BF16> __global__ __launch_bounds__(256) void sample_scan_kernel(c
     float x[32];
     r.load(chunk, lane, x);
     const Settings s = settings_of(a, row);
+    if (index == 0 && lane == 0) *a.wides = 0;
     float mine = kNegInf;
 #pragma unroll
-    for (int i = 0; i < 32; i++) mine = fmaxf(mine, x[i]);
-    const float most = over_lanes(mine, [](float p, float q) { return fmaxf(p, q); });
-    int at = 0x7FFFFFFF;
+    for (int i = 0; i < 32; i++) mine = fmaxf(mine, x[i]);  // (a NaN is not taken)
+    const float most = value_of(over_lanes(key_of(mine), Most{}));
+    Chunk c{0.0, most, 0, kAll, 0};
+    if (s.first) {
+        int at = 0x7FFFFFFF;
 #pragma unroll
-    for (int i = 31; i >= 0; i--) at = x[i] == most ? Row<BF16>::place(chunk, lane, i) - r.lead : at;
-    at = over_lanes(at, [](int p, int q) { return min(p, q); });
-    Chunk c{0.0, most, at, kAll, 0};
-    if (!s.first && most > kNegInf) {
+        for (int i = 31; i >= 0; i--) at = x[i] == most ? Row<BF16>::place(chunk, lane, i) - r.lead : at;
+        c.at = (int)over_lanes((uint32_t)at, Least{});
+    } else if (most > kNegInf) {
         double sum = 0.0;
+        const float lowest = (float)((double)most - 693.0 * s.t);  // weighs 2^-999.8; a NaN and minus infinity count as that
+        const double least_weight = ((double)lowest - (double)most) * s.rate;
+        if (least_weight <= -950.0 && least_weight >= -1010.0) {  // (not so where 32 bits have no such number, near infinity or zero temperature)
 #pragma unroll
-        for (int i = 0; i < 32; i++) sum += weight(x[i], most, s.rate);
-        c.sum = over_lanes(sum, [](double p, double q) { return p + q; });
+            for (int i = 0; i < 32; i++) sum += power_of_two(((double)fmaxf(x[i], lowest) - (double)most) * s.rate);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < 32; i++) sum += x[i] > kNegInf ? weight(x[i], most, s.rate) : 0.0;
+        }
+        c.sum = sum_of_lanes(sum);
         if (s.cuts()) {
             const uint32_t top = key_of(mine);
             uint32_t level = 0;
 #pragma unroll
             for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
                 if (__popcll(__ballot(top >= (level | bit))) >= 32) level |= bit;
+            const float least = value_of(max(level, key_of(-3.402823466e38f)));  // (minus infinity is in no list)
             uint32_t *keys = a.keys + index * kChunkKeys;
             int count = 0;
 #pragma unroll
             for (int i = 0; i < 32; i++) {
-                const uint32_t key = key_of(x[i]);
-                const bool in = key >= level && x[i] > kNegInf;
+                const bool in = x[i] >= least;
                 const uint64_t all = __ballot(in);
+                if (!all) continue;
                 const int to = count + __popcll(all & ((1ull << lane) - 1));
-                if (in && to < kChunkKeys) keys[to] = key;
+                if (in && to < kChunkKeys) keys[to] = key_of(x[i]);
                 count += __popcll(all);
             }
             if (count <= kChunkKeys) { c.level = level; c.count = count; }
@@ -198,18 +253,13 @@ template <bool BF16> __global__ __launch_bounds__(256) void sample_scan_kernel(c
 // ---- the second launch ------------------------------------------------------------------------------------------------
 
 // Sums of the threads in front of each, in order; `total` of all of them.
-template <class T> __device__ __forceinline__ T threads_in_front(T v, T *waves, T &total) {
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    T upto = v;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const T o = __shfl_up(upto, m);
-        if (lane >= m) upto += o;
-    }
+__device__ __forceinline__ uint64_t threads_in_front(uint64_t v, uint64_t *waves, uint64_t &total) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const uint64_t upto = scan_lanes(v, (uint64_t)0, Sum{});
     __syncthreads();
-    if (lane == 63) waves[wave] = upto;
+    if (((int)threadIdx.x & 63) == 63) waves[wave] = upto;
     __syncthreads();
-    T front = 0;
+    uint64_t front = 0;
     total = 0;
 #pragma unroll
     for (int i = 0; i < kPickWaves; i++) {
@@ -219,11 +269,10 @@ template <class T> __device__ __forceinline__ T threads_in_front(T v, T *waves, 
     return front + upto - v;
 }
 
-// The last kept token: the kept ones are those of larger key and the first `ties` of this one; how many are above it, and their weight.
+// The last kept token: the kept ones are those of larger key and the first `ties` of this one; how many are above it, or what they weigh.
 struct Cut {
     uint32_t key, ties;
-    uint32_t above;
-    uint64_t above_weight;
+    uint64_t above;  // tokens, where the cut is one of tokens, or weight
 };
 
 struct PickLds {
@@ -234,281 +283,231 @@ struct PickLds {
     uint64_t chunk_weight[kMostChunks];
     uint32_t chunk_ties[kMostChunks];
     uint64_t waves[kPickWaves];
-    uint64_t found_weight;
-    uint32_t found, found_count, listed;
+    uint64_t found_above;
+    uint32_t few[kFew];
+    uint64_t few_weights[kFew];
+    uint32_t found, found_key, found_same, listed, fews;
 };
 
-// The first of the bins, from bin 0 on, up to which `want` is reached, of tokens (by count) or of weight; what is in front of it.  kBins: none.
-__device__ __forceinline__ uint32_t find_bin(PickLds &l, bool by_count, uint64_t want, uint32_t &above, uint64_t &above_weight) {
-    constexpr int N = kBins / kPickThreads;
-    const int first = (int)threadIdx.x * N;
-    uint64_t weights = 0, counts = 0, total;
-    if (threadIdx.x == 0) l.found = kBins;
+template <class T, class F> __device__ __forceinline__ T over_threads(T v, uint64_t *waves, F f) {
+    v = over_lanes(v, f);
+    __syncthreads();
+    if (((int)threadIdx.x & 63) == 0) waves[(int)threadIdx.x >> 6] = (uint64_t)v;
+    __syncthreads();
+    v = (T)waves[0];
 #pragma unroll
-    for (int i = 0; i < N; i++) { weights += l.weights[first + i]; counts += l.counts[first + i]; }
-    uint64_t w = threads_in_front(weights, l.waves, total) + above_weight, c = threads_in_front(counts, l.waves, total) + above;
+    for (int i = 1; i < kPickWaves; i++) v = f(v, (T)waves[i]);
+    return v;
+}
+__device__ __forceinline__ uint64_t sum_of_threads(uint64_t v, uint64_t *waves) { return over_threads(v, waves, Sum{}); }
+
+// The first of the bins, from bin 0 on, up to which `want` is reached, of tokens (by count) or of weight; `above`: what is in front of it.  BINS: none.
+template <int BINS> __device__ __forceinline__ uint32_t find_bin(PickLds &l, bool by_count, uint64_t want, uint64_t &above) {
+    constexpr int N = BINS / kPickThreads;
+    const int first = (int)threadIdx.x * N;
+    if (threadIdx.x == 0) l.found = BINS;
+    uint64_t bins[N], mine = 0, total;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const uint64_t bw = l.weights[first + i], bc = l.counts[first + i];
-        const uint64_t before = by_count ? c : w, after = by_count ? c + bc : w + bw;
-        if (before < want && want <= after) {
+        bins[i] = by_count ? l.counts[first + i] : l.weights[first + i];
+        mine += bins[i];
+    }
+    uint64_t at = threads_in_front(mine, l.waves, total) + above;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (at < want && want <= at + bins[i]) {
             l.found = (uint32_t)(first + i);
-            l.found_count = (uint32_t)c;
-            l.found_weight = w;
+            l.found_above = at;
         }
-        w += bw;
-        c += bc;
+        at += bins[i];
     }
     __syncthreads();
     const uint32_t bin = l.found;
-    if (bin < kBins) { above = l.found_count; above_weight = l.found_weight; }
+    if (bin < BINS) above = l.found_above;
     __syncthreads();
     return bin;
 }
 
-__device__ __forceinline__ void clear_bins(PickLds &l) {
+template <int BINS> __device__ __forceinline__ void clear_bins(PickLds &l) {
     __syncthreads();
-    for (int i = (int)threadIdx.x; i < kBins; i += kPickThreads) { l.weights[i] = 0; l.counts[i] = 0; }
+    for (int i = (int)threadIdx.x; i < BINS; i += kPickThreads) { l.weights[i] = 0; l.counts[i] = 0; }
     __syncthreads();
 }
-__device__ __forceinline__ void add_to_bin(PickLds &l, uint32_t bin, uint64_t weight) {
-    atomicAdd(reinterpret_cast<unsigned long long *>(&l.weights[bin]), (unsigned long long)weight);
+__device__ __forceinline__ void add_to_bin(PickLds &l, uint32_t bin, bool with_weight, uint64_t weight) {
+    if (with_weight) atomicAdd(reinterpret_cast<unsigned long long *>(&l.weights[bin]), (unsigned long long)weight);
     atomicAdd(&l.counts[bin], 1u);
 }
+// how many of the tokens of the cut's key are kept
+__device__ __forceinline__ uint32_t ties_of(uint64_t want, uint64_t above, uint64_t each, uint32_t all) {
+    const uint64_t ties = (want - above + each - 1) / each;
+    return ties < all ? (uint32_t)ties : all;
+}
 
-// The cut at `want` tokens (or weight) among the keys that `each` passes on, with `cut` as what is above all of these: digit by digit, 11, 11 and 10 bits.  False: they
-// do not reach it.
-template <class Each, class Weight> __device__ __forceinline__ bool find_cut(PickLds &l, Each each, Weight weight_of, bool by_count, uint64_t want, Cut &cut) {
+// The cut at `want` tokens (or weight) among the l.listed keys in LDS, with cut.above as what is above all of them: by nine bits at a time of a key's distance from the largest, until so few
+// are left that each is held against all of them.  False: they do not reach it.
+template <class Weight> __device__ __forceinline__ bool cut_of_list(PickLds &l, Weight weight_of, bool by_count, uint64_t want, Cut &cut) {
+    const int tid = (int)threadIdx.x, n = (int)l.listed;
+    uint32_t top = kAll, left = (uint32_t)n;
+    int width = 32;  // keys from top down to top - 2^width + 1 are looked at
+    if (n == 0) return false;
+    if (n > kFew) {
+        uint32_t low = kAll;
+        top = 0;
+        for (int i = tid; i < n; i += kPickThreads) { low = min(low, l.keys[i]); top = max(top, l.keys[i]); }
+        low = over_threads(low, l.waves, Least{});
+        top = over_threads(top, l.waves, Most{});
+        width = 32 - __clz((int)(top - low));
+        do {
+            const uint32_t last = width < 32 ? (1u << width) - 1u : kAll;
+            const int shift = width > 9 ? width - 9 : 0;
+            clear_bins<kListBins>(l);
+            for (int i = tid; i < n; i += kPickThreads) {
+                const uint32_t key = l.keys[i], d = top - key;
+                if (key <= top && d <= last) add_to_bin(l, d >> shift, !by_count, by_count ? 0 : weight_of(key));
+            }
+            __syncthreads();
+            const uint32_t bin = find_bin<kListBins>(l, by_count, want, cut.above);
+            if (bin >= kListBins) return false;  // (the first time, or never)
+            left = l.counts[bin];
+            top -= bin << shift;
+            width = shift;
+        } while (width && left > kFew);
+        if (width == 0) {
+            cut.key = top;
+            cut.ties = ties_of(want, cut.above, by_count ? 1 : weight_of(top), left);
+            __syncthreads();
+            return true;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) { l.fews = 0; l.found_same = 0; }
+    __syncthreads();
+    for (int i = tid; i < n; i += kPickThreads) {
+        const uint32_t key = l.keys[i];
+        if (key <= top && (width == 32 || top - key < (1u << width))) l.few[atomicAdd(&l.fews, 1u)] = key;
+    }
+    __syncthreads();
+    if (tid < (int)left) l.few_weights[tid] = by_count ? 1 : weight_of(l.few[tid]);
+    __syncthreads();
+    // eight threads a key, an eighth of the others each
+    const int mine = tid / 8;
+    if (mine < (int)left) {
+        const uint32_t key = l.few[mine];
+        uint64_t above = 0;
+        uint32_t same = 0;
+#pragma unroll
+        for (int i = 0; i < kFew / 8; i++) {
+            const int other = tid % 8 + 8 * i;
+            const uint32_t k = l.few[other];
+            const bool there = other < (int)left;
+            above += there && k > key ? l.few_weights[other] : 0;
+            same += there && k == key;
+        }
+#pragma unroll
+        for (int m = 1; m < 8; m <<= 1) {
+            above += __shfl_xor(above, m);
+            same += __shfl_xor(same, m);
+        }
+        above += cut.above;
+        const uint64_t w = l.few_weights[mine];
+        if (above < want && want <= above + same * w) {  // (all of one key write the same)
+            l.found_key = key;
+            l.found_above = above;
+            l.found_same = ties_of(want, above, w, same);
+        }
+    }
+    __syncthreads();
+    cut.key = l.found_key;
+    cut.above = l.found_above;
+    cut.ties = l.found_same;
+    __syncthreads();
+    return cut.ties != 0;
+}
+
+// What the cut keeps of the list weighs; only keys from the cut's on stay in it.
+template <class Weight> __device__ __forceinline__ uint64_t keep_of_list(PickLds &l, Weight weight_of, const Cut &cut) {
+    constexpr int N = kListMost / kPickThreads;
+    const int tid = (int)threadIdx.x, lane = tid & 63, n = (int)l.listed;
+    uint32_t keys[N], kept = 0;
+    uint16_t chunks[N];
+    uint64_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int at = tid + i * kPickThreads;
+        keys[i] = at < n ? l.keys[at] : 0u;
+        chunks[i] = at < n ? l.chunks[at] : 0;
+        kept += keys[i] >= cut.key;
+    }
+    __syncthreads();
+    if (tid == 0) l.listed = 0;
+    __syncthreads();
+    const uint32_t upto = scan_lanes(kept, 0u, Sum{}), all = last_lane(upto);
+    uint32_t to = 0;
+    if (lane == 0 && all) to = atomicAdd(&l.listed, all);
+    to = __builtin_amdgcn_readfirstlane(to) + upto - kept;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (keys[i] < cut.key) continue;
+        l.keys[to] = keys[i];
+        l.chunks[to++] = chunks[i];
+    }
+    __syncthreads();
+    for (int i = tid; i < (int)l.listed; i += kPickThreads) sum += l.keys[i] > cut.key ? weight_of(l.keys[i]) : 0;
+    return sum_of_threads(sum, l.waves) + cut.ties * weight_of(cut.key);
+}
+
+// The same among the keys that `each` passes on, however many: digit by digit, 11, 11 and 10 bits.
+template <class Each, class Weight> __device__ __forceinline__ bool cut_of_many(PickLds &l, Each each, Weight weight_of, bool by_count, uint64_t want, Cut &cut) {
     uint32_t prefix = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 3; pass++) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, done = pass == 0 ? 32 : pass == 1 ? 21 : 10;
-        clear_bins(l);
+        const uint32_t digits = pass == 2 ? 1023u : 2047u;
+        clear_bins<kBins>(l);
         each([&](uint32_t key, int) {
             if (done < 32 && key >> done != prefix >> done) return;
-            const uint32_t digits = pass == 2 ? 1023u : 2047u;
-            add_to_bin(l, digits - (key >> shift & digits), weight_of(key));  // (the largest first)
+            add_to_bin(l, digits - (key >> shift & digits), !by_count, by_count ? 0 : weight_of(key));  // (the largest first)
         });
         __syncthreads();
-        const uint32_t bin = find_bin(l, by_count, want, cut.above, cut.above_weight);
+        const uint32_t bin = find_bin<kBins>(l, by_count, want, cut.above);
         if (bin >= kBins) return false;
-        prefix |= ((pass == 2 ? 1023u : 2047u) - bin) << shift;
-        if (pass == 2) {
-            const uint32_t all = l.counts[bin];
-            const uint64_t left = want - (by_count ? cut.above : cut.above_weight), w = by_count ? 1 : weight_of(prefix);
-            const uint64_t ties = (left + w - 1) / w;
-            cut.ties = ties < all ? (uint32_t)ties : all;
-        }
+        prefix |= (digits - bin) << shift;
+        if (pass == 2) cut.ties = ties_of(want, cut.above, by_count ? 1 : weight_of(prefix), l.counts[bin]);
     }
     cut.key = prefix;
     __syncthreads();
     return true;
 }
 
-template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleArgs a) {
-    __shared__ PickLds l;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t row = blockIdx.x;
-    const Row<BF16> r(a, row);
-    const Settings s = settings_of(a, row);
-    const int chunks = r.chunks();
-    const Chunk *chunk = a.chunk + row * a.chunks;
+// Bins of 1/32 in powers of two below the largest logit.
+__device__ __forceinline__ uint32_t bin_of(uint32_t key, float most, uint32_t most_key, float rate) {
+    const float d = (most - value_of(key)) * rate * 32.0f;
+    return key == most_key ? 0u : (uint32_t)fminf(d, (float)(kBins - 1));
+}
+// the weight that top-p asks for
+__device__ __forceinline__ uint64_t share_of(const Settings &s, uint64_t w) {
+    const double p = ceil(s.top_p * (double)w);
+    return p < 1.0 ? (uint64_t)1 : (uint64_t)p;
+}
 
-    // the row's largest logit; where; the level from which on the lists have every key; their length
-    float most = kNegInf;
-    int at = 0x7FFFFFFF;
-    uint32_t level = 0;
-    for (int c = tid; c < chunks; c += kPickThreads) {
-        const float m = chunk[c].most;
-        if (m > most) { most = m; at = chunk[c].at; }
-        if (m > kNegInf) level = max(level, chunk[c].level);
-    }
-    const float wave_most = over_lanes(most, [](float p, float q) { return fmaxf(p, q); });
-    at = over_lanes(most == wave_most ? at : 0x7FFFFFFF, [](int p, int q) { return min(p, q); });
-    level = over_lanes(level, [](uint32_t p, uint32_t q) { return max(p, q); });
-    if (lane == 0) {
-        l.weights[wave] = key_of(wave_most);
-        l.counts[wave] = (uint32_t)at;
-        l.counts[kPickWaves + wave] = level;
-    }
-    __syncthreads();
-    uint32_t most_key = 0;
-#pragma unroll
-    for (int i = 0; i < kPickWaves; i++) {
-        const uint32_t k = (uint32_t)l.weights[i];
-        at = k > most_key ? (int)l.counts[i] : k == most_key ? min(at, (int)l.counts[i]) : at;
-        most_key = max(most_key, k);
-        level = max(level, l.counts[kPickWaves + i]);
-    }
-    most = value_of(most_key);
-    if (s.first || most == kNegInf) {  // (a row without a number has no token)
-        if (tid == 0) {
-            a.tokens[row] = most == kNegInf ? -1 : at;
-            if (a.probabilities) a.probabilities[row] = most == kNegInf ? 0.0f : 1.0f;
-        }
-        return;
-    }
-    const auto weight_of = [&](uint32_t key) { return units(weight(value_of(key), most, s.rate)); };
-    const auto each_listed = [&](auto f) {
-        for (int i = tid; i < (int)l.listed; i += kPickThreads) f(l.keys[i], (int)l.chunks[i]);
-    };
-    const auto each_of_row = [&](auto f) {
-#pragma unroll 1
-        for (int c = wave; c < chunks; c += kPickWaves) {
-            float x[32];
-            r.load(c, lane, x);
-#pragma unroll
-            for (int i = 0; i < 32; i++)
-                if (x[i] > kNegInf) f(key_of(x[i]), c);
-        }
-    };
+// A token's weight and what min-p asks of keys, given the row's largest.
+__device__ __forceinline__ uint32_t floor_of(const Settings &s, float most, uint32_t most_key) {
+    if (!(s.min_p > 0.0)) return 0;
+    const double least = (double)most + s.t * log(s.min_p);
+    float f = (float)least;
+    if ((double)f < least) f = value_of(key_of(f) + 1);
+    return most == __builtin_huge_valf() ? most_key : min(most_key, key_of(clean(f)));
+}
 
-    // the cut: nothing, to begin with
-    Cut cut{0u, kAll, 0u, 0u};
-    uint32_t floor_key = 0;  // what min-p asks for
-    if (s.min_p > 0.0) {
-        const double least = (double)most + s.t * log(s.min_p);
-        float f = (float)least;
-        if ((double)f < least) f = value_of(key_of(f) + 1);
-        floor_key = most == __builtin_huge_valf() ? most_key : min(most_key, key_of(clean(f)));
-    }
-    const bool orders = s.k || s.top_p < 1.0;
-    bool from_lists = s.cuts() && level != kAll && (orders || floor_key >= level);
-    if (from_lists) {
-        if (tid == 0) l.listed = 0;
-        __syncthreads();
-#pragma unroll 1
-        for (int c = wave; c < chunks; c += kPickWaves) {
-            const int count = chunk[c].most > kNegInf ? chunk[c].count : 0;
-            const uint32_t *keys = a.keys + (row * a.chunks + c) * kChunkKeys;
-            for (int i = lane; i < count; i += 64) {
-                const uint32_t key = keys[i];
-                if (key < level) continue;
-                const uint32_t to = atomicAdd(&l.listed, 1u);
-                if (to < (uint32_t)kListMost) { l.keys[to] = key; l.chunks[to] = (uint16_t)c; }
-            }
-        }
-        __syncthreads();
-        from_lists = l.listed <= (uint32_t)kListMost;
-    }
-    // the weight of the row, for top-p without top-k
-    uint64_t all = 0;
-    if (!s.k && s.top_p < 1.0) {
-        double sum = 0.0;
-        for (int c = tid; c < chunks; c += kPickThreads)
-            if (chunk[c].most > kNegInf) sum += chunk[c].sum * weight(chunk[c].most, most, s.rate);
-        uint64_t total;
-        threads_in_front(units(sum), l.waves, total);
-        all = total;
-    }
-    const auto share = [&](uint64_t w) {
-        const double p = ceil(s.top_p * (double)w);
-        return p < 1.0 ? (uint64_t)1 : (uint64_t)p;
-    };
-    if (from_lists && orders) {
-        if (s.k) {
-            Cut c{0u, 0u, 0u, 0u};
-            from_lists = find_cut(l, each_listed, weight_of, true, (uint64_t)s.k, c);
-            if (from_lists) {
-                cut = c;
-                all = c.above_weight + c.ties * weight_of(c.key);
-            }
-        }
-        if (from_lists && s.top_p < 1.0) {
-            Cut c{0u, 0u, 0u, 0u};
-            from_lists = find_cut(l, each_listed, weight_of, false, share(all), c);
-            if (from_lists) cut = c;
-        }
-    }
-    if (s.cuts() && !from_lists && orders) {
-        // over the row again: bins of 1/32 in powers of two, then the keys of the one with the cut in it
-        const auto bin_of = [&](uint32_t key) {
-            const float d = (most - value_of(key)) * (float)s.rate * 32.0f;
-            return key == most_key ? 0u : (uint32_t)fminf(d, (float)(kBins - 1));
-        };
-        const auto cut_at = [&](bool by_count, uint64_t want, Cut &c) {
-            clear_bins(l);
-            each_of_row([&](uint32_t key, int) { add_to_bin(l, bin_of(key), weight_of(key)); });
-            __syncthreads();
-            if (!by_count && !s.k) {  // (the sum of these very numbers)
-                uint64_t mine = 0;
-                for (int i = tid; i < kBins; i += kPickThreads) mine += l.weights[i];
-                threads_in_front(mine, l.waves, all);
-                want = share(all);
-            }
-            const uint32_t bin = find_bin(l, by_count, want, c.above, c.above_weight);
-            if (bin >= kBins) return false;
-            const bool fits = l.counts[bin] <= (uint32_t)kListMost;
-            __syncthreads();
-            if (!fits)
-                return find_cut(l, [&](auto f) { each_of_row([&](uint32_t key, int at_chunk) { if (bin_of(key) == bin) f(key, at_chunk); }); }, weight_of, by_count, want, c);
-            if (tid == 0) l.listed = 0;
-            __syncthreads();
-            each_of_row([&](uint32_t key, int at_chunk) {
-                if (bin_of(key) != bin) return;
-                const uint32_t to = atomicAdd(&l.listed, 1u);
-                l.keys[to] = key;
-                l.chunks[to] = (uint16_t)at_chunk;
-            });
-            __syncthreads();
-            return find_cut(l, each_listed, weight_of, by_count, want, c);
-        };
-        if (s.k) {
-            Cut c{0u, 0u, 0u, 0u};
-            if (cut_at(true, (uint64_t)s.k, c)) {
-                cut = c;
-                all = c.above_weight + c.ties * weight_of(c.key);
-            } else if (s.top_p < 1.0) {  // (fewer numbers than k: all of them)
-                uint64_t mine = 0;
-                for (int i = tid; i < kBins; i += kPickThreads) mine += l.weights[i];
-                threads_in_front(mine, l.waves, all);
-            }
-        }
-        if (s.top_p < 1.0) {
-            Cut c{0u, 0u, 0u, 0u};
-            if (cut_at(false, share(all), c)) cut = c;
-        }
-    }
-    if (floor_key > cut.key) cut = Cut{floor_key, kAll, 0u, 0u};
-
-    // the kept weight of every chunk, and its tokens that equal the cut's
-    if (from_lists) {
-        __syncthreads();
-        for (int c = tid; c < chunks; c += kPickThreads) { l.chunk_weight[c] = 0; l.chunk_ties[c] = 0; }
-        __syncthreads();
-        each_listed([&](uint32_t key, int c) {
-            if (key > cut.key) atomicAdd(reinterpret_cast<unsigned long long *>(&l.chunk_weight[c]), (unsigned long long)weight_of(key));
-            else if (key == cut.key) atomicAdd(&l.chunk_ties[c], 1u);
-        });
-    } else if (s.cuts()) {
-#pragma unroll 1
-        for (int c = wave; c < chunks; c += kPickWaves) {
-            float x[32];
-            r.load(c, lane, x);
-            uint64_t sum = 0;
-            uint32_t ties = 0;
-#pragma unroll
-            for (int i = 0; i < 32; i++) {
-                const uint32_t key = key_of(x[i]);
-                if (x[i] > kNegInf && key > cut.key) sum += weight_of(key);
-                ties += x[i] > kNegInf && key == cut.key;
-            }
-            sum = over_lanes(sum, [](uint64_t p, uint64_t q) { return p + q; });
-            ties = over_lanes(ties, [](uint32_t p, uint32_t q) { return p + q; });
-            if (lane == 0) { l.chunk_weight[c] = sum; l.chunk_ties[c] = ties; }
-        }
-    } else {
-        for (int c = tid; c < chunks; c += kPickThreads) {
-            l.chunk_weight[c] = chunk[c].most > kNegInf ? units(chunk[c].sum * weight(chunk[c].most, most, s.rate)) : 0;
-            l.chunk_ties[c] = 0;
-        }
-    }
-    __syncthreads();
-
+// The token, once the cut is known: chunks in l.chunk_weight (without the cut's ties) and l.chunk_ties.
+template <bool BF16>
+__device__ __forceinline__ void draw(const SampleArgs &a, PickLds &l, const Row<BF16> &r, const Settings &s, int64_t row, int chunks, float most, const Cut &cut) {
+    const int tid = (int)threadIdx.x;
+    const bool cuts = s.cuts();
     // the chunk: two neighbouring ones a thread
-    const uint64_t cut_weight = s.cuts() ? weight_of(cut.key) : 0;
+    const uint64_t cut_weight = cuts ? units(weight(value_of(cut.key), most, s.rate)) : 0;
     constexpr int N = kMostChunks / kPickThreads;
-    uint64_t kept[N], mine = 0, total;
+    uint64_t kept[N], tie_at[N], mine = 0, total, tie_total;
     uint32_t ties[N], my_ties = 0;
     const int c0 = tid * N;
 #pragma unroll
@@ -517,9 +516,7 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_pick
         ties[i] = c0 + i < chunks ? l.chunk_ties[c0 + i] : 0;
         my_ties += ties[i];
     }
-    uint64_t tie_total;
     uint64_t tie_front = threads_in_front((uint64_t)my_ties, l.waves, tie_total);
-    uint64_t tie_at[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
         tie_at[i] = tie_front;
@@ -537,9 +534,9 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_pick
     for (int i = 0; i < N; i++) {
         if (front <= want && want < front + kept[i]) {
             l.found = (uint32_t)(c0 + i);
-            l.found_weight = front;
+            l.found_above = front;
             l.chunk_weight[0] = kept[i];
-            l.found_count = (uint32_t)min(tie_at[i], (uint64_t)kAll);
+            l.found_same = (uint32_t)min(tie_at[i], (uint64_t)kAll);
         }
         front += kept[i];
     }
@@ -547,19 +544,18 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_pick
 
     // the token: four neighbouring ones a thread
     const int c = (int)l.found;
-    want -= l.found_weight;
+    want -= l.found_above;
     const uint64_t of_chunk = l.chunk_weight[0];
-    uint32_t rank = l.found_count;
+    uint32_t rank = l.found_same;
     // (with nothing cut off the chunk's weight is a sum in 64 bits, not one of these units, of which its tokens may have none: in parts of the chunk then)
-    const float unit_most = s.cuts() ? most : chunk[c].most;
-    __syncthreads();
+    const float unit_most = cuts ? most : a.chunk[row * a.chunks + c].most;
     constexpr int M = kChunk / kPickThreads;
     float x[M];
     my_ties = 0;
 #pragma unroll
     for (int i = 0; i < M; i++) {
-        x[i] = r.one(c * kChunk + tid * M + i);
-        my_ties += s.cuts() && x[i] > kNegInf && key_of(x[i]) == cut.key;
+        x[i] = clean(r.one(c * kChunk + tid * M + i));
+        my_ties += cuts && x[i] > kNegInf && key_of(x[i]) == cut.key;
     }
     rank += (uint32_t)threads_in_front((uint64_t)my_ties, l.waves, tie_total);
     mine = 0;
@@ -567,15 +563,15 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_pick
 #pragma unroll
     for (int i = 0; i < M; i++) {
         const uint32_t key = key_of(x[i]);
-        const bool tie = s.cuts() && key == cut.key;
-        const bool keep = x[i] > kNegInf && (!s.cuts() || key > cut.key || (tie && rank < cut.ties));
+        const bool tie = cuts && key == cut.key;
+        const bool keep = x[i] > kNegInf && (!cuts || key > cut.key || (tie && rank < cut.ties));
         if (tie && x[i] > kNegInf) rank++;
         w[i] = keep ? units(weight(x[i], unit_most, s.rate)) : 0;
         mine += w[i];
     }
     uint64_t in_chunk;
     front = threads_in_front(mine, l.waves, in_chunk);
-    if (!s.cuts()) want = (uint64_t)((double)want / (double)of_chunk * (double)in_chunk);
+    if (!cuts) want = (uint64_t)((double)want / (double)of_chunk * (double)in_chunk);
     want = min(want, in_chunk - 1);
 #pragma unroll
     for (int i = 0; i < M; i++) {
@@ -585,6 +581,351 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_pick
         }
         front += w[i];
     }
+}
+
+// The kept weight of every chunk from the list in LDS, added to what is in l.chunk_weight, and its tokens that equal the cut's.
+template <class Weight> __device__ __forceinline__ void chunks_of_list(PickLds &l, Weight weight_of, const Cut &cut, int chunks, bool clear) {
+    __syncthreads();
+    for (int c = (int)threadIdx.x; c < chunks; c += kPickThreads) {
+        if (clear) l.chunk_weight[c] = 0;
+        l.chunk_ties[c] = 0;
+    }
+    __syncthreads();
+    for (int i = (int)threadIdx.x; i < (int)l.listed; i += kPickThreads) {
+        const uint32_t key = l.keys[i];
+        const int c = l.chunks[i];
+        if (key > cut.key) atomicAdd(reinterpret_cast<unsigned long long *>(&l.chunk_weight[c]), (unsigned long long)weight_of(key));
+        else if (key == cut.key) atomicAdd(&l.chunk_ties[c], 1u);
+    }
+    __syncthreads();
+}
+
+// All of a flat row in one workgroup: its bins, the keys of the one with the cut in it, then its chunks.
+template <bool BF16>
+__device__ __forceinline__ void draw_alone(const SampleArgs &a, PickLds &l, const Row<BF16> &r, const Settings &s, int64_t row, int chunks, float most, uint32_t most_key, uint32_t floor_key) {
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float rate = (float)s.rate;
+    const auto weight_of = [&](uint32_t key) { return units(weight(value_of(key), most, s.rate)); };
+    const auto each_of_row = [&](auto f) {
+#pragma unroll 1
+        for (int at = wave * 4; at < chunks * 4; at += at % 4 == 3 ? (kPickWaves - 1) * 4 + 1 : 1) {  // (a quarter of a chunk at a time: few registers)
+            float x[8];
+            r.load(at / 4, lane, x, at % 4 * 8);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (x[i] > kNegInf) f(key_of(x[i]), at / 4);
+        }
+    };
+    Cut cut{0u, kAll, 0};
+    uint64_t all = 0;
+#pragma unroll 1
+    for (int turn = s.k ? 0 : 1; turn < (s.top_p < 1.0 ? 2 : 1); turn++) {
+        const bool by_count = turn == 0;
+        Cut c{0u, 0u, 0};
+        clear_bins<kBins>(l);
+        each_of_row([&](uint32_t key, int) { add_to_bin(l, bin_of(key, most, most_key, rate), true, weight_of(key)); });
+        __syncthreads();
+        if (turn == (s.k ? 0 : 1)) {  // (what all of the row weighs, where fewer numbers than k are there too)
+            uint64_t mine = 0;
+            for (int i = tid; i < kBins; i += kPickThreads) mine += l.weights[i];
+            all = sum_of_threads(mine, l.waves);
+        }
+        const uint64_t want = by_count ? (uint64_t)s.k : share_of(s, all);
+        const uint32_t bin = find_bin<kBins>(l, by_count, want, c.above);
+        if (bin >= kBins) continue;
+        const uint32_t in_bin = l.counts[bin];
+        __syncthreads();
+        if (in_bin > (uint32_t)kListMost) {
+            cut_of_many(l, [&](auto f) { each_of_row([&](uint32_t key, int at) { if (bin_of(key, most, most_key, rate) == bin) f(key, at); }); }, weight_of, by_count, want, c);
+        } else {
+            if (tid == 0) l.listed = 0;
+            __syncthreads();
+            each_of_row([&](uint32_t key, int at) {
+                if (bin_of(key, most, most_key, rate) != bin) return;
+                const uint32_t to = atomicAdd(&l.listed, 1u);
+                l.keys[to] = key;
+                l.chunks[to] = (uint16_t)at;
+            });
+            __syncthreads();
+            cut_of_list(l, weight_of, by_count, want, c);
+        }
+        cut = c;
+        if (by_count && s.top_p < 1.0) {
+            uint64_t mine = 0;
+            each_of_row([&](uint32_t key, int) { mine += key > cut.key ? weight_of(key) : 0; });
+            all = sum_of_threads(mine, l.waves) + cut.ties * weight_of(cut.key);
+        }
+    }
+    if (floor_key > cut.key) cut = Cut{floor_key, kAll, 0};
+    __syncthreads();
+#pragma unroll 1
+    for (int c = wave; c < chunks; c += kPickWaves) {
+        uint64_t sum = 0;
+        uint32_t ties = 0;
+#pragma unroll 1
+        for (int from = 0; from < 32; from += 8) {
+            float x[8];
+            r.load(c, lane, x, from);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t key = key_of(x[i]);
+                if (x[i] > kNegInf && key > cut.key) sum += weight_of(key);
+                ties += x[i] > kNegInf && key == cut.key;
+            }
+        }
+        sum = over_lanes(sum, Sum{});
+        ties = over_lanes(ties, Sum{});
+        if (lane == 0) { l.chunk_weight[c] = sum; l.chunk_ties[c] = ties; }
+    }
+    __syncthreads();
+    draw(a, l, r, s, row, chunks, most, cut);
+}
+
+template <bool BF16> __global__ __launch_bounds__(kPickThreads, 4) void sample_pick_kernel(const SampleArgs a) {
+    __shared__ PickLds l;
+    const int tid = (int)threadIdx.x, lane = tid & 63;
+    const int64_t row = blockIdx.x;
+    const Row<BF16> r(a, row);
+    const Settings s = settings_of(a, row);
+    const int chunks = r.chunks();
+    const Chunk *chunk = a.chunk + row * a.chunks;
+
+    // the row's largest logit, and the level from which on the lists have every key
+    uint32_t most_key = 0, level = 0;
+    for (int c = tid; c < chunks; c += kPickThreads) {
+        const float m = chunk[c].most;
+        const bool some = m > kNegInf;
+        most_key = max(most_key, some ? key_of(m) : 0u);
+        level = max(level, some ? chunk[c].level : 0u);
+        l.chunk_ties[c] = some ? (uint32_t)chunk[c].count : 0u;
+    }
+    most_key = over_threads(most_key, l.waves, Most{});
+    level = over_threads(level, l.waves, Most{});
+    const float most = value_of(most_key);
+    if (most_key == 0 || s.first) {  // (a row without a number has no token)
+        uint32_t at = kAll;
+        for (int c = tid; c < chunks; c += kPickThreads)
+            if (most_key && key_of(chunk[c].most) == most_key) at = min(at, (uint32_t)chunk[c].at);
+        at = over_threads(at, l.waves, Least{});
+        if (tid == 0) {
+            a.tokens[row] = (int32_t)at;
+            if (a.probabilities) a.probabilities[row] = most_key ? 1.0f : 0.0f;
+        }
+        return;
+    }
+    const auto weight_of = [&](uint32_t key) { return units(weight(value_of(key), most, s.rate)); };
+    if (!s.cuts()) {
+        for (int c = tid; c < chunks; c += kPickThreads) {
+            l.chunk_weight[c] = chunk[c].most > kNegInf ? units(chunk[c].sum * weight(chunk[c].most, most, s.rate)) : 0;
+            l.chunk_ties[c] = 0;
+        }
+        __syncthreads();
+        draw(a, l, r, s, row, chunks, most, Cut{0u, kAll, 0});
+        return;
+    }
+    const uint32_t floor_key = floor_of(s, most, most_key);
+    Cut cut{0u, kAll, 0};
+    bool from_lists = level != kAll && (s.orders() || floor_key >= level);
+    if (from_lists) {
+        if (tid == 0) l.listed = 0;
+        __syncthreads();
+        // (sixteen loads on their way at a time)
+        constexpr int AHEAD = 16;
+        const uint32_t *keys = a.keys + row * a.chunks * kChunkKeys;
+        const int slots = chunks * kChunkKeys;
+#pragma unroll 1
+        for (int i0 = tid; i0 < slots + lane; i0 += AHEAD * kPickThreads) {  // (whole wavefronts)
+            uint32_t key[AHEAD], in = 0;
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const int at = i0 + i * kPickThreads;
+                key[i] = at < slots && at % kChunkKeys < (int)l.chunk_ties[at / kChunkKeys] ? keys[at] : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) in += key[i] >= level && key[i];
+            const uint32_t upto = scan_lanes(in, 0u, Sum{}), all = last_lane(upto);
+            uint32_t to = 0;
+            if (lane == 0 && all) to = atomicAdd(&l.listed, all);
+            to = __builtin_amdgcn_readfirstlane(to) + upto - in;
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                if (key[i] < level || !key[i]) continue;
+                if (to < (uint32_t)kListMost) { l.keys[to] = key[i]; l.chunks[to] = (uint16_t)((i0 + i * kPickThreads) / kChunkKeys); }
+                to++;
+            }
+        }
+        __syncthreads();
+        from_lists = l.listed <= (uint32_t)kListMost;
+    }
+    uint64_t all = 0;
+    if (from_lists && s.k) {
+        cut = Cut{0u, 0u, 0};
+        from_lists = cut_of_list(l, weight_of, true, (uint64_t)s.k, cut);
+        if (from_lists && s.top_p < 1.0) all = keep_of_list(l, weight_of, cut);
+    } else if (from_lists && s.top_p < 1.0) {
+        double sum = 0.0;
+        for (int c = tid; c < chunks; c += kPickThreads)
+            if (chunk[c].most > kNegInf) sum += chunk[c].sum * weight(chunk[c].most, most, s.rate);
+        all = sum_of_threads(units(sum), l.waves);
+    }
+    if (from_lists && s.top_p < 1.0) {
+        cut = Cut{0u, 0u, 0};
+        from_lists = cut_of_list(l, weight_of, false, share_of(s, all), cut);
+    }
+    if (from_lists) {
+        if (floor_key > cut.key) cut = Cut{floor_key, kAll, 0};
+        chunks_of_list(l, weight_of, cut, chunks, true);
+        draw(a, l, r, s, row, chunks, most, cut);
+        return;
+    }
+    // a flat row: into the launches for those, where there are any and they have room (with both bounds the second needs the first's answer)
+    __syncthreads();
+    if (a.wide && !(s.k && s.top_p < 1.0)) {
+        if (tid == 0) l.found = atomicAdd(a.wides, 1u);
+        __syncthreads();
+        const uint32_t slot = l.found;
+        if (slot < (uint32_t)a.wide_rows) {
+            Wide &w = a.wide[slot];
+            for (int i = tid; i < kBins; i += kPickThreads) { w.weights[i] = 0; w.counts[i] = 0; }
+            if (tid == 0) { w.row = row; w.most = most; w.floor_key = floor_key; w.listed = 0; }
+            return;
+        }
+    }
+    draw_alone(a, l, r, s, row, chunks, most, most_key, floor_key);
+}
+
+// ---- the launches for flat rows: eight chunks a workgroup ------------------------------------------------------------------
+
+__device__ __forceinline__ Wide *wide_of(const SampleArgs &a, int slot) { return slot < a.wide_rows && (uint32_t)slot < *a.wides ? a.wide + slot : nullptr; }
+
+template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_bins_kernel(const SampleArgs a, int parts) {
+    __shared__ uint64_t weights[kBins];
+    __shared__ uint32_t counts[kBins];
+    const int slot = (int)blockIdx.x / parts, tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Wide *w = wide_of(a, slot);
+    if (!w) return;
+    const int64_t row = w->row;
+    const Row<BF16> r(a, row);
+    const Settings s = settings_of(a, row);
+    const int c = ((int)blockIdx.x - slot * parts) * kPickWaves + wave;
+    if (!s.orders()) return;
+    float x[32];
+    if (c < r.chunks()) r.load(c, lane, x);
+    for (int i = tid; i < kBins; i += kPickThreads) { weights[i] = 0; counts[i] = 0; }
+    __syncthreads();
+    const float most = w->most;
+    const uint32_t most_key = key_of(most);
+    if (c < r.chunks()) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            if (!(x[i] > kNegInf)) continue;
+            const uint32_t bin = bin_of(key_of(x[i]), most, most_key, (float)s.rate);
+            if (!s.k) atomicAdd(reinterpret_cast<unsigned long long *>(&weights[bin]), (unsigned long long)units(weight(x[i], most, s.rate)));
+            atomicAdd(&counts[bin], 1u);
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kPickThreads) {
+        if (!counts[i]) continue;
+        if (!s.k) atomicAdd(reinterpret_cast<unsigned long long *>(&w->weights[i]), (unsigned long long)weights[i]);
+        atomicAdd(&w->counts[i], counts[i]);
+    }
+}
+
+// The bin with the row's cut in it; above: tokens or weight in front of it; want: what the cut is at; in_bin: its tokens.  kBins: everything is kept.
+__device__ __forceinline__ uint32_t bin_of_cut(PickLds &l, const Settings &s, const Wide &w, uint64_t &above, uint64_t &want, uint32_t &in_bin) {
+    uint64_t all = 0;
+    if (!s.orders()) return kBins;
+    for (int i = (int)threadIdx.x; i < kBins; i += kPickThreads) {
+        if (s.k) l.counts[i] = w.counts[i];
+        else all += l.weights[i] = w.weights[i];
+    }
+    all = sum_of_threads(all, l.waves);
+    want = s.k ? (uint64_t)s.k : share_of(s, all);
+    above = 0;
+    const uint32_t bin = find_bin<kBins>(l, s.k != 0, want, above);
+    in_bin = bin < kBins ? w.counts[bin] : 0;
+    return bin;
+}
+
+template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_gather_kernel(const SampleArgs a, int parts) {
+    __shared__ PickLds l;
+    const int slot = (int)blockIdx.x / parts, tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Wide *w = wide_of(a, slot);
+    if (!w) return;
+    const int64_t row = w->row;
+    const Row<BF16> r(a, row);
+    const Settings s = settings_of(a, row);
+    const int c = ((int)blockIdx.x - slot * parts) * kPickWaves + wave;
+    float x[32];
+    if (c < r.chunks()) r.load(c, lane, x);
+    uint64_t above, want;
+    uint32_t in_bin = 0;
+    const uint32_t bin = bin_of_cut(l, s, *w, above, want, in_bin);
+    if (c >= r.chunks() || in_bin > (uint32_t)kListMost) return;
+    const float most = w->most;
+    const uint32_t most_key = key_of(most), floor_key = w->floor_key;
+    uint64_t sum = 0;
+    uint32_t in = 0, found = 0;  // which of the lane's are in the bin; how many of the wavefront's
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+        const uint32_t key = key_of(x[i]);
+        const uint32_t mine = x[i] > kNegInf && key >= floor_key ? bin_of(key, most, most_key, (float)s.rate) : kAll;
+        if (mine < bin) sum += units(weight(x[i], most, s.rate));
+        in |= (uint32_t)(mine == bin) << i;
+        found += __popcll(__ballot(mine == bin));
+    }
+    if (found) {
+        uint32_t to = 0;
+        if (lane == 0) to = atomicAdd(&w->listed, found);
+        to = __builtin_amdgcn_readfirstlane(to);
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            const uint64_t all = __ballot(in >> i & 1u);
+            if (in >> i & 1u) {
+                const uint32_t at = to + __popcll(all & ((1ull << lane) - 1));
+                w->keys[at] = key_of(x[i]);
+                w->chunks[at] = (uint16_t)c;
+            }
+            to += __popcll(all);
+        }
+    }
+    sum = over_lanes(sum, Sum{});
+    if (lane == 0) w->chunk_weight[c] = sum;
+}
+
+template <bool BF16> __global__ __launch_bounds__(kPickThreads, 4) void sample_wide_kernel(const SampleArgs a) {
+    __shared__ PickLds l;
+    const int tid = (int)threadIdx.x;
+    const Wide *w = wide_of(a, (int)blockIdx.x);
+    if (!w) return;
+    const int64_t row = w->row;
+    const Row<BF16> r(a, row);
+    const Settings s = settings_of(a, row);
+    const int chunks = r.chunks();
+    const float most = w->most;
+    const uint32_t most_key = key_of(most), floor_key = w->floor_key;
+    const auto weight_of = [&](uint32_t key) { return units(weight(value_of(key), most, s.rate)); };
+    uint64_t want;
+    Cut cut{0u, kAll, 0}, c{0u, 0u, 0};
+    uint32_t in_bin = 0;
+    const uint32_t bin = bin_of_cut(l, s, *w, c.above, want, in_bin);
+    if (in_bin > (uint32_t)kListMost) {
+        __syncthreads();
+        draw_alone(a, l, r, s, row, chunks, most, most_key, floor_key);
+        return;
+    }
+    __syncthreads();
+    // the keys of the bin that min-p leaves: where it leaves none of them, or not as many as the cut keeps, it is the cut
+    const int n = bin < kBins ? (int)w->listed : 0;
+    for (int i = tid; i < n; i += kPickThreads) { l.keys[i] = w->keys[i]; l.chunks[i] = w->chunks[i]; }
+    for (int i = tid; i < chunks; i += kPickThreads) l.chunk_weight[i] = w->chunk_weight[i];
+    if (tid == 0) l.listed = (uint32_t)n;
+    __syncthreads();
+    if (n && cut_of_list(l, weight_of, s.k != 0, want, c)) cut = c;
+    if (floor_key > cut.key) cut = Cut{floor_key, kAll, 0};
+    chunks_of_list(l, weight_of, cut, chunks, false);
+    draw(a, l, r, s, row, chunks, most, cut);
 }
 
 }  // namespace
@@ -599,10 +940,20 @@ int launch_sample(const void *logits, bool bf16, int64_t rows, int64_t vocab, in
     // as many rows at a time as 256 MB of workspace hold
     const size_t a_row = (size_t)a.chunks * (sizeof(Chunk) + kChunkKeys * 4);
     const int64_t batch = std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)(((size_t)256 << 20) / a_row)));
+    // Flat rows have launches of their own where one bound may lead below a chunk's list (not a small top-k, which the lists nearly always hold) and a workgroup would
+    // go over a row in several rounds.
+    const bool cuts = how.top_ks || how.top_ps || how.min_ps || how.top_k > 0 || how.top_p < 1.0 || how.min_p > 0.0;
+    const bool wide = cuts && (how.top_ks || how.top_k <= 0 || how.top_k > 256) && a.chunks > kPickWaves;
+    a.wide_rows = (int)std::min<int64_t>(batch, kWideRows);
+    const size_t lists = (size_t)batch * a_row, wides = (lists + 255) / 256 * 256, flat = wides + 256;
     void *ws = nullptr;
-    if (int rc = stream_workspace(s, (size_t)batch * a_row, &ws)) return rc;
-    a.chunk = static_cast<Chunk *>(ws);
+    if (int rc = stream_workspace(s, flat + (wide ? a.wide_rows * sizeof(Wide) : 0), &ws)) return rc;
+    unsigned char *at = static_cast<unsigned char *>(ws);
+    a.chunk = reinterpret_cast<Chunk *>(at);
     a.keys = reinterpret_cast<uint32_t *>(a.chunk + batch * a.chunks);
+    a.wides = reinterpret_cast<uint32_t *>(at + wides);
+    a.wide = wide ? reinterpret_cast<Wide *>(at + flat) : nullptr;
+    const int parts = (a.chunks + kPickWaves - 1) / kPickWaves;
     for (int64_t row = 0; row < rows; row += batch) {
         const int64_t n = std::min(batch, rows - row), waves = n * a.chunks;
         a.logits = static_cast<const uint8_t *>(logits) + row * a.row_bytes;
@@ -614,8 +965,13 @@ int launch_sample(const void *logits, bool bf16, int64_t rows, int64_t vocab, in
         a.uniform = uniform + row;
         a.tokens = tokens + row;
         a.probabilities = probabilities ? probabilities + row : nullptr;
+        const dim3 block(kPickThreads), slices((unsigned)(a.wide_rows * parts));
         if (int rc = launch(bf16 ? sample_scan_kernel<true> : sample_scan_kernel<false>, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, a, waves)) return rc;
-        if (int rc = launch(bf16 ? sample_pick_kernel<true> : sample_pick_kernel<false>, dim3((unsigned)n), dim3(kPickThreads), 0, s, a)) return rc;
+        if (int rc = launch(bf16 ? sample_pick_kernel<true> : sample_pick_kernel<false>, dim3((unsigned)n), block, 0, s, a)) return rc;
+        if (!wide) continue;
+        if (int rc = launch(bf16 ? sample_bins_kernel<true> : sample_bins_kernel<false>, slices, block, 0, s, a, parts)) return rc;
+        if (int rc = launch(bf16 ? sample_gather_kernel<true> : sample_gather_kernel<false>, slices, block, 0, s, a, parts)) return rc;
+        if (int rc = launch(bf16 ? sample_wide_kernel<true> : sample_wide_kernel<false>, dim3((unsigned)a.wide_rows), block, 0, s, a)) return rc;
     }
     return GQ_OK;
 }

@@ -353,6 +353,15 @@ def test_samples_of_rows_with_holes(gpu, how):
     assert tokens[3] == -1 and tokens[2] == 4321 and tokens[7] == 4999 and tokens[4] in (17, 4000)
 
 
+def test_samples_of_more_flat_rows_than_their_launches_take(gpu):
+    torch = gpu
+    rng = np.random.default_rng(10)
+    x = logits(rng, 150, 20000, sure=False)
+    x[::7] = np.round(x[::7])
+    for how in (dict(top_p=0.8), dict(top_k=3000), dict(min_p=0.01), dict(top_p=0.9, min_p=0.02)):
+        check_samples(torch, torch.from_numpy(x).cuda(), rng.random(150), **how)
+
+
 def test_samples_with_settings_of_each_row(gpu):
     torch = gpu
     rng = np.random.default_rng(6)
