@@ -28,6 +28,10 @@ template <int D, bool TWO> __device__ __forceinline__ float reference(float most
     const float set = most - Weights<D, TWO>::kSet;
     return passes<D, TWO>(most, set) ? most : set;
 }
+// With many rows a weight comes from a score's exact product with the scale, less a reference that is a rounded one: one instruction, and from references of
+// this size on an error of a 2^-8 th and more of a factor of 2 (at 2^27, of more than fp16 numbers have room for).  There the product is rounded as the reference was.
+// (bfloat16 alone: float32 queries take all of the scale but a power of two, by which products are exact.)
+constexpr float kCoarse = 65536.0f;
 
 __device__ __forceinline__ h2 as_h2(uint32_t u) { return __builtin_bit_cast(h2, u); }
 __device__ __forceinline__ h2 both(float v) { h2 r = {(_Float16)v, (_Float16)v}; return r; }

@@ -23,11 +23,6 @@ namespace gq {
 
 namespace {
 
-// With many rows a weight comes from a score's exact product with the scale, less a reference that is a rounded one: one instruction, and from references of
-// this size on an error of a 2^-8 th and more of a factor of 2 (at 2^27, of more than fp16 numbers have room for).  There the product is rounded as the reference was.
-// (bfloat16 alone: float32 queries take all of the scale but a power of two, by which products are exact.)
-constexpr float kCoarse = 65536.0f;
-
 struct AttendArgs {
     KvCall kv;
     HeadRows q;

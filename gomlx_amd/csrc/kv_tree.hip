@@ -17,7 +17,7 @@ namespace gq {
 
 namespace {
 
-constexpr int kMostTreeWorkgroups = 2048;
+constexpr int kLeastShare = 4;  // tiles of a workgroup, at least: one a wavefront
 
 struct TreeArgs {
     KvCall kv;
@@ -27,8 +27,7 @@ struct TreeArgs {
     const int32_t *tree;    // [rows, words]
     int words;
     void *out;              // [rows, heads, D]
-    float *part, *part_ml;  // of workgroups whose unit has several: sums [rows, D], (reference, sum) [rows, 2]
-    int workgroups;         // that all units together are cut into, about
+    float *part, *part_ml;  // of units that several workgroups work on: sums [workgroups, 2, rows, D], (reference, sum) [workgroups, 2, rows, 2]
     int blocks, rows;       // row blocks of a sequence and rows of a block, at most
     int2 *pieces;           // per unit: the first workgroup that works on it, and how many do
 };
@@ -46,50 +45,56 @@ __device__ __forceinline__ int tree_tiles(const TreeArgs &a, const KvSeq &s) {
     return s.news ? max(1, ((hi + 31) >> 5) - (lo >> 5)) : 0;
 }
 
-// Pieces of one length, a multiple of the wavefronts, of which all units together have about a.workgroups; the lengths are known on the device only, so that every
-// wavefront finds its place by a sum over them, 64 sequences at a time, one a lane.  (All tiles together: less than 2^31.)
-struct TreePiece {
-    int b, h, block, nth;  // b < 0: there is none
-    int share, tiles;      // tiles of a piece, of the unit
+// The tiles of all units stand in one line, and every workgroup takes the same number of them: the end of a unit, perhaps some whole ones, the beginning of another.  (Pieces
+// of units, one a workgroup, take as long as the longest: 32 sequences of 2048 to 8192 tokens, 16 nodes, 104 us for 66.)  The lengths are known on the device only, so that every wavefront finds
+// its place by a sum over them, 64 sequences at a time, one a lane.  (All tiles together: less than 2^31.)
+struct TreePlace {
+    int b, unit, tile;  // sequence; of its units; tile of the unit
+    int left, share;    // tiles of the workgroup; b < 0: it has none
     KvSeq seq;
-    __device__ __forceinline__ int pieces() const { return (tiles + share - 1) / share; }
+    // (the same for the whole wavefront: in scalar registers)
+    __device__ __forceinline__ void uniform() {
+        for (int *v : {&b, &unit, &tile, &left, &share, &seq.length, &seq.news, &seq.row0, &seq.first}) *v = __builtin_amdgcn_readfirstlane(*v);
+    }
 };
-__device__ __forceinline__ TreePiece tree_piece_of(const TreeArgs &a, int index, int block_rows) {
+__device__ __forceinline__ TreePlace tree_place_of(const TreeArgs &a, int index, int workgroups, int block_rows) {
     const int lane = (int)threadIdx.x & 63, seqs = a.kv.seqs, heads = a.kv.kv_heads;
-    TreePiece p;
+    TreePlace p;
     p.b = -1;
     KvSeq mine{};
-    int tiles = 0, units = 0, total = 0;
-    for (int base = (seqs - 1) & ~63; base >= 0; base -= 64) {  // (the first 64 last: they stay)
+    int each = 0, units = 0, total = 0, wide = 0;  // tiles of a unit of the lane's sequence, and such units; of all; with every unit's rounded up to the least share
+    const auto up = [](int n) { return (n + kLeastShare - 1) / kLeastShare * kLeastShare; };
+    const auto look = [&](int base) {
         mine = KvSeq{};
         if (base + lane < seqs) mine = kv_seq(a.kv, base + lane);
-        tiles = tree_tiles(a, mine);
+        each = tree_tiles(a, mine);
         units = blocks_of(a, mine, block_rows) * heads;
-        total += __builtin_amdgcn_readlane(lane_scan(tiles * units), 63);
+    };
+    for (int base = (seqs - 1) & ~63; base >= 0; base -= 64) {  // (the first 64 last: they stay)
+        look(base);
+        total += __builtin_amdgcn_readlane(lane_scan(each * units), 63);
+        wide += min(1 << 24, __builtin_amdgcn_readlane(lane_scan(min(1 << 18, up(each) * units)), 63));  // (so many do not fit)
     }
-    const int least = (total + a.workgroups - 1) / a.workgroups;
-    p.share = max(1, (least + kSplitWaves - 1) / kSplitWaves) * kSplitWaves;
-    int front = 0;  // pieces in front
+    // Where the workgroups are more than enough none works on two units.
+    const bool apart = wide <= workgroups * kLeastShare;
+    p.share = apart ? kLeastShare : (total + workgroups - 1) / workgroups;
+    if (apart) total = wide;
+    const int at = index * p.share;
+    if (index > (total - 1) / p.share) return p;
+    p.left = min(p.share, total - at);
+    int front = 0;
     for (int base = 0; base < seqs; base += 64) {
-        if (base) {
-            mine = KvSeq{};
-            if (base + lane < seqs) mine = kv_seq(a.kv, base + lane);
-            tiles = tree_tiles(a, mine);
-            units = blocks_of(a, mine, block_rows) * heads;
-        }
-        const int each = (tiles + p.share - 1) / p.share, upto = lane_scan(each * units);
-        const uint64_t past = __ballot(front + upto > index);
+        if (base) look(base);
+        const int tiles = (apart ? up(each) : each) * units, upto = lane_scan(tiles);
+        const uint64_t past = __ballot(front + upto > at);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             p.b = base + l;
             p.seq = seq_of_lane(mine, l);
-            p.tiles = __builtin_amdgcn_readlane(tiles, l);
-            const int all = __builtin_amdgcn_readlane(each * units, l), in = index - (front + __builtin_amdgcn_readlane(upto, l) - all);
-            const int blocks = blocks_of(a, p.seq, block_rows), per_head = all / heads;
-            p.h = in / per_head;
-            const int rest = in - p.h * per_head;
-            p.nth = rest / blocks;
-            p.block = rest - p.nth * blocks;  // (blocks of one piece of the tokens are neighbours)
+            const int in = at - (front + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l)), own = __builtin_amdgcn_readlane(each, l), line = apart ? up(own) : own;
+            p.unit = in / line;
+            p.tile = in - p.unit * line;
+            if (apart) p.left = min(p.left, own - p.tile);
             break;
         }
         front += __builtin_amdgcn_readlane(upto, 63);
@@ -97,29 +102,22 @@ __device__ __forceinline__ TreePiece tree_piece_of(const TreeArgs &a, int index,
     return p;
 }
 
-// What a row sees: context tokens from `lo` on, and from there the tokens of the tree whose bit is set.
-struct Sight { int lo; const int32_t *mask; };
-__device__ __forceinline__ Sight sight_of(const TreeArgs &a, const KvSeq &s, int node) {
-    Sight v;
-    v.mask = a.tree + (int64_t)(s.row0 + node) * a.words;
-    v.lo = 0;
-    if (a.window) {
-        const int words = (s.news + 31) >> 5;
-        const auto word = [&](int w) { return (uint32_t)v.mask[w] & (s.news - 32 * w < 32 ? (1u << (s.news - 32 * w)) - 1u : 0xFFFFFFFFu); };  // (bits behind the last node are none)
-        int left = a.window;
-        for (int w = words - 1; w >= 0; w--) {
-            uint32_t bits = word(w);
-            const int n = __popc(bits);
-            if (n >= left) {  // the last `left` of these, and nothing in front
-                for (int drop = n - left; drop > 0; drop--) bits &= bits - 1;
-                v.lo = s.first + 32 * w + __ffs((int)bits) - 1;
-                return v;
-            }
-            left -= n;
+// What a row sees: tokens of the context from this one on, and from there on those of the tree whose bit is set.
+__device__ __forceinline__ int sight_of(const TreeArgs &a, const KvSeq &s, int node) {
+    if (!a.window) return 0;
+    const int32_t *mask = a.tree + (int64_t)(s.row0 + node) * a.words;
+    int left = a.window;
+    for (int w = ((s.news + 31) >> 5) - 1; w >= 0; w--) {
+        uint32_t bits = (uint32_t)mask[w];
+        if (s.news - 32 * w < 32) bits &= (1u << (s.news - 32 * w)) - 1u;  // (those behind the last node are none)
+        const int n = __popc(bits);
+        if (n >= left) {  // the last `left` of these, and nothing in front
+            for (int drop = n - left; drop > 0; drop--) bits &= bits - 1;
+            return s.first + 32 * w + __ffs((int)bits) - 1;
         }
-        v.lo = s.first - left;
+        left -= n;
     }
-    return v;
+    return s.first - left;
 }
 // eight bits of a row's mask from token `at` of the tree on (nothing is looked up outside its words)
 __device__ __forceinline__ uint32_t mask_bits(const int32_t *mask, int words, int at) {
@@ -131,7 +129,8 @@ __device__ __forceinline__ uint32_t mask_bits(const int32_t *mask, int words, in
 template <int D, bool BF16, int RG> struct TreeLds {
     static constexpr int kOperands = RG * (D / 32) * 1024, kQueries = kOperands * (BF16 ? 1 : 2);  // bytes
     static constexpr int kRing = kSplitWaves * kSplitSlots * SplitLds<D>::kSlot;
-    static constexpr int kSums = kSplitWaves * 16 * (D + 4) * 4;
+    static constexpr int kJoin = RG < 256 / D ? RG : D == 256 ? (RG < 2 ? RG : 2) : 256 / D;  // groups of sixteen rows whose results meet at a time
+    static constexpr int kSums = kSplitWaves * 16 * kJoin * (D + 4) * 4;
     static constexpr int kBytes = (kQueries + kRing > kSums ? kQueries + kRing : kSums);
 };
 
@@ -142,276 +141,363 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 1 : 2) void kv_tree_ke
     typedef TreeLds<D, BF16, RG> Lds;
     __shared__ __align__(16) uint8_t lds[Lds::kBytes];
     __shared__ float refs[kSplitWaves][ROWS], totals[kSplitWaves][ROWS], scales[ROWS];
-    __shared__ int lows[ROWS];
+    __shared__ float factors[kSplitWaves][ROWS];  // what a wavefront multiplies its scores by as it takes their exponentials
+    __shared__ int lows[ROWS], mask_rows[ROWS];  // (read where a tile needs masks: in registers they would take what the results need)
     const KvCall &kv = a.kv;
     const int tid = (int)threadIdx.x, lane = tid & 63, r = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const TreePiece piece = tree_piece_of(a, (int)blockIdx.x, ROWS);
-    if (piece.b < 0) return;
-    const int b = piece.b, h = piece.h;
-    const KvSeq &seq = piece.seq;
-    const int row_first = piece.block * ROWS, rows = min(ROWS, seq.news * a.group - row_first);
-    int lo, hi;
-    tokens_of(a, seq, lo, hi);
-    const int tile0 = (lo >> 5) + piece.nth * piece.share, tile1 = min((lo >> 5) + min((piece.nth + 1) * piece.share, piece.tiles), (hi + 31) >> 5);
+    TreePlace at = tree_place_of(a, (int)blockIdx.x, (int)gridDim.x, ROWS);
+    if (at.b < 0) return;
     const Unpack unpack;
-
-    TileWalk<KvTile<D>::kBytes, kSplitWaves> walk(kv, b, h, tile0 + wave, tile1);
     uint8_t *ring = lds + Lds::kQueries + wave * kSplitSlots * SplitLds<D>::kSlot;
     const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)ring);
-    const uint8_t *mem = walk.next();
-    if (mem) fetch_tile<D>(ring_at, mem);
-    // the rows' queries, sixteen rows a wavefront at a time
     h8 *operands = reinterpret_cast<h8 *>(lds);
+
 #pragma unroll 1
-    for (int m = wave; m < RG; m += kSplitWaves) {
-        const int idx = row_first + 16 * m + r;
-        const bool live = 16 * m + r < rows;
-        const int node = live ? idx / a.group : 0, head = h * a.group + (live ? idx - node * a.group : 0);
-        h8 qh[G], ql[TWO ? G : 1];
-        float to_log2;
-        load_queries<D, 16, BF16, TWO>(a.q, (int64_t)(seq.row0 + node) * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, to_log2);
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-            operands[(m * G + g) * 64 + lane] = qh[g];
-            if constexpr (TWO) operands[Lds::kOperands / 16 + (m * G + g) * 64 + lane] = ql[g];
-        }
-        if (j == 0) {
-            scales[16 * m + r] = to_log2;
-            lows[16 * m + r] = live ? sight_of(a, seq, node).lo : 0;
-        }
-    }
-    __syncthreads();
-    float to_log2[RG];
-    int all_lo = 0;  // from here on every row sees the context
-#pragma unroll
-    for (int m = 0; m < RG; m++) {
-        to_log2[m] = scales[16 * m + r];
-        all_lo = max(all_lo, lows[16 * m + r]);
-    }
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) all_lo = max(all_lo, __shfl_xor(all_lo, m));
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    for (;;) {
+        at.uniform();
+        const KvSeq seq = at.seq;
+        const int blocks = blocks_of(a, seq, ROWS), h = at.unit / blocks, block = at.unit - h * blocks;
+        const int row_first = block * ROWS, rows = min(ROWS, seq.news * a.group - row_first);
+        int lo, hi;
+        tokens_of(a, seq, lo, hi);
+        const int tiles = tree_tiles(a, seq), here = min(at.left, tiles - at.tile);
+        const int tile0 = (lo >> 5) + at.tile, tile1 = min(tile0 + here, (hi + 31) >> 5);
 
-    f4 o[RG][W];
-    float ref[RG], total[RG];  // the rows' references, and the lane's share of their sums
+        TileWalk<KvTile<D>::kBytes, kSplitWaves> walk(kv, at.b, h, tile0 + wave, tile1);
+        const uint8_t *mem = walk.next();
+        if (mem) fetch_tile<D>(ring_at, mem);
+        // the rows' queries, sixteen rows a wavefront at a time
+#pragma unroll 1
+        for (int m = wave; m < RG; m += kSplitWaves) {
+            const int idx = row_first + 16 * m + r;
+            const bool live = 16 * m + r < rows;
+            const int node = live ? idx / a.group : 0, head = h * a.group + (live ? idx - node * a.group : 0);
+            h8 qh[G], ql[TWO ? G : 1];
+            float to_log2;
+            load_queries<D, 16, BF16, TWO>(a.q, (int64_t)(seq.row0 + node) * a.q.row + head * a.q.head, live, a.wide, a.scale_log2, qh, ql, to_log2);
+            to_log2 = to_log2 < 0x1p-122f ? 0x1p-122f : to_log2;  // (not 0, so that its product with -infinity stays that; a scale of NaN stays one)
 #pragma unroll
-    for (int m = 0; m < RG; m++) {
-        ref[m] = kNegInf;
-        total[m] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; w++) o[m][w] = f4{0.f, 0.f, 0.f, 0.f};
-    }
-
-    int turn = 0;
-    for (int tile = tile0 + wave; tile < tile1; tile += kSplitWaves) {
-        const uint8_t *mem_next = walk.next();
-        if (mem_next) {
-            fetch_tile<D>(ring_at + (uint32_t)(turn ^ 1) * SplitLds<D>::kSlot, mem_next);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(SplitLds<D>::kLoads) : "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            for (int g = 0; g < G; g++) {
+                operands[(m * G + g) * 64 + lane] = qh[g];
+                if constexpr (TWO) operands[Lds::kOperands / 16 + (m * G + g) * 64 + lane] = ql[g];
+            }
+            if (j == 0) {
+                scales[16 * m + r] = to_log2;
+                lows[16 * m + r] = live ? sight_of(a, seq, node) : 0;
+                mask_rows[16 * m + r] = live ? seq.row0 + node : -1;
+            }
         }
-        if (mem) {
-            const int t0 = tile * 32;
-            float s[RG][8];
-            {
-                KeyWords<D> k;
-                k.load(ring + turn * SplitLds<D>::kSlot);
-                f4 acc[RG][2];
+        __syncthreads();
+        int all_lo = 0;  // from here on every row sees the context
 #pragma unroll
-                for (int m = 0; m < RG; m++) acc[m][0] = acc[m][1] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int m = 0; m < RG; m++) {
+            factors[wave][16 * m + r] = scales[16 * m + r];
+            all_lo = max(all_lo, lows[16 * m + r]);
+        }
+        if (a.window) {
 #pragma unroll
-                for (int g = 0; g < G; g++) {
-                    const h8 k0 = k.operand(unpack, 0, g), k1 = k.operand(unpack, 1, g);
+            for (int m = 1; m < 16; m <<= 1) all_lo = max(all_lo, __shfl_xor(all_lo, m));
+        }
+        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+
+        f4 o[RG][W];
+        float ref[RG], total[RG];  // the rows' references, and the lane's share of their sums
+        bool coarse = false;       // one of the references is large: scores are multiplied by their scale first, and the factors are 1
+#pragma unroll
+        for (int m = 0; m < RG; m++) {
+            ref[m] = kNegInf;
+            total[m] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; w++) o[m][w] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+
+        int turn = 0;
+        for (int tile = tile0 + wave; tile < tile1; tile += kSplitWaves) {
+            const uint8_t *mem_next = walk.next();
+            if (mem_next) {
+                fetch_tile<D>(ring_at + (uint32_t)(turn ^ 1) * SplitLds<D>::kSlot, mem_next);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(SplitLds<D>::kLoads) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            if (mem) {
+                const int t0 = tile * 32;
+                f4 s[RG][2];  // scores as the products leave them: what they are multiplied by is not negative
+                {
+                    // The rows' operands are read three steps (of sixteen rows and a group) ahead, and the next group's codes widened between the matrix instructions.
+                    constexpr int AHEAD = TWO ? 1 : 3, STEPS = G * RG;
+                    h8 q[AHEAD + 1], rest[TWO ? 2 : 1], keys[2][2];
+                    const auto read = [&](int i) __attribute__((always_inline)) {
+                        q[i % (AHEAD + 1)] = operands[(i % RG * G + i / RG) * 64 + lane];
+                        if constexpr (TWO) rest[i % 2] = operands[Lds::kOperands / 16 + (i % RG * G + i / RG) * 64 + lane];
+                    };
+                    KeyWords<D> k;
+                    k.load(ring + turn * SplitLds<D>::kSlot);
+#pragma unroll
+                    for (int i = 0; i < AHEAD; i++)
+                        if (i < STEPS) read(i);
+                    keys[0][0] = k.operand(unpack, 0, 0);
+                    keys[0][1] = k.operand(unpack, 1, 0);
+#pragma unroll
+                    for (int m = 0; m < RG; m++) s[m][0] = s[m][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < STEPS; i++) {
+                        const int g = i / RG, m = i % RG;
+                        __builtin_amdgcn_sched_barrier(0);  // (the order as written: left alone the compiler widens everything first and reads an operand as it needs it)
+                        if (i + AHEAD < STEPS) read(i + AHEAD);
+                        if (g + 1 < G) {
+                            if (m == 0) keys[(g + 1) & 1][0] = k.operand(unpack, 0, g + 1);
+                            if (m == RG / 2) keys[(g + 1) & 1][1] = k.operand(unpack, 1, g + 1);
+                        }
+                        s[m][0] = mfma(keys[g & 1][0], q[i % (AHEAD + 1)], s[m][0]);
+                        s[m][1] = mfma(keys[g & 1][1], q[i % (AHEAD + 1)], s[m][1]);
+                        if constexpr (TWO) {
+                            s[m][0] = mfma(keys[g & 1][0], rest[i % 2], s[m][0]);
+                            s[m][1] = mfma(keys[g & 1][1], rest[i % 2], s[m][1]);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (t0 < all_lo || t0 + 32 > seq.first) {
 #pragma unroll
                     for (int m = 0; m < RG; m++) {
-                        const h8 q = operands[(m * G + g) * 64 + lane];
-                        acc[m][0] = mfma(k0, q, acc[m][0]);
-                        acc[m][1] = mfma(k1, q, acc[m][1]);
-                        if constexpr (TWO) {
-                            const h8 rest = operands[Lds::kOperands / 16 + (m * G + g) * 64 + lane];
-                            acc[m][0] = mfma(k0, rest, acc[m][0]);
-                            acc[m][1] = mfma(k1, rest, acc[m][1]);
+                        const int row = mask_rows[16 * m + r], from = row < 0 ? hi : lows[16 * m + r], first = t0 + 8 * j;
+                        uint32_t bits = row < 0 ? 0u : mask_bits(a.tree + (int64_t)row * a.words, a.words, first - seq.first);
+                        // bit e: token first + e is seen
+                        const int context = seq.first - first, behind = from - first, end = hi - first;
+                        bits |= context >= 8 ? 255u : context > 0 ? (1u << context) - 1u : 0u;
+                        bits &= behind >= 8 ? 0u : behind > 0 ? 255u << behind : 255u;
+                        bits &= end >= 8 ? 255u : end > 0 ? (1u << end) - 1u : 0u;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) s[m][e >> 2][e & 3] = bits >> e & 1u ? s[m][e >> 2][e & 3] : kNegInf;
+                    }
+                }
+                if (!TWO && coarse) {
+#pragma unroll
+                    for (int m = 0; m < RG; m++) { s[m][0] *= scales[16 * m + r]; s[m][1] *= scales[16 * m + r]; }
+                }
+                float by[RG], most[RG];
+                bool beyond = false;
+#pragma unroll
+                for (int m = 0; m < RG; m++) by[m] = factors[wave][16 * m + r];
+#pragma unroll
+                for (int m = 0; m < RG; m++) {
+                    // (the maximum that takes a NaN, which makes the row one anyway: the other would first have to make sure of every score's kind)
+                    const auto larger = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };
+                    most[m] = larger(larger(larger(s[m][0].x, s[m][0].y), larger(s[m][0].z, s[m][0].w)), larger(larger(s[m][1].x, s[m][1].y), larger(s[m][1].z, s[m][1].w)));
+                    most[m] *= by[m];
+                    beyond = beyond || passes<D, TWO>(most[m], ref[m]);
+                }
+                if (__any(beyond)) {  // (the first score of a row among them: its reference is -infinity)
+                    bool large = false;
+#pragma unroll
+                    for (int m = 0; m < RG; m++) {
+                        if (!__any(passes<D, TWO>(most[m], ref[m]))) continue;
+                        most[m] = fmaxf(most[m], __shfl_xor(most[m], 16));
+                        most[m] = fmaxf(most[m], __shfl_xor(most[m], 32));
+                        const float next = fmaxf(ref[m], reference<D, TWO>(most[m]));
+                        const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref[m] - next);
+                        ref[m] = next;
+                        large = large || (fabsf(next) >= kCoarse && next != kNegInf);
+                        total[m] *= shrink;
+#pragma unroll
+                        for (int w = 0; w < W; w++) o[m][w] *= shrink;
+                    }
+                    if (!TWO && !coarse && __any(large)) {  // (this tile's scores too)
+                        coarse = true;
+#pragma unroll
+                        for (int m = 0; m < RG; m++) {
+                            s[m][0] *= scales[16 * m + r];
+                            s[m][1] *= scales[16 * m + r];
+                            factors[wave][16 * m + r] = by[m] = 1.0f;
                         }
                     }
                 }
-#pragma unroll
-                for (int m = 0; m < RG; m++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) s[m][e] = acc[m][e >> 2][e & 3] * to_log2[m];
-            }
-            if (t0 < all_lo || t0 + 32 > seq.first) {
+                h8 ph[RG], pl[TWO ? RG : 1];
 #pragma unroll
                 for (int m = 0; m < RG; m++) {
-                    const int idx = row_first + 16 * m + r;
-                    const bool live = 16 * m + r < rows;
-                    const int from = live ? lows[16 * m + r] : hi, at = t0 + 8 * j;
-                    const uint32_t bits = live ? mask_bits(a.tree + (int64_t)(seq.row0 + idx / a.group) * a.words, a.words, at - seq.first) : 0u;
+                    const float less = ref[m] == kNegInf ? 0.0f : -ref[m];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) s[m][e] = at + e >= from && at + e < hi && (at + e < seq.first || (bits >> e & 1u)) ? s[m][e] : kNegInf;
+                    for (int e = 0; e < 8; e += 2) {
+                        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][e & 3], by[m], less)), p1 = __builtin_amdgcn_exp2f(fmaf(s[m][e >> 2][(e & 3) + 1], by[m], less));
+                        ph[m][e] = (_Float16)p0;
+                        ph[m][e + 1] = (_Float16)p1;
+                        if constexpr (TWO) {
+                            total[m] += p0;
+                            total[m] += p1;
+                            pl[m][e] = (_Float16)(p0 - (float)ph[m][e]);
+                            pl[m][e + 1] = (_Float16)(p1 - (float)ph[m][e + 1]);
+                        } else {  // the weights as they are used, two in one instruction
+                            const h2 pair = {ph[m][e], ph[m][e + 1]}, ones = {(_Float16)1.0f, (_Float16)1.0f};
+                            total[m] = __builtin_amdgcn_fdot2(pair, ones, total[m], false);
+                        }
+                    }
+                }
+                ValueWords<D> v;
+                v.load(ring + turn * SplitLds<D>::kSlot);
+                h8 x[2];
+                x[0] = v.operand(unpack, 0);
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (w + 1 < W) x[(w + 1) & 1] = v.operand(unpack, w + 1);
+#pragma unroll
+                    for (int m = 0; m < RG; m++) {
+                        o[m][w] = mfma(x[w & 1], ph[m], o[m][w]);
+                        if constexpr (TWO) o[m][w] = mfma(x[w & 1], pl[m], o[m][w]);
+                    }
                 }
             }
-            float most[RG];
-            bool beyond = false;
-#pragma unroll
-            for (int m = 0; m < RG; m++) {
-                most[m] = fmaxf(fmaxf(fmaxf(s[m][0], s[m][1]), fmaxf(s[m][2], s[m][3])), fmaxf(fmaxf(s[m][4], s[m][5]), fmaxf(s[m][6], s[m][7])));
-                beyond = beyond || passes<D, TWO>(most[m], ref[m]);
-            }
-            if (__any(beyond)) {  // (the first score of a row among them: its reference is -infinity)
-#pragma unroll
-                for (int m = 0; m < RG; m++) {
-                    if (!__any(passes<D, TWO>(most[m], ref[m]))) continue;
-                    most[m] = fmaxf(most[m], __shfl_xor(most[m], 16));
-                    most[m] = fmaxf(most[m], __shfl_xor(most[m], 32));
-                    const float next = fmaxf(ref[m], reference<D, TWO>(most[m]));
-                    const float shrink = next == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ref[m] - next);
-                    ref[m] = next;
-                    total[m] *= shrink;
-#pragma unroll
-                    for (int w = 0; w < W; w++) o[m][w] *= shrink;
-                }
-            }
-            h8 ph[RG], pl[TWO ? RG : 1];
-#pragma unroll
-            for (int m = 0; m < RG; m++) {
-                const float less = ref[m] == kNegInf ? 0.0f : ref[m];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float p = __builtin_amdgcn_exp2f(s[m][e] - less);
-                    total[m] += p;
-                    ph[m][e] = (_Float16)p;
-                    if constexpr (TWO) pl[m][e] = (_Float16)(p - (float)ph[m][e]);
-                }
-            }
-            ValueWords<D> v;
-            v.load(ring + turn * SplitLds<D>::kSlot);
-#pragma unroll
-            for (int w = 0; w < W; w++) {
-                const h8 x = v.operand(unpack, w);
-#pragma unroll
-                for (int m = 0; m < RG; m++) {
-                    o[m][w] = mfma(x, ph[m], o[m][w]);
-                    if constexpr (TWO) o[m][w] = mfma(x, pl[m], o[m][w]);
-                }
-            }
+            mem = mem_next;
+            turn ^= 1;
         }
-        mem = mem_next;
-        turn ^= 1;
-    }
 
-    // the wavefronts' results, sixteen rows at a time, in the place of queries and tiles
-    float(*sums)[16][D + 4] = reinterpret_cast<float(*)[16][D + 4]>(lds);
-    const int pieces = piece.pieces();
-    if (a.pieces && piece.nth == 0 && tid == 0) a.pieces[(b * kv.kv_heads + h) * a.blocks + piece.block] = make_int2((int)blockIdx.x, pieces);
+        // the wavefronts' results, a few groups of rows at a time, in the place of queries and tiles
+        constexpr int JOIN = Lds::kJoin;
+        int thread = tid;
+        asm volatile("" : "+v"(thread));  // (or what follows from it is made in front of all units, for registers that the tiles need)
+        const int in_row = thread & 15, in_four = (thread >> 4) & 3;
+        float(*sums)[16 * JOIN][D + 4] = reinterpret_cast<float(*)[16 * JOIN][D + 4]>(lds);
+        const bool begins = at.tile == 0, whole = begins && here == tiles;
+        if (a.pieces && begins && tid == 0) a.pieces[(at.b * kv.kv_heads + h) * a.blocks + block] = make_int2((int)blockIdx.x, 1 + (tiles - here + at.share - 1) / at.share);
 #pragma unroll
-    for (int m = 0; m < RG; m++) {
-        total[m] += __shfl_xor(total[m], 16);
-        total[m] += __shfl_xor(total[m], 32);
-        if (j == 0) {
-            refs[wave][16 * m + r] = ref[m];
-            totals[wave][16 * m + r] = total[m];
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < RG; m++) {
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < W; w++) *reinterpret_cast<f4 *>(&sums[wave][r][16 * w + 4 * j]) = o[m][w];
-        __syncthreads();
-        const int here = min(16, rows - 16 * m);
-        for (int i = tid; i < here * (D / 4); i += 64 * kSplitWaves) {
-            const int in = i / (D / 4), rr = 16 * m + in, d = (i - in * (D / 4)) * 4;
-            float top = kNegInf;
-#pragma unroll
-            for (int w = 0; w < kSplitWaves; w++) top = fmaxf(top, refs[w][rr]);
-            f4 sum = {0.f, 0.f, 0.f, 0.f};
-            float all = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kSplitWaves; w++) {
-                const float f = refs[w][rr] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(refs[w][rr] - top);
-                // (a wavefront without a reference has seen no number: its sum is zero, or NaN)
-                all += refs[w][rr] == kNegInf ? totals[w][rr] : totals[w][rr] * f;
-                sum += *reinterpret_cast<const f4 *>(&sums[w][in][d]) * f;
+        for (int m = 0; m < RG; m++) {
+            total[m] += __shfl_xor(total[m], 16);
+            total[m] += __shfl_xor(total[m], 32);
+            if (j == 0) {
+                refs[wave][16 * m + r] = ref[m];
+                totals[wave][16 * m + r] = total[m];
             }
-            if (pieces == 1) {
-                const int node = (row_first + rr) / a.group;
-                const int64_t out = (int64_t)(seq.row0 + node) * a.heads + h * a.group + (row_first + rr - node * a.group);
-                store_result<BF16>(a.out, out * D + d, sum, all);
-            } else {
-                const int64_t line = (int64_t)blockIdx.x * a.rows + rr;
-                *reinterpret_cast<f4 *>(a.part + line * D + d) = sum;
-                if (d == 0) {
-                    a.part_ml[line * 2] = top;
-                    a.part_ml[line * 2 + 1] = all;
+        }
+#pragma unroll
+        for (int m0 = 0; m0 < RG; m0 += JOIN) {
+            __syncthreads();
+            if (m0 == 0 && thread < ROWS) {  // what each wavefront's sums are multiplied by; the row's reference and sum
+                float top = kNegInf, all = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kSplitWaves; w++) top = fmaxf(top, refs[w][thread]);
+#pragma unroll
+                for (int w = 0; w < kSplitWaves; w++) {
+                    const float by = refs[w][thread], f = by == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(by - top);
+                    // (a wavefront without a reference has seen no number: its sum is zero, or NaN)
+                    all += by == kNegInf ? totals[w][thread] : totals[w][thread] * f;
+                    factors[w][thread] = f;
+                }
+                refs[0][thread] = top;
+                totals[0][thread] = all;
+            }
+#pragma unroll
+            for (int m = m0; m < m0 + JOIN && m < RG; m++)
+#pragma unroll
+                for (int w = 0; w < W; w++) *reinterpret_cast<f4 *>(&sums[wave][16 * (m - m0) + in_row][16 * w + 4 * in_four]) = o[m][w];
+            __syncthreads();
+            const int count = min(16 * JOIN, rows - 16 * m0);
+            for (int i = thread; i < count * (D / 4); i += 64 * kSplitWaves) {
+                const int in = i / (D / 4), rr = 16 * m0 + in, d = (i - in * (D / 4)) * 4;
+                f4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < kSplitWaves; w++) sum += *reinterpret_cast<const f4 *>(&sums[w][in][d]) * factors[w][rr];
+                if (whole) {
+                    const int node = (row_first + rr) / a.group;
+                    const int64_t out = (int64_t)(seq.row0 + node) * a.heads + h * a.group + (row_first + rr - node * a.group);
+                    store_result<BF16>(a.out, out * D + d, sum, totals[0][rr]);
+                } else {
+                    const int64_t line = ((int64_t)blockIdx.x * 2 + begins) * a.rows + rr;
+                    *reinterpret_cast<f4 *>(a.part + line * D + d) = sum;
+                    if (d == 0) {
+                        a.part_ml[line * 2] = refs[0][rr];
+                        a.part_ml[line * 2 + 1] = totals[0][rr];
+                    }
                 }
             }
         }
+        at.left -= here;
+        if (at.left <= 0) break;
+        // the next unit, of the next sequence that has one where this was the last
+        at.tile = 0;
+        if (++at.unit == blocks * kv.kv_heads) {
+            at.unit = 0;
+            do {
+                at.seq = kv_seq(kv, ++at.b);
+            } while (at.seq.news == 0);  // (tiles are left: there is one)
+        }
+        __syncthreads();
     }
 }
 
-// Joins the pieces of the units that more than one workgroup has worked on: one workgroup per unit and row.
-template <int D, bool BF16>
+// Joins the pieces of the units that more than one workgroup has worked on: SHARES threads for four values of a row.
+template <int D, bool BF16, int SHARES>
 __global__ __launch_bounds__(256) void kv_tree_join_kernel(const TreeArgs a, int block_rows) {
-    constexpr int L = D / 4, S = 256 / L;  // lanes of a row's values, and the shares into which the pieces are divided
-    __shared__ f4 sums[S][L];
-    __shared__ float factors[kMostTreeWorkgroups], tops[4], alls[4];
-    const int block = (int)blockIdx.x / a.rows, rr = (int)blockIdx.x - block * a.rows, h = (int)blockIdx.y, b = (int)blockIdx.z, tid = (int)threadIdx.x;
-    const KvSeq seq = kv_seq(a.kv, b);
-    if (block * block_rows + rr >= seq.news * a.group) return;  // (without rows nobody has written the unit's pieces)
+    constexpr int L = D / 4, R = 256 / L / SHARES;  // lanes of a row's values; rows of a workgroup
+    __shared__ f4 sums[256];
+    __shared__ float tops[256 / L], alls[256 / L];
+    const int per_block = (a.rows + R - 1) / R, block = (int)blockIdx.x / per_block, h = (int)blockIdx.y, b = (int)blockIdx.z, tid = (int)threadIdx.x;
+    const int rr = ((int)blockIdx.x - block * per_block) * R + tid / L / SHARES, share = tid / L % SHARES, d = tid % L * 4;
     const int unit = (b * a.kv.kv_heads + h) * a.blocks + block;
+    const KvSeq seq = kv_seq(a.kv, b);
+    if (block * block_rows >= seq.news * a.group) return;  // (without rows nobody has written the unit's pieces)
     const int2 piece = a.pieces[unit];
-    const int first = piece.x, pieces = piece.y, stride = blocks_of(a, seq, block_rows);  // (between the pieces of a unit lie its neighbours')
+    const int first = piece.x, pieces = piece.y;
     if (pieces == 1) return;
-    const auto line = [&](int i) { return (int64_t)(first + i * stride) * a.rows + rr; };
-    float top = kNegInf;
-    for (int i = tid; i < pieces; i += 256) top = fmaxf(top, a.part_ml[line(i) * 2]);
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-    if ((tid & 63) == 0) tops[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    float all = 0.0f;
-    for (int i = tid; i < pieces; i += 256) {
-        const float ref = a.part_ml[line(i) * 2], t = a.part_ml[line(i) * 2 + 1];
-        const float f = ref == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
-        factors[i] = f;
-        all += ref == kNegInf ? t : t * f;
-    }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) all += __shfl_xor(all, m);
-    if ((tid & 63) == 0) alls[tid >> 6] = all;
-    __syncthreads();
-    all = (alls[0] + alls[1]) + (alls[2] + alls[3]);
-    const int l = tid % L, part = tid / L;
+    const bool live = rr < a.rows && block * block_rows + rr < seq.news * a.group;
+    const auto line = [&](int i) { return ((int64_t)(first + i) * 2 + (i == 0)) * a.rows + (live ? rr : 0); };
+    float top = kNegInf, all = 0.0f;
     f4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = part; i < pieces; i += S) sum += *reinterpret_cast<const f4 *>(a.part + line(i) * D + l * 4) * factors[i];
-    sums[part][l] = sum;
-    __syncthreads();
-    if (part) return;
-    sum = sums[0][l];
-    for (int i = 1; i < S; i++) sum += sums[i][l];
+    for (int i = share; i < pieces; i += SHARES) top = fmaxf(top, a.part_ml[line(i) * 2]);
+#pragma unroll 4
+    for (int i = share; i < pieces; i += SHARES) {
+        const float ref = a.part_ml[line(i) * 2], t = a.part_ml[line(i) * 2 + 1];
+        const float f = ref == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
+        all += ref == kNegInf ? t : t * f;
+        sum += *reinterpret_cast<const f4 *>(a.part + line(i) * D + d) * f;
+    }
+    if constexpr (SHARES > 1) {
+        sums[tid] = sum;
+        if (d == 0) { tops[tid / L] = top; alls[tid / L] = all; }
+        __syncthreads();
+        if (share) return;
+        const int mine = tid / L;
+#pragma unroll
+        for (int i = 0; i < SHARES; i++) top = fmaxf(top, tops[mine + i]);
+        sum = f4{0.f, 0.f, 0.f, 0.f};
+        all = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SHARES; i++) {
+            const float f = tops[mine + i] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(tops[mine + i] - top);
+            all += tops[mine + i] == kNegInf ? alls[mine + i] : alls[mine + i] * f;
+            sum += sums[tid + i * L] * f;
+        }
+    }
+    if (!live) return;
     const int node = (block * block_rows + rr) / a.group;
     const int64_t out = (int64_t)(seq.row0 + node) * a.heads + h * a.group + (block * block_rows + rr - node * a.group);
-    store_result<BF16>(a.out, out * D + l * 4, sum, all);
+    store_result<BF16>(a.out, out * D + d, sum, all);
 }
 
-template <int D, bool BF16, int RG> int tree_attend(const TreeArgs &a, hipStream_t s) {
-    const KvCall &kv = a.kv;
-    const unsigned grid = (unsigned)(a.workgroups + (int64_t)kv.seqs * kv.kv_heads * a.blocks);  // (a unit's last piece may be short)
-    if (int rc = launch(kv_tree_kernel<D, BF16, RG>, dim3(grid), dim3(64 * kSplitWaves), 0, s, a)) return rc;
-    if (!a.pieces) return GQ_OK;
-    return launch(kv_tree_join_kernel<D, BF16>, dim3((unsigned)(a.blocks * a.rows), (unsigned)kv.kv_heads, (unsigned)kv.seqs), dim3(256), 0, s, a, 16 * RG);
+template <int D, bool BF16, int SHARES> int tree_join(const TreeArgs &a, int block_rows, hipStream_t s) {
+    constexpr int R = 1024 / D / SHARES;
+    const dim3 grid((unsigned)(a.blocks * ((a.rows + R - 1) / R)), (unsigned)a.kv.kv_heads, (unsigned)a.kv.seqs);
+    return launch(kv_tree_join_kernel<D, BF16, SHARES>, grid, dim3(256), 0, s, a, block_rows);
 }
-template <int D, bool BF16> int tree_attend(const TreeArgs &a, int row_groups, hipStream_t s) {
+template <int D, bool BF16, int RG> int tree_attend(const TreeArgs &a, int workgroups, hipStream_t s) {
+    if (int rc = launch(kv_tree_kernel<D, BF16, RG>, dim3((unsigned)workgroups), dim3(64 * kSplitWaves), 0, s, a)) return rc;
+    if (!a.pieces) return GQ_OK;
+    // (with many pieces a unit the threads of a row share them)
+    const int64_t units = (int64_t)a.kv.seqs * a.kv.kv_heads * a.blocks;
+    constexpr int most = 1024 / D;
+    return workgroups > 8 * units ? tree_join<D, BF16, most>(a, 16 * RG, s) : tree_join<D, BF16, 1>(a, 16 * RG, s);
+}
+template <int D, bool BF16> int tree_attend(const TreeArgs &a, int row_groups, int workgroups, hipStream_t s) {
     switch (row_groups) {
-    case 1: return tree_attend<D, BF16, 1>(a, s);
-    case 2: return tree_attend<D, BF16, 2>(a, s);
+    case 1: return tree_attend<D, BF16, 1>(a, workgroups, s);
+    case 2: return tree_attend<D, BF16, 2>(a, workgroups, s);
+    case 3:
+        if constexpr (D < 256) return tree_attend<D, BF16, 3>(a, workgroups, s);
     default:
-        if constexpr (D == 256) return tree_attend<D, BF16, 2>(a, s);
-        else return tree_attend<D, BF16, 4>(a, s);
+        if constexpr (D == 256) return tree_attend<D, BF16, 2>(a, workgroups, s);
+        else return tree_attend<D, BF16, 4>(a, workgroups, s);
     }
 }
 
@@ -422,7 +508,7 @@ struct TreePlan { int row_groups, rows; int64_t blocks, tiles; };
 static TreePlan tree_plan(const KvCall &kv, int heads, int window) {
     TreePlan p;
     const int64_t most_rows = (int64_t)kv.max_new * (heads / kv.kv_heads), room = (int64_t)kv.max_pages * kv.page_tokens / 32;
-    p.row_groups = most_rows <= 16 ? 1 : most_rows <= 32 || kv.head_dim == 256 ? 2 : 4;
+    p.row_groups = (int)std::min<int64_t>((most_rows + 15) / 16, kv.head_dim == 256 ? 2 : 4);
     p.rows = (int)std::min<int64_t>(most_rows, 16 * p.row_groups);
     p.blocks = (most_rows + 16 * p.row_groups - 1) / (16 * p.row_groups);
     p.tiles = std::max<int64_t>(1, window ? std::min<int64_t>(room, ((int64_t)window + kv.max_new + 31) / 32 + 1) : room);
@@ -456,10 +542,11 @@ int launch_kv_tree_attention(const KvCall &kv, const HeadRows &q, int heads, flo
     a.rows = p.rows;
     a.blocks = (int)p.blocks;
     const int64_t tiles = p.tiles, units = (int64_t)kv.seqs * kv.kv_heads * a.blocks;
+    // (as many workgroups as run at a time)
     const int per_cu = kv.head_dim == 256 ? 1 : 2;
-    a.workgroups = (int)std::min<int64_t>(std::min(kMostTreeWorkgroups, device_cu_count() * per_cu), (units * tiles + kSplitWaves - 1) / kSplitWaves);
-    if (tiles > kSplitWaves) {
-        const size_t lines = (size_t)(a.workgroups + units) * a.rows;
+    const int workgroups = (int)std::min<int64_t>(device_cu_count() * per_cu, units * ((tiles + kLeastShare - 1) / kLeastShare));
+    if (tiles > 1) {
+        const size_t lines = (size_t)workgroups * 2 * a.rows;
         const auto up = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
         const size_t ml = up(lines * kv.head_dim * 4), pieces = ml + up(lines * 8), all = pieces + (size_t)units * 8;
         void *ws = nullptr;
@@ -470,9 +557,9 @@ int launch_kv_tree_attention(const KvCall &kv, const HeadRows &q, int heads, flo
         a.pieces = reinterpret_cast<int2 *>(at + pieces);
     }
     switch (kv.head_dim) {
-    case 64: return q.bf16 ? tree_attend<64, true>(a, p.row_groups, s) : tree_attend<64, false>(a, p.row_groups, s);
-    case 128: return q.bf16 ? tree_attend<128, true>(a, p.row_groups, s) : tree_attend<128, false>(a, p.row_groups, s);
-    default: return q.bf16 ? tree_attend<256, true>(a, p.row_groups, s) : tree_attend<256, false>(a, p.row_groups, s);
+    case 64: return q.bf16 ? tree_attend<64, true>(a, p.row_groups, workgroups, s) : tree_attend<64, false>(a, p.row_groups, workgroups, s);
+    case 128: return q.bf16 ? tree_attend<128, true>(a, p.row_groups, workgroups, s) : tree_attend<128, false>(a, p.row_groups, workgroups, s);
+    default: return q.bf16 ? tree_attend<256, true>(a, p.row_groups, workgroups, s) : tree_attend<256, false>(a, p.row_groups, workgroups, s);
     }
 }
 
