@@ -4,10 +4,12 @@
 //            with a window the last `window` of all these
 //     o_i  = sum_j P_ij v_j,  P_i = softmax(s_i);  a row that sees nothing gets zeros
 //
-// Every row of a sequence sees the same long context, so that a key head's (node, query head) pairs, 16 RG of them, go over the cache together: a wavefront widens a tile's
+// Every row of a sequence sees the same long context, so that a key head's (node, query head) pairs, up to 64 of them, go over the cache together: a wavefront widens a tile's
 // codes once, in registers, and contracts them with all of these rows (queries in LDS, as operands; results in registers).  Widening costs 208 vector instructions a
-// tile of 32 tokens at D = 128, every 16 rows 32 matrix instructions of 16 cycles (twice that in float32) and some 75 vector instructions for their weights: at 64 rows a tile's share of the
-// memory's rate and of the vector units' about meet.
+// tile of 32 tokens at D = 128, every 16 rows 16 matrix instructions of 16 cycles (in float32 32) and some 47 vector instructions, eight of them exponentials of four times the
+// usual length, for their weights.  These bound it, for next to matrix instructions little else is issued: at 64 rows some 2000 cycles of the one and 1000 of the other a
+// tile, 3100 as measured (two wavefronts a SIMD; one alone takes 3500).  us a call, D = 128, bfloat16, 8 key heads of 4 queries: 32 sequences of 2048 to 8192 tokens with 8
+// to 16 nodes each 79 (460 TFLOP/s, 2.5 TB/s of cache); 32 nodes over 131072 tokens 96 (715 TFLOP/s); 16 sequences of 2048 to 8192 tokens with 32 to 64 nodes 124 (580).
 #include "kv_attend.hpp"
 
 #include <algorithm>
@@ -46,7 +48,7 @@ __device__ __forceinline__ int tree_tiles(const TreeArgs &a, const KvSeq &s) {
 }
 
 // The tiles of all units stand in one line, and every workgroup takes the same number of them: the end of a unit, perhaps some whole ones, the beginning of another.  (Pieces
-// of units, one a workgroup, take as long as the longest: 32 sequences of 2048 to 8192 tokens, 16 nodes, 104 us for 66.)  The lengths are known on the device only, so that every wavefront finds
+// of units, one a workgroup, take as long as the longest: 32 sequences of 2048 to 8192 tokens, 16 nodes, 8 heads of 4 queries, D = 128, 104 us for 84.)  The lengths are known on the device only, so that every wavefront finds
 // its place by a sum over them, 64 sequences at a time, one a lane.  (All tiles together: less than 2^31.)
 struct TreePlace {
     int b, unit, tile;  // sequence; of its units; tile of the unit
@@ -73,7 +75,8 @@ __device__ __forceinline__ TreePlace tree_place_of(const TreeArgs &a, int index,
     for (int base = (seqs - 1) & ~63; base >= 0; base -= 64) {  // (the first 64 last: they stay)
         look(base);
         total += __builtin_amdgcn_readlane(lane_scan(each * units), 63);
-        wide += min(1 << 24, __builtin_amdgcn_readlane(lane_scan(min(1 << 18, up(each) * units)), 63));  // (so many do not fit)
+        const int mine_up = (int)min((int64_t)up(each) * units, (int64_t)1 << 18);
+        wide = min(wide + __builtin_amdgcn_readlane(lane_scan(mine_up), 63), 1 << 24);  // (so many do not fit)
     }
     // Where the workgroups are more than enough none works on two units.
     const bool apart = wide <= workgroups * kLeastShare;
@@ -117,7 +120,7 @@ __device__ __forceinline__ int sight_of(const TreeArgs &a, const KvSeq &s, int n
         }
         left -= n;
     }
-    return s.first - left;
+    return s.first > left ? s.first - left : 0;
 }
 // eight bits of a row's mask from token `at` of the tree on (nothing is looked up outside its words)
 __device__ __forceinline__ uint32_t mask_bits(const int32_t *mask, int words, int at) {

@@ -625,3 +625,55 @@ def test_steps_with_drafts_leave_what_steps_without_leave(gpu, dtype):
                 for x, y in zip(*(nn.kv_cache_read(z[n], table[b:b + 1], lengths[b:b + 1].contiguous(), **how) for z in (drafted, plain))):
                     assert torch.equal(x, y)
     assert sum(short) > 6 * seqs  # (some drafts were accepted)
+
+
+def _example():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "drafted_decoding.py")
+    spec = importlib.util.spec_from_file_location("drafted_decoding", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    return m
+
+
+def test_example_takes_drafts_through_the_layer_as_single_tokens(gpu):
+    """A step's accepted rows against the same tokens one by one, over a cache of their own.  Each way of the layer is within 1e-2 of its output's 2-norm by
+    the projections' contract (four in a chain within 1e-3 of their rows' largest), two of them within 2e-2 of each other."""
+    torch = gpu
+    from gomlx_amd import nn
+    ex = _example()
+    model = ex.Model(200, 512, 8, 2, 768, seed=4, positions=200)
+    drafts = ex.Drafts(3, (3, 2, 1))
+    assert drafts.nodes == 16 and drafts.parents[:16].tolist() == [-1, 0, 0, 0, 1, 1, 2, 2, 3, 3, 4, 5, 6, 7, 8, 9]
+    caches, plain = (ex.Caches(model.layer, 3, 150, 32) for _ in range(2))
+    roots, seen = torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda"), []
+    forward = model.forward
+    model.forward = lambda *a, **k: (seen.append((a[1], forward(*a, **k))), seen[-1][1])[1]
+    taken = 0
+    for _ in range(8):
+        path, after = ex.step(model, caches, drafts, roots, torch.rand(48, device="cuda"), temperature=0.3)
+        tokens, h = seen.pop()
+        for i in range(path.shape[1]):
+            on = path[:, i] >= 0
+            if not on.any():
+                break
+            for b in on.nonzero()[:, 0].tolist():
+                row = 16 * b + path[b, i].item()
+                at = plain.lengths[b:b + 1].clone()
+                plain.lengths[b] += 1
+                one = ex.Caches.__new__(ex.Caches)
+                one.data, one.table = plain.data, plain.table[b:b + 1]
+                single = forward(one, tokens[row:row + 1], at, plain.lengths[b:b + 1].clone(), None, 1)
+                assert (single - h[row]).norm() <= 2e-2 * single.norm()
+                taken += 1
+        roots = after
+        assert torch.equal(caches.lengths, plain.lengths)
+    assert taken > 24  # (some drafts were right)
+
+
+def test_example_runs(gpu, monkeypatch, capsys):
+    ex = _example()
+    monkeypatch.setattr("sys.argv", ["drafted_decoding.py", "--steps", "4", "--seqs", "3", "--prompt", "40", "--vocab", "300", "--shape", "512", "8", "2", "768"])
+    ex.main()
+    assert "tokens a sequence and step" in capsys.readouterr().out
