@@ -1,8 +1,8 @@
 """Decoding with drafted tokens: the operators of gomlx_amd.nn as a serving loop with speculation calls them.
 
 ``python examples/drafted_decoding.py [--steps N]`` takes prompts through one Llama-3-8B-shaped layer (synthetic weights) between a token table and an
-output head, then decodes: a cheap guess (the head on the token's own row of the table, without the layer) drafts a tree of continuations of every sequence, one pass
-takes all of them through the layer over its 4-bit cache, a token is sampled behind each of them, and the path that the samples follow is kept.
+output head, then decodes: a cheap guess (the layer without its attention) drafts a tree of continuations of every sequence, one pass takes all of them through the layer over
+its 4-bit cache, a token is sampled behind each of them, and the path that the samples follow is kept.
 """
 from __future__ import annotations
 
@@ -28,10 +28,18 @@ class Model:
 
     def embed(self, tokens: torch.Tensor) -> torch.Tensor:
         x = nn.quantized_gather(self.table, tokens[:, None], self.quant)
-        return 16.0 * nn.rms_norm(x, nn.RMSNorm())  # (large beside what the layer adds, so that the cheap guess is a guess)
+        return 512.0 * nn.rms_norm(x, nn.RMSNorm())  # (large beside what attention over random keys adds, so that the cheap guess is a good one)
 
     def logits(self, x: torch.Tensor) -> torch.Tensor:
         return nn.quantized_dense(x, self.head, self.quant, norm=nn.RMSNorm())
+
+    def feed_forward(self, h: torch.Tensor) -> torch.Tensor:
+        w, q4 = self.layer.weights, self.layer.quant
+        f = nn.gated_feed_forward(h, w["gate"], w["up"], q4, nn.Activation.SILU, norm=self.layer.norms[1])
+        return nn.quantized_dense(f, w["down"], q4, residual=h)
+
+    def guess(self, tokens: torch.Tensor) -> torch.Tensor:
+        return self.logits(self.feed_forward(self.embed(tokens)))
 
     def forward(self, caches: Caches, tokens, positions, lengths, starts, max_new, tree=None) -> torch.Tensor:
         """float32 [rows, hidden] of the sequences' new tokens, which ``lengths`` counts; with ``tree`` they are drafted ones."""
@@ -45,9 +53,7 @@ class Model:
             a = nn.cached_attention(q, caches.data, caches.table, lengths, starts=starts, max_new=max_new)
         else:
             a = nn.tree_attention(q, caches.data, caches.table, lengths, tree, starts=starts, max_new=max_new)
-        h = nn.quantized_dense(a.view(rows, layer.hidden), w["o"], q4, residual=x)
-        f = nn.gated_feed_forward(h, w["gate"], w["up"], q4, nn.Activation.SILU, norm=layer.norms[1])
-        return nn.quantized_dense(f, w["down"], q4, residual=h)
+        return self.feed_forward(nn.quantized_dense(a.view(rows, layer.hidden), w["o"], q4, residual=x))
 
 
 class Drafts:
@@ -63,10 +69,10 @@ class Drafts:
         self.starts = torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * self.nodes
 
     def draft(self, model: Model, roots: torch.Tensor) -> torch.Tensor:
-        """int32 [sequences * nodes]: under each node the tokens that the head likes best without the layer."""
+        """int32 [sequences * nodes]: under each node the likeliest tokens by the guess."""
         levels = [roots[:, None]]
         for width in self.widths:
-            best = model.logits(model.embed(levels[-1].reshape(-1))).topk(width).indices
+            best = model.guess(levels[-1].reshape(-1)).topk(width).indices
             levels.append(best.int().view(len(roots), -1))
         return torch.cat(levels, 1).reshape(-1)
 
@@ -89,7 +95,7 @@ def main() -> None:
     p.add_argument("--prompt", type=int, default=500)
     p.add_argument("--vocab", type=int, default=32000)
     p.add_argument("--widths", type=int, nargs="+", default=(3, 2, 1))
-    p.add_argument("--temperature", type=float, default=0.7)
+    p.add_argument("--temperature", type=float, default=0.05)
     p.add_argument("--shape", type=int, nargs=4, default=(4096, 32, 8, 14336), metavar=("HIDDEN", "HEADS", "KV_HEADS", "FFN"))
     a = p.parse_args()
     drafts = Drafts(a.seqs, a.widths)

@@ -637,8 +637,9 @@ def _example():
     return m
 
 
-def test_example_takes_drafts_through_the_layer_as_single_tokens(gpu):
-    """A step's accepted rows against the same tokens one by one, over a cache of their own.  Each way of the layer is within 1e-2 of its output's 2-norm by
+def test_example_takes_drafts_through_the_layer_as_single_tokens(gpu, monkeypatch):
+    """A step's accepted rows against the same tokens one by one over the keys and values that the step has left in the cache (of its own a single token would write
+    others: projections by other kernels differ enough to round some of their values to the next of 16).  Each way of the layer is within 1e-2 of its output's 2-norm by
     the projections' contract (four in a chain within 1e-3 of their rows' largest), two of them within 2e-2 of each other."""
     torch = gpu
     from gomlx_amd import nn
@@ -646,30 +647,25 @@ def test_example_takes_drafts_through_the_layer_as_single_tokens(gpu):
     model = ex.Model(200, 512, 8, 2, 768, seed=4, positions=200)
     drafts = ex.Drafts(3, (3, 2, 1))
     assert drafts.nodes == 16 and drafts.parents[:16].tolist() == [-1, 0, 0, 0, 1, 1, 2, 2, 3, 3, 4, 5, 6, 7, 8, 9]
-    caches, plain = (ex.Caches(model.layer, 3, 150, 32) for _ in range(2))
+    caches = ex.Caches(model.layer, 3, 150, 32)
     roots, seen = torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda"), []
     forward = model.forward
     model.forward = lambda *a, **k: (seen.append((a[1], forward(*a, **k))), seen[-1][1])[1]
-    taken = 0
     for _ in range(8):
-        path, after = ex.step(model, caches, drafts, roots, torch.rand(48, device="cuda"), temperature=0.3)
+        before = caches.lengths.tolist()
+        path, roots = ex.step(model, caches, drafts, roots, torch.rand(48, device="cuda"), temperature=0.0)
         tokens, h = seen.pop()
-        for i in range(path.shape[1]):
-            on = path[:, i] >= 0
-            if not on.any():
-                break
-            for b in on.nonzero()[:, 0].tolist():
-                row = 16 * b + path[b, i].item()
-                at = plain.lengths[b:b + 1].clone()
-                plain.lengths[b] += 1
+        assert path[:, 0].tolist() == [0, 0, 0]
+        assert caches.lengths.tolist() == [n + int((p >= 0).sum()) for n, p in zip(before, path)]
+        with monkeypatch.context() as m:
+            m.setattr(nn, "kv_cache_append", lambda *a, **k: None)
+            for b in range(3):
                 one = ex.Caches.__new__(ex.Caches)
-                one.data, one.table = plain.data, plain.table[b:b + 1]
-                single = forward(one, tokens[row:row + 1], at, plain.lengths[b:b + 1].clone(), None, 1)
-                assert (single - h[row]).norm() <= 2e-2 * single.norm()
-                taken += 1
-        roots = after
-        assert torch.equal(caches.lengths, plain.lengths)
-    assert taken > 24  # (some drafts were right)
+                one.data, one.table = caches.data, caches.table[b:b + 1]
+                for i, node in enumerate(n for n in path[b].tolist() if n >= 0):
+                    row, at = 16 * b + node, ints(torch, [before[b] + i])
+                    single = forward(one, tokens[row:row + 1], at, at + 1, None, 1)
+                    assert (single - h[row]).norm() <= 2e-2 * single.norm()
 
 
 def test_example_runs(gpu, monkeypatch, capsys):
