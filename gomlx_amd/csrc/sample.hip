@@ -12,7 +12,7 @@
 // Weights are formed in 64 bits: next to a border, of which a vocabulary has as many as tokens, 32 would give another token once in some hundred rows.  Where order must
 // not matter (histograms, sums that several threads add to) they are whole numbers of 2^-42 of the largest.  The same arguments always give the same token.
 //
-// The first launch reads the logits once: a wavefront a chunk, which leaves its maximum, its sum and its largest keys (32 at least, some 45, complete from
+// The first launch reads the logits once: a wavefront a chunk, which leaves its maximum, its sum and its largest keys (48 at least, some 90, complete from
 // a level on).  In the second a workgroup a row finds the cut among the keys that the chunks have left, and reads a single chunk again.  Where the cut lies
 // below what they have left (a flat distribution under top-p) the row is gone over twice more, by all its chunks at a time in launches that find nothing to do otherwise; where the
 // call's settings make that unlikely these launches are left out, and the second one does it by itself.
@@ -27,7 +27,7 @@ namespace {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int kChunk = 2048, kChunkKeys = 128, kMostChunks = 1024;
+constexpr int kChunk = 2048, kChunkKeys = 128, kLevelLanes = 48, kMostChunks = 1024;
 constexpr int kPickThreads = 512, kPickWaves = kPickThreads / 64, kBins = 2048, kListBins = 512, kListMost = 6144, kFew = 64;
 constexpr int kWideRows = 128;  // flat rows that the launches for them have room for; the others are gone over in the second launch
 constexpr uint32_t kAll = 0xFFFFFFFFu;
@@ -190,8 +190,8 @@ __device__ __forceinline__ double sum_of_lanes(double v) {
     return v;
 }
 
-// One wavefront a chunk.  The level: of the lanes' largest keys the 32nd (its upper 16 bits), so that 32 keys at least are at or above it and, where the large ones
-// lie anywhere, some 45 of 2048.
+// One wavefront a chunk.  The level: of the lanes' largest keys the 48th (its upper 16 bits), so that 48 keys at least are at or above it and, where the large ones
+// lie anywhere, some 90 of 2048, of the 128 that there is room for.
 template <bool BF16> __global__ __launch_bounds__(256) void sample_scan_kernel(const SampleArgs a, int64_t waves) {
     const int lane = (int)threadIdx.x & 63;
     const int64_t index = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -231,7 +231,7 @@ template <bool BF16> __global__ __launch_bounds__(256) void sample_scan_kernel(c
             uint32_t level = 0;
 #pragma unroll
             for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
-                if (__popcll(__ballot(top >= (level | bit))) >= 32) level |= bit;
+                if (__popcll(__ballot(top >= (level | bit))) >= kLevelLanes) level |= bit;
             const float least = value_of(max(level, key_of(-3.402823466e38f)));  // (minus infinity is in no list)
             uint32_t *keys = a.keys + index * kChunkKeys;
             int count = 0;
@@ -778,9 +778,9 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads, 4) void sample_p
         draw(a, l, r, s, row, chunks, most, cut);
         return;
     }
-    // a flat row: into the launches for those, where there are any and they have room (with both bounds the second needs the first's answer)
+    // a flat row: into the launches for those, where there are any and they have room
     __syncthreads();
-    if (a.wide && !(s.k && s.top_p < 1.0)) {
+    if (a.wide) {
         if (tid == 0) l.found = atomicAdd(a.wides, 1u);
         __syncthreads();
         const uint32_t slot = l.found;
@@ -820,32 +820,57 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_bins
         for (int i = 0; i < 32; i++) {
             if (!(x[i] > kNegInf)) continue;
             const uint32_t bin = bin_of(key_of(x[i]), most, most_key, (float)s.rate);
-            if (!s.k) atomicAdd(reinterpret_cast<unsigned long long *>(&weights[bin]), (unsigned long long)units(weight(x[i], most, s.rate)));
+            if (s.top_p < 1.0) atomicAdd(reinterpret_cast<unsigned long long *>(&weights[bin]), (unsigned long long)units(weight(x[i], most, s.rate)));
             atomicAdd(&counts[bin], 1u);
         }
     }
     __syncthreads();
     for (int i = tid; i < kBins; i += kPickThreads) {
         if (!counts[i]) continue;
-        if (!s.k) atomicAdd(reinterpret_cast<unsigned long long *>(&w->weights[i]), (unsigned long long)weights[i]);
+        if (s.top_p < 1.0) atomicAdd(reinterpret_cast<unsigned long long *>(&w->weights[i]), (unsigned long long)weights[i]);
         atomicAdd(&w->counts[i], counts[i]);
     }
 }
 
-// The bin with the row's cut in it; above: tokens or weight in front of it; want: what the cut is at; in_bin: its tokens.  kBins: everything is kept.
-__device__ __forceinline__ uint32_t bin_of_cut(PickLds &l, const Settings &s, const Wide &w, uint64_t &above, uint64_t &want, uint32_t &in_bin) {
-    uint64_t all = 0;
-    if (!s.orders()) return kBins;
-    for (int i = (int)threadIdx.x; i < kBins; i += kPickThreads) {
+// The bins in which a row's cuts lie: that of its top-k in the last of them, that of its top-p in one of them (with both it depends on what the first k weigh, of which the
+// bins in front of the last tell the least).  What is above them, and their tokens.  first == kBins: everything is kept.
+struct CutBins {
+    uint32_t first, last;
+    uint64_t above, above_weight;  // tokens and weight
+    uint32_t tokens;
+    bool counted;  // the top-k cuts something off
+    uint64_t all;  // without a top-k that does: the weight of the row
+};
+__device__ __forceinline__ CutBins bins_of_cuts(PickLds &l, const Settings &s, const Wide &w) {
+    const int tid = (int)threadIdx.x;
+    CutBins c{kBins, kBins, 0, 0, 0, false, 0};
+    if (!s.orders()) return c;
+    const bool weighs = s.top_p < 1.0;
+    for (int i = tid; i < kBins; i += kPickThreads) {
         if (s.k) l.counts[i] = w.counts[i];
-        else all += l.weights[i] = w.weights[i];
+        if (weighs) l.weights[i] = w.weights[i];
     }
-    all = sum_of_threads(all, l.waves);
-    want = s.k ? (uint64_t)s.k : share_of(s, all);
-    above = 0;
-    const uint32_t bin = find_bin<kBins>(l, s.k != 0, want, above);
-    in_bin = bin < kBins ? w.counts[bin] : 0;
-    return bin;
+    __syncthreads();
+    if (s.k) c.last = find_bin<kBins>(l, true, (uint64_t)s.k, c.above);
+    c.counted = c.last < kBins;
+    c.first = c.last;
+    if (weighs) {
+        uint64_t mine = 0;
+        for (int i = tid; i < (int)c.last; i += kPickThreads) mine += l.weights[i];
+        c.all = sum_of_threads(mine, l.waves);
+        c.first = find_bin<kBins>(l, false, share_of(s, c.all), c.above_weight);
+        if (!c.counted) c.last = c.first;
+    }
+    if (c.first >= kBins) return c;
+    if (c.first == c.last) {
+        c.tokens = w.counts[c.first];
+    } else {
+        uint64_t in = 0, above = 0;
+        for (int i = tid; i <= (int)c.last; i += kPickThreads) (i < (int)c.first ? above : in) += l.counts[i];
+        c.above = sum_of_threads(above, l.waves);
+        c.tokens = (uint32_t)sum_of_threads(in, l.waves);
+    }
+    return c;
 }
 
 template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_gather_kernel(const SampleArgs a, int parts) {
@@ -859,21 +884,20 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads) void sample_gath
     const int c = ((int)blockIdx.x - slot * parts) * kPickWaves + wave;
     float x[32];
     if (c < r.chunks()) r.load(c, lane, x);
-    uint64_t above, want;
-    uint32_t in_bin = 0;
-    const uint32_t bin = bin_of_cut(l, s, *w, above, want, in_bin);
-    if (c >= r.chunks() || in_bin > (uint32_t)kListMost) return;
+    const CutBins bins = bins_of_cuts(l, s, *w);
+    if (c >= r.chunks() || bins.tokens > (uint32_t)kListMost) return;
     const float most = w->most;
     const uint32_t most_key = key_of(most), floor_key = w->floor_key;
     uint64_t sum = 0;
-    uint32_t in = 0, found = 0;  // which of the lane's are in the bin; how many of the wavefront's
+    uint32_t in = 0, found = 0;  // which of the lane's are in the bins; how many of the wavefront's
 #pragma unroll
     for (int i = 0; i < 32; i++) {
         const uint32_t key = key_of(x[i]);
-        const uint32_t mine = x[i] > kNegInf && key >= floor_key ? bin_of(key, most, most_key, (float)s.rate) : kAll;
-        if (mine < bin) sum += units(weight(x[i], most, s.rate));
-        in |= (uint32_t)(mine == bin) << i;
-        found += __popcll(__ballot(mine == bin));
+        const uint32_t mine = x[i] > kNegInf ? bin_of(key, most, most_key, (float)s.rate) : kAll;
+        if (mine < bins.first && key >= floor_key) sum += units(weight(x[i], most, s.rate));
+        const bool listed = mine >= bins.first && mine <= bins.last && mine < kBins;  // (whatever min-p says: top-p goes by all of the first k)
+        in |= (uint32_t)listed << i;
+        found += __popcll(__ballot(listed));
     }
     if (found) {
         uint32_t to = 0;
@@ -906,23 +930,30 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads, 4) void sample_w
     const float most = w->most;
     const uint32_t most_key = key_of(most), floor_key = w->floor_key;
     const auto weight_of = [&](uint32_t key) { return units(weight(value_of(key), most, s.rate)); };
-    uint64_t want;
-    Cut cut{0u, kAll, 0}, c{0u, 0u, 0};
-    uint32_t in_bin = 0;
-    const uint32_t bin = bin_of_cut(l, s, *w, c.above, want, in_bin);
-    if (in_bin > (uint32_t)kListMost) {
+    const CutBins bins = bins_of_cuts(l, s, *w);
+    if (bins.tokens > (uint32_t)kListMost) {
         __syncthreads();
         draw_alone(a, l, r, s, row, chunks, most, most_key, floor_key);
         return;
     }
     __syncthreads();
-    // the keys of the bin that min-p leaves: where it leaves none of them, or not as many as the cut keeps, it is the cut
-    const int n = bin < kBins ? (int)w->listed : 0;
+    const int n = bins.first < kBins ? (int)w->listed : 0;
     for (int i = tid; i < n; i += kPickThreads) { l.keys[i] = w->keys[i]; l.chunks[i] = w->chunks[i]; }
     for (int i = tid; i < chunks; i += kPickThreads) l.chunk_weight[i] = w->chunk_weight[i];
     if (tid == 0) l.listed = (uint32_t)n;
     __syncthreads();
-    if (n && cut_of_list(l, weight_of, s.k != 0, want, c)) cut = c;
+    Cut cut{0u, kAll, 0};
+    uint64_t all = bins.all;
+    if (n && bins.counted) {
+        Cut c{0u, 0u, bins.above};
+        if (cut_of_list(l, weight_of, true, (uint64_t)s.k, c)) cut = c;
+        all = bins.above_weight;
+        if (s.top_p < 1.0) all += keep_of_list(l, weight_of, cut);
+    }
+    if (n && s.top_p < 1.0) {
+        Cut c{0u, 0u, bins.above_weight};
+        if (cut_of_list(l, weight_of, false, share_of(s, all), c)) cut = c;
+    }
     if (floor_key > cut.key) cut = Cut{floor_key, kAll, 0};
     chunks_of_list(l, weight_of, cut, chunks, false);
     draw(a, l, r, s, row, chunks, most, cut);
@@ -940,10 +971,10 @@ int launch_sample(const void *logits, bool bf16, int64_t rows, int64_t vocab, in
     // as many rows at a time as 256 MB of workspace hold
     const size_t a_row = (size_t)a.chunks * (sizeof(Chunk) + kChunkKeys * 4);
     const int64_t batch = std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)(((size_t)256 << 20) / a_row)));
-    // Flat rows have launches of their own where one bound may lead below a chunk's list (not a small top-k, which the lists nearly always hold) and a workgroup would
+    // Flat rows have launches of their own where a bound may lead below a chunk's list (not a small top-k, which the lists nearly always hold) and a workgroup would
     // go over a row in several rounds.
     const bool cuts = how.top_ks || how.top_ps || how.min_ps || how.top_k > 0 || how.top_p < 1.0 || how.min_p > 0.0;
-    const bool wide = cuts && (how.top_ks || how.top_k <= 0 || how.top_k > 256) && a.chunks > kPickWaves;
+    const bool wide = cuts && (how.top_ks || how.top_k <= 0 || how.top_k > 64) && a.chunks > kPickWaves;
     a.wide_rows = (int)std::min<int64_t>(batch, kWideRows);
     const size_t lists = (size_t)batch * a_row, wides = (lists + 255) / 256 * 256, flat = wides + 256;
     void *ws = nullptr;

@@ -319,7 +319,8 @@ def test_samples(gpu, vocab, dtype, how):
     check_samples(torch, x, u, **how)
 
 
-@pytest.mark.parametrize("how", SETTINGS, ids=lambda h: "-".join(f"{k}{v}" for k, v in h.items()) or "plain")
+@pytest.mark.parametrize("how", SETTINGS + [dict(top_k=300, top_p=0.9), dict(top_k=3000, top_p=0.7, min_p=0.05), dict(top_k=3000, top_p=0.9, min_p=0.3), dict(top_k=39999, top_p=0.9),
+                                            dict(top_k=20000, top_p=0.001), dict(top_k=20000, min_p=0.01)], ids=lambda h: "-".join(f"{k}{v}" for k, v in h.items()) or "plain")
 def test_samples_of_flat_distributions(gpu, how):
     """The cut lies below what the first launch leaves of each chunk: the row is gone over again."""
     torch = gpu
@@ -358,7 +359,7 @@ def test_samples_of_more_flat_rows_than_their_launches_take(gpu):
     rng = np.random.default_rng(10)
     x = logits(rng, 150, 20000, sure=False)
     x[::7] = np.round(x[::7])
-    for how in (dict(top_p=0.8), dict(top_k=3000), dict(min_p=0.01), dict(top_p=0.9, min_p=0.02)):
+    for how in (dict(top_p=0.8), dict(top_k=3000), dict(min_p=0.01), dict(top_p=0.9, min_p=0.02), dict(top_k=2000, top_p=0.8, min_p=0.01)):
         check_samples(torch, torch.from_numpy(x).cuda(), rng.random(150), **how)
 
 
