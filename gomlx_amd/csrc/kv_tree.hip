@@ -31,6 +31,7 @@ struct TreeArgs {
     void *out;              // [rows, heads, D]
     float *part, *part_ml;  // of units that several workgroups work on: sums [workgroups, 2, rows, D], (reference, sum) [workgroups, 2, rows, 2]
     int blocks, rows;       // row blocks of a sequence and rows of a block, at most
+    int all_blocks;         // of all sequences, at most, where the join finds them by number; 0: it is laid out by `blocks`
     int2 *pieces;           // per unit: the first workgroup that works on it, and how many do
 };
 
@@ -436,10 +437,33 @@ __global__ __launch_bounds__(256) void kv_tree_join_kernel(const TreeArgs a, int
     constexpr int L = D / 4, R = 256 / L / SHARES;  // lanes of a row's values; rows of a workgroup
     __shared__ f4 sums[256];
     __shared__ float tops[256 / L], alls[256 / L];
-    const int per_block = (a.rows + R - 1) / R, block = (int)blockIdx.x / per_block, h = (int)blockIdx.y, b = (int)blockIdx.z, tid = (int)threadIdx.x;
+    const int per_block = (a.rows + R - 1) / R, h = (int)blockIdx.y, tid = (int)threadIdx.x;
+    int block = (int)blockIdx.x / per_block, b = (int)blockIdx.z;
     const int rr = ((int)blockIdx.x - block * per_block) * R + tid / L / SHARES, share = tid / L % SHARES, d = tid % L * 4;
+    KvSeq seq{};
+    if (a.all_blocks) {
+        const int index = block, lane = tid & 63;
+        int front = 0;
+        b = -1;
+        for (int base = 0; base < a.kv.seqs; base += 64) {
+            KvSeq mine{};
+            if (base + lane < a.kv.seqs) mine = kv_seq(a.kv, base + lane);
+            const int blocks = blocks_of(a, mine, block_rows), upto = lane_scan(blocks);
+            const uint64_t past = __ballot(front + upto > index);
+            if (past) {
+                const int l = __ffsll((unsigned long long)past) - 1;
+                b = base + l;
+                seq = seq_of_lane(mine, l);
+                block = index - (front + __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(blocks, l));
+                break;
+            }
+            front += __builtin_amdgcn_readlane(upto, 63);
+        }
+        if (b < 0) return;
+    } else {
+        seq = kv_seq(a.kv, b);
+    }
     const int unit = (b * a.kv.kv_heads + h) * a.blocks + block;
-    const KvSeq seq = kv_seq(a.kv, b);
     if (block * block_rows >= seq.news * a.group) return;  // (without rows nobody has written the unit's pieces)
     const int2 piece = a.pieces[unit];
     const int first = piece.x, pieces = piece.y;
@@ -482,7 +506,8 @@ __global__ __launch_bounds__(256) void kv_tree_join_kernel(const TreeArgs a, int
 
 template <int D, bool BF16, int SHARES> int tree_join(const TreeArgs &a, int block_rows, hipStream_t s) {
     constexpr int R = 1024 / D / SHARES;
-    const dim3 grid((unsigned)(a.blocks * ((a.rows + R - 1) / R)), (unsigned)a.kv.kv_heads, (unsigned)a.kv.seqs);
+    const int per_block = (a.rows + R - 1) / R;
+    const dim3 grid((unsigned)((a.all_blocks ? a.all_blocks : a.blocks) * per_block), (unsigned)a.kv.kv_heads, a.all_blocks ? 1u : (unsigned)a.kv.seqs);
     return launch(kv_tree_join_kernel<D, BF16, SHARES>, grid, dim3(256), 0, s, a, block_rows);
 }
 template <int D, bool BF16, int RG> int tree_attend(const TreeArgs &a, int workgroups, hipStream_t s) {
@@ -508,13 +533,16 @@ template <int D, bool BF16> int tree_attend(const TreeArgs &a, int row_groups, i
 }  // namespace
 
 // How a call's rows are cut into blocks: 16 RG (node, query head) pairs of a key head.
-struct TreePlan { int row_groups, rows; int64_t blocks, tiles; };
+struct TreePlan { int row_groups, rows; int64_t blocks, tiles, all_blocks; };
 static TreePlan tree_plan(const KvCall &kv, int heads, int window) {
     TreePlan p;
     const int64_t most_rows = (int64_t)kv.max_new * (heads / kv.kv_heads), room = (int64_t)kv.max_pages * kv.page_tokens / 32;
     p.row_groups = (int)std::min<int64_t>((most_rows + 15) / 16, kv.head_dim == 256 ? 2 : 4);
     p.rows = (int)std::min<int64_t>(most_rows, 16 * p.row_groups);
     p.blocks = (most_rows + 16 * p.row_groups - 1) / (16 * p.row_groups);
+    // (one large tree beside many small ones: nearly all of a grid laid out for the largest would have nothing to do)
+    p.all_blocks = (int64_t)kv.rows * (heads / kv.kv_heads) / (16 * p.row_groups) + kv.seqs;
+    if (p.blocks * kv.seqs <= 2 * p.all_blocks) p.all_blocks = 0;
     p.tiles = std::max<int64_t>(1, window ? std::min<int64_t>(room, ((int64_t)window + kv.max_new + 31) / 32 + 1) : room);
     return p;
 }
@@ -522,8 +550,9 @@ static TreePlan tree_plan(const KvCall &kv, int heads, int window) {
 int check_kv_tree_attention(const char *fn, const KvCall &kv, int heads, int window) {
     const TreePlan p = tree_plan(kv, heads, window);
     const int64_t units = (int64_t)kv.seqs * kv.kv_heads * p.blocks;
-    // (threads of a launch are counted in 32 bits: fewer than 2^24 workgroups, of which a unit has one for every 1024 values that are joined; and so are the tiles of all units)
-    if (p.blocks > INT32_MAX / kv.kv_heads / kv.seqs || units * ((p.rows * kv.head_dim + 1023) / 1024) > (1 << 24) - 4096 || units > (INT32_MAX - 4096) / p.tiles)
+    // (threads of a launch are counted in 32 bits: fewer than 2^24 workgroups, of which a block of rows has one for every 1024 values that are joined; and so are the tiles of all units)
+    const int64_t joined = p.all_blocks ? p.all_blocks * kv.kv_heads : units;
+    if (p.blocks > INT32_MAX / kv.kv_heads / kv.seqs || joined * ((p.rows * kv.head_dim + 1023) / 1024) > (1 << 24) - 4096 || units > (INT32_MAX - 4096) / p.tiles)
         return fail(GQ_ERR_INVALID, "%s: %d sequences of up to %d rows of %d heads over up to %lld tiles: too many (pass the page table's first columns)", fn, kv.seqs, kv.max_new, heads,
                     (long long)p.tiles);
     return GQ_OK;
@@ -545,6 +574,7 @@ int launch_kv_tree_attention(const KvCall &kv, const HeadRows &q, int heads, flo
     const TreePlan p = tree_plan(kv, heads, window);
     a.rows = p.rows;
     a.blocks = (int)p.blocks;
+    a.all_blocks = (int)p.all_blocks;
     const int64_t tiles = p.tiles, units = (int64_t)kv.seqs * kv.kv_heads * a.blocks;
     // (as many workgroups as run at a time)
     const int per_cu = kv.head_dim == 256 ? 1 : 2;

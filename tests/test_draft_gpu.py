@@ -167,6 +167,17 @@ def test_attention_over_more_than_64_sequences(gpu):
     check_attention(c, news, 4, [ref.ancestors(random_parents(rng, n)) if n else [] for n in news], "bf16")
 
 
+def test_attention_of_one_large_tree_beside_small_ones(gpu):
+    torch = gpu
+    rng = np.random.default_rng(3)
+    news = [int(n) for n in rng.integers(0, 3, 90)]
+    news[66] = 300
+    lengths = [n + int(x) for n, x in zip(news, rng.integers(0, 300, 90))]
+    for dim in (64, 256):
+        c = Case(torch, lengths, kv_heads=2, dim=dim, page=32, seed=2).fill()
+        check_attention(c, news, 6, [ref.ancestors(random_parents(rng, n)) if n else [] for n in news], "bf16")
+
+
 def test_a_chain_is_attention_of_new_tokens(gpu):
     torch = gpu
     c = Case(torch, [500, 90], seed=5).fill()
@@ -674,3 +685,106 @@ def test_example_runs(gpu, monkeypatch, capsys):
     monkeypatch.setattr("sys.argv", ["drafted_decoding.py", "--steps", "4", "--seqs", "3", "--prompt", "40", "--vocab", "300", "--shape", "512", "8", "2", "768"])
     ex.main()
     assert "tokens a sequence and step" in capsys.readouterr().out
+
+
+def test_a_step_replays_from_a_graph(gpu):
+    """Everything between the projections of a step, recorded once and replayed over other inputs with eager calls in between; some rows belong to no sequence."""
+    torch = gpu
+    from gomlx_amd import nn
+    rng = np.random.default_rng(12)
+    seqs, nodes, padding, heads, kv_heads, dim, vocab = 3, 9, 4, 8, 2, 64, 3000
+    rows = seqs * nodes + padding
+    table = torch.arange(seqs * 8, dtype=torch.int32, device="cuda").view(seqs, 8)
+    starts = ints(torch, [0, 9, 18, 27])
+    head = torch.randn(heads * dim, vocab, device="cuda")
+
+    def inputs(seed):
+        g = torch.Generator("cuda").manual_seed(seed)
+        normal = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+        parents = sum((random_parents(rng, nodes) for _ in range(seqs)), []) + [0] * padding
+        return dict(lengths=ints(torch, [40 + seed, 9, 200 - seed]), parents=ints(torch, parents), tokens=ints(torch, rng.integers(0, 5, rows)), q=normal(rows, heads, dim), k=normal(rows, kv_heads, dim),
+                    v=normal(rows, kv_heads, dim), u=torch.rand(rows, device="cuda", generator=g), cache=torch.randint(0, 100, (seqs * 8, kv_heads, 1, 36 * dim), dtype=torch.uint8, device="cuda", generator=g),
+                    weights=normal(seqs * 8, kv_heads, 32).abs())
+
+    def step(s):
+        tree, positions = nn.draft_tree(s["parents"], s["lengths"], starts=starts, max_new=nodes)
+        nn.kv_cache_append(s["cache"], s["k"], s["v"], table, s["lengths"], starts=starts, max_new=nodes, weights=s["weights"])
+        a = nn.tree_attention(s["q"], s["cache"], table, s["lengths"], tree, starts=starts, max_new=nodes)
+        drawn, shares = nn.sample(a.view(rows, -1) @ head, s["u"], 0.8, 0, 0.9, probabilities=True)
+        path, token, lengths = nn.kv_cache_accept(s["cache"], table, s["lengths"], s["parents"], s["tokens"], drawn % 5, starts=starts, max_new=nodes, weights=s["weights"])
+        real = slice(0, seqs * nodes)
+        return [tree[real], positions[real], a[real], drawn[real], shares[real], path, token, lengths, s["cache"], s["weights"]]
+
+    copy = lambda s: {k: t.clone() for k, t in s.items()}  # noqa: E731
+    states = [inputs(i) for i in range(4)]
+    held, stream = copy(states[0]), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step(copy(states[0]))
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(held)
+    for i in (1, 2, 3, 0, 2):
+        for k, t in states[i].items():
+            held[k].copy_(t)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        eager = step(copy(states[i]))
+        torch.cuda.synchronize()
+        for n, (x, y) in enumerate(zip(out, eager)):
+            assert torch.equal(x, y), f"state {i}, output {n}"
+
+
+def test_attention_of_very_many_sequences(gpu):
+    """Trees of a root alone are single new tokens."""
+    torch = gpu
+    from gomlx_amd import nn
+    seqs = 9000
+    cache = nn.kv_cache(seqs, 1, 64, 32)
+    table = torch.randperm(seqs, device="cuda").int().view(seqs, 1)
+    lengths = torch.randint(1, 33, (seqs,), dtype=torch.int32, device="cuda")
+    starts = torch.cat([torch.zeros(1, device="cuda"), lengths.cumsum(0)]).int()
+    rows = int(starts[-1])
+    nn.kv_cache_append(cache, torch.randn(rows, 1, 64, device="cuda"), torch.randn(rows, 1, 64, device="cuda"), table, lengths, starts=starts, max_new=32)
+    q = torch.randn(seqs, 4, 64, device="cuda")
+    got = nn.tree_attention(q, cache, table, lengths, torch.ones(seqs, 1, dtype=torch.int32, device="cuda"))
+    want = nn.cached_attention(q, cache, table, lengths)
+    # (each within a few 2^-22 of 64 bits, times values of up to 5 that weights of 1 average)
+    assert (got - want).abs().max() <= 1e-5
+
+
+def test_calls_from_two_threads_on_streams_of_their_own(gpu):
+    torch = gpu
+    import threading
+    from gomlx_amd import nn
+    rng = np.random.default_rng(13)
+    xs = [torch.from_numpy(logits(rng, 40, 30000, sure=i == 0)).cuda() for i in range(2)]
+    us = [torch.rand(40, device="cuda") for _ in range(2)]
+    cases = [Case(torch, [3000, 2000], seed=20 + i).fill() for i in range(2)]
+    sets = [[ref.ancestors(random_parents(rng, 20)) for _ in range(2)] for _ in range(2)]
+    trees = [torch.from_numpy(np.concatenate([ref.masks(s, 1) for s in ss])).cuda() for ss in sets]
+    qs = [torch.randn(40, 8, 128, device="cuda") for _ in range(2)]
+
+    def work(i):
+        c = cases[i]
+        return nn.sample(xs[i], us[i], 1.0, 0, 0.9), nn.tree_attention(qs[i], c.cache, c.d_table, c.ints([3000, 2000]), trees[i], starts=c.ints([0, 20, 40]), max_new=20)
+
+    want = [work(i) for i in range(2)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def thread(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = work(i)
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(x, y) for x, y in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
