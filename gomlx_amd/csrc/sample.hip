@@ -236,17 +236,17 @@ template <bool BF16> __global__ __launch_bounds__(256) void sample_scan_kernel(c
                 if (__popcll(__ballot(top >= (level | bit))) >= kLevelLanes) level |= bit;
             const float least = value_of(max(level, key_of(-3.402823466e38f)));  // (minus infinity is in no list)
             uint32_t *keys = a.keys + index * kChunkKeys;
-            int count = 0;
+            // (a lane has one or two of them, and reads these again: to look for one in each of its registers takes 12 instructions a register)
+            uint32_t in = 0;
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
-                const bool in = x[i] >= least;
-                const uint64_t all = __ballot(in);
-                if (!all) continue;
-                const int to = count + __popcll(all & ((1ull << lane) - 1));
-                if (in && to < kChunkKeys) keys[to] = key_of(x[i]);
-                count += __popcll(all);
+            for (int i = 0; i < 32; i++) in |= x[i] >= least ? 1u << i : 0u;
+            const uint32_t mine_in = (uint32_t)__popc(in), upto = scan_lanes(mine_in, 0u, Sum{});
+            const int count = (int)last_lane(upto);
+            if (count <= kChunkKeys) {
+                for (uint32_t to = upto - mine_in; in; in &= in - 1, to++) keys[to] = key_of(r.one(Row<BF16>::place(chunk, lane, __ffs((int)in) - 1)));
+                c.level = level;
+                c.count = count;
             }
-            if (count <= kChunkKeys) { c.level = level; c.count = count; }
         }
     }
     if (lane == 0) a.chunk[index] = c;
