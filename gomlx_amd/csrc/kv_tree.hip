@@ -9,7 +9,7 @@
 // tile of 32 tokens at D = 128, every 16 rows 16 matrix instructions of 16 cycles (in float32 32) and some 47 vector instructions, eight of them exponentials of four times the
 // usual length, for their weights.  These bound it, for next to matrix instructions little else is issued: at 64 rows some 2000 cycles of the one and 1000 of the other a
 // tile, 3100 as measured (two wavefronts a SIMD; one alone takes 3500).  us a call, D = 128, bfloat16, 8 key heads of 4 queries: 32 sequences of 2048 to 8192 tokens with 8
-// to 16 nodes each 79 (460 TFLOP/s, 2.5 TB/s of cache); 32 nodes over 131072 tokens 96 (715 TFLOP/s); 16 sequences of 2048 to 8192 tokens with 32 to 64 nodes 124 (580).
+// to 16 nodes each 79 (460 TFLOP/s, 2.5 TB/s of cache); 32 nodes over 131072 tokens 93 (740 TFLOP/s); 16 sequences of 2048 to 8192 tokens with 32 to 64 nodes 124 (580).
 #include "kv_attend.hpp"
 
 #include <algorithm>

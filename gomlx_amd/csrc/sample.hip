@@ -193,7 +193,8 @@ __device__ __forceinline__ double sum_of_lanes(double v) {
 // One wavefront a chunk.  The level: of the lanes' largest keys the 48th (its upper 16 bits), so that 48 keys at least are at or above it and, where the large ones
 // lie anywhere, some 90 of 2048, of the 128 that there is room for.
 //
-// Vector instructions bound it where there are many rows, 30 a logit, 16 of them in 64 bits: 512 rows of 128256 in float32 67 us, 3.9 TB/s (of 4.9 that a copy reaches).  One row: 7 us.
+// The reading bounds it where there are many rows: 512 rows of 128256 in float32 65 us, 4.04 TB/s (a plain sum reads 3.99, a copy moves 4.9), of which 26 vector instructions a logit,
+// 16 of them in 64 bits, take 48.  One row: 7 us.
 template <bool BF16> __global__ __launch_bounds__(256) void sample_scan_kernel(const SampleArgs a, int64_t waves) {
     const int lane = (int)threadIdx.x & 63;
     const int64_t index = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
