@@ -1416,6 +1416,7 @@ int gq_sample(int dtype, const void *dLogits, int64_t rows, int64_t vocab, int64
     if (rows < 0 || vocab < 1 || row_stride < 0) return fail(GQ_ERR_INVALID, "%s: %lld rows of %lld logits, %lld apart", fn, (long long)rows, (long long)vocab, (long long)row_stride);
     if (!how) return fail(GQ_ERR_INVALID, "%s: null settings", fn);
     if (rows == 0) return GQ_OK;
+    if (vocab > kMostLogits) return fail(GQ_ERR_INVALID, "%s: a vocabulary of %lld tokens: at most %lld", fn, (long long)vocab, (long long)kMostLogits);
     if (!dLogits || !dUniform || !dTokens) return fail(GQ_ERR_INVALID, "%s: null device pointer", fn);
     if (!aligned_to(dLogits, dtype == GQ_BF16 ? 2 : 4)) return fail(GQ_ERR_INVALID, "%s: logits are not aligned to their elements", fn);
     for (const void *p : {(const void *)dUniform, (const void *)dTokens, (const void *)dProbabilities, (const void *)how->dTemperature, (const void *)how->dTopP, (const void *)how->dMinP, (const void *)how->dTopK})

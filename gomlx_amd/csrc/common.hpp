@@ -186,6 +186,7 @@ int launch_kv_tree_attention(const KvCall &kv, const HeadRows &q, int heads, flo
 int launch_kv_accept(const KvCall &kv, const int32_t *parents, const int32_t *tokens, const int32_t *sampled, float *accounts, int32_t *path, int path_columns, int32_t *next,
                      int32_t *new_lengths, hipStream_t s);
 // A token for every row of logits (sample.hip).  Settings: where a pointer is not null it has one for each row.
+constexpr int64_t kMostLogits = ((int64_t)1 << 21) - 7;  // of a row
 struct Sampling {
     double temperature, top_p, min_p;
     int top_k;

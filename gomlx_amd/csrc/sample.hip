@@ -30,6 +30,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int kChunk = 2048, kChunkKeys = 128, kLevelLanes = 48, kMostChunks = 1024;
 constexpr int kPickThreads = 512, kPickWaves = kPickThreads / 64, kBins = 2048, kListBins = 512, kListMost = 6144, kFew = 64;
 constexpr int kWideRows = 128;  // flat rows that the launches for them have room for; the others are gone over in the second launch
+static_assert((kMostLogits + 7 + kChunk - 1) / kChunk <= kMostChunks, "a row's chunks have room in LDS, wherever its first logit lies");
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -974,7 +975,6 @@ int launch_sample(const void *logits, bool bf16, int64_t rows, int64_t vocab, in
     a.row_bytes = row_stride * (bf16 ? 2 : 4);
     a.vocab = (int)vocab;
     a.chunks = (int)((vocab + 7 + kChunk - 1) / kChunk);
-    if (a.chunks > kMostChunks) return fail(GQ_ERR_INVALID, "sample: a vocabulary of %lld tokens: at most %d", (long long)vocab, kMostChunks * kChunk - 7);
     // as many rows at a time as 256 MB of workspace hold
     const size_t a_row = (size_t)a.chunks * (sizeof(Chunk) + kChunkKeys * 4);
     const int64_t batch = std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)(((size_t)256 << 20) / a_row)));

@@ -112,6 +112,14 @@ def test_sample_refusals():
     assert call(rows=0)[0] == _lib.OK
 
 
+@pytest.mark.parametrize("vocab", [2 ** 21 - 6, 2 ** 21, 2 ** 31, 2 ** 42, 2 ** 43 - 2 ** 11, 2 ** 43, 2 ** 62, 2 ** 63 - 1])
+def test_sample_refuses_vocabularies_that_32_bits_do_not_count(vocab):
+    L, p = _lib.lib(), Buffers()
+    d = _lib.SamplingDesc(1.0, 1.0, 0.0, 0)
+    rc, text = _error(L.gq_sample(_lib.F32, p(), 1, vocab, vocab, p(), ctypes.byref(d), p(), None, None))
+    assert rc == _lib.ERR_INVALID and f"{vocab} tokens: at most {2 ** 21 - 7}" in text
+
+
 def test_accept_refusals():
     L, p = _lib.lib(), Buffers()
 
