@@ -625,13 +625,20 @@ def tree_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
     return out
 
 
+def _sampling_number(name: str, value, least, most) -> None:
+    if not least <= value <= most:
+        raise ValueError(f"{name} must be between {least} and {most}, got {value}")
+    if name == "top_k" and value % 1 != 0:  # (infinity among them: no bound is 0)
+        raise ValueError(f"top_k must be a whole number, got {value}")
+
+
 def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, probabilities: bool = False):
     """A token for every row of logits [rows, vocabulary] (float32 or bfloat16, strided rows allowed) from a given number of [0, 1) for each, ``uniform`` (float32 [rows]).
 
     With weights exp((x - max x) / temperature) and tokens in order of their logits, equal ones by index, stay: the first ``top_k``; of these the shortest
     beginning that weighs at least ``top_p`` of them, one token at least; of these those that weigh ``min_p`` of the largest and more.  The token is the lowest index up
     to which what stays weighs more than ``uniform`` of it all.  A temperature of 0 asks for the first in order; ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0 are no bounds.  Each
-    of the four is one number, or a tensor with one for each row (float32, ``top_k`` int32; values outside their range count as the nearest in it, NaN as no bound, a temperature of NaN as 0).
+    of the four is one number (``top_k`` a whole one), or a tensor with one for each row (float32, ``top_k`` int32; values outside their range count as the nearest in it, NaN as no bound, a temperature of NaN as 0).
     A NaN logit counts as minus infinity; a row without a number above that gets token -1.  Weights and sums are formed in 64 bits: the same arguments give the same token.
 
     Returns int32 [rows]; with ``probabilities`` also float32 [rows], what share of the weight that stays the token has."""
@@ -656,9 +663,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0
             if value.dtype != dtype or tuple(value.shape) != (rows,) or value.device != logits.device:
                 raise ValueError(f"{name} must be a number or a {dtype} [{rows}] tensor on {logits.device}, got {value.dtype} {tuple(value.shape)} on {value.device}")
             setattr(d, field, value.data_ptr())
-        elif not least <= value <= most:
-            raise ValueError(f"{name} must be between {least} and {most}, got {value}")
         else:
+            _sampling_number(name, value, least, most)
             setattr(d, name, min(int(value), 2 ** 31 - 1) if name == "top_k" else float(value))
     if uniform.device != logits.device:
         raise ValueError("uniform and logits must be on one device")

@@ -465,6 +465,24 @@ def test_sample_refuses(gpu):
         nn.sample(x.half(), u)
 
 
+@pytest.mark.parametrize("native", (True, False))
+def test_sample_takes_whole_numbers_as_top_k(gpu, monkeypatch, native):
+    torch = gpu
+    from gomlx_amd import _lib, nn
+    if not native:
+        monkeypatch.setattr(_lib, "fast", None)
+    x, u = torch.randn(40, 100, device="cuda"), torch.rand(40, device="cuda")
+    for bad in (0.5, 2.9, 99.999, math.inf, math.nan, -0.5, np.float32(1.5)):
+        with pytest.raises(ValueError, match="top_k"):
+            nn.sample(x, u, top_k=bad)
+    three, all_of_it = nn.sample(x, u, top_k=3), nn.sample(x, u)
+    assert not torch.equal(three, all_of_it)
+    for k in (3.0, np.int64(3), np.float32(3), torch.full((40,), 3, dtype=torch.int32, device="cuda")):
+        assert torch.equal(nn.sample(x, u, top_k=k), three)
+    for k in (0.0, 100, 2 ** 31 - 1, 2 ** 31, 2 ** 70):
+        assert torch.equal(nn.sample(x, u, top_k=k), all_of_it)
+
+
 # ---- the end of a step ----------------------------------------------------------------------------------------------------
 
 

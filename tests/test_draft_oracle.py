@@ -120,6 +120,19 @@ def test_sample_refuses_vocabularies_that_32_bits_do_not_count(vocab):
     assert rc == _lib.ERR_INVALID and f"{vocab} tokens: at most {2 ** 21 - 7}" in text
 
 
+def test_top_k_is_a_whole_number():
+    from gomlx_amd import nn
+    for k in (0, 1, 50, 50.0, np.int64(7), np.float32(7), 2 ** 70):
+        nn._sampling_number("top_k", k, 0, math.inf)
+    for k in (0.5, 2.9, np.float32(1.5), -1, -0.5, math.inf, math.nan):
+        with pytest.raises(ValueError, match="top_k"):
+            nn._sampling_number("top_k", k, 0, math.inf)
+    nn._sampling_number("temperature", 0.5, 0.0, math.inf)
+    nn._sampling_number("temperature", math.inf, 0.0, math.inf)
+    with pytest.raises(ValueError, match="top_p"):
+        nn._sampling_number("top_p", 1.5, 0.0, 1.0)
+
+
 def test_accept_refusals():
     L, p = _lib.lib(), Buffers()
 
