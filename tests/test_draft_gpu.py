@@ -365,6 +365,75 @@ def test_samples_of_rows_with_holes(gpu, how):
     assert tokens[3] == -1 and tokens[2] == 4321 and tokens[7] == 4999 and tokens[4] in (17, 4000)
 
 
+def kernel_us(call, times=5):
+    """The least time that the kernels of a call have taken."""
+    import ctypes
+    from gomlx_amd import _lib
+    n, us, out = ctypes.c_int(), ctypes.c_double(), []
+    for _ in range(times):
+        _lib.check(_lib.lib().gq_profile_begin())
+        call()
+        _lib.check(_lib.lib().gq_profile_end(ctypes.byref(n), ctypes.byref(us)))
+        out.append(us.value)
+    return min(out)
+
+
+def masked(rng, x, allowed, value):
+    """All but `allowed` tokens of every row at one value."""
+    out = np.full_like(x, value)
+    for r in range(len(x)):
+        keep = np.concatenate([np.argsort(-x[r])[:allowed // 2], rng.choice(x.shape[1], allowed - allowed // 2, replace=False)])
+        out[r, keep] = x[r, keep]
+    return out
+
+
+@pytest.mark.parametrize("how", [dict(top_k=50, top_p=0.9, temperature=0.8), dict(top_k=50), dict(top_k=3), dict(top_p=0.9), dict(top_p=0.9999), dict(min_p=0.05), dict(min_p=1e-9), dict(top_k=200, top_p=0.95),
+                                 dict(top_k=3000, min_p=0.01), dict(top_k=40, temperature=30.0), dict(top_p=0.5, temperature=1e9)], ids=str)
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+def test_samples_of_rows_with_many_equal_logits(gpu, how, dtype):
+    torch = gpu
+    rng = np.random.default_rng(14)
+    vocab = 20003
+    x = logits(rng, 10, vocab)
+    x[0] = masked(rng, x[:1], 300, -1e9)[0]
+    x[1] = masked(rng, x[1:2], 12, -1e9)[0]
+    x[2] = masked(rng, x[2:3], 2000, -30.0)[0]
+    x[3, 5000:] = 0.0                         # padding, of chunks that have nothing else
+    x[4, 12000:16000] = 9.0                   # among the likely ones
+    x[5] = np.where(rng.random(vocab) < 0.001, 4.0, np.where(rng.random(vocab) < 0.1, 3.0, -2.0))
+    x[6, rng.random(vocab) < 0.1] = np.inf
+    x[7] = -1e9
+    x[8] = -20.0
+    x[8, (np.arange(vocab) // 4) % 64 < 10] = 1.0 + np.arange(vocab)[(np.arange(vocab) // 4) % 64 < 10] * 1e-4  # all large ones of a chunk in ten lanes
+    x[9] = masked(rng, x[9:], 400, -3e38)[0]
+    check_samples(torch, torch.from_numpy(x).cuda().to(torch.float32 if dtype == "f32" else torch.bfloat16), rng.random(10), **how)
+
+
+@pytest.mark.parametrize("how", [dict(top_k=50, top_p=0.9, temperature=0.8), dict(top_k=50), dict(top_p=0.9)], ids=str)
+@pytest.mark.parametrize("value", (-1e9, -200.0))
+def test_a_mask_by_a_finite_value_takes_no_longer(gpu, how, value):
+    """... than one by minus infinity: chunks full of equal logits leave the others' lists alone.  (A row that is gone over alone takes five times as long and more.)"""
+    torch = gpu
+    from gomlx_amd import nn
+    rng = np.random.default_rng(15)
+    x = logits(rng, 1, 128256)
+    u = torch.rand(1, device="cuda")
+    times = []
+    for v in (-np.inf, value):
+        d = torch.from_numpy(masked(np.random.default_rng(16), x, 300, v)).cuda()
+        nn.sample(d, u, **how)
+        times.append(kernel_us(lambda: nn.sample(d, u, **how)))  # noqa: B023
+    assert times[1] <= 2 * times[0], times
+    # padding behind the vocabulary, which ends anywhere in a chunk of 2048
+    for rest in (0, 130, 180, 190, 300, 1500):
+        x[0, -3000 - rest:] = 0.0
+        d = torch.from_numpy(x).cuda()
+        padded = kernel_us(lambda: nn.sample(d, u, **how))  # noqa: B023
+        x[0, -3000 - rest:] = -np.inf
+        e = torch.from_numpy(x).cuda()
+        assert padded <= 2 * kernel_us(lambda: nn.sample(e, u, **how)), rest  # noqa: B023
+
+
 def test_samples_of_more_flat_rows_than_their_launches_take(gpu):
     torch = gpu
     rng = np.random.default_rng(10)
