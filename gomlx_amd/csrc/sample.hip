@@ -785,7 +785,12 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads, 4) void sample_p
     uint64_t all = 0;
     if (from_lists && s.k) {
         cut = Cut{0u, 0u, 0};
-        from_lists = cut_of_list(l, weight_of, true, (uint64_t)s.k, cut);
+        // (Fewer than k: all of them stay, and what the lists do not have adds nothing where it weighs nothing.  A mask that leaves ten tokens of 128256 under top-k 50 and
+        // top-p 0.9: 19 us for minus infinity, 20 for -1e9; 74 and 836 with the row gone over for more.)
+        if (!cut_of_list(l, weight_of, true, (uint64_t)s.k, cut)) {
+            from_lists = level < most_key && weight_of(level) == 0;
+            cut = Cut{level, kAll, 0};
+        }
         if (from_lists && s.top_p < 1.0) all = keep_of_list(l, weight_of, cut);
     } else if (from_lists && s.top_p < 1.0) {
         double sum = 0.0;

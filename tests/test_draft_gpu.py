@@ -434,6 +434,34 @@ def test_a_mask_by_a_finite_value_takes_no_longer(gpu, how, value):
         assert padded <= 2 * kernel_us(lambda: nn.sample(e, u, **how)), rest  # noqa: B023
 
 
+@pytest.mark.parametrize("how", [dict(top_k=50, top_p=0.9, temperature=0.8), dict(top_k=50), dict(top_k=300, top_p=0.99), dict(top_k=50, min_p=0.01), dict(top_k=50, min_p=1e-300),
+                                 dict(top_k=50, temperature=0.01), dict(top_k=50, top_p=0.9, temperature=7.0), dict(top_k=40, temperature=1e12)], ids=str)
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+def test_samples_of_rows_with_fewer_tokens_than_top_k(gpu, how, dtype):
+    torch = gpu
+    rng = np.random.default_rng(17)
+    x = np.concatenate([masked(rng, logits(rng, 1, 20003), n, v) for v in (-np.inf, -1e9, -200.0, -20.0, 0.0) for n in (2, 10, 47)])
+    x = np.concatenate([x, np.full((2, 20003), -3e38, np.float32)])
+    x[-1, 7], x[-2, [5, 19000]] = -2.9e38, 3e38
+    check_samples(torch, torch.from_numpy(x).cuda().to(torch.float32 if dtype == "f32" else torch.bfloat16), rng.random(len(x)), **how)
+
+
+@pytest.mark.parametrize("how", [dict(top_k=50, top_p=0.9, temperature=0.8), dict(top_k=50), dict(top_k=300, top_p=0.9)], ids=str)
+@pytest.mark.parametrize("value", (-np.inf, -1e9, -200.0))
+def test_a_mask_that_leaves_fewer_tokens_than_top_k_takes_no_longer(gpu, how, value):
+    """... than the same under a top-k that they reach: what is masked weighs nothing, so that the row need not be gone over for more."""
+    torch = gpu
+    from gomlx_amd import nn
+    rng = np.random.default_rng(18)
+    x, u = torch.from_numpy(masked(rng, logits(rng, 1, 128256), 10, value)).cuda(), torch.rand(1, device="cuda")
+    times = []
+    for k in (5, how["top_k"]):
+        nn.sample(x, u, **{**how, "top_k": k})
+        times.append(kernel_us(lambda: nn.sample(x, u, **{**how, "top_k": k})))  # noqa: B023
+    # (a top-k of more than 64 has the launches for flat rows behind it, three of which find nothing to do: each some 3 us)
+    assert times[1] <= 2 * times[0] + (10 if how["top_k"] > 64 else 0), times
+
+
 def test_samples_of_more_flat_rows_than_their_launches_take(gpu):
     torch = gpu
     rng = np.random.default_rng(10)
