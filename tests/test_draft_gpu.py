@@ -903,3 +903,55 @@ def test_calls_from_two_threads_on_streams_of_their_own(gpu):
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_threads_finish_every_call(gpu):
+    """Two threads at a time on streams of their own, and two on one stream: an error in a thread, or calls that it has not come to, fail the test as wrong results do."""
+    torch = gpu
+    import threading
+    from gomlx_amd import nn
+    rng = np.random.default_rng(19)
+    calls, threads = 20, 4
+    xs = [torch.from_numpy(logits(rng, 30, 30000, sure=i % 2 == 0)).cuda() for i in range(threads)]
+    us = [torch.rand(30, device="cuda") for _ in range(threads)]
+    cases = [Case(torch, [3000, 2000], seed=30 + i).fill() for i in range(threads)]
+    caches = [c.cache.clone() for c in cases]
+    parents = [[random_parents(rng, 20) for _ in range(2)] for _ in range(threads)]
+    ups = [ints(torch, sum(p, [])) for p in parents]
+    words = [ints(torch, rng.integers(0, 4, 40)) for _ in range(threads)]
+    qs = [torch.randn(40, 8, 128, device="cuda") for _ in range(threads)]
+    lengths, starts = ints(torch, [3000, 2000]), ints(torch, [0, 20, 40])
+
+    def work(i):
+        caches[i].copy_(cases[i].cache)
+        tree, positions = nn.draft_tree(ups[i], lengths, starts=starts, max_new=20)
+        out = nn.tree_attention(qs[i], caches[i], cases[i].d_table, lengths, tree, starts=starts, max_new=20)
+        drawn, shares = nn.sample(xs[i], us[i], 1.0, 0, 0.9, probabilities=True)
+        path, token, left = nn.kv_cache_accept(caches[i], cases[i].d_table, lengths, ups[i], words[i], words[i], starts=starts, max_new=20)
+        return tree, positions, out, drawn, shares, path, token, left, caches[i].clone()
+
+    want = [work(i) for i in range(threads)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    streams.append(streams[1])
+    streams.append(torch.cuda.Stream())
+    done, errors = [0] * threads, []
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(streams[i]):
+                for _ in range(calls):
+                    got = work(i)
+                    streams[i].synchronize()
+                    assert all(torch.equal(x, y) for x, y in zip(got, want[i])), f"thread {i}, call {done[i]}"
+                    done[i] += 1
+        except BaseException as e:  # noqa: BLE001 (a thread's own traceback is only printed)
+            errors.append(e)
+
+    running = [threading.Thread(target=thread, args=(i,)) for i in range(threads)]
+    for t in running:
+        t.start()
+    for t in running:
+        t.join()
+    assert not errors, errors
+    assert done == [calls] * threads
