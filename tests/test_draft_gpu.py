@@ -955,3 +955,64 @@ def test_threads_finish_every_call(gpu):
         t.join()
     assert not errors, errors
     assert done == [calls] * threads
+
+
+def test_native_host_path(gpu, monkeypatch):
+    """The native steps serve the calls of a step with drafts, with the Python steps' results; what they do not know they leave alone."""
+    torch = gpu
+    from gomlx_amd import _lib, nn
+    rng = np.random.default_rng(20)
+    c = Case(torch, [90, 33], 2, 64, 32, seed=21, wide_table=1).fill()
+    n, starts = c.ints([90, 33]), c.ints([0, 6, 11])
+    up = ints(torch, random_parents(rng, 6) + random_parents(rng, 5))
+    words, drawn = ints(torch, rng.integers(0, 3, 11)), ints(torch, rng.integers(0, 3, 11))
+    q = torch.randn(11, 4, 64, device="cuda")
+    x, u = torch.randn(11, 3000, device="cuda"), torch.rand(11, device="cuda")
+    t, k = torch.rand(11, device="cuda"), ints(torch, rng.integers(0, 60, 11))
+    p, m = torch.rand(11, device="cuda"), 0.1 * torch.rand(11, device="cuda")
+    fast = _lib.fast
+    assert fast is not None
+
+    def calls():
+        cache, w = c.cache.clone(), torch.arange(c.pages * 2 * 32, device="cuda").float().view(c.pages, 2, 32)
+        tree, positions = nn.draft_tree(up, n, starts=starts, max_new=6)
+        out = [tree, positions, *nn.draft_tree(up[:2].contiguous(), n)]
+        out.append(nn.tree_attention(q, cache, c.d_table, n, tree, starts=starts, max_new=6))
+        out.append(nn.tree_attention(q.bfloat16(), cache, c.d_table, n, tree, starts, 6, 0.3, 9))
+        out.append(nn.tree_attention(q[:2], cache, c.d_table, n, tree[:2]))
+        for y in (x, x.bfloat16(), x[:, 1:2990]):
+            out += [nn.sample(y, u), nn.sample(y, u, 0), *nn.sample(y, u, 0.7, 40, 0.9, 0.01, True), *nn.sample(y, u, t, k, p, m, probabilities=True), nn.sample(y, u, t, 5, p)]
+        out += [*nn.kv_cache_accept(cache, c.d_table, n, up, words, drawn, starts=starts, max_new=6, weights=w), cache.clone(), w]
+        out += [*nn.kv_cache_accept(cache, c.d_table, n, up[:2].contiguous(), words[:2].contiguous(), drawn[:2].contiguous()), cache]
+        return out
+
+    native = calls()
+    served = []
+
+    class Spy:
+        def __getattr__(self, name):
+            def call(*args):
+                result = getattr(fast, name)(*args)
+                served.append((name, result is not None))
+                return result
+            return call
+
+    monkeypatch.setattr(_lib, "fast", Spy())
+    spied = calls()
+    assert all(ok for _, ok in served) and {name for name, _ in served} == {"draft_tree", "tree_attention", "sample", "kv_accept"}
+    monkeypatch.setattr(_lib, "fast", None)
+    plain = calls()
+    assert len(native) == len(plain) == len(spied)
+    for a, b, d in zip(native, plain, spied):
+        assert torch.equal(a, b) and torch.equal(a, d) and a.dtype == b.dtype and a.stride() == b.stride() and a.device == b.device
+    tree = native[0]
+    attend, accept = (q, c.cache, c.d_table, n, tree, starts, 6, None, 0), (c.cache, c.d_table, n, up, words, drawn, starts, 6, None)
+    change = lambda args, i, v: args[:i] + (v,) + args[i + 1:]  # noqa: E731
+    for f, args in ((fast.draft_tree, (up.long(), n, starts, 6)), (fast.draft_tree, (up, n[:1], starts, 6)), (fast.draft_tree, (up, n, None, 6)), (fast.draft_tree, (up, n, starts, 0)), (fast.draft_tree, (up.cpu(), n, starts, 6)),
+                    (fast.tree_attention, change(attend, 0, q.half())), (fast.tree_attention, change(attend, 0, q[:, :3])), (fast.tree_attention, change(attend, 4, tree.long())),
+                    (fast.tree_attention, change(attend, 4, tree[:10])), (fast.tree_attention, change(attend, 4, tree[:, :0])), (fast.tree_attention, change(attend, 8, -1)),
+                    (fast.tree_attention, change(attend, 0, q.cpu())), (fast.sample, (x, u, 1.0, 0.5, 1.0, 0.0, False)), (fast.sample, (x, u, -1.0, 0, 1.0, 0.0, False)), (fast.sample, (x, u, 1.0, 0, 1.5, 0.0, False)),
+                    (fast.sample, (x, u[:3], 1.0, 0, 1.0, 0.0, False)), (fast.sample, (x.half(), u, 1.0, 0, 1.0, 0.0, False)), (fast.sample, (x, u, 1.0, t, 1.0, 0.0, False)), (fast.sample, (x, u, t[:4], 0, 1.0, 0.0, False)),
+                    (fast.sample, (x.t(), u, 1.0, 0, 1.0, 0.0, False)), (fast.kv_accept, change(accept, 4, words.long())), (fast.kv_accept, change(accept, 5, drawn[:10])), (fast.kv_accept, change(accept, 3, up.view(1, 11))),
+                    (fast.kv_accept, change(accept, 7, 0)), (fast.kv_accept, change(accept, 6, None))):
+        assert f(*args) is None
