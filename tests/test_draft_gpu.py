@@ -1016,3 +1016,19 @@ def test_native_host_path(gpu, monkeypatch):
                     (fast.sample, (x.t(), u, 1.0, 0, 1.0, 0.0, False)), (fast.kv_accept, change(accept, 4, words.long())), (fast.kv_accept, change(accept, 5, drawn[:10])), (fast.kv_accept, change(accept, 3, up.view(1, 11))),
                     (fast.kv_accept, change(accept, 7, 0)), (fast.kv_accept, change(accept, 6, None))):
         assert f(*args) is None
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16"))
+@pytest.mark.parametrize("window", (0, 6))
+@pytest.mark.parametrize("more", (1, 2, 9))
+def test_attention_with_masks_wider_than_needed(gpu, dtype, window, more):
+    """Words behind those that the largest tree needs, some with bits set: they count for nothing."""
+    torch = gpu
+    c = Case(torch, [130, 40, 31], dim=64, page=32, seed=22).fill()
+    news = [33, 9, 31]
+    words = 2 + more
+    sets = [ref.ancestors(random_parents(c.rng, n)) for n in news]
+    for s in sets:
+        for row in s:
+            row.update(int(j) for j in c.rng.choice(np.arange(66, 32 * words), 5, replace=False))
+    check_attention(c, news, 8, sets, dtype, window=window, words=words)
