@@ -9,7 +9,8 @@
 // tile of 32 tokens at D = 128, every 16 rows 16 matrix instructions of 16 cycles (in float32 32) and some 47 vector instructions, eight of them exponentials of four times the
 // usual length, for their weights.  These bound it, for next to matrix instructions little else is issued: at 64 rows some 2000 cycles of the one and 1000 of the other a
 // tile, 3100 as measured (two wavefronts a SIMD; one alone takes 3500).  us a call, D = 128, bfloat16, 8 key heads of 4 queries: 32 sequences of 2048 to 8192 tokens with 8
-// to 16 nodes each 79 (460 TFLOP/s, 2.5 TB/s of cache); 32 nodes over 131072 tokens 93 (740 TFLOP/s); 16 sequences of 2048 to 8192 tokens with 32 to 64 nodes 124 (580).
+// to 16 nodes each 80 (450 TFLOP/s, 2.5 TB/s of cache); 32 nodes over 131072 tokens 96 (720 TFLOP/s); 16 sequences of 2048 to 8192 tokens with 32 to 64 nodes 124 (580).  (One of hundreds of
+// calls behind one another; of the first ten, before the clock has risen, 86, 104 and 138.)
 #include "kv_attend.hpp"
 
 #include <algorithm>
@@ -576,7 +577,9 @@ int launch_kv_tree_attention(const KvCall &kv, const HeadRows &q, int heads, flo
     a.blocks = (int)p.blocks;
     a.all_blocks = (int)p.all_blocks;
     const int64_t tiles = p.tiles, units = (int64_t)kv.seqs * kv.kv_heads * a.blocks;
-    // (as many workgroups as run at a time)
+    // Two workgroups a CU, as many as run at a time with 64 rows (with 16 there is room for more, of whose pieces more have to be joined): 16 nodes of 32 sequences of 2048 to 8192
+    // tokens, 1, 2, 3 and 4 a CU: bfloat16 at D = 128 99 80 101 98 us, at D = 64 71 54 68 64, float32 129 110 125 128; 4 nodes at D = 128 65 52 53 60, at D = 64 47 34 31 31; 32 nodes over 131072 tokens
+    // 107 95 109 105.  At D = 256 one runs at a time: 130 140 157 175.
     const int per_cu = kv.head_dim == 256 ? 1 : 2;
     const int workgroups = (int)std::min<int64_t>(device_cu_count() * per_cu, units * ((tiles + kLeastShare - 1) / kLeastShare));
     if (tiles > 1) {

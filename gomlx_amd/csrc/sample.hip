@@ -29,7 +29,9 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kChunk = 2048, kChunkKeys = 128, kLevelLanes = 48, kMostChunks = 1024;
 constexpr int kPickThreads = 512, kPickWaves = kPickThreads / 64, kBins = 2048, kListBins = 512, kListMost = 6144, kFew = 64;
-constexpr int kWideRows = 128;  // flat rows that the launches for them have room for; the others are gone over in the second launch
+// Flat rows that the launches for them have room for (68 KB each); the others are gone over in the second launch.  Of 512 rows of an output head that is unsure of every eighth some 14 to 25 are flat.
+// us for 64, 128, 256 and 512 rows of 128256 that all are, under top-p 0.95: 92 135 312 426, with room for 512 of them 92 134 209 368, for 32 of them 232 247 265 381.
+constexpr int kWideRows = 128;
 static_assert((kMostLogits + 7 + kChunk - 1) / kChunk <= kMostChunks, "a row's chunks have room in LDS, wherever its first logit lies");
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 constexpr float kNegInf = -__builtin_huge_valf();
@@ -196,8 +198,9 @@ __device__ __forceinline__ double sum_of_lanes(double v) {
 // number, padding) the level goes up over them, so that such a chunk takes nothing from the row's other lists: one row of 128256 with 200 numbers among -1e9 takes 22 us under top-k 50
 // and top-p 0.9, and 512 rows without a mask 86; with an empty list in the chunk's place, and all of the row gone over by its workgroup, 530 and 285.
 //
-// The reading bounds it where there are many rows: 512 rows of 128256 in float32 65 us, 4.04 TB/s (a plain sum reads 3.99, a copy moves 4.9), of which 26 vector instructions a logit,
-// 16 of them in 64 bits, take 48.  One row: 7 us.
+// 512 rows of 128256 in float32 take 64 us, 4.1 TB/s.  The memory gives 5.9 to a kernel that only reads (123 MB; 45 us for these), and 26 vector instructions a logit, 16 of them in 64 bits for the chunk's sum, take 48:
+// each wavefront loads its chunk first and works on it then, so that the two overlap by what other wavefronts do alone.  Keys that are read again come from the memory too (some 90 a chunk, 0.44 times
+// as many requests as the logits ask for).  One row: 7 us.
 template <bool BF16> __global__ __launch_bounds__(256) void sample_scan_kernel(const SampleArgs a, int64_t waves) {
     const int lane = (int)threadIdx.x & 63;
     const int64_t index = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -704,7 +707,7 @@ __device__ __forceinline__ void draw_alone(const SampleArgs &a, PickLds &l, cons
     draw(a, l, r, s, row, chunks, most, cut);
 }
 
-// A chain of passes over the lists behind barriers: 17 us for one row of 128256 under top-k and top-p, 26 for 512 (two a CU).  Keys by bins of their distance from the largest and few keys held
+// A chain of passes over the lists behind barriers: 17 us for one row of 128256 under top-k and top-p, 25 for 512 (two a CU).  Keys by bins of their distance from the largest and few keys held
 // against each other took the first of these from 31; the lists' loads sixteen at a time, scans by lane moves and the list cut down to what top-k keeps are in it.
 template <bool BF16> __global__ __launch_bounds__(kPickThreads, 4) void sample_pick_kernel(const SampleArgs a) {
     __shared__ PickLds l;
@@ -825,7 +828,7 @@ template <bool BF16> __global__ __launch_bounds__(kPickThreads, 4) void sample_p
 }
 
 // ---- the launches for flat rows: eight chunks a workgroup ------------------------------------------------------------------
-// 10 + 16 + 14 us for a few rows of 50257 in bfloat16, 16 + 20 + 20 for some 60 of 128256 in float32: loads, 64-bit exponentials and barriers one behind the other.  (One workgroup a row, as in draw_alone,
+// 10 + 16 + 14 us for a few rows of 50257 in bfloat16, 14 + 19 + 16 for some 20 of 128256 in float32: loads, 64-bit exponentials and barriers one behind the other.  (One workgroup a row, as in draw_alone,
 // took 70 us more than these for the first, 100 to 200 for the second.)
 
 __device__ __forceinline__ Wide *wide_of(const SampleArgs &a, int slot) { return slot < a.wide_rows && (uint32_t)slot < *a.wides ? a.wide + slot : nullptr; }
@@ -1002,8 +1005,9 @@ int launch_sample(const void *logits, bool bf16, int64_t rows, int64_t vocab, in
     // as many rows at a time as 256 MB of workspace hold
     const size_t a_row = (size_t)a.chunks * (sizeof(Chunk) + kChunkKeys * 4);
     const int64_t batch = std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)(((size_t)256 << 20) / a_row)));
-    // Flat rows have launches of their own where a bound may lead below a chunk's list (not a small top-k, which the lists nearly always hold) and a workgroup would
-    // go over a row in several rounds.
+    // Flat rows have launches of their own where a bound may lead below a chunk's list (not a small top-k, which the lists hold: 48 keys of a chunk at least, and all of the row's large ones) and a workgroup
+    // would go over a row in several rounds.  Where they find nothing to do they add 6 us: one row of 128256 under top-k 50 and top-p 0.9 23 us without them and 29 with them, 512 rows 100 and 104; a row that
+    // needs them and has none takes 70 to 200 more.
     const bool cuts = how.top_ks || how.top_ps || how.min_ps || how.top_k > 0 || how.top_p < 1.0 || how.min_p > 0.0;
     const bool wide = cuts && (how.top_ks || how.top_k <= 0 || how.top_k > 64) && a.chunks > kPickWaves;
     a.wide_rows = (int)std::min<int64_t>(batch, kWideRows);
