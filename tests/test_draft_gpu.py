@@ -365,7 +365,7 @@ def test_samples_of_rows_with_holes(gpu, how):
     assert tokens[3] == -1 and tokens[2] == 4321 and tokens[7] == 4999 and tokens[4] in (17, 4000)
 
 
-def kernel_us(call, times=5):
+def kernel_us(call, times=15):
     """The least time that the kernels of a call have taken."""
     import ctypes
     from gomlx_amd import _lib
