@@ -12,8 +12,8 @@
 // Weights are formed in 64 bits: next to a border, of which a vocabulary has as many as tokens, 32 would give another token once in some hundred rows.  Where order must
 // not matter (histograms, sums that several threads add to) they are whole numbers of 2^-42 of the largest.  The same arguments always give the same token.
 //
-// The first launch reads the logits once: a wavefront a chunk, which leaves its maximum, its sum and its largest keys (48 at least, some 90, complete from
-// a level on).  In the second a workgroup a row finds the cut among the keys that the chunks have left, and reads a single chunk again.  Where the cut lies
+// The first launch reads the logits once: a wavefront a chunk, which leaves its maximum, its sum and its largest keys (some 90, fewer where many are
+// equal, complete from a level on).  In the second a workgroup a row finds the cut among the keys that the chunks have left, and reads a single chunk again.  Where the cut lies
 // below what they have left (a flat distribution under top-p) the row is gone over twice more, by all its chunks at a time in launches that find nothing to do otherwise; where the
 // call's settings make that unlikely these launches are left out, and the second one does it by itself.
 #include "common.hpp"
@@ -1005,7 +1005,7 @@ int launch_sample(const void *logits, bool bf16, int64_t rows, int64_t vocab, in
     // as many rows at a time as 256 MB of workspace hold
     const size_t a_row = (size_t)a.chunks * (sizeof(Chunk) + kChunkKeys * 4);
     const int64_t batch = std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)(((size_t)256 << 20) / a_row)));
-    // Flat rows have launches of their own where a bound may lead below a chunk's list (not a small top-k, which the lists hold: 48 keys of a chunk at least, and all of the row's large ones) and a workgroup
+    // Flat rows have launches of their own where a bound may lead below a chunk's list (not a small top-k, which the lists hold: 48 keys of a chunk and more, where not too many of them are equal) and a workgroup
     // would go over a row in several rounds.  Where they find nothing to do they add 6 us: one row of 128256 under top-k 50 and top-p 0.9 23 us without them and 29 with them, 512 rows 100 and 104; a row that
     // needs them and has none takes 70 to 200 more.
     const bool cuts = how.top_ks || how.top_ps || how.min_ps || how.top_k > 0 || how.top_p < 1.0 || how.min_p > 0.0;
